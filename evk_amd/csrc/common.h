@@ -221,6 +221,10 @@ DEV float gelu_fast(float x) {
     return 0.5f * x * (1.0f + tanh_fast(ka * (x + kb * x * x * x)));
 }
 
+// x / (1 + e^-x) on the hardware exponential and reciprocal
+DEV float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x)); }
+DEV float silu_f(float x) { return x * sigmoid_fast(x); }
+
 // 16-byte accesses at any fp16 address
 DEV half8 ld_h8(const f16* p) {
     half8 v;

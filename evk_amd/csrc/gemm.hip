@@ -87,6 +87,30 @@ DEV void tile_to_lds(__amdgpu_buffer_rsrc_t res, int64_t ld, int r0, int c0, int
     }
 }
 
+// The columns of a GEMM_GLU tile: blocks of 16, in turn of the gate's matrix
+// and of the second one, so that a wave's accumulators hold both for the same
+// columns.  Chunk ch (8 columns) of a tile row: column glu_col(ch) from the
+// tile's first one, in matrix glu_mat(ch).
+DEV int glu_mat(int ch) { return (ch >> 1) & 1; }
+DEV int glu_col(int ch) { return (ch >> 2) * 16 + (ch & 1) * 8; }
+
+// tile_to_lds of a GEMM_GLU tile: rows r0.. of columns c0.. of both matrices,
+// each nr x nc, one behind the other
+template <int ROWS, int COLS, int NWV>
+DEV void glu_to_lds(__amdgpu_buffer_rsrc_t res, int r0, int c0, int nr, int nc, f16* lds, int wave, int lane) {
+    constexpr int CPR = COLS / 8, RPI = 64 / CPR, PER = ROWS / RPI / NWV;
+    static_assert(PER >= 1 && CPR >= 8, "tile shape");
+#pragma unroll
+    for (int t = 0; t < PER; ++t) {
+        const int q = wave * PER + t;
+        const int row = q * RPI + lane / CPR, ch = (lane % CPR) ^ (2 * (row & 3));
+        const int col = c0 + glu_col(ch);
+        const bool ok = r0 + row < nr && col < nc;
+        const uint32_t off = oob_or(ok, (uint32_t)((((int64_t)glu_mat(ch) * nr + r0 + row) * nc + col) * 2));
+        dma16(res, off, lds_addr(lds + q * 512));
+    }
+}
+
 // fragment of a k-contiguous tile: row r, k chunk kc (8 halves)
 DEV half8 frag_k(const f16* t, int r, int kc) {
     return *reinterpret_cast<const half8*>(t + r * MB_K + ((kc ^ (r & 7)) << 3));
@@ -114,10 +138,14 @@ struct RagTile {
     static_assert(PER >= 1 && ROWS * CPR % NT == 0, "tile shape");
     u32x4 r[PER];
 
+    // GLU: the columns of both matrices (nr x nc each, ld == nc)
+    template <bool GLU = false>
     DEV void load(const f16* src, int64_t ld, int64_t r0, int64_t c0, int nr, int nc, int tid) {
-        const int row = tid / CPR, col = (tid % CPR) * 8;  // chunk i: NT / CPR rows further each
+        const int ch = tid % CPR;
+        const int row = tid / CPR, col = GLU ? glu_col(ch) : ch * 8;  // chunk i: NT / CPR rows further each
         const f16* p = src + (r0 + row) * ld + c0 + col;
-        if (r0 + ROWS <= nr && c0 + COLS <= nc) {  // workgroup-uniform: the tile is whole
+        if constexpr (GLU) p += (int64_t)glu_mat(ch) * nr * nc;
+        if (r0 + ROWS <= nr && c0 + (GLU ? COLS / 2 : COLS) <= nc) {  // workgroup-uniform: the tile is whole
 #pragma unroll
             for (int i = 0; i < PER; ++i) __builtin_memcpy(&r[i], p + (int64_t)i * (NT / CPR) * ld, 16);
             return;
@@ -184,14 +212,21 @@ DEV void wait_vmcnt(int n) {
     }
 }
 
-template <int BM, int BN, bool TA, bool TB, int NWV, int KG, int NST, bool RAG>
+// KIND GEMM_ONE: a product.  GEMM_GLU: two products of A, with the two matrices
+// of B, joined in the epilogue (C = act(A B0) * A B1); a tile holds BN / 2
+// columns of each.  GEMM_PAIR: the sum of two products, A0 B0 + A1 B1 (each
+// second operand behind the first one), whose K tiles follow each other.
+template <int BM, int BN, bool TA, bool TB, int NWV, int KG, int NST, bool RAG, int KIND = GEMM_ONE>
 __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int tiles_m, int tiles_n) {
+    constexpr bool GLU = KIND == GEMM_GLU, PAIR = KIND == GEMM_PAIR;
+    static_assert(!GLU || (!TA && !TB), "rows of A against both matrices as they are");
     constexpr int WGN = NWV / 2;  // waves along N (2 along M)
     constexpr int BK = MB_K, WM = BM / 2, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
     constexpr int A_EL = BM * BK, B_EL = BN * BK, STAGE = A_EL + B_EL;
     static_assert(!RAG || NST == 2, "two stages through registers");
     constexpr int LPT = (BM * BK / 512 + BN * BK / 512) / NWV;  // DMA loads per wave per tile
-    constexpr int OUT_LD = WN + 8;
+    constexpr int OW = GLU ? WN / 2 : WN;  // columns of C in a wave's part
+    constexpr int OUT_LD = OW + 8;
     constexpr int OUT_EL = NWV * WM * OUT_LD;
     constexpr int LDS_EL = OUT_EL > KG * NST * STAGE ? OUT_EL : KG * NST * STAGE;
     static_assert(KG == 1 || (KG - 1) * NWV * FM * FN * 64 * 8 <= KG * NST * STAGE,
@@ -210,7 +245,7 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
     constexpr int GM = 4;
     const int grp = t / (GM * tiles_n), first = grp * GM, gsz = min(GM, tiles_m - first);
     const int tm = first + (t % (GM * tiles_n)) % gsz, tn = (t % (GM * tiles_n)) / gsz;
-    const int m0 = tm * BM, n0 = tn * BN;
+    const int m0 = tm * BM, n0 = tn * (GLU ? BN / 2 : BN);
 
     const int lane = threadIdx.x & 63;
     // KG > 1: KG groups of NWV waves; group kg takes the kg-th range of the
@@ -224,20 +259,43 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
     // RAG: every chunk is bounds-checked against the matrix; the descriptors
     // (whose sizes are 32-bit) serve the other form only
     const __amdgpu_buffer_rsrc_t ares = buf_rsrc(A, RAG ? 0u : (uint32_t)((int64_t)M * K * 2));
-    const __amdgpu_buffer_rsrc_t bres = buf_rsrc(B, RAG ? 0u : (uint32_t)((int64_t)K * N * 2));
+    const __amdgpu_buffer_rsrc_t bres = buf_rsrc(B, RAG ? 0u : (uint32_t)((int64_t)K * N * (GLU ? 4 : 2)));
     RagTile<TA ? BK : BM, TA ? BM : BK, !TA, 64 * NWV> ra;
     RagTile<TB ? BN : BK, TB ? BK : BN, TB, 64 * NWV> rb;
     const int gtid = wave * 64 + lane;
-    auto fetch = [&](int k0) {
-        if constexpr (TA) ra.load(A, M, k0, m0, K, M, gtid);
-        else ra.load(A, K, m0, k0, M, K, gtid);
-        if constexpr (TB) rb.load(B, K, n0, k0, N, K, gtid);
-        else rb.load(B, N, k0, n0, K, N, gtid);
+    constexpr int KSEG = PAIR ? 2 : 1;  // ranges of K, each in tiles of its own
+    const int kt_seg = (K + BK - 1) / BK;
+    auto fetch = [&](int kt) {
+        int k0 = kt * BK;
+        const f16 *fa = A, *fb = B;
+        if constexpr (PAIR) {
+            if (kt >= kt_seg) {
+                k0 = (kt - kt_seg) * BK;
+                fa += (int64_t)M * K;
+                fb += (int64_t)K * N;
+            }
+        }
+        if constexpr (TA) ra.load(fa, M, k0, m0, K, M, gtid);
+        else ra.load(fa, K, m0, k0, M, K, gtid);
+        if constexpr (TB) rb.load(fb, K, n0, k0, N, K, gtid);
+        else rb.template load<GLU>(fb, N, k0, n0, K, N, gtid);
     };
-    auto issue = [&](int k0, f16* sa, f16* sb) {
+    auto issue = [&](int kt, f16* sa, f16* sb) {
+        int k0 = kt * BK;
+        if constexpr (PAIR) {
+            static_assert(!PAIR || (!TA && TB), "the order of the input's gradient");
+            const bool second = kt >= kt_seg;
+            k0 = (kt - (second ? kt_seg : 0)) * BK;
+            const __amdgpu_buffer_rsrc_t as = buf_rsrc(A + (second ? (int64_t)M * K : 0), (uint32_t)((int64_t)M * K * 2));
+            const __amdgpu_buffer_rsrc_t bs = buf_rsrc(B + (second ? (int64_t)K * N : 0), (uint32_t)((int64_t)K * N * 2));
+            tile_to_lds<BM, BK, true, NWV>(as, K, m0, k0, M, K, sa, wave, lane);
+            tile_to_lds<BN, BK, true, NWV>(bs, K, n0, k0, N, K, sb, wave, lane);
+            return;
+        }
         if constexpr (TA) tile_to_lds<BK, BM, false, NWV>(ares, M, k0, m0, K, M, sa, wave, lane);
         else tile_to_lds<BM, BK, true, NWV>(ares, K, m0, k0, M, K, sa, wave, lane);
         if constexpr (TB) tile_to_lds<BN, BK, true, NWV>(bres, K, n0, k0, N, K, sb, wave, lane);
+        else if constexpr (GLU) glu_to_lds<BK, BN, NWV>(bres, k0, n0, K, N, sb, wave, lane);
         else tile_to_lds<BK, BN, false, NWV>(bres, N, k0, n0, K, N, sb, wave, lane);
     };
 
@@ -253,18 +311,19 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
     // allow it, so that they are there when the last product is (C
     // read at the end: 3072 x 768 over 2560 rows 33.4 us, now 30.0; the whole
     // MLP step 184 us with 2-byte reads and writes of C, 171, now 162).
-    constexpr int CPR = WN / 8, CQ = WM * CPR / 64;
+    constexpr int CPR = OW / 8, CQ = (WM * CPR + 63) / 64;
     constexpr bool C_EARLY = CQ <= 8;
     f16* ot = smem + wave * WM * OUT_LD;
     auto each_chunk = [&](auto&& f) {  // f(q, C address, LDS address, columns inside C)
 #pragma unroll
         for (int q = 0; q < CQ; ++q) {
             const int r = (lane + 64 * q) / CPR, cc = ((lane + 64 * q) % CPR) * 8;
-            const int row = m0 + wm0 + r, col = n0 + wn0 + cc;
+            const int row = m0 + wm0 + r, col = n0 + (GLU ? wn0 / 2 : wn0) + cc;
+            if (WM * CPR % 64 != 0 && r >= WM) continue;  // fewer chunks than lanes
             if (row < M && col < N) f(q, Cp + (int64_t)row * N + col, ot + r * OUT_LD + cc, N - col);
         }
     };
-    const bool adds = p.acc || p.epi == GEMM_RESIDUAL;
+    const bool adds = !GLU && (p.acc || p.epi == GEMM_RESIDUAL);
     u32x4 prior[CQ];
     auto load_c = [&] {
         each_chunk([&](int q, const f16* c, f16*, int left) {
@@ -321,7 +380,7 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
 
     // tile kt of the group's range lives in stage kt % NST; NST-1 tiles are
     // in flight.  Every group runs the same number of barrier steps.
-    const int KT_ALL = (K + BK - 1) / BK, per = (KT_ALL + KG - 1) / KG;
+    const int KT_ALL = KSEG * kt_seg, per = (KT_ALL + KG - 1) / KG;
     const int kt_base = kg * per, KT = max(0, min(KT_ALL - kt_base, per));
     f16* gsm = smem + kg * NST * STAGE;
     if constexpr (RAG) {
@@ -329,12 +388,12 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
         // and written to the other stage after (everyone has left that stage
         // once the barrier that published tile kt is passed)
         if (KT > 0) {
-            fetch(kt_base * BK);
+            fetch(kt_base);
             ra.store(gsm, gtid);
             rb.store(gsm + A_EL, gtid);
         }
         for (int kt = 0; kt < per; ++kt) {
-            if (kt + 1 < KT) fetch((kt_base + kt + 1) * BK);
+            if (kt + 1 < KT) fetch(kt_base + kt + 1);
             __syncthreads();
             if (kt >= KT) continue;
             const f16* cur = gsm + (kt % 2) * STAGE;
@@ -348,7 +407,7 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
     } else {
 #pragma unroll
         for (int t2 = 0; t2 < NST - 1; ++t2)
-            if (t2 < KT) issue((kt_base + t2) * BK, gsm + t2 * STAGE, gsm + t2 * STAGE + A_EL);
+            if (t2 < KT) issue(kt_base + t2, gsm + t2 * STAGE, gsm + t2 * STAGE + A_EL);
         for (int kt = 0; kt < per; ++kt) {
             // this wave's loads of tile kt are in LDS once at most the loads of
             // the younger tiles in flight remain (loads complete in order)
@@ -356,7 +415,7 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
             __syncthreads();  // everyone's; the stage of tile kt-1 is free again
             if (kt + NST - 1 < KT) {
                 f16* nxt = gsm + ((kt + NST - 1) % NST) * STAGE;
-                issue((kt_base + kt + NST - 1) * BK, nxt, nxt + A_EL);
+                issue(kt_base + kt + NST - 1, nxt, nxt + A_EL);
             }
             if (kt >= KT) continue;
             const f16* cur = gsm + (kt % NST) * STAGE;
@@ -393,6 +452,53 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
         __builtin_amdgcn_wave_barrier();
     };
+    auto write_out = [&](f16* dst) {  // the LDS tile to its place in dst, laid out as C
+        each_chunk([&](int, f16* c, const f16* o, int left) {
+            c = dst + (c - Cp);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(o);
+            if constexpr (RAG) {
+                if (left >= 8) {
+                    __builtin_memcpy(c, &v, 16);
+                } else {
+                    const half8 h = as_half8(v);
+#pragma unroll
+                    for (int e = 0; e < 7; ++e)
+                        if (e < left) c[e] = h[e];
+                }
+            } else {
+                // nontemporal: C is written once (QKV shape 0.785 -> 0.763 ms)
+                __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(c));
+            }
+        });
+    };
+    if constexpr (GLU) {
+        // gate and second product of column 16 j + l16 of the wave's part:
+        // acc[i][2 j] and acc[i][2 j + 1].  A training step keeps both rounded
+        // to fp16; C comes from the unrounded sums and is rounded once.
+        auto stage2 = [&](auto&& f) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN / 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        ot[(16 * i + 4 * g + e) * OUT_LD + 16 * j + l16] = (f16)f(acc[i][2 * j][e], acc[i][2 * j + 1][e]);
+            wave_lds();
+        };
+        if (p.gate_up) {
+            stage2([](float a, float) { return a; });
+            write_out(p.gate_up);
+            wave_lds();
+            stage2([](float, float b) { return b; });
+            write_out(p.gate_up + (int64_t)M * N);
+            wave_lds();
+        }
+        if (p.act == EVKHIP_ACT_SILU) stage2([](float a, float b) { return silu_f(a) * b; });
+        else if (p.act == EVKHIP_ACT_GELU) stage2([](float a, float b) { return gelu_fast(a) * b; });
+        else stage2([](float a, float b) { return (a < 0.0f ? 0.0f : a) * b; });
+        write_out(Cp);
+        return;
+    }
     auto stage = [&](auto&& f) {  // LDS tile = fp16(f(sum, what it holds))
 #pragma unroll
         for (int i = 0; i < FM; ++i)
@@ -440,22 +546,7 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
             return;
         }
     }
-    each_chunk([&](int, f16* c, const f16* o, int left) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(o);
-        if constexpr (RAG) {
-            if (left >= 8) {
-                __builtin_memcpy(c, &v, 16);
-            } else {
-                const half8 h = as_half8(v);
-#pragma unroll
-                for (int e = 0; e < 7; ++e)
-                    if (e < left) c[e] = h[e];
-            }
-        } else {
-            // nontemporal: C is written once (QKV shape 0.785 -> 0.763 ms)
-            __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(c));
-        }
-    });
+    write_out(Cp);
 }
 
 // ---- skinny GEMV: C(M,N) = A(M,K) B(K,N), M <= 16, B row-major -------------
@@ -901,6 +992,43 @@ hipError_t launch_plan_rag(int plan, const GemmArgs& a, int batch, bool ta, bool
     }
 }
 
+// The gated linear unit and the sum of two products: the same instances, the
+// plan by the cost of what they amount to (twice the columns, twice the K).
+template <int PLAN, bool RAG, int KIND>
+hipError_t launch_kind(const GemmArgs& a, hipStream_t st) {
+    constexpr GemmPlan P = kPlans[PLAN];
+    constexpr int CN = KIND == GEMM_GLU ? P.bn / 2 : P.bn;
+    const int tm = (a.M + P.bm - 1) / P.bm, tn = (a.N + CN - 1) / CN;
+    hipLaunchKernelGGL((gemm_mfma<P.bm, P.bn, false, KIND == GEMM_PAIR, P.waves, P.kg, RAG ? 2 : P.stages, RAG, KIND>),
+                       dim3((unsigned)(tm * tn)), dim3(64 * P.waves * P.kg), 0, st, a, tm, tn);
+    return hipGetLastError();
+}
+
+template <int KIND>
+hipError_t launch_kind_plan(const GemmArgs& a, bool direct, hipStream_t st) {
+    GemmArgs as = a;
+    if (KIND == GEMM_GLU) as.N = 2 * a.N;
+    else as.K = 2 * a.K;
+    const int plan = choose_plan(as, 1, direct ? kRowPlans : kRagPlans);
+    if (!direct) {
+        switch (plan) {
+            case 1: return launch_kind<1, true, KIND>(a, st);
+            case 4: return launch_kind<4, true, KIND>(a, st);
+            default: return launch_kind<6, true, KIND>(a, st);
+        }
+    }
+    switch (plan) {
+        case 0: return launch_kind<0, false, KIND>(a, st);
+        case 1: return launch_kind<1, false, KIND>(a, st);
+        case 2: return launch_kind<2, false, KIND>(a, st);
+        case 3: return launch_kind<3, false, KIND>(a, st);
+        case 4: return launch_kind<4, false, KIND>(a, st);
+        case 5: return launch_kind<5, false, KIND>(a, st);
+        case 6: return launch_kind<6, false, KIND>(a, st);
+        default: return launch_kind<7, false, KIND>(a, st);
+    }
+}
+
 // Library workspace for the split-K GEMV (grow-only): partials, and the
 // per-column-block arrival counters in an allocation of their own (zeroed
 // once; the last arrival of every launch leaves its counter at zero).
@@ -969,6 +1097,20 @@ int noalloc_scratch(GemvScratch* out) {
     out->part = reinterpret_cast<float*>(base + kScratchCounterBytes);
     out->part_elems = EVKHIP_NOALLOC_PART_BYTES / sizeof(float);
     return EVKHIP_OK;
+}
+
+int glu_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st) {
+    const bool direct = vec_ok && (int64_t)a.M * a.K * 2 < INT32_MAX && (int64_t)a.K * a.N * 4 < INT32_MAX &&
+                        (int64_t)a.M * a.N < INT32_MAX;
+    const hipError_t e = launch_kind_plan<GEMM_GLU>(a, direct, st);
+    return e == hipSuccess ? EVKHIP_OK : check_hip(e, "gated_linear launch");
+}
+
+int pair_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st) {
+    const bool direct = vec_ok && (int64_t)a.M * a.K * 2 < INT32_MAX && (int64_t)a.K * a.N * 2 < INT32_MAX &&
+                        (int64_t)a.M * a.N < INT32_MAX;
+    const hipError_t e = launch_kind_plan<GEMM_PAIR>(a, direct, st);
+    return e == hipSuccess ? EVKHIP_OK : check_hip(e, "gated_linear_backward launch");
 }
 
 int gemm_dispatch(const GemmArgs& a, int batch, bool ta, bool tb, bool vec_ok, hipStream_t st,

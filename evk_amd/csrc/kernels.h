@@ -22,12 +22,20 @@ struct GemmArgs {
     int acc;             // C = fp16(C + A B)
     int epi;             // GEMM_*, without acc
     QkvDest qkv;         // GEMM_QKV (C is not written)
+    f16* gate_up;        // glu_dispatch: both products, (2, M, N), or null
+    int act;             // glu_dispatch: EVKHIP_ACT_*
 };
 // Ops folded into the store of a product, with the roundings of the separate
 // ops: C = fp16(C + fp16(A B)), C = fp16(gelu(fp16(A B))), and rope of the q
 // and k columns of fp16(A B), regrouped per head and into the cache (A and B
 // row-major, N % 24 == 0).
 enum { GEMM_STORE = 0, GEMM_RESIDUAL = 1, GEMM_GELU = 2, GEMM_QKV = 3 };
+// gemm_mfma's forms: one product, a gated linear unit, a sum of two products
+enum { GEMM_ONE = 0, GEMM_GLU = 1, GEMM_PAIR = 2 };
+// C (M, N) = act(A B[0]) * (A B[1]): A (M, K), B (2, K, N).
+int glu_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st);
+// C (M, N) = A[0] B[0]^T + A[1] B[1]^T: A (2, M, K), B (2, N, K).
+int pair_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st);
 // Caller-provided split-K scratch of the skinny (M <= 16) path: partials and
 // arrival counters.  With it, gemm_dispatch allocates nothing.
 struct GemvScratch {
@@ -136,12 +144,43 @@ int cross_entropy_launch(const f16* logits, const uint16_t* tgt, f16* grad, f16*
                          bool vec, hipStream_t st);
 int sum_batch_launch(const f16* in, f16* out, int batch, int64_t per_batch, hipStream_t st);
 int causal_mask_launch(f16* scores, int64_t batch, int N, hipStream_t st);
+int glu_bwd_launch(const f16* gate_up, const f16* dh, f16* dgu, int64_t n, int act, hipStream_t st);
 int position_add_launch(const f16* in, const f16* pos, f16* out, int B, int64_t per_batch, hipStream_t st);
 int position_add_bwd_launch(const f16* gout, f16* gin, f16* gpos, int B, int64_t per_batch, hipStream_t st);
 int rope_bwd_launch(const f16* gout, f16* gin, int B, int S, int E, float base, hipStream_t st);
 int embed_bwd_launch(const f16* gout, const uint16_t* idx, f16* gemb, int64_t n_idx, int dim, int vocab,
                      hipStream_t st);
 void train_ops_free_workspace();
+
+// ---- qkv_rope.hip ----
+struct QkvRopeArgs {
+    const f16* qkv;        // (B, N, (H + 2 KV) dh)
+    const f16 *wq, *wk;    // (dh) or null
+    f16 *q, *k, *v;        // (B, N, H dh), (B, R, KV dh) twice
+    const f16 *dq, *dk, *dv;  // backward: (B, N, H dh), (B, N, KV dh) twice
+    f16 *dqkv, *dwq, *dwk;    // as qkv; (dh) or null
+    const int* offsets;    // (B) positions of the first tokens, or null: p0
+    int B, N, H, KV, R, dh, p0;
+    float eps, base;
+    int accumulate;        // dwq, dwk += instead of =
+};
+int qkv_rope_forward(const QkvRopeArgs& a, hipStream_t st);
+uint64_t qkv_rope_bwd_workspace(uint64_t tokens, int dh);
+int qkv_rope_backward(const QkvRopeArgs& a, float* part, hipStream_t st);  // part: that workspace, or null
+
+// ---- window.hip ----
+struct WindowArgs {
+    const f16 *q, *k, *v;   // (B, N, H dh), (B, R, KV dh) twice
+    const f16 *o, *dO;      // backward
+    f16 *out, *dK, *dV;     // O (forward) or dQ
+    float* lse;             // (B, H, N), null where the forward's caller wants none
+    const int* offsets;     // (B) positions of the first queries, or null: p0
+    int B, N, H, KV, R, dh, p0;
+    int window, sinks;      // window: INT32_MAX for none
+    float scale;
+};
+int window_forward(const WindowArgs& a, hipStream_t st);
+int window_backward(const WindowArgs& a, hipStream_t st);  // R == N, p0 == 0
 
 // ---- model.hip ----
 void model_free_workspace();

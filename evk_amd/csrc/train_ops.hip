@@ -137,6 +137,41 @@ __global__ __launch_bounds__(EW_NT) void gelu_bwd_k(const f16* gout, const f16* 
     st8(gin, i0, n, vec, a);
 }
 
+// Gated linear unit h = act(g) u: dg = dh u act'(g), du = dh act(g), from the
+// fp16 products of the forward; both gradients are rounded to fp16, the
+// operands of the products that follow.  Memory-bound: five values of n.
+DEV float act_of(float g, int act, float* grad) {
+    if (act == EVKHIP_ACT_SILU) {
+        const float sg = sigmoid_fast(g);
+        *grad = sg * (1.0f + g * (1.0f - sg));
+        return g * sg;
+    }
+    if (act == EVKHIP_ACT_GELU) {
+        *grad = gelu_grad(g);
+        return gelu_fast(g);
+    }
+    *grad = g > 0.0f ? 1.0f : 0.0f;
+    return g < 0.0f ? 0.0f : g;
+}
+__global__ __launch_bounds__(EW_NT) void glu_bwd_k(const f16* gate_up, const f16* dh, f16* dgu, int64_t n, int act,
+                                                   bool vec) {
+    const int64_t i0 = first8();
+    if (i0 >= n) return;
+    float g[8], u[8], h[8];
+    ld8(gate_up, i0, n, vec, g);
+    ld8(gate_up + n, i0, n, vec, u);
+    ld8(dh, i0, n, vec, h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float da;
+        const float a = act_of(g[e], act, &da);
+        g[e] = h[e] * u[e] * da;
+        u[e] = h[e] * a;
+    }
+    st8(dgu, i0, n, vec, g);
+    st8(dgu + n, i0, n, vec, u);
+}
+
 // sgd.comp: param = fp16(param - lr * grad)
 __global__ __launch_bounds__(EW_NT) void sgd_k(f16* param, const f16* grad, float lr, int64_t n, bool vec) {
     const int64_t i0 = first8();
@@ -778,6 +813,12 @@ int gelu_bwd_launch(const f16* gout, const f16* in, f16* gin, int64_t n, bool ve
     if (n == 0) return EVKHIP_OK;
     hipLaunchKernelGGL(gelu_bwd_k, dim3(ew_grid8(n)), dim3(EW_NT), 0, st, gout, in, gin, n, vec);
     return launched("gelu_backward launch");
+}
+int glu_bwd_launch(const f16* gate_up, const f16* dh, f16* dgu, int64_t n, int act, hipStream_t st) {
+    if (n == 0) return EVKHIP_OK;
+    const bool vec = n % 8 == 0 && aligned16(gate_up) && aligned16(dh) && aligned16(dgu);
+    hipLaunchKernelGGL(glu_bwd_k, dim3(ew_grid8(n)), dim3(EW_NT), 0, st, gate_up, dh, dgu, n, act, vec);
+    return launched("gated_linear_backward launch");
 }
 int sgd_launch(f16* param, const f16* grad, float lr, int64_t n, bool vec, hipStream_t st) {
     if (n == 0) return EVKHIP_OK;

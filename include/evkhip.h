@@ -293,6 +293,98 @@ int evkhip_embed_backward(const evkhip_tensor* grad_out, const evkhip_tensor* in
                           const evkhip_tensor* grad_embeddings, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Operators of a grouped-query transformer block (no reference counterparts:
+ * its block has one key head, no norm weights, sees every earlier position and
+ * ends in gelu).  H query heads share KV key and value heads of head_dim
+ * values; query head h reads key head h / (H / KV).  Position p is the number
+ * of tokens before a token in its sequence.
+ *
+ * `workspace` is device memory of the caller, 16-byte aligned, of at least the
+ * bytes that the operator's *_workspace function names for the shapes (0: may
+ * be NULL); its content does not matter and is not kept.  Calls whose
+ * workspaces do not overlap may run at the same time, and a captured call uses
+ * the workspace it was captured with.  Outputs may not overlap inputs, each
+ * other or the workspace (EVKHIP_ERR_INVALID_ARG).
+ * ------------------------------------------------------------------------- */
+
+/* Norms of queries and keys for each head with the position rotation, the
+ * values and the cache rows in one pass over the products of Wqkv.
+ * qkv (B,N,(H+2KV)*head_dim): the queries' heads, the keys', the values'.
+ * q (B,N,H*head_dim), k and v (B,rows,KV*head_dim).  Token t of sequence b has
+ * position p = position_offset + t, or offsets[b] + t (offsets: device int32
+ * (B), then position_offset is 0):
+ *   q[b,t], k[b,p] = turn_p(x * w / sqrt(mean(x^2) + eps)),  v[b,p] = x
+ * with mean over the head, w = q_weight / k_weight (head_dim; NULL: ones) and
+ * turn_p as evkhip_rope turns (frequencies by head_dim; the angle is formed in
+ * 64 bits).  Other rows of k and v keep their values, and rows that offsets
+ * put outside [0,rows) are not written.  head_dim even, at most 256;
+ * rows == N and position_offset 0 without a cache. */
+int evkhip_qkv_norm_rope(const evkhip_tensor* qkv, const evkhip_tensor* q_weight, const evkhip_tensor* k_weight,
+                         const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v, uint32_t head_dim,
+                         float eps, float rotary_base, uint32_t position_offset, const int32_t* offsets,
+                         void* stream);
+
+/* Its gradient: dq (B,N,H*head_dim), dk and dv (B,N,KV*head_dim) in; dqkv (as
+ * qkv) is written; dq_weight and dk_weight (head_dim, NULL: not wanted) are
+ * written, or added to with accumulate (summed in 32 bits in a fixed order,
+ * rounded once). */
+uint64_t evkhip_qkv_norm_rope_backward_workspace(uint64_t tokens, uint32_t head_dim);
+int evkhip_qkv_norm_rope_backward(const evkhip_tensor* qkv, const evkhip_tensor* q_weight,
+                                  const evkhip_tensor* k_weight, const evkhip_tensor* dq, const evkhip_tensor* dk,
+                                  const evkhip_tensor* dv, const evkhip_tensor* dqkv, const evkhip_tensor* dq_weight,
+                                  const evkhip_tensor* dk_weight, uint32_t head_dim, float eps, float rotary_base,
+                                  uint32_t position_offset, int accumulate, void* workspace,
+                                  uint64_t workspace_bytes, void* stream);
+
+/* Attention over a sliding window and the first tokens.  q, o
+ * (B,N,H*head_dim); k, v (B,rows,KV*head_dim), a cache or the sequence itself;
+ * scale 1/sqrt(head_dim).  Query t of sequence b stands at position
+ * p = position_offset + t, or offsets[b] + t (offsets: device int32 (B), then
+ * position_offset is 0), and sees the rows j <= p with j > p - window or
+ * j < sinks; window 0 shows every row up to p.  Rows that a query does not see
+ * do not reach its output, whatever they hold.  A query that sees no row (an
+ * offset below 0) has output 0 and log-sum-exp -inf.  lse: NULL or fp32
+ * (B,H,N).  N == 1 is a decode step.  head_dim up to 256. */
+uint64_t evkhip_window_attention_workspace(uint32_t batch, uint32_t n, uint32_t rows, uint32_t heads,
+                                           uint32_t kv_heads, uint32_t head_dim, uint32_t window, uint32_t sinks);
+int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,
+                            const evkhip_tensor* o, uint32_t head_dim, uint32_t window, uint32_t sinks,
+                            uint32_t position_offset, const int32_t* offsets, float* lse, void* workspace,
+                            uint64_t workspace_bytes, void* stream);
+
+/* Its gradient over a whole sequence (rows == N, positions from 0) from the
+ * forward's o and lse: dQ (as q), dK and dV (as k) are written, dK and dV
+ * summed over the heads that share them, in a fixed order. */
+uint64_t evkhip_window_attention_bwd_workspace(uint32_t batch, uint32_t n, uint32_t heads, uint32_t kv_heads,
+                                               uint32_t head_dim, uint32_t window, uint32_t sinks);
+int evkhip_window_attention_bwd(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,
+                                const evkhip_tensor* o, const evkhip_tensor* dO, const evkhip_tensor* dQ,
+                                const evkhip_tensor* dK, const evkhip_tensor* dV, const float* lse,
+                                uint32_t head_dim, uint32_t window, uint32_t sinks, void* workspace,
+                                uint64_t workspace_bytes, void* stream);
+
+/* Gated linear unit, the first half of a gated feed-forward block:
+ * h = act(x w[0]) * (x w[1]); x (...,D), w (2,D,F), h (...,F).  gate_up: NULL
+ * or (2,...,F), which receives both products for the backward pass.  h comes
+ * from the unrounded 32-bit products. */
+#define EVKHIP_ACT_SILU 0
+#define EVKHIP_ACT_GELU 1 /* the tanh form of evkhip_gelu */
+#define EVKHIP_ACT_RELU 2
+uint64_t evkhip_gated_linear_workspace(uint64_t tokens, uint32_t d, uint32_t f);
+int evkhip_gated_linear(const evkhip_tensor* x, const evkhip_tensor* w, const evkhip_tensor* h,
+                        const evkhip_tensor* gate_up, int activation, void* workspace, uint64_t workspace_bytes,
+                        void* stream);
+
+/* Its gradient from the forward's gate_up: dx (as x) is written; dw (as w) is
+ * written, or added to with accumulate.  Either may be NULL (not wanted).  The
+ * gradients of both products pass through fp16 once. */
+uint64_t evkhip_gated_linear_backward_workspace(uint64_t tokens, uint32_t d, uint32_t f);
+int evkhip_gated_linear_backward(const evkhip_tensor* x, const evkhip_tensor* w, const evkhip_tensor* gate_up,
+                                 const evkhip_tensor* dh, const evkhip_tensor* dx, const evkhip_tensor* dw,
+                                 int activation, int accumulate, void* workspace, uint64_t workspace_bytes,
+                                 void* stream);
+
+/* ---------------------------------------------------------------------------
  * KV-cached greedy decode (the caller the single-query path exists for; the
  * reference decodes by full recompute, example/main_llm.cpp:622-654).  The
  * model is the reference block (main_llm.cpp:528-546) in multi-head,
