@@ -42,7 +42,7 @@ def _run(cmd):
 
 # Files whose MFMA accumulators fit in the architectural VGPRs: keep them there
 # (no AGPR<->VGPR copies around the softmax / epilogue arithmetic).
-VGPR_MFMA = {"flash.hip", "flash_wide.hip"}
+VGPR_MFMA = {"flash.hip", "flash_wide.hip", "window.hip"}
 
 
 def _compile(src: str) -> str:

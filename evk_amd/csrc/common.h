@@ -169,6 +169,32 @@ DEV float buf_load_f16(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
 // it returns zeros, so predicated loads need no branch.
 DEV uint32_t oob_or(bool ok, uint32_t off) { return ok ? off : 0x80000000u; }
 
+typedef __attribute__((address_space(3))) void lds_void;
+
+// 16 bytes per lane from a buffer straight into LDS: lane i writes
+// lds_base + 16 i (lds_base: wave-uniform LDS byte address).  Written as
+// inline assembly so that the compiler does not make every later LDS read
+// wait for these loads (it cannot tell the two stages apart); the kernel
+// waits for them itself (vmcnt) before the barrier that publishes a stage.
+// M0 carries the LDS address; nothing else in the kernels that use this
+// keeps a value in M0.
+DEV void dma16(__amdgpu_buffer_rsrc_t res, uint32_t voff, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :
+                 : "v"(voff), "s"(res), "s"(lds_base)
+                 : "memory");
+}
+DEV uint32_t lds_addr(const f16* p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_void*)p);
+}
+
+// Workgroup w runs on XCD w % 8; each XCD takes a contiguous range of tiles
+// (the first total % 8 XCDs one more than the others).
+DEV int xcd_tile(int w, int total) {
+    const int x = w % 8;
+    return x * (total / 8) + min(x, total % 8) + w / 8;
+}
+
 DEV float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));

@@ -48,25 +48,6 @@ namespace {
 // such chunks too, and rounds the fp32 sum once.
 constexpr int MB_K = 64;  // BK
 
-typedef __attribute__((address_space(3))) void lds_void;
-
-// 16 bytes per lane from a buffer straight into LDS: lane i writes
-// lds_base + 16 i (lds_base: wave-uniform LDS byte address).  Written as
-// inline assembly so that the compiler does not make every later LDS read
-// wait for these loads (it cannot tell the two stages apart); the kernel
-// waits for them itself (vmcnt) before the barrier that publishes a stage.
-// M0 carries the LDS address; nothing else in the kernels that use this
-// keeps a value in M0.
-DEV void dma16(__amdgpu_buffer_rsrc_t res, uint32_t voff, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-                 :
-                 : "v"(voff), "s"(res), "s"(lds_base)
-                 : "memory");
-}
-DEV uint32_t lds_addr(const f16* p) {
-    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const lds_void*)p);
-}
-
 // One operand tile (ROWS x COLS halves as stored in memory; the matrix is
 // nr x nc with leading dimension ld, the tile starts at (r0, c0)) into LDS.
 template <int ROWS, int COLS, bool KCONTIG, int NWV = 4>
@@ -192,13 +173,6 @@ DEV half8 rope8(const half8& x, const float2* t) {
         r[2 * u + 1] = (f16)(x0 * sn[u] + x1 * cs[u]);
     }
     return r;
-}
-
-// Workgroup w runs on XCD w % 8; each XCD takes a contiguous range of tiles
-// (the first total % 8 XCDs one more than the others).
-DEV int xcd_tile(int w, int total) {
-    const int x = w % 8;
-    return x * (total / 8) + min(x, total % 8) + w / 8;
 }
 
 // s_waitcnt with vmcnt(n) (n < 64) and the other counters left alone

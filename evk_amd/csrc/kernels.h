@@ -178,6 +178,7 @@ struct WindowArgs {
     int B, N, H, KV, R, dh, p0;
     int window, sinks;      // window: INT32_MAX for none
     float scale;
+    int big;                // MFMA kernels: a sequence's rows of K pass 2 GiB
 };
 int window_forward(const WindowArgs& a, hipStream_t st);
 int window_backward(const WindowArgs& a, hipStream_t st);  // R == N, p0 == 0
