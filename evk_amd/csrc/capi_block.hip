@@ -283,8 +283,12 @@ int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, cons
 
 uint64_t evkhip_window_attention_bwd_workspace(uint32_t batch, uint32_t n, uint32_t heads, uint32_t kv_heads,
                                                uint32_t head_dim, uint32_t window, uint32_t sinks) {
-    (void)batch, (void)n, (void)heads, (void)kv_heads, (void)head_dim, (void)window, (void)sinks;
-    return 0;
+    // shapes that the call refuses need nothing
+    if (batch == 0 || n == 0 || heads == 0 || kv_heads == 0 || head_dim == 0 || head_dim > 256 ||
+        (uint64_t)batch * n * heads > kMaxRows || (uint64_t)batch * n * kv_heads > kMaxRows || n > kMaxRows)
+        return 0;
+    return window_bwd_workspace((int)batch, (int)n, (int)heads, (int)kv_heads, (int)head_dim,
+                                window ? clamp_int(window) : INT32_MAX, clamp_int(sinks));
 }
 
 int evkhip_window_attention_bwd(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,
@@ -321,7 +325,7 @@ int evkhip_window_attention_bwd(const evkhip_tensor* q, const evkhip_tensor* k, 
     a.dK = (f16*)dK->data;
     a.dV = (f16*)dV->data;
     a.lse = const_cast<float*>(lse);
-    return window_backward(a, as_stream(stream));
+    return window_backward(a, workspace, as_stream(stream));
 }
 
 uint64_t evkhip_gated_linear_workspace(uint64_t tokens, uint32_t d, uint32_t f) {

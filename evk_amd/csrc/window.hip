@@ -530,12 +530,380 @@ __global__ __launch_bounds__(256, 2) void window_fwd(WindowArgs a, int tiles) {
         fwd_row(a, ((int64_t)b * a.N + r / group) * a.H + c * group + r % group, reinterpret_cast<RowLds*>(smem)[wave], lane);
 }
 
+// Backward, dQ and the rows' statistics.  Workgroup as in the forward:
+//   S^T = K Q^T, dP^T = V dO^T, P = 2^(S c - lse), dS = P (dP - D),
+//   dQ^T += K^T dS^T (K^T by transposed reads of the same tile),
+// dS rounded to fp16 for the product.  Stores (lse log2 e, D) of every row,
+// flat by key head, for the kernel of dK and dV.
+template <int DH, int QB>
+__global__ __launch_bounds__(256, 2) void window_dq(WindowArgs a, int tiles, float2* stats) {
+    using G = Geo<DH>;
+    constexpr int KS = G::KS, DT = G::DT, W = G::W, TILE = BK * W, ROWS = 64 * QB;
+    __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4, trow = l16 >> 2, tcol = (l16 & 3) * 4;
+    const int at = xcd_tile(blockIdx.x, gridDim.x);
+    const int tile = tiles - 1 - at % tiles, bc = at / tiles, c = bc % a.KV, b = bc / a.KV;
+    const int group = a.H / a.KV, NR = a.N * group, R0 = tile * ROWS, wr0 = R0 + wave * 16 * QB;
+    const List list(a, b, R0 / group, (min(R0 + ROWS, NR) - 1) / group, a.big);
+    const KvTiles kv(a, b, c);
+    const int nt = (list.n + BK - 1) / BK;
+    kv.load<DH, 4>(a, list, 0, smem, smem + TILE, wave, lane);
+
+    half8 qf[QB][KS], gf[QB][KS];
+    int qp[QB];
+    float lse2[QB], dsum[QB];
+    const int64_t q0 = ((int64_t)b * a.N * a.H + c * group) * a.dh;
+    auto row_at = [&](int r) { return q0 + ((int64_t)(r / group) * a.H + r % group) * a.dh; };
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int r = min(wr0 + 16 * q + l16, NR - 1);
+        qp[q] = r / group;
+        lse2[q] = a.lse[((int64_t)b * a.H + c * group + r % group) * a.N + r / group] * kLog2e;
+        float sum = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            half8 of = {};
+            qf[q][ks] = gf[q][ks] = half8{};
+            if (32 * ks + 8 * g < a.dh) {
+                const int64_t src = row_at(r) + 32 * ks + 8 * g;
+                qf[q][ks] = *reinterpret_cast<const half8*>(a.q + src);
+                gf[q][ks] = *reinterpret_cast<const half8*>(a.dO + src);
+                of = *reinterpret_cast<const half8*>(a.o + src);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += (float)gf[q][ks][i] * (float)of[i];
+        }
+        dsum[q] = query_sum(sum);
+        if (g == 0 && wr0 + 16 * q + l16 < NR) stats[(int64_t)bc * NR + r] = float2{lse2[q], dsum[q]};
+    }
+    const float c2 = a.scale * kLog2e;
+    floatx4 acc[DT][QB];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int q = 0; q < QB; ++q) acc[d][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    half2_t wild = {(f16)0.0f, (f16)0.0f};
+    for (int t = 0; t < nt; ++t) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
+        __syncthreads();                     // everyone's; the other stage is free
+        f16* const sk = smem + (t & 1) * 2 * TILE;
+        f16* const sv = sk + TILE;
+        if (t + 1 < nt) {
+            f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
+            kv.load<DH, 4>(a, list, (t + 1) * BK, nx, nx + TILE, wave, lane);
+        }
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {  // 32 entries at a time
+            floatx4 s[2][QB], dp[2][QB];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int q = 0; q < QB; ++q) s[kb][q] = dp[kb][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const half8 kf = row_frag<W>(sk, 32 * k2 + 16 * kb + l16, 4 * ks + g);
+                    const half8 vf = row_frag<W>(sv, 32 * k2 + 16 * kb + l16, 4 * ks + g);
+#pragma unroll
+                    for (int q = 0; q < QB; ++q) {
+                        s[kb][q] = mfma16(kf, qf[q][ks], s[kb][q]);
+                        dp[kb][q] = mfma16(vf, gf[q][ks], dp[kb][q]);
+                    }
+                }
+            const bool plain = list.plain(a, t * BK + 32 * k2, 32);  // workgroup-uniform
+            half8 ds[QB];
+#pragma unroll
+            for (int q = 0; q < QB; ++q) {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][q][i % 4], c2, -lse2[q]));
+                    e[i] = p * (dp[i / 4][q][i % 4] - dsum[q]);
+                }
+                if (!plain) {
+                    const Seen see(a, list, qp[q]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) e[i] = see(t * BK + 32 * k2 + 16 * (i / 4) + 4 * g + i % 4) ? e[i] : 0.0f;
+                }
+                ds[q] = as_half8(u32x4{pack_h2(e[0], e[1]), pack_h2(e[2], e[3]), pack_h2(e[4], e[5]), pack_h2(e[6], e[7])});
+            }
+            half8 kt[DT];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) kt[d] = col_frag<W>(sk, 32 * k2 + 4 * g + trow, d, tcol);
+            if (!plain) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) wild = wild2(kt[d], wild);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int q = 0; q < QB; ++q) acc[d][q] = mfma16(kt[d], ds[q], acc[d][q]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int r = wr0 + 16 * q + l16;
+        if (r >= NR) continue;
+        f16* dst = a.out + row_at(r);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            if (16 * d + 4 * g < a.dh)
+                *reinterpret_cast<uint2*>(dst + 16 * d + 4 * g) = uint2{pack_h2(acc[d][q][0] * a.scale, acc[d][q][1] * a.scale),
+                                                                        pack_h2(acc[d][q][2] * a.scale, acc[d][q][3] * a.scale)};
+    }
+    static_assert(4 * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
+    const bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
+    if (!__syncthreads_or(again) || !again) return;
+#pragma unroll 1
+    for (int r = wr0; r < min(wr0 + 16 * QB, NR); ++r)
+        dq_row(a, ((int64_t)b * a.N + r / group) * a.H + c * group + r % group, reinterpret_cast<RowLds*>(smem)[wave], lane);
+}
+
+// Backward, dK and dV.  Workgroup: 4 waves of 16 KB rows (keys) of one key head
+// and one part of the queries that see any of them; Q and dO come in tiles of
+// QT flat rows through two LDS stages.
+//   S = Q K^T and dP = dO V^T (a lane: one key, rows 4 g + j of a 16-row
+//   block), P and dS are then the B operands of dV^T += dO^T P and
+//   dK^T += Q^T dS, whose A operands are transposed reads of the same tiles.
+// The sum over the heads of a group is part of the sum over rows.
+//
+// Parts: the queries from the first key's position to the last one that sees
+// the block are cut every `unit` positions (KEYS times Parts::q).  A block with
+// one part writes dK and dV; the others (the sinks' blocks, which every later
+// query sees, and all where the grid would not fill the chip otherwise) leave
+// 32-bit sums that window_dkdv_join adds in the order of the parts.
+struct Parts {
+    int q;         // key blocks' lengths of queries per part
+    int blocks;    // key blocks of a sequence
+    int full;      // the first of them, seen by every later query
+    int rest;      // parts of each other block
+    int64_t items;  // parts of one key head, slots of one key head
+    int64_t slots;
+    __host__ __device__ __forceinline__ int64_t sum(int64_t n) const {  // of ceil(m / q) for m = 1 .. n
+        const int64_t k = n / q;
+        return q * k * (k + 1) / 2 + (n - q * k) * (k + 1);
+    }
+    // parts before block i
+    __host__ __device__ __forceinline__ int64_t before(int i) const {
+        const int f = i < full ? i : full;
+        return sum(blocks) - sum(blocks - f) + (int64_t)(i - f) * rest;
+    }
+    __host__ __device__ __forceinline__ int parts_of(int i) const { return i < full ? (blocks - i + q - 1) / q : rest; }
+    DEV int block_of(int64_t item) const {  // the block that holds part `item`
+        int lo = 0, hi = blocks - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (before(mid) <= item) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    }
+};
+
+template <int DH, int KB>
+__global__ __launch_bounds__(256, KB == 1 && DH > 128 ? 1 : 2) void window_dkdv(WindowArgs a, Parts pt, const float2* stats, float* ws) {
+    using G = Geo<DH>;
+    constexpr int KS = G::KS, DT = G::DT, W = G::W, KEYS = 64 * KB, QT = 32, TILE = QT * W;
+    __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
+    __shared__ float2 sst[2][QT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4, trow = l16 >> 2, tcol = (l16 & 3) * 4;
+    const int64_t at = (int64_t)xcd_tile(blockIdx.x, gridDim.x);
+    const int bc = (int)(at / pt.items), c = bc % a.KV, b = bc / a.KV;
+    const int64_t item = at % pt.items;
+    const int blk = pt.block_of(item), part = (int)(item - pt.before(blk)), nparts = pt.parts_of(blk);
+    const int group = a.H / a.KV, NR = a.N * group;
+    const int k0 = blk * KEYS, klast = min(k0 + KEYS, a.N) - 1;
+    // queries of this part: flat rows [ra, rb)
+    const int64_t unit = (int64_t)pt.q * KEYS;
+    const int64_t t_end = k0 < a.sinks ? a.N : min((int64_t)a.N, (int64_t)klast + a.window);
+    const int ta = (int)min(t_end, k0 + part * unit), tb = (int)min(t_end, k0 + (part + 1) * unit);
+    const int ra = ta * group, rb = tb * group;
+    const int nt = (rb - ra + QT - 1) / QT;
+
+    const int64_t qb0 = (int64_t)b * a.N * a.H + c * group;  // row of (position 0, head 0 of the group)
+    auto load = [&](int r0, f16* sq, f16* sg) {
+        const int t0 = r0 / group;
+        const int64_t base = (qb0 + (int64_t)t0 * a.H) * a.dh;
+        const uint32_t span = (uint32_t)min(((int64_t)a.B * a.N * a.H * a.dh - base) * 2, (int64_t)INT32_MAX);
+        auto off = [&](int r) -> int64_t {
+            const int row = r0 + r;
+            return row < rb ? ((int64_t)(row / group - t0) * a.H + row % group) * a.dh * 2 : -1;
+        };
+        rows_to_lds<DH, QT, 4>(buf_rsrc(a.q + base, span), a.dh, sq, wave, lane, off);
+        rows_to_lds<DH, QT, 4>(buf_rsrc(a.dO + base, span), a.dh, sg, wave, lane, off);
+    };
+    float2 st = {0.0f, 0.0f};
+    auto load_stats = [&](int r0) {
+        if (threadIdx.x < QT) st = r0 + (int)threadIdx.x < rb ? stats[(int64_t)bc * NR + r0 + threadIdx.x] : float2{0.0f, 0.0f};
+    };
+    if (nt > 0) {
+        load(ra, smem, smem + TILE);
+        load_stats(ra);
+    }
+    half8 kf[KB][KS], vf[KB][KS];
+    int key[KB];
+    const int64_t kv_ld = (int64_t)a.KV * a.dh, kv0 = (int64_t)b * a.R * kv_ld + (int64_t)c * a.dh;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+        key[kb] = k0 + (wave * KB + kb) * 16 + l16;
+        const int64_t src = kv0 + min(key[kb], a.N - 1) * kv_ld;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            kf[kb][ks] = vf[kb][ks] = half8{};
+            if (32 * ks + 8 * g < a.dh) {
+                kf[kb][ks] = *reinterpret_cast<const half8*>(a.k + src + 32 * ks + 8 * g);
+                vf[kb][ks] = *reinterpret_cast<const half8*>(a.v + src + 32 * ks + 8 * g);
+            }
+        }
+    }
+    floatx4 gk[DT][KB], gv[DT][KB];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) gk[d][kb] = gv[d][kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    const float c2 = a.scale * kLog2e;
+    half2_t wild = {(f16)0.0f, (f16)0.0f};
+    for (int t = 0; t < nt; ++t) {
+        if (threadIdx.x < QT) sst[t & 1][threadIdx.x] = st;
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
+        __syncthreads();                     // everyone's; the other stage is free
+        f16* const sq = smem + (t & 1) * 2 * TILE;
+        f16* const sg = sq + TILE;
+        const int r0 = ra + t * QT;
+        if (t + 1 < nt) {
+            f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
+            load(r0 + QT, nx, nx + TILE);
+            load_stats(r0 + QT);
+        }
+        floatx4 s[2][KB], dp[2][KB];
+#pragma unroll
+        for (int rb2 = 0; rb2 < 2; ++rb2) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) s[rb2][kb] = dp[rb2][kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const half8 qf = row_frag<W>(sq, 16 * rb2 + l16, 4 * ks + g);
+                const half8 gf = row_frag<W>(sg, 16 * rb2 + l16, 4 * ks + g);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    s[rb2][kb] = mfma16(qf, kf[kb][ks], s[rb2][kb]);
+                    dp[rb2][kb] = mfma16(gf, vf[kb][ks], dp[rb2][kb]);
+                }
+            }
+        }
+        // every query of the tile sees every key of the block: the first query the last key, the last query the first
+        // key outside the sinks
+        const int tf = r0 / group, tl = min(r0 + QT, rb) - 1;
+        const bool plain = (r0 + QT <= rb) & (klast <= tf) &
+                           ((klast < a.sinks) | (max(k0, a.sinks) > tl / group - a.window));
+        half8 p[KB], ds[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            float e[8], f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 q = sst[t & 1][16 * (i / 4) + 4 * g + i % 4];
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][kb][i % 4], c2, -q.x));
+                f[i] = e[i] * (dp[i / 4][kb][i % 4] - q.y);
+            }
+            if (!plain) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = r0 + 16 * (i / 4) + 4 * g + i % 4, pos = r / group;
+                    const bool see = (r < rb) & (key[kb] <= pos) & ((key[kb] > pos - a.window) | (key[kb] < a.sinks));
+                    e[i] = see ? e[i] : 0.0f;
+                    f[i] = see ? f[i] : 0.0f;
+                }
+            }
+            p[kb] = as_half8(u32x4{pack_h2(e[0], e[1]), pack_h2(e[2], e[3]), pack_h2(e[4], e[5]), pack_h2(e[6], e[7])});
+            ds[kb] = as_half8(u32x4{pack_h2(f[0], f[1]), pack_h2(f[2], f[3]), pack_h2(f[4], f[5]), pack_h2(f[6], f[7])});
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const half8 gt = col_frag<W>(sg, 4 * g + trow, d, tcol), qt = col_frag<W>(sq, 4 * g + trow, d, tcol);
+            if (!plain) wild = wild2(qt, wild2(gt, wild));
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                gv[d][kb] = mfma16(gt, p[kb], gv[d][kb]);
+                gk[d][kb] = mfma16(qt, ds[kb], gk[d][kb]);
+            }
+        }
+    }
+    bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+        if (nparts > 1) {
+            // [key][dK, dV]; the parts of blocks that have one come after these
+            float* dst = ws + ((int64_t)bc * pt.slots + item) * (2 * KEYS * DH) + ((wave * KB + kb) * 16 + l16) * (2 * DH);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                *reinterpret_cast<floatx4*>(dst + 16 * d + 4 * g) = gk[d][kb];
+                *reinterpret_cast<floatx4*>(dst + DH + 16 * d + 4 * g) = gv[d][kb];
+            }
+            continue;
+        }
+        if (key[kb] >= a.N) continue;
+        const int64_t dst = kv0 + key[kb] * kv_ld;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            if (16 * d + 4 * g < a.dh) {
+                *reinterpret_cast<uint2*>(a.dK + dst + 16 * d + 4 * g) =
+                    uint2{pack_h2(gk[d][kb][0] * a.scale, gk[d][kb][1] * a.scale), pack_h2(gk[d][kb][2] * a.scale, gk[d][kb][3] * a.scale)};
+                *reinterpret_cast<uint2*>(a.dV + dst + 16 * d + 4 * g) =
+                    uint2{pack_h2(gv[d][kb][0], gv[d][kb][1]), pack_h2(gv[d][kb][2], gv[d][kb][3])};
+            }
+    }
+    if (nparts > 1) again = false;  // window_dkdv_join looks at the sums
+    static_assert(4 * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
+    if (!__syncthreads_or(again) || !again) return;
+#pragma unroll 1
+    for (int j = k0 + wave * 16 * KB; j < min(k0 + (wave + 1) * 16 * KB, a.N); ++j)
+        dkdv_row(a, ((int64_t)b * a.R + j) * a.KV + c, reinterpret_cast<RowLds*>(smem)[wave], lane);
+}
+
+// The sums of the parts of one key, a wave each.  A sum that is not finite may
+// be a hidden NaN's work: that key is computed again, row by row.
+template <int DH, int KEYS>
+__global__ __launch_bounds__(64) void window_dkdv_join(WindowArgs a, Parts pt, int blocks, const float* ws) {
+    constexpr int PER = 2 * DH / 64;
+    __shared__ RowLds lds;
+    const int lane = threadIdx.x, j = blockIdx.x % (blocks * KEYS), bc = blockIdx.x / (blocks * KEYS);
+    const int blk = j / KEYS, nparts = pt.parts_of(blk), c = bc % a.KV, b = bc / a.KV;
+    if (nparts < 2 || j >= a.N) return;
+    const float* src = ws + ((int64_t)bc * pt.slots + pt.before(blk)) * (2 * KEYS * DH) + (j % KEYS) * (2 * DH) + lane * PER;
+    float v[PER] = {};
+    for (int p = 0; p < nparts; ++p)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] += src[(int64_t)p * (2 * KEYS * DH) + i];
+    const int64_t row = ((int64_t)b * a.R + j) * a.KV + c;
+    const bool is_k = lane < 32;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        bad |= !(fabsf(v[i]) < INFINITY);
+        const int d = lane % 32 * PER + i;
+        if (d < a.dh) (is_k ? a.dK : a.dV)[row * a.dh + d] = (f16)(is_k ? v[i] * a.scale : v[i]);
+    }
+    if (__any(bad)) dkdv_row(a, row, lds, lane);
+}
+
 // The MFMA kernels' shapes
 bool mfma_ok(const WindowArgs& a) {
     if (a.dh % 8 || !aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.out)) return false;
     if (a.dO && (!aligned16(a.dO) || !aligned16(a.o) || !aligned16(a.dK) || !aligned16(a.dV))) return false;
     // a tile's rows behind one descriptor
     return (int64_t)a.KV * a.dh * 2 * (BK + 1) < INT32_MAX && (int64_t)a.H * a.dh * 2 * 260 < INT32_MAX;
+}
+template <class F>
+hipError_t by_head64(int dh, F&& f) {
+    if (dh <= 64) f(std::integral_constant<int, 64>{});
+    else if (dh <= 96) f(std::integral_constant<int, 96>{});
+    else if (dh <= 128) f(std::integral_constant<int, 128>{});
+    else f(std::integral_constant<int, 256>{});
+    return hipGetLastError();
 }
 template <class F>
 hipError_t by_head(int dh, F&& f) {
@@ -568,11 +936,69 @@ int window_forward(const WindowArgs& args, hipStream_t st) {
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "window_attention launch");
 }
 
-int window_backward(const WindowArgs& a, hipStream_t st) {
+namespace {
+// dK, dV workgroups: keys of one (64 KB), by head size
+constexpr int kv_blocks(int dh) { return dh <= 128 ? 2 : 1; }
+
+Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
+    const int64_t keys = 64 * kv_blocks(dh);
+    Parts p{};
+    p.blocks = (int)((N + keys - 1) / keys);
+    p.full = window >= N ? p.blocks : (int)std::min<int64_t>(p.blocks, (sinks + keys - 1) / keys);
+    // queries that see a block, in key blocks' lengths: the window, or every later one
+    const int64_t span = p.full == p.blocks ? p.blocks : ((int64_t)window + keys - 2) / keys + 1;
+    auto set = [&](int64_t q) {
+        p.q = (int)q;
+        p.rest = (int)((span + q - 1) / q);
+        p.items = p.before(p.blocks);
+        p.slots = p.rest > 1 ? p.items : p.before(p.full);
+    };
+    // long parts, as few as fill the chip
+    int64_t q = p.full == p.blocks ? std::max<int64_t>(1, span / 4) : span;
+    set(q);
+    while (q > 1 && p.items * B * KV < 768) set(q = q / 2);
+    return p;
+}
+}  // namespace
+
+uint64_t window_bwd_workspace(int B, int N, int H, int KV, int dh, int window, int sinks) {
+    if (dh % 8) return 0;
+    const Parts p = parts_for(B, N, KV, dh, window, sinks);
+    uint64_t row = 0;
+    (void)by_head64(dh, [&](auto dhc) { row = 2 * decltype(dhc)::value * sizeof(float); });
+    return ((uint64_t)B * N * H + 1) / 2 * 2 * sizeof(float2) + (uint64_t)B * KV * p.slots * 64 * kv_blocks(dh) * row;
+}
+
+int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
+    WindowArgs a = args;
+    a.big = (int64_t)a.R * a.KV * a.dh * 2 >= INT32_MAX;
     const int64_t rows = (int64_t)a.B * a.N * a.H, kv_rows = (int64_t)a.B * a.R * a.KV;
-    hipLaunchKernelGGL(window_dkdv_rows, dim3((unsigned)kv_rows), dim3(64), 0, st, a);
-    hipLaunchKernelGGL(window_dq_rows, dim3((unsigned)rows), dim3(64), 0, st, a);
-    const hipError_t e = hipGetLastError();
+    hipError_t e;
+    if (mfma_ok(a)) {
+        // stats first: 8 bytes a row, rounded up so that the sums behind them are aligned
+        float2* const stats = (float2*)ws;
+        float* const sums = (float*)(stats + (rows + 1) / 2 * 2);
+        e = by_head(a.dh, [&](auto dhc) {
+            constexpr int DH = decltype(dhc)::value, QB = DH <= 128 ? 2 : 1;
+            const int64_t nr = (int64_t)a.N * (a.H / a.KV);
+            const int tiles = (int)((nr + 64 * QB - 1) / (64 * QB));
+            hipLaunchKernelGGL((window_dq<DH, QB>), dim3((unsigned)((int64_t)tiles * a.B * a.KV)), dim3(256), 0, st, a, tiles, stats);
+        });
+        const Parts p = parts_for(a.B, a.N, a.KV, a.dh, a.window, a.sinks);
+        if (e == hipSuccess)
+            e = by_head64(a.dh, [&](auto dhc) {
+                constexpr int DH = decltype(dhc)::value, KB = kv_blocks(DH), KEYS = 64 * KB;
+                hipLaunchKernelGGL((window_dkdv<DH, KB>), dim3((unsigned)(p.items * a.B * a.KV)), dim3(256), 0, st, a, p, stats, sums);
+                const int joined = p.rest > 1 ? p.blocks : p.full;
+                if (p.slots > 0 && joined > 0)
+                    hipLaunchKernelGGL((window_dkdv_join<DH, KEYS>), dim3((unsigned)((int64_t)joined * KEYS * a.B * a.KV)), dim3(64), 0, st, a,
+                                       p, joined, sums);
+            });
+    } else {
+        hipLaunchKernelGGL(window_dkdv_rows, dim3((unsigned)kv_rows), dim3(64), 0, st, a);
+        hipLaunchKernelGGL(window_dq_rows, dim3((unsigned)rows), dim3(64), 0, st, a);
+        e = hipGetLastError();
+    }
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "window_attention_bwd launch");
 }
 
