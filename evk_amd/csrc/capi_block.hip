@@ -102,6 +102,12 @@ int check_norm(const char* op, float eps, float base) {
 
 int clamp_int(uint32_t v) { return v > (uint32_t)INT32_MAX ? INT32_MAX : (int)v; }
 
+// Whether the call takes these sizes; those that it refuses need no workspace.
+bool window_sizes(uint32_t B, uint32_t N, uint32_t R, uint32_t H, uint32_t KV, uint32_t dh) {
+    return B && N && R && H && KV && H % KV == 0 && dh && dh <= 256 && N <= kMaxRows && R <= kMaxRows &&
+           (uint64_t)B * N <= kMaxRows / H && (uint64_t)B * R <= kMaxRows / KV;
+}
+
 WindowArgs window_args(const Heads& s, uint32_t dh, uint32_t window, uint32_t sinks) {
     WindowArgs a{};
     a.B = (int)s.B;
@@ -251,8 +257,9 @@ int evkhip_qkv_norm_rope_backward(const evkhip_tensor* qkv, const evkhip_tensor*
 
 uint64_t evkhip_window_attention_workspace(uint32_t batch, uint32_t n, uint32_t rows, uint32_t heads,
                                            uint32_t kv_heads, uint32_t head_dim, uint32_t window, uint32_t sinks) {
-    (void)batch, (void)n, (void)rows, (void)heads, (void)kv_heads, (void)head_dim, (void)window, (void)sinks;
-    return 0;
+    if (!window_sizes(batch, n, rows, heads, kv_heads, head_dim)) return 0;
+    return window_fwd_workspace((int)batch, (int)n, (int)rows, (int)heads, (int)kv_heads, (int)head_dim,
+                                window ? clamp_int(window) : INT32_MAX, clamp_int(sinks));
 }
 
 int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,
@@ -278,15 +285,12 @@ int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, cons
     a.lse = lse;
     a.offsets = offsets;
     a.p0 = (int)position_offset;
-    return window_forward(a, as_stream(stream));
+    return window_forward(a, workspace, as_stream(stream));
 }
 
 uint64_t evkhip_window_attention_bwd_workspace(uint32_t batch, uint32_t n, uint32_t heads, uint32_t kv_heads,
                                                uint32_t head_dim, uint32_t window, uint32_t sinks) {
-    // shapes that the call refuses need nothing
-    if (batch == 0 || n == 0 || heads == 0 || kv_heads == 0 || head_dim == 0 || head_dim > 256 ||
-        (uint64_t)batch * n * heads > kMaxRows || (uint64_t)batch * n * kv_heads > kMaxRows || n > kMaxRows)
-        return 0;
+    if (!window_sizes(batch, n, n, heads, kv_heads, head_dim)) return 0;
     return window_bwd_workspace((int)batch, (int)n, (int)heads, (int)kv_heads, (int)head_dim,
                                 window ? clamp_int(window) : INT32_MAX, clamp_int(sinks));
 }

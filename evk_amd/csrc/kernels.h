@@ -180,7 +180,8 @@ struct WindowArgs {
     float scale;
     int big;                // MFMA kernels: a sequence's rows of K pass 2 GiB
 };
-int window_forward(const WindowArgs& a, hipStream_t st);
+uint64_t window_fwd_workspace(int B, int N, int R, int H, int KV, int dh, int window, int sinks);
+int window_forward(const WindowArgs& a, void* ws, hipStream_t st);
 uint64_t window_bwd_workspace(int B, int N, int H, int KV, int dh, int window, int sinks);
 int window_backward(const WindowArgs& a, void* ws, hipStream_t st);  // R == N, p0 == 0
 

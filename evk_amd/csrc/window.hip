@@ -240,38 +240,59 @@ struct Geo {
     static constexpr int W = DH <= 32 ? 32 : DH <= 64 ? 64 : DH <= 128 ? 128 : 256;  // halves of an LDS row
     static constexpr int CPR = W / 8;                                               // 16-byte chunks of it
 };
-// Chunk c of row r lies at slot c ^ swz(r): the reads of eight rows at one
-// chunk and of four rows at one pair of chunks both hit distinct banks.
+// Chunk c of row r lies at slot c ^ swz(r): the 64 banks serve the reads of 16
+// rows at one chunk, and the transposed reads of 8 rows at one pair of chunks,
+// without conflicts.
 template <int W>
 DEV int swz(int r) {
-    return W == 32 ? 2 * ((r >> 1) & 1) | ((r >> 2) & 1) : 2 * (r & 3) | ((r >> 2) & 1);
+    const int pair = W >= 128 ? r & 7 : W == 64 ? (r >> 1) & 3 : (r >> 2) & 1;  // rows that meet in the banks
+    return pair << 1 | ((r >> 3) & 1);
 }
-template <int W>
-DEV half8 row_frag(const f16* t, int r, int chunk) {
-    return *reinterpret_cast<const half8*>(t + r * W + ((chunk ^ swz<W>(r)) << 3));
-}
-// rows r .. r + 3 and r + 16 .. r + 19 (r = 4 g + trow of a 32-row step) of the 16 columns of block d
-template <int W>
-DEV half8 col_frag(const f16* t, int r, int d, int tcol) {
-    auto at = [&](int q) { return t + q * W + (((2 * d + (tcol >> 3)) ^ swz<W>(q)) << 3 | (tcol & 7)); };
-    return cat4(lds_read_tr(at(r)), lds_read_tr(at(r + 16)));
+// A lane's places in a tile: offsets are sums of a row's and exclusive ors of
+// a chunk's part.
+template <int DH>
+struct Frag {
+    static constexpr int W = Geo<DH>::W;
+    int row_at, col_at;
+    DEV explicit Frag(int lane) {
+        const int l16 = lane & 15, g = lane >> 4, r = 4 * g + (l16 >> 2), c = l16 & 3;
+        row_at = l16 * W + ((g ^ swz<W>(l16)) << 3);
+        col_at = r * W + (((c >> 1) ^ swz<W>(r)) << 3) + (c & 1) * 4;
+    }
+    // row r0 + l16 (r0 a multiple of 16), chunk 4 ks + g
+    DEV half8 row(const f16* t, int r0, int ks) const {
+        return *reinterpret_cast<const half8*>(t + r0 * W + (row_at ^ (ks << 5)));
+    }
+    // column 16 d + l16 of rows r0 + 4 g .. + 3 and 16 further (r0 a multiple of 32): two transposed reads
+    DEV half8 col(const f16* t, int r0, int d) const {
+        const f16* p = t + r0 * W + (col_at ^ (d << 4));
+        return cat4(lds_read_tr(p), lds_read_tr(p + 16 * W));
+    }
+};
+
+// buf_rsrc of values that are the same in the whole wave, wherever they were computed
+DEV __amdgpu_buffer_rsrc_t wave_rsrc(const f16* base, uint32_t bytes) {
+    const uint64_t p = (uint64_t)base;
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)p), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32));
+    return buf_rsrc((const void*)(hi << 32 | lo), (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
 }
 
-// ROWS rows of 16-byte chunks into LDS; off(row): byte offset of row `row` from the descriptor's base, or < 0 for
-// none.  Rows and chunks that are not there read as zeros.
-template <int DH, int ROWS, int NWV, class F>
-DEV void rows_to_lds(__amdgpu_buffer_rsrc_t res, int dh, f16* lds, int wave, int lane, F&& off) {
+// ROWS rows of 16-byte chunks into LDS by NWV waves: the lane's share of one
+// tile is chunk `chunk(i)` of row `row(i)`, i < PER, each 16 bytes to
+// lds + 1 KB (wave PER + i) + 16 lane.
+template <int DH, int ROWS, int NWV>
+struct TileDma {
     using G = Geo<DH>;
-    constexpr int RPI = 64 / G::CPR, PER = ROWS / RPI / NWV;
+    static constexpr int RPI = 64 / G::CPR, PER = ROWS / RPI / NWV;
     static_assert(PER >= 1 && ROWS % (RPI * NWV) == 0, "tile shape");
+    int wave, lane;
+    DEV int row(int i) const { return (wave * PER + i) * RPI + lane / G::CPR; }
+    DEV int chunk(int i) const { return (lane % G::CPR) ^ swz<G::W>(row(i)); }
+    DEV void go(__amdgpu_buffer_rsrc_t res, const uint32_t (&off)[PER], f16* lds) const {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int q = wave * PER + i, row = q * RPI + lane / G::CPR;
-        const int chunk = (lane % G::CPR) ^ swz<G::W>(row);
-        const int64_t o = off(row);
-        dma16(res, oob_or(o >= 0 && chunk * 8 < dh, (uint32_t)(o + chunk * 16)), lds_addr(lds + q * 512));
+        for (int i = 0; i < PER; ++i) dma16(res, off[i], lds_addr(lds + (wave * PER + i) * 512));
     }
-}
+};
 
 // The list of the rows that the queries t0 .. t1 of sequence b see.
 struct List {
@@ -280,8 +301,8 @@ struct List {
     int sl, n;       // entries before the window (s, or padded to whole tiles), entries
     int first;       // entries below this one are sinks
     DEV List(const WindowArgs& a, int b, int t0, int t1, bool pad) {
-        pmin = position_of(a, b, t0);
-        pmax = position_of(a, b, t1);
+        pmin = __builtin_amdgcn_readfirstlane(position_of(a, b, t0));
+        pmax = __builtin_amdgcn_readfirstlane(position_of(a, b, t1));
         hi = pmax < 0 ? 0 : min(pmax, a.R - 1) + 1;
         lo = min(max(0, pmin - a.window + 1), hi);
         s = a.sinks;
@@ -307,32 +328,45 @@ struct Seen {
     DEV bool operator()(int i) const { return (i <= hi) & ((i < first) | (i >= lo)); }
 };
 
-// K and V of one sequence and key head behind buffer descriptors.  While a
-// sequence's rows stay below 2 GiB one descriptor serves any row; past that
-// (WindowArgs::big) the sinks are padded to whole tiles and every tile has a
-// descriptor from its own first row on.
+// K and V of one sequence and key head behind buffer descriptors that start at
+// a tile's first row and end with the list (what lies past them reads as
+// zeros): a lane's offsets are the same in every tile.  Only a tile that holds
+// both sinks and window forms its own; while a sequence's rows stay below 2 GiB
+// their distance fits the offset, past that (WindowArgs::big) the sinks are
+// padded to whole tiles.
+template <int DH, int NWV>
 struct KvTiles {
+    using Dma = TileDma<DH, BK, NWV>;
     const f16 *k, *v;
-    int64_t bytes;  // of the sequence's rows from k on
-    uint32_t ld;    // bytes of a row
-    DEV KvTiles(const WindowArgs& a, int b, int c) {
+    uint32_t ld;  // bytes of a row
+    Dma dma;
+    uint32_t off[Dma::PER];
+    DEV KvTiles(const WindowArgs& a, int b, int c, int wave, int lane) : dma{wave, lane} {
         ld = (uint32_t)a.KV * a.dh * 2;
         const int64_t at = (int64_t)b * a.R * a.KV * a.dh + (int64_t)c * a.dh;
         k = a.k + at;
         v = a.v + at;
-        bytes = (int64_t)a.R * ld - (int64_t)c * a.dh * 2;
+#pragma unroll
+        for (int i = 0; i < Dma::PER; ++i) off[i] = oob_or(dma.chunk(i) * 8 < a.dh, dma.row(i) * ld + dma.chunk(i) * 16);
     }
-    template <int DH, int NWV>
-    DEV void load(const WindowArgs& a, const List& l, int i0, f16* sk, f16* sv, int wave, int lane) const {
-        const int first = a.big ? l.row(i0) : 0;
-        const int64_t skip = (int64_t)first * ld;
-        const uint32_t span = (uint32_t)min(bytes - skip, (int64_t)INT32_MAX);
-        auto off = [&](int r) -> int64_t {
-            const int i = i0 + r;
-            return (i < l.n) & ((i < l.s) | (i >= l.sl)) ? (int64_t)(l.row(i) - first) * ld : -1;
-        };
-        rows_to_lds<DH, BK, NWV>(buf_rsrc(k + skip / 2, span), a.dh, sk, wave, lane, off);
-        rows_to_lds<DH, BK, NWV>(buf_rsrc(v + skip / 2, span), a.dh, sv, wave, lane, off);
+    DEV void load(const List& l, int i0, f16* sk, f16* sv) const {
+        const int64_t skip = (int64_t)l.row(i0) * (ld / 2);
+        if (i0 < l.sl && i0 + BK > l.s) {  // sinks, then the window (or padding)
+            const int gap = l.sl == l.s ? l.lo - l.sl : l.hi;
+            const uint32_t rows = l.sl == l.s ? min(i0 + BK, l.n) - i0 + gap : l.s - i0;
+            uint32_t o[Dma::PER];
+#pragma unroll
+            for (int i = 0; i < Dma::PER; ++i) {
+                const bool far = i0 + dma.row(i) >= l.s;
+                o[i] = oob_or((off[i] < 0x80000000u) & !(far & (l.sl != l.s)), off[i] + (far ? (uint32_t)gap * ld : 0u));
+            }
+            dma.go(wave_rsrc(k + skip, rows * ld), o, sk);
+            dma.go(wave_rsrc(v + skip, rows * ld), o, sv);
+            return;
+        }
+        const uint32_t span = (uint32_t)min(l.n - i0, BK) * ld;
+        dma.go(wave_rsrc(k + skip, span), off, sk);
+        dma.go(wave_rsrc(v + skip, span), off, sv);
     }
 };
 
@@ -350,6 +384,14 @@ DEV float query_sum(float m) {
     const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
     return __uint_as_float(t[0]) + __uint_as_float(t[1]);
 }
+
+// n / d for 0 <= n < d + 2^16, d < 2^21: the quotient of n + 1/2 is at least
+// 1 / (2 d) from a whole number, its error at most 2^-22.
+struct SmallDiv {
+    float inv;
+    DEV explicit SmallDiv(int d) : inv(1.0f / (float)d) {}
+    DEV int operator()(int n) const { return (int)(((float)n + 0.5f) * inv); }
+};
 
 // NaN or infinity among the values: a product with 0 is 0 for every other one
 DEV half2_t wild2(const half8& x, half2_t w) {
@@ -425,20 +467,21 @@ struct Softmax {
 // that some query does not wholly see is looked at for such values in V; a wave
 // that meets one computes its rows again at the end, row by row.
 template <int DH, int QB>
-__global__ __launch_bounds__(256, 2) void window_fwd(WindowArgs a, int tiles) {
+__global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a, int tiles) {
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, TILE = BK * W, ROWS = 64 * QB;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l16 = lane & 15, g = lane >> 4, trow = l16 >> 2, tcol = (l16 & 3) * 4;
+    const int l16 = lane & 15, g = lane >> 4;
+    const Frag<DH> fr(lane);
     // an XCD takes tiles that follow each other, which share most of their rows
     const int at = xcd_tile(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - at % tiles, bc = at / tiles, c = bc % a.KV, b = bc / a.KV;
     const int group = a.H / a.KV, NR = a.N * group, R0 = tile * ROWS, wr0 = R0 + wave * 16 * QB;
     const List list(a, b, R0 / group, (min(R0 + ROWS, NR) - 1) / group, a.big);
-    const KvTiles kv(a, b, c);
+    const KvTiles<DH, 4> kv(a, b, c, wave, lane);
     const int nt = (list.n + BK - 1) / BK;
-    if (nt > 0) kv.load<DH, 4>(a, list, 0, smem, smem + TILE, wave, lane);
+    if (nt > 0) kv.load(list, 0, smem, smem + TILE);
 
     half8 qf[QB][KS];
     int qp[QB];
@@ -465,7 +508,7 @@ __global__ __launch_bounds__(256, 2) void window_fwd(WindowArgs a, int tiles) {
         f16* const sv = sk + TILE;
         if (t + 1 < nt) {
             f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
-            kv.load<DH, 4>(a, list, (t + 1) * BK, nx, nx + TILE, wave, lane);
+            kv.load(list, (t + 1) * BK, nx, nx + TILE);
         }
         floatx4 s[4][QB];
 #pragma unroll
@@ -474,7 +517,7 @@ __global__ __launch_bounds__(256, 2) void window_fwd(WindowArgs a, int tiles) {
             for (int q = 0; q < QB; ++q) s[kb][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const half8 kf = row_frag<W>(sk, 16 * kb + l16, 4 * ks + g);
+                const half8 kf = fr.row(sk, 16 * kb, ks);
 #pragma unroll
                 for (int q = 0; q < QB; ++q) s[kb][q] = mfma16(kf, qf[q][ks], s[kb][q]);
             }
@@ -497,7 +540,7 @@ __global__ __launch_bounds__(256, 2) void window_fwd(WindowArgs a, int tiles) {
         for (int k2 = 0; k2 < 2; ++k2) {
             half8 vf[DT];
 #pragma unroll
-            for (int d = 0; d < DT; ++d) vf[d] = col_frag<W>(sv, 32 * k2 + 4 * g + trow, d, tcol);
+            for (int d = 0; d < DT; ++d) vf[d] = fr.col(sv, 32 * k2, d);
             if (!plain) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) wild = wild2(vf[d], wild);
@@ -530,25 +573,206 @@ __global__ __launch_bounds__(256, 2) void window_fwd(WindowArgs a, int tiles) {
         fwd_row(a, ((int64_t)b * a.N + r / group) * a.H + c * group + r % group, reinterpret_cast<RowLds*>(smem)[wave], lane);
 }
 
+// Forward for few query rows (single tokens, short prompts): a workgroup takes
+// 16 rows of one key head, its NW waves every NW-th step of 32 entries, each
+// with a softmax of its own; the waves' states meet in LDS.  K goes from memory
+// straight into A operands, V through the wave's own LDS slot, no barrier
+// before the end: what counts is that every wave has its loads in flight.  A
+// long list is split over workgroups as well, whose states window_join adds.
+template <int DH>
+struct SplitGeo {
+    static constexpr int NW = DH <= 128 ? 8 : 4;  // waves
+};
+
+template <int DH>
+__global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void window_split(WindowArgs a, int tiles, int splits, float* ws) {
+    using G = Geo<DH>;
+    constexpr int KS = G::KS, DT = G::DT, W = G::W, NW = SplitGeo<DH>::NW, VPER = 32 * G::CPR / 64, OW = DH + 4;
+    constexpr int SLOT = 32 * W * 2, STATE = 16 * OW * 4;  // bytes of a wave's V, then of its state
+    constexpr int EACH = SLOT > STATE ? SLOT : STATE;
+    constexpr int BYTES = NW * (EACH > (int)sizeof(RowLds) ? EACH : (int)sizeof(RowLds));
+    __shared__ __attribute__((aligned(16))) char smem[BYTES];
+    __shared__ float sm_m[NW][16], sm_l[NW][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const Frag<DH> fr(lane);
+    const int at = xcd_tile(blockIdx.x, gridDim.x);
+    const int split = at % splits, tile = at / splits % tiles, bc = at / splits / tiles, c = bc % a.KV, b = bc / a.KV;
+    const int group = a.H / a.KV, NR = a.N * group, R0 = tile * 16;
+    const List list(a, b, R0 / group, (min(R0 + 16, NR) - 1) / group, false);
+    const int steps = (list.n + 31) / 32;
+    const int c0 = (int)((int64_t)steps * split / splits), c1 = (int)((int64_t)steps * (split + 1) / splits);
+    const int64_t ld = (int64_t)a.KV * a.dh, kv0 = (int64_t)b * a.R * ld + (int64_t)c * a.dh;
+    f16* const slot = reinterpret_cast<f16*>(smem + wave * SLOT);
+
+    u32x4 kr[2][KS], vr[VPER];
+    auto load_k = [&](int step) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const f16* src = a.k + kv0 + list.row(min(32 * step + 16 * kb + l16, list.n - 1)) * ld;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                kr[kb][ks] = u32x4{0u, 0u, 0u, 0u};
+                if (32 * ks + 8 * g < a.dh) kr[kb][ks] = *reinterpret_cast<const u32x4*>(src + 32 * ks + 8 * g);
+            }
+        }
+    };
+    auto load_v = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < VPER; ++i) {
+            const int row = (lane + 64 * i) / G::CPR, chunk = (lane + 64 * i) % G::CPR ^ swz<W>(row);
+            vr[i] = u32x4{0u, 0u, 0u, 0u};
+            if (chunk * 8 < a.dh)
+                vr[i] = *reinterpret_cast<const u32x4*>(a.v + kv0 + list.row(min(32 * step + row, list.n - 1)) * ld + chunk * 8);
+        }
+    };
+    int step = c0 + wave;
+    if (step < c1) {
+        load_k(step);
+        load_v(step);
+    }
+    const int r = min(R0 + l16, NR - 1), qp = position_of(a, b, r / group);
+    const int64_t q_at = ((int64_t)b * a.N + r / group) * a.H + c * group + r % group;  // row of q
+    half8 qf[1][KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        qf[0][ks] = half8{};
+        if (32 * ks + 8 * g < a.dh) qf[0][ks] = *reinterpret_cast<const half8*>(a.q + q_at * a.dh + 32 * ks + 8 * g);
+    }
+    const float c2 = a.scale * kLog2e;
+    Softmax<DH, 1> sm;
+    half2_t wild = {(f16)0.0f, (f16)0.0f};
+    for (; step < c1; step += NW) {
+#pragma unroll
+        for (int i = 0; i < VPER; ++i) *reinterpret_cast<u32x4*>(slot + (lane + 64 * i) * 8) = vr[i];
+        if (step + NW < c1) load_v(step + NW);
+        half8 vf[DT];
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vf[d] = fr.col(slot, 0, d);
+        floatx4 s[2][1];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            s[kb][0] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[kb][0] = mfma16(as_half8(kr[kb][ks]), qf[0][ks], s[kb][0]);
+        }
+        if (step + NW < c1) load_k(step + NW);
+        if (!list.plain(a, 32 * step, 32)) {
+            const Seen see(a, list, qp);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[kb][0][j] = see(32 * step + 16 * kb + 4 * g + j) ? s[kb][0][j] : -INFINITY;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) wild = wild2(vf[d], wild);
+        }
+        half8 p[1][1];
+        sm.template probs<2>(s, c2, p);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) sm.o[d][0] = mfma16(vf[d], p[0][0], sm.o[d][0]);
+    }
+    const bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
+    // the states, one row of OW floats a query; the slots have been read
+    const int any_again = __syncthreads_or(again);
+    float* const st = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<floatx4*>(st + (wave * 16 + l16) * OW + 16 * d + 4 * g) = sm.o[d][0];
+    const float l = query_sum(sm.l[0]);
+    if (g == 0) {
+        sm_m[wave][l16] = sm.m[0];
+        sm_l[wave][l16] = l;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * (DH / 4); e += 64 * NW) {
+        const int q = e / (DH / 4), d = e % (DH / 4) * 4, row = R0 + q;
+        if (row >= NR) continue;
+        float m = -INFINITY, ls = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, sm_m[w][q]);
+        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float f = sm_m[w][q] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm_m[w][q] - m);
+            ls += f * sm_l[w][q];
+            o += f * *reinterpret_cast<const floatx4*>(st + (w * 16 + q) * OW + d);
+        }
+        if (splits > 1) {
+            float* dst = ws + (((int64_t)bc * NR + row) * splits + split) * (DH + 4);
+            *reinterpret_cast<floatx4*>(dst + 4 + d) = o;
+            if (d == 0) dst[0] = m, dst[1] = ls;
+            continue;
+        }
+        const int64_t at_row = ((int64_t)b * a.N + row / group) * a.H + c * group + row % group;
+        const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+        if (d < a.dh)
+            *reinterpret_cast<uint2*>(a.out + at_row * a.dh + d) = uint2{pack_h2(o[0] * inv, o[1] * inv), pack_h2(o[2] * inv, o[3] * inv)};
+        if (a.lse && d == 0)
+            a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = ls == 0.0f ? -INFINITY : (m + log2f(ls)) * kLn2;
+    }
+    if (splits > 1 || !any_again) return;
+    __syncthreads();
+#pragma unroll 1
+    for (int q = wave; q < 16 && R0 + q < NR; q += NW) {
+        const int row = R0 + q;
+        fwd_row(a, ((int64_t)b * a.N + row / group) * a.H + c * group + row % group, reinterpret_cast<RowLds*>(smem)[wave], lane);
+    }
+}
+
+// The states of one query row's splits, a wave each, in their order.  What is
+// not finite may be a hidden NaN's work: that row is computed again.
+template <int DH>
+__global__ __launch_bounds__(64) void window_join(WindowArgs a, int splits, const float* ws) {
+    constexpr int PER = (DH + 63) / 64;
+    __shared__ RowLds lds;
+    const int lane = threadIdx.x, group = a.H / a.KV, NR = a.N * group;
+    const int row = blockIdx.x % NR, bc = blockIdx.x / NR, c = bc % a.KV, b = bc / a.KV;
+    const float* src = ws + (int64_t)blockIdx.x * splits * (DH + 4);
+    float m = -INFINITY;
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, src[s * (DH + 4)]);
+    float l = 0.0f, o[PER] = {};
+    for (int s = 0; s < splits; ++s) {
+        const float* p = src + s * (DH + 4);
+        const float f = p[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[0] - m);
+        l += f * p[1];
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (lane * PER + i < DH) o[i] += f * p[4 + lane * PER + i];
+    }
+    const int64_t at = ((int64_t)b * a.N + row / group) * a.H + c * group + row % group;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    bool bad = !(fabsf(l) < INFINITY);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int d = lane * PER + i;
+        if (d >= a.dh) continue;
+        bad |= !(fabsf(o[i]) < INFINITY);
+        a.out[at * a.dh + d] = (f16)(o[i] * inv);
+    }
+    if (a.lse && lane == 0)
+        a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    if (__any(bad)) fwd_row(a, at, lds, lane);
+}
+
 // Backward, dQ and the rows' statistics.  Workgroup as in the forward:
 //   S^T = K Q^T, dP^T = V dO^T, P = 2^(S c - lse), dS = P (dP - D),
 //   dQ^T += K^T dS^T (K^T by transposed reads of the same tile),
 // dS rounded to fp16 for the product.  Stores (lse log2 e, D) of every row,
 // flat by key head, for the kernel of dK and dV.
 template <int DH, int QB>
-__global__ __launch_bounds__(256, 2) void window_dq(WindowArgs a, int tiles, float2* stats) {
+__global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a, int tiles, float2* stats) {
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, TILE = BK * W, ROWS = 64 * QB;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l16 = lane & 15, g = lane >> 4, trow = l16 >> 2, tcol = (l16 & 3) * 4;
+    const int l16 = lane & 15, g = lane >> 4;
+    const Frag<DH> fr(lane);
     const int at = xcd_tile(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - at % tiles, bc = at / tiles, c = bc % a.KV, b = bc / a.KV;
     const int group = a.H / a.KV, NR = a.N * group, R0 = tile * ROWS, wr0 = R0 + wave * 16 * QB;
     const List list(a, b, R0 / group, (min(R0 + ROWS, NR) - 1) / group, a.big);
-    const KvTiles kv(a, b, c);
+    const KvTiles<DH, 4> kv(a, b, c, wave, lane);
     const int nt = (list.n + BK - 1) / BK;
-    kv.load<DH, 4>(a, list, 0, smem, smem + TILE, wave, lane);
+    kv.load(list, 0, smem, smem + TILE);
 
     half8 qf[QB][KS], gf[QB][KS];
     int qp[QB];
@@ -591,7 +815,7 @@ __global__ __launch_bounds__(256, 2) void window_dq(WindowArgs a, int tiles, flo
         f16* const sv = sk + TILE;
         if (t + 1 < nt) {
             f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
-            kv.load<DH, 4>(a, list, (t + 1) * BK, nx, nx + TILE, wave, lane);
+            kv.load(list, (t + 1) * BK, nx, nx + TILE);
         }
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {  // 32 entries at a time
@@ -604,8 +828,8 @@ __global__ __launch_bounds__(256, 2) void window_dq(WindowArgs a, int tiles, flo
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    const half8 kf = row_frag<W>(sk, 32 * k2 + 16 * kb + l16, 4 * ks + g);
-                    const half8 vf = row_frag<W>(sv, 32 * k2 + 16 * kb + l16, 4 * ks + g);
+                    const half8 kf = fr.row(sk, 32 * k2 + 16 * kb, ks);
+                    const half8 vf = fr.row(sv, 32 * k2 + 16 * kb, ks);
 #pragma unroll
                     for (int q = 0; q < QB; ++q) {
                         s[kb][q] = mfma16(kf, qf[q][ks], s[kb][q]);
@@ -631,7 +855,7 @@ __global__ __launch_bounds__(256, 2) void window_dq(WindowArgs a, int tiles, flo
             }
             half8 kt[DT];
 #pragma unroll
-            for (int d = 0; d < DT; ++d) kt[d] = col_frag<W>(sk, 32 * k2 + 4 * g + trow, d, tcol);
+            for (int d = 0; d < DT; ++d) kt[d] = fr.col(sk, 32 * k2, d);
             if (!plain) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) wild = wild2(kt[d], wild);
@@ -675,45 +899,49 @@ __global__ __launch_bounds__(256, 2) void window_dq(WindowArgs a, int tiles, flo
 // query sees, and all where the grid would not fill the chip otherwise) leave
 // 32-bit sums that window_dkdv_join adds in the order of the parts.
 struct Parts {
-    int q;         // key blocks' lengths of queries per part
-    int blocks;    // key blocks of a sequence
-    int full;      // the first of them, seen by every later query
-    int rest;      // parts of each other block
-    int64_t items;  // parts of one key head, slots of one key head
-    int64_t slots;
-    __host__ __device__ __forceinline__ int64_t sum(int64_t n) const {  // of ceil(m / q) for m = 1 .. n
-        const int64_t k = n / q;
+    int q;       // key blocks' lengths of queries per part
+    int blocks;  // key blocks of a sequence
+    int full;    // the first of them, seen by every later query: block i has ceil((blocks - i) / q) parts
+    int rest;    // parts of each other block
+    int items;   // parts of one key head
+    int slots;   // of them with sums in the workspace, the first ones
+    __host__ __device__ __forceinline__ int parts_of(int i) const { return i < full ? (blocks - i + q - 1) / q : rest; }
+    __host__ __device__ __forceinline__ int sum(int n) const {  // of ceil(m / q) for m = 1 .. n
+        const int k = n / q;
         return q * k * (k + 1) / 2 + (n - q * k) * (k + 1);
     }
-    // parts before block i
-    __host__ __device__ __forceinline__ int64_t before(int i) const {
+    __host__ __device__ __forceinline__ int before(int i) const {  // parts before block i
         const int f = i < full ? i : full;
-        return sum(blocks) - sum(blocks - f) + (int64_t)(i - f) * rest;
+        return sum(blocks) - sum(blocks - f) + (i - f) * rest;
     }
-    __host__ __device__ __forceinline__ int parts_of(int i) const { return i < full ? (blocks - i + q - 1) / q : rest; }
-    DEV int block_of(int64_t item) const {  // the block that holds part `item`
-        int lo = 0, hi = blocks - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (before(mid) <= item) lo = mid;
-            else hi = mid - 1;
+    // the block and the part that item `it` is: the first blocks in groups of q of equally many parts
+    DEV void find(int it, int* blk, int* part) const {
+        int k = (blocks + q - 1) / q, first = 0, n = min(full, blocks - (k - 1) * q);
+        while (first < full && it >= n * k) {
+            it -= n * k--;
+            first += n;
+            n = min(q, full - first);
         }
-        return lo;
+        if (first >= full) k = rest;
+        *blk = first + it / k;
+        *part = it % k;
     }
 };
 
 template <int DH, int KB>
-__global__ __launch_bounds__(256, KB == 1 && DH > 128 ? 1 : 2) void window_dkdv(WindowArgs a, Parts pt, const float2* stats, float* ws) {
+__global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void window_dkdv(WindowArgs a, Parts pt, const float2* stats, float* ws) {
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, KEYS = 64 * KB, QT = 32, TILE = QT * W;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
     __shared__ float2 sst[2][QT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l16 = lane & 15, g = lane >> 4, trow = l16 >> 2, tcol = (l16 & 3) * 4;
-    const int64_t at = (int64_t)xcd_tile(blockIdx.x, gridDim.x);
-    const int bc = (int)(at / pt.items), c = bc % a.KV, b = bc / a.KV;
-    const int64_t item = at % pt.items;
-    const int blk = pt.block_of(item), part = (int)(item - pt.before(blk)), nparts = pt.parts_of(blk);
+    const int l16 = lane & 15, g = lane >> 4;
+    const Frag<DH> fr(lane);
+    const int at = xcd_tile(blockIdx.x, gridDim.x);
+    const int bc = at / pt.items, c = bc % a.KV, b = bc / a.KV, item = at % pt.items;
+    int blk, part;
+    pt.find(item, &blk, &part);
+    const int nparts = pt.parts_of(blk);
     const int group = a.H / a.KV, NR = a.N * group;
     const int k0 = blk * KEYS, klast = min(k0 + KEYS, a.N) - 1;
     // queries of this part: flat rows [ra, rb)
@@ -724,16 +952,32 @@ __global__ __launch_bounds__(256, KB == 1 && DH > 128 ? 1 : 2) void window_dkdv(
     const int nt = (rb - ra + QT - 1) / QT;
 
     const int64_t qb0 = (int64_t)b * a.N * a.H + c * group;  // row of (position 0, head 0 of the group)
+    const SmallDiv by_group(group);
+    // a tile's rows begin with row m0 of a position's `group`; where tiles hold whole positions m0 is 0 throughout
+    using Dma = TileDma<DH, QT, 4>;
+    const Dma dma{wave, lane};
+    auto offset = [&](int i, int m0) {
+        const int m = m0 + dma.row(i), t = by_group(m);
+        return oob_or(dma.chunk(i) * 8 < a.dh, (uint32_t)((t * a.H + (m - t * group)) * a.dh + dma.chunk(i) * 8) * 2);
+    };
+    uint32_t off[Dma::PER];
+#pragma unroll
+    for (int i = 0; i < Dma::PER; ++i) off[i] = offset(i, 0);
     auto load = [&](int r0, f16* sq, f16* sg) {
-        const int t0 = r0 / group;
+        const int t0 = r0 / group, m0 = r0 - t0 * group, rows = min(QT, rb - r0);
         const int64_t base = (qb0 + (int64_t)t0 * a.H) * a.dh;
-        const uint32_t span = (uint32_t)min(((int64_t)a.B * a.N * a.H * a.dh - base) * 2, (int64_t)INT32_MAX);
-        auto off = [&](int r) -> int64_t {
-            const int row = r0 + r;
-            return row < rb ? ((int64_t)(row / group - t0) * a.H + row % group) * a.dh * 2 : -1;
-        };
-        rows_to_lds<DH, QT, 4>(buf_rsrc(a.q + base, span), a.dh, sq, wave, lane, off);
-        rows_to_lds<DH, QT, 4>(buf_rsrc(a.dO + base, span), a.dh, sg, wave, lane, off);
+        // up to the end of the last row
+        const int tl = by_group(m0 + rows - 1);
+        const uint32_t span = (uint32_t)(tl * a.H + (m0 + rows - 1 - tl * group) + 1) * a.dh * 2;
+        uint32_t o[Dma::PER];
+#pragma unroll
+        for (int i = 0; i < Dma::PER; ++i) {
+            o[i] = m0 ? offset(i, m0) : off[i];
+            // rows past the last one may lie before its end in memory (other heads' rows of the same position)
+            if (rows < QT) o[i] = oob_or(dma.row(i) < rows, o[i]);
+        }
+        dma.go(wave_rsrc(a.q + base, span), o, sq);
+        dma.go(wave_rsrc(a.dO + base, span), o, sg);
     };
     float2 st = {0.0f, 0.0f};
     auto load_stats = [&](int r0) {
@@ -744,12 +988,10 @@ __global__ __launch_bounds__(256, KB == 1 && DH > 128 ? 1 : 2) void window_dkdv(
         load_stats(ra);
     }
     half8 kf[KB][KS], vf[KB][KS];
-    int key[KB];
     const int64_t kv_ld = (int64_t)a.KV * a.dh, kv0 = (int64_t)b * a.R * kv_ld + (int64_t)c * a.dh;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-        key[kb] = k0 + (wave * KB + kb) * 16 + l16;
-        const int64_t src = kv0 + min(key[kb], a.N - 1) * kv_ld;
+        const int64_t src = kv0 + min(k0 + (wave * KB + kb) * 16 + l16, a.N - 1) * kv_ld;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             kf[kb][ks] = vf[kb][ks] = half8{};
@@ -766,6 +1008,52 @@ __global__ __launch_bounds__(256, KB == 1 && DH > 128 ? 1 : 2) void window_dkdv(
         for (int kb = 0; kb < KB; ++kb) gk[d][kb] = gv[d][kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     const float c2 = a.scale * kLog2e;
     half2_t wild = {(f16)0.0f, (f16)0.0f};
+    // the tiles with queries that do not see some key run a body of their own
+    auto scores = [&](int t, int r0, const f16* sq, const f16* sg, half8 (&p)[KB], half8 (&ds)[KB], auto mask) {
+        constexpr bool MASK = decltype(mask)::value;
+        const int tf = r0 / group, m0 = r0 - tf * group;
+#pragma unroll
+        for (int rb2 = 0; rb2 < 2; ++rb2) {
+            floatx4 s[KB], dp[KB];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) s[kb] = dp[kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const half8 qf = fr.row(sq, 16 * rb2, ks), gf = fr.row(sg, 16 * rb2, ks);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    s[kb] = mfma16(qf, kf[kb][ks], s[kb]);
+                    dp[kb] = mfma16(gf, vf[kb][ks], dp[kb]);
+                }
+            }
+            float2 st4[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) st4[j] = sst[t & 1][16 * rb2 + 4 * g + j];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                float e[4], f[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][j], c2, -st4[j].x));
+                    f[j] = e[j] * (dp[kb][j] - st4[j].y);
+                    if constexpr (MASK) {
+                        const int r = 16 * rb2 + 4 * g + j, pos = tf + by_group(m0 + r);
+                        const int key = k0 + (wave * KB + kb) * 16 + l16;
+                        const bool see = (r0 + r < rb) & (key <= pos) & ((key > pos - a.window) | (key < a.sinks));
+                        e[j] = see ? e[j] : 0.0f;
+                        f[j] = see ? f[j] : 0.0f;
+                    }
+                }
+                u32x4 pu = as_u32x4(p[kb]), du = as_u32x4(ds[kb]);
+                pu[2 * rb2] = pack_h2(e[0], e[1]);
+                pu[2 * rb2 + 1] = pack_h2(e[2], e[3]);
+                du[2 * rb2] = pack_h2(f[0], f[1]);
+                du[2 * rb2 + 1] = pack_h2(f[2], f[3]);
+                p[kb] = as_half8(pu);
+                ds[kb] = as_half8(du);
+            }
+        }
+    };
     for (int t = 0; t < nt; ++t) {
         if (threadIdx.x < QT) sst[t & 1][threadIdx.x] = st;
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
@@ -778,53 +1066,20 @@ __global__ __launch_bounds__(256, KB == 1 && DH > 128 ? 1 : 2) void window_dkdv(
             load(r0 + QT, nx, nx + TILE);
             load_stats(r0 + QT);
         }
-        floatx4 s[2][KB], dp[2][KB];
-#pragma unroll
-        for (int rb2 = 0; rb2 < 2; ++rb2) {
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) s[rb2][kb] = dp[rb2][kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const half8 qf = row_frag<W>(sq, 16 * rb2 + l16, 4 * ks + g);
-                const half8 gf = row_frag<W>(sg, 16 * rb2 + l16, 4 * ks + g);
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    s[rb2][kb] = mfma16(qf, kf[kb][ks], s[rb2][kb]);
-                    dp[rb2][kb] = mfma16(gf, vf[kb][ks], dp[rb2][kb]);
-                }
-            }
-        }
         // every query of the tile sees every key of the block: the first query the last key, the last query the first
         // key outside the sinks
-        const int tf = r0 / group, tl = min(r0 + QT, rb) - 1;
-        const bool plain = (r0 + QT <= rb) & (klast <= tf) &
-                           ((klast < a.sinks) | (max(k0, a.sinks) > tl / group - a.window));
+        const int tf = r0 / group, tl = (r0 + QT - 1) / group;
+        const bool plain = (r0 + QT <= rb) & (klast <= tf) & ((klast < a.sinks) | (max(k0, a.sinks) > tl - a.window));
         half8 p[KB], ds[KB];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            float e[8], f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float2 q = sst[t & 1][16 * (i / 4) + 4 * g + i % 4];
-                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][kb][i % 4], c2, -q.x));
-                f[i] = e[i] * (dp[i / 4][kb][i % 4] - q.y);
-            }
-            if (!plain) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int r = r0 + 16 * (i / 4) + 4 * g + i % 4, pos = r / group;
-                    const bool see = (r < rb) & (key[kb] <= pos) & ((key[kb] > pos - a.window) | (key[kb] < a.sinks));
-                    e[i] = see ? e[i] : 0.0f;
-                    f[i] = see ? f[i] : 0.0f;
-                }
-            }
-            p[kb] = as_half8(u32x4{pack_h2(e[0], e[1]), pack_h2(e[2], e[3]), pack_h2(e[4], e[5]), pack_h2(e[6], e[7])});
-            ds[kb] = as_half8(u32x4{pack_h2(f[0], f[1]), pack_h2(f[2], f[3]), pack_h2(f[4], f[5]), pack_h2(f[6], f[7])});
+        if (plain) {
+            scores(t, r0, sq, sg, p, ds, std::false_type{});
+        } else {
+            scores(t, r0, sq, sg, p, ds, std::true_type{});
+            for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sq, 0, d), wild2(fr.col(sg, 0, d), wild));
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-            const half8 gt = col_frag<W>(sg, 4 * g + trow, d, tcol), qt = col_frag<W>(sq, 4 * g + trow, d, tcol);
-            if (!plain) wild = wild2(qt, wild2(gt, wild));
+            const half8 gt = fr.col(sg, 0, d), qt = fr.col(sq, 0, d);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 gv[d][kb] = mfma16(gt, p[kb], gv[d][kb]);
@@ -845,8 +1100,9 @@ __global__ __launch_bounds__(256, KB == 1 && DH > 128 ? 1 : 2) void window_dkdv(
             }
             continue;
         }
-        if (key[kb] >= a.N) continue;
-        const int64_t dst = kv0 + key[kb] * kv_ld;
+        const int key = k0 + (wave * KB + kb) * 16 + l16;
+        if (key >= a.N) continue;
+        const int64_t dst = kv0 + key * kv_ld;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
             if (16 * d + 4 * g < a.dh) {
@@ -917,21 +1173,52 @@ hipError_t by_head(int dh, F&& f) {
 
 }  // namespace
 
-int window_forward(const WindowArgs& args, hipStream_t st) {
+namespace {
+// How the forward of a shape runs: 16-row tiles with the list split `splits`
+// ways, or (splits 0) tiles of 128 rows.
+int fwd_splits(int B, int N, int R, int H, int KV, int dh, int window, int sinks) {
+    const int64_t rows = (int64_t)N * (H / KV), heads = (int64_t)B * KV, wide = dh <= 128 ? 128 : 64;
+    const int64_t tiles = heads * ((rows + 15) / 16);
+    if (rows > 64 && heads * ((rows + wide - 1) / wide) >= 128) return 0;
+    const int64_t waves = dh <= 128 ? 8 : 4;
+    const int64_t list = std::min<int64_t>(R, (int64_t)window + sinks + 16), steps = (list + 31) / 32;
+    return (int)std::max<int64_t>(1, std::min((steps + 4 * waves - 1) / (4 * waves), 512 / tiles));
+}
+}  // namespace
+
+uint64_t window_fwd_workspace(int B, int N, int R, int H, int KV, int dh, int window, int sinks) {
+    if (dh % 8) return 0;
+    const int splits = fwd_splits(B, N, R, H, KV, dh, window, sinks);
+    uint64_t row = 0;
+    (void)by_head(dh, [&](auto dhc) { row = (decltype(dhc)::value + 4) * sizeof(float); });
+    return splits > 1 ? (uint64_t)B * N * H * splits * row : 0;
+}
+
+int window_forward(const WindowArgs& args, void* ws, hipStream_t st) {
     WindowArgs a = args;
     a.big = (int64_t)a.R * a.KV * a.dh * 2 >= INT32_MAX;
     const int64_t rows = (int64_t)a.B * a.N * a.H;
+    const int64_t nr = (int64_t)a.N * (a.H / a.KV), heads = (int64_t)a.B * a.KV;
+    const int splits = fwd_splits(a.B, a.N, a.R, a.H, a.KV, a.dh, a.window, a.sinks);
     hipError_t e;
-    if (mfma_ok(a)) {
-        e = by_head(a.dh, [&](auto dhc) {
-            constexpr int DH = decltype(dhc)::value, QB = DH <= 128 ? 2 : 1;
-            const int64_t nr = (int64_t)a.N * (a.H / a.KV);
-            const int tiles = (int)((nr + 64 * QB - 1) / (64 * QB));
-            hipLaunchKernelGGL((window_fwd<DH, QB>), dim3((unsigned)((int64_t)tiles * a.B * a.KV)), dim3(256), 0, st, a, tiles);
-        });
-    } else {
+    if (!mfma_ok(a)) {
         hipLaunchKernelGGL(window_fwd_rows, dim3((unsigned)rows), dim3(64), 0, st, a);
         e = hipGetLastError();
+    } else if (splits == 0) {
+        e = by_head(a.dh, [&](auto dhc) {
+            constexpr int DH = decltype(dhc)::value, QB = DH <= 128 ? 2 : 1;
+            const int tiles = (int)((nr + 64 * QB - 1) / (64 * QB));
+            hipLaunchKernelGGL((window_fwd<DH, QB>), dim3((unsigned)(tiles * heads)), dim3(256), 0, st, a, tiles);
+        });
+    } else {
+        e = by_head(a.dh, [&](auto dhc) {
+            constexpr int DH = decltype(dhc)::value;
+            const int tiles = (int)((nr + 15) / 16);
+            hipLaunchKernelGGL(window_split<DH>, dim3((unsigned)(tiles * splits * heads)), dim3(64 * SplitGeo<DH>::NW), 0, st, a, tiles, splits,
+                               (float*)ws);
+            if (splits > 1)
+                hipLaunchKernelGGL(window_join<DH>, dim3((unsigned)(nr * heads)), dim3(64), 0, st, a, splits, (const float*)ws);
+        });
     }
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "window_attention launch");
 }
@@ -941,22 +1228,29 @@ namespace {
 constexpr int kv_blocks(int dh) { return dh <= 128 ? 2 : 1; }
 
 Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
-    const int64_t keys = 64 * kv_blocks(dh);
-    Parts p{};
-    p.blocks = (int)((N + keys - 1) / keys);
-    p.full = window >= N ? p.blocks : (int)std::min<int64_t>(p.blocks, (sinks + keys - 1) / keys);
+    const int64_t keys = 64 * kv_blocks(dh), heads = (int64_t)B * KV;
+    const int64_t blocks = (N + keys - 1) / keys;
+    const int64_t full = window >= N ? blocks : std::min<int64_t>(blocks, ((int64_t)sinks + keys - 1) / keys);
     // queries that see a block, in key blocks' lengths: the window, or every later one
-    const int64_t span = p.full == p.blocks ? p.blocks : ((int64_t)window + keys - 2) / keys + 1;
-    auto set = [&](int64_t q) {
-        p.q = (int)q;
-        p.rest = (int)((span + q - 1) / q);
-        p.items = p.before(p.blocks);
-        p.slots = p.rest > 1 ? p.items : p.before(p.full);
+    const int64_t span = full == blocks ? blocks : std::min(blocks, ((int64_t)window + keys - 2) / keys + 1);
+    auto items = [&](int64_t q) {
+        auto sum = [&](int64_t n) {
+            const int64_t k = n / q;
+            return q * k * (k + 1) / 2 + (n - q * k) * (k + 1);
+        };
+        return sum(blocks) - sum(blocks - full) + (blocks - full) * ((span + q - 1) / q);
     };
-    // long parts, as few as fill the chip
-    int64_t q = p.full == p.blocks ? std::max<int64_t>(1, span / 4) : span;
-    set(q);
-    while (q > 1 && p.items * B * KV < 768) set(q = q / 2);
+    // long parts, as few as fill the chip (and fewer than 2^24)
+    int64_t q = full == blocks ? std::max<int64_t>(1, span / 4) : span;
+    while (q > 1 && items(q) * heads < 768) q /= 2;
+    while (items(q) * heads > (1 << 24) && q < blocks) q *= 2;
+    Parts p{};
+    p.q = (int)q;
+    p.blocks = (int)blocks;
+    p.full = (int)full;
+    p.rest = (int)((span + q - 1) / q);
+    p.items = (int)items(q);
+    p.slots = p.rest > 1 ? p.items : p.items - (int)(blocks - full);
     return p;
 }
 }  // namespace
