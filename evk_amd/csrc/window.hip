@@ -240,13 +240,13 @@ struct Geo {
     static constexpr int W = DH <= 32 ? 32 : DH <= 64 ? 64 : DH <= 128 ? 128 : 256;  // halves of an LDS row
     static constexpr int CPR = W / 8;                                               // 16-byte chunks of it
 };
-// Chunk c of row r lies at slot c ^ swz(r): the 64 banks serve the reads of 16
-// rows at one chunk, and the transposed reads of 8 rows at one pair of chunks,
-// without conflicts.
+// Chunk c of row r lies at slot c ^ swz(r).  LDS serves a transposed read in
+// halves of the wave (rows 0 .. 7, 8 .. 15 at one pair of chunks) and a 16-byte
+// read in four sets of lanes, each with all 16 rows, rows 4 .. 11 at the chunk
+// of the neighbouring g: both meet every bank once (measured: no conflicts).
 template <int W>
 DEV int swz(int r) {
-    const int pair = W >= 128 ? r & 7 : W == 64 ? (r >> 1) & 3 : (r >> 2) & 1;  // rows that meet in the banks
-    return pair << 1 | ((r >> 3) & 1);
+    return 2 * (W >= 128 ? r & 7 : W == 64 ? (r >> 1) & 3 : (r >> 2) & 1);
 }
 // A lane's places in a tile: offsets are sums of a row's and exclusive ors of
 // a chunk's part.
@@ -885,7 +885,7 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
         dq_row(a, ((int64_t)b * a.N + r / group) * a.H + c * group + r % group, reinterpret_cast<RowLds*>(smem)[wave], lane);
 }
 
-// Backward, dK and dV.  Workgroup: 4 waves of 16 KB rows (keys) of one key head
+// Backward, dK and dV.  Workgroup: NWV waves of 16 KB rows (keys) of one key head
 // and one part of the queries that see any of them; Q and dO come in tiles of
 // QT flat rows through two LDS stages.
 //   S = Q K^T and dP = dO V^T (a lane: one key, rows 4 g + j of a 16-row
@@ -928,10 +928,16 @@ struct Parts {
     }
 };
 
-template <int DH, int KB>
-__global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void window_dkdv(WindowArgs a, Parts pt, const float2* stats, float* ws) {
+template <int DH>
+struct KvGrad {
+    static constexpr int KB = 1, NWV = DH <= 128 ? 8 : 4;  // 16-key blocks of a wave, waves
+    static constexpr int KEYS = 16 * KB * NWV, QT = Geo<DH>::W >= 128 ? 32 : 64;
+};
+template <int DH>
+__global__ __launch_bounds__(64 * KvGrad<DH>::NWV, KvGrad<DH>::NWV / 4) void window_dkdv(WindowArgs a, Parts pt, const float2* stats, float* ws) {
     using G = Geo<DH>;
-    constexpr int KS = G::KS, DT = G::DT, W = G::W, KEYS = 64 * KB, QT = 32, TILE = QT * W;
+    constexpr int KS = G::KS, DT = G::DT, W = G::W, KB = KvGrad<DH>::KB, NWV = KvGrad<DH>::NWV, KEYS = KvGrad<DH>::KEYS;
+    constexpr int QT = KvGrad<DH>::QT, TILE = QT * W;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
     __shared__ float2 sst[2][QT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -954,7 +960,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void window_dkdv(WindowArgs a
     const int64_t qb0 = (int64_t)b * a.N * a.H + c * group;  // row of (position 0, head 0 of the group)
     const SmallDiv by_group(group);
     // a tile's rows begin with row m0 of a position's `group`; where tiles hold whole positions m0 is 0 throughout
-    using Dma = TileDma<DH, QT, 4>;
+    using Dma = TileDma<DH, QT, NWV>;
     const Dma dma{wave, lane};
     auto offset = [&](int i, int m0) {
         const int m = m0 + dma.row(i), t = by_group(m);
@@ -1009,7 +1015,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void window_dkdv(WindowArgs a
     const float c2 = a.scale * kLog2e;
     half2_t wild = {(f16)0.0f, (f16)0.0f};
     // the tiles with queries that do not see some key run a body of their own
-    auto scores = [&](int t, int r0, const f16* sq, const f16* sg, half8 (&p)[KB], half8 (&ds)[KB], auto mask) {
+    auto scores = [&](int t, int r0, int h, const f16* sq, const f16* sg, half8 (&p)[KB], half8 (&ds)[KB], auto mask) {
         constexpr bool MASK = decltype(mask)::value;
         const int tf = r0 / group, m0 = r0 - tf * group;
 #pragma unroll
@@ -1019,7 +1025,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void window_dkdv(WindowArgs a
             for (int kb = 0; kb < KB; ++kb) s[kb] = dp[kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const half8 qf = fr.row(sq, 16 * rb2, ks), gf = fr.row(sg, 16 * rb2, ks);
+                const half8 qf = fr.row(sq, 32 * h + 16 * rb2, ks), gf = fr.row(sg, 32 * h + 16 * rb2, ks);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
                     s[kb] = mfma16(qf, kf[kb][ks], s[kb]);
@@ -1028,7 +1034,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void window_dkdv(WindowArgs a
             }
             float2 st4[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) st4[j] = sst[t & 1][16 * rb2 + 4 * g + j];
+            for (int j = 0; j < 4; ++j) st4[j] = sst[t & 1][32 * h + 16 * rb2 + 4 * g + j];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 float e[4], f[4];
@@ -1037,7 +1043,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void window_dkdv(WindowArgs a
                     e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][j], c2, -st4[j].x));
                     f[j] = e[j] * (dp[kb][j] - st4[j].y);
                     if constexpr (MASK) {
-                        const int r = 16 * rb2 + 4 * g + j, pos = tf + by_group(m0 + r);
+                        const int r = 32 * h + 16 * rb2 + 4 * g + j, pos = tf + by_group(m0 + r);
                         const int key = k0 + (wave * KB + kb) * 16 + l16;
                         const bool see = (r0 + r < rb) & (key <= pos) & ((key > pos - a.window) | (key < a.sinks));
                         e[j] = see ? e[j] : 0.0f;
@@ -1070,20 +1076,23 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void window_dkdv(WindowArgs a
         // key outside the sinks
         const int tf = r0 / group, tl = (r0 + QT - 1) / group;
         const bool plain = (r0 + QT <= rb) & (klast <= tf) & ((klast < a.sinks) | (max(k0, a.sinks) > tl - a.window));
-        half8 p[KB], ds[KB];
-        if (plain) {
-            scores(t, r0, sq, sg, p, ds, std::false_type{});
-        } else {
-            scores(t, r0, sq, sg, p, ds, std::true_type{});
-            for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sq, 0, d), wild2(fr.col(sg, 0, d), wild));
-        }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            const half8 gt = fr.col(sg, 0, d), qt = fr.col(sq, 0, d);
+        for (int h = 0; h < QT / 32; ++h) {
+            half8 p[KB], ds[KB];
+            if (plain) {
+                scores(t, r0, h, sq, sg, p, ds, std::false_type{});
+            } else {
+                scores(t, r0, h, sq, sg, p, ds, std::true_type{});
+                for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sq, 32 * h, d), wild2(fr.col(sg, 32 * h, d), wild));
+            }
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                gv[d][kb] = mfma16(gt, p[kb], gv[d][kb]);
-                gk[d][kb] = mfma16(qt, ds[kb], gk[d][kb]);
+            for (int d = 0; d < DT; ++d) {
+                const half8 gt = fr.col(sg, 32 * h, d), qt = fr.col(sq, 32 * h, d);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    gv[d][kb] = mfma16(gt, p[kb], gv[d][kb]);
+                    gk[d][kb] = mfma16(qt, ds[kb], gk[d][kb]);
+                }
             }
         }
     }
@@ -1113,7 +1122,7 @@ __global__ __launch_bounds__(256, DH > 96 ? 1 : 2) void window_dkdv(WindowArgs a
             }
     }
     if (nparts > 1) again = false;  // window_dkdv_join looks at the sums
-    static_assert(4 * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
+    static_assert(NWV * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
     if (!__syncthreads_or(again) || !again) return;
 #pragma unroll 1
     for (int j = k0 + wave * 16 * KB; j < min(k0 + (wave + 1) * 16 * KB, a.N); ++j)
@@ -1224,11 +1233,8 @@ int window_forward(const WindowArgs& args, void* ws, hipStream_t st) {
 }
 
 namespace {
-// dK, dV workgroups: keys of one (64 KB), by head size
-constexpr int kv_blocks(int dh) { return dh <= 128 ? 2 : 1; }
-
 Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
-    const int64_t keys = 64 * kv_blocks(dh), heads = (int64_t)B * KV;
+    const int64_t keys = dh <= 128 ? KvGrad<128>::KEYS : KvGrad<256>::KEYS, heads = (int64_t)B * KV;
     const int64_t blocks = (N + keys - 1) / keys;
     const int64_t full = window >= N ? blocks : std::min<int64_t>(blocks, ((int64_t)sinks + keys - 1) / keys);
     // queries that see a block, in key blocks' lengths: the window, or every later one
@@ -1258,9 +1264,9 @@ Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
 uint64_t window_bwd_workspace(int B, int N, int H, int KV, int dh, int window, int sinks) {
     if (dh % 8) return 0;
     const Parts p = parts_for(B, N, KV, dh, window, sinks);
-    uint64_t row = 0;
-    (void)by_head64(dh, [&](auto dhc) { row = 2 * decltype(dhc)::value * sizeof(float); });
-    return ((uint64_t)B * N * H + 1) / 2 * 2 * sizeof(float2) + (uint64_t)B * KV * p.slots * 64 * kv_blocks(dh) * row;
+    uint64_t part = 0;
+    (void)by_head64(dh, [&](auto dhc) { part = KvGrad<decltype(dhc)::value>::KEYS * 2 * decltype(dhc)::value * sizeof(float); });
+    return ((uint64_t)B * N * H + 1) / 2 * 2 * sizeof(float2) + (uint64_t)B * KV * p.slots * part;
 }
 
 int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
@@ -1281,8 +1287,8 @@ int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
         const Parts p = parts_for(a.B, a.N, a.KV, a.dh, a.window, a.sinks);
         if (e == hipSuccess)
             e = by_head64(a.dh, [&](auto dhc) {
-                constexpr int DH = decltype(dhc)::value, KB = kv_blocks(DH), KEYS = 64 * KB;
-                hipLaunchKernelGGL((window_dkdv<DH, KB>), dim3((unsigned)(p.items * a.B * a.KV)), dim3(256), 0, st, a, p, stats, sums);
+                constexpr int DH = decltype(dhc)::value, KEYS = KvGrad<DH>::KEYS;
+                hipLaunchKernelGGL(window_dkdv<DH>, dim3((unsigned)(p.items * a.B * a.KV)), dim3(64 * KvGrad<DH>::NWV), 0, st, a, p, stats, sums);
                 const int joined = p.rest > 1 ? p.blocks : p.full;
                 if (p.slots > 0 && joined > 0)
                     hipLaunchKernelGGL((window_dkdv_join<DH, KEYS>), dim3((unsigned)((int64_t)joined * KEYS * a.B * a.KV)), dim3(64), 0, st, a,
