@@ -370,6 +370,32 @@ struct KvTiles {
     }
 };
 
+// N steps, each of M MFMAs on fragments that R LDS reads brought: the reads of
+// step i + AHEAD go out before the MFMAs of step i (read(i, slot) into slot
+// i % (AHEAD + 1) of a ring, use(i, slot)).  start() requests the first ones,
+// ahead of work that hides them; `pin` holds the scheduler to this order.
+template <int N, int AHEAD>
+struct Ring {
+    static constexpr int SLOTS = AHEAD + 1;
+    template <int R, class F>
+    static DEV void start(F&& read) {
+        static_for<AHEAD>([&](auto i) { read(i, i); });
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * R, 0);
+    }
+    template <int M, int R, class F, class U>
+    static DEV void run(F&& read, U&& use) {
+        static_for<N>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            if constexpr (i + AHEAD < N) {
+                read(std::integral_constant<int, i + AHEAD>{}, std::integral_constant<int, (i + AHEAD) % SLOTS>{});
+                __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+            }
+            use(ic, std::integral_constant<int, i % SLOTS>{});
+            __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+        });
+    }
+};
+
 DEV float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 // over the four lanes of a query (16 and 32 apart)
 DEV float query_max(float m) {
@@ -510,20 +536,19 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
             f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
             kv.load(list, (t + 1) * BK, nx, nx + TILE);
         }
+        using Rows = Ring<4 * KS, 3>;
+        using Cols = Ring<2 * DT, 2>;
         floatx4 s[4][QB];
+        half8 kf[Rows::SLOTS], vf[Cols::SLOTS];
+        auto row = [&](auto i, auto slot) { kf[slot] = fr.row(sk, 16 * (i / KS), i % KS); };
+        auto col = [&](auto i, auto slot) { vf[slot] = fr.col(sv, 32 * (i / DT), i % DT); };
+        Rows::template start<1>(row);
+        Rows::template run<QB, 1>(row, [&](auto i, auto slot) {
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-#pragma unroll
-            for (int q = 0; q < QB; ++q) s[kb][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const half8 kf = fr.row(sk, 16 * kb, ks);
-#pragma unroll
-                for (int q = 0; q < QB; ++q) s[kb][q] = mfma16(kf, qf[q][ks], s[kb][q]);
-            }
-        }
-        const bool plain = list.plain(a, t * BK, BK);  // workgroup-uniform
-        if (!plain) {
+            for (int q = 0; q < QB; ++q)
+                s[i / KS][q] = mfma16(kf[slot], qf[q][i % KS], i % KS ? s[i / KS][q] : floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+        });
+        if (!list.plain(a, t * BK, BK)) {  // workgroup-uniform
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
                 const Seen see(a, list, qp[q]);
@@ -533,23 +558,15 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
                     for (int j = 0; j < 4; ++j)
                         s[kb][q][j] = see(t * BK + 16 * kb + 4 * g + j) ? s[kb][q][j] : -INFINITY;
             }
+            for (int i = 0; i < 2 * DT; ++i) wild = wild2(fr.col(sv, i & 1 ? 32 : 0, i / 2), wild);
         }
         half8 p[2][QB];
         sm.template probs<4>(s, c2, p);
+        Cols::template start<2>(col);
+        Cols::template run<QB, 2>(col, [&](auto i, auto slot) {
 #pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-            half8 vf[DT];
-#pragma unroll
-            for (int d = 0; d < DT; ++d) vf[d] = fr.col(sv, 32 * k2, d);
-            if (!plain) {
-#pragma unroll
-                for (int d = 0; d < DT; ++d) wild = wild2(vf[d], wild);
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int q = 0; q < QB; ++q) sm.o[d][q] = mfma16(vf[d], p[k2][q], sm.o[d][q]);
-        }
+            for (int q = 0; q < QB; ++q) sm.o[i % DT][q] = mfma16(vf[slot], p[i / DT][q], sm.o[i % DT][q]);
+        });
     }
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
@@ -817,25 +834,26 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
             f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
             kv.load(list, (t + 1) * BK, nx, nx + TILE);
         }
+        using Rows = Ring<2 * KS, 2>;
+        using Cols = Ring<DT, 2>;
+        half8 kf[Rows::SLOTS], vf[Rows::SLOTS], kt[Cols::SLOTS];
 #pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {  // 32 entries at a time
+        for (int k2 = 0; k2 < 2; ++k2) {
+            auto row = [&](auto i, auto slot) {
+                kf[slot] = fr.row(sk, 32 * k2 + 16 * (i / KS), i % KS);
+                vf[slot] = fr.row(sv, 32 * k2 + 16 * (i / KS), i % KS);
+            };
+            auto col = [&](auto i, auto slot) { kt[slot] = fr.col(sk, 32 * k2, i); };
             floatx4 s[2][QB], dp[2][QB];
+            Rows::template start<2>(row);
+            Rows::template run<2 * QB, 2>(row, [&](auto i, auto slot) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int q = 0; q < QB; ++q) s[kb][q] = dp[kb][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const half8 kf = fr.row(sk, 32 * k2 + 16 * kb, ks);
-                    const half8 vf = fr.row(sv, 32 * k2 + 16 * kb, ks);
-#pragma unroll
-                    for (int q = 0; q < QB; ++q) {
-                        s[kb][q] = mfma16(kf, qf[q][ks], s[kb][q]);
-                        dp[kb][q] = mfma16(vf, gf[q][ks], dp[kb][q]);
-                    }
+                for (int q = 0; q < QB; ++q) {
+                    const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                    s[i / KS][q] = mfma16(kf[slot], qf[q][i % KS], i % KS ? s[i / KS][q] : zero);
+                    dp[i / KS][q] = mfma16(vf[slot], gf[q][i % KS], i % KS ? dp[i / KS][q] : zero);
                 }
+            });
             const bool plain = list.plain(a, t * BK + 32 * k2, 32);  // workgroup-uniform
             half8 ds[QB];
 #pragma unroll
@@ -853,17 +871,13 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
                 }
                 ds[q] = as_half8(u32x4{pack_h2(e[0], e[1]), pack_h2(e[2], e[3]), pack_h2(e[4], e[5]), pack_h2(e[6], e[7])});
             }
-            half8 kt[DT];
+            if (!plain)
+                for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sk, 32 * k2, d), wild);
+            Cols::template start<2>(col);
+            Cols::template run<QB, 2>(col, [&](auto i, auto slot) {
 #pragma unroll
-            for (int d = 0; d < DT; ++d) kt[d] = fr.col(sk, 32 * k2, d);
-            if (!plain) {
-#pragma unroll
-                for (int d = 0; d < DT; ++d) wild = wild2(kt[d], wild);
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int q = 0; q < QB; ++q) acc[d][q] = mfma16(kt[d], ds[q], acc[d][q]);
+                for (int q = 0; q < QB; ++q) acc[i][q] = mfma16(kt[slot], ds[q], acc[i][q]);
+            });
         }
     }
 #pragma unroll
@@ -930,11 +944,11 @@ struct Parts {
 
 template <int DH>
 struct KvGrad {
-    static constexpr int KB = 1, NWV = DH <= 128 ? 8 : 4;  // 16-key blocks of a wave, waves
+    static constexpr int KB = 1, NWV = 4;  // 16-key blocks of a wave, waves
     static constexpr int KEYS = 16 * KB * NWV, QT = Geo<DH>::W >= 128 ? 32 : 64;
 };
 template <int DH>
-__global__ __launch_bounds__(64 * KvGrad<DH>::NWV, KvGrad<DH>::NWV / 4) void window_dkdv(WindowArgs a, Parts pt, const float2* stats, float* ws) {
+__global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void window_dkdv(WindowArgs a, Parts pt, const float2* stats, float* ws) {
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, KB = KvGrad<DH>::KB, NWV = KvGrad<DH>::NWV, KEYS = KvGrad<DH>::KEYS;
     constexpr int QT = KvGrad<DH>::QT, TILE = QT * W;
@@ -950,12 +964,12 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, KvGrad<DH>::NWV / 4) void win
     const int nparts = pt.parts_of(blk);
     const int group = a.H / a.KV, NR = a.N * group;
     const int k0 = blk * KEYS, klast = min(k0 + KEYS, a.N) - 1;
-    // queries of this part: flat rows [ra, rb)
+    // queries of this part: flat rows [ra, rb_end)
     const int64_t unit = (int64_t)pt.q * KEYS;
     const int64_t t_end = k0 < a.sinks ? a.N : min((int64_t)a.N, (int64_t)klast + a.window);
     const int ta = (int)min(t_end, k0 + part * unit), tb = (int)min(t_end, k0 + (part + 1) * unit);
-    const int ra = ta * group, rb = tb * group;
-    const int nt = (rb - ra + QT - 1) / QT;
+    const int ra = ta * group, rb_end = tb * group;
+    const int nt = (rb_end - ra + QT - 1) / QT;
 
     const int64_t qb0 = (int64_t)b * a.N * a.H + c * group;  // row of (position 0, head 0 of the group)
     const SmallDiv by_group(group);
@@ -970,7 +984,7 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, KvGrad<DH>::NWV / 4) void win
 #pragma unroll
     for (int i = 0; i < Dma::PER; ++i) off[i] = offset(i, 0);
     auto load = [&](int r0, f16* sq, f16* sg) {
-        const int t0 = r0 / group, m0 = r0 - t0 * group, rows = min(QT, rb - r0);
+        const int t0 = r0 / group, m0 = r0 - t0 * group, rows = min(QT, rb_end - r0);
         const int64_t base = (qb0 + (int64_t)t0 * a.H) * a.dh;
         // up to the end of the last row
         const int tl = by_group(m0 + rows - 1);
@@ -987,7 +1001,7 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, KvGrad<DH>::NWV / 4) void win
     };
     float2 st = {0.0f, 0.0f};
     auto load_stats = [&](int r0) {
-        if (threadIdx.x < QT) st = r0 + (int)threadIdx.x < rb ? stats[(int64_t)bc * NR + r0 + threadIdx.x] : float2{0.0f, 0.0f};
+        if (threadIdx.x < QT) st = r0 + (int)threadIdx.x < rb_end ? stats[(int64_t)bc * NR + r0 + threadIdx.x] : float2{0.0f, 0.0f};
     };
     if (nt > 0) {
         load(ra, smem, smem + TILE);
@@ -1014,51 +1028,74 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, KvGrad<DH>::NWV / 4) void win
         for (int kb = 0; kb < KB; ++kb) gk[d][kb] = gv[d][kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     const float c2 = a.scale * kLog2e;
     half2_t wild = {(f16)0.0f, (f16)0.0f};
-    // the tiles with queries that do not see some key run a body of their own
-    auto scores = [&](int t, int r0, int h, const f16* sq, const f16* sg, half8 (&p)[KB], half8 (&ds)[KB], auto mask) {
-        constexpr bool MASK = decltype(mask)::value;
+    // 32 rows of a tile
+    auto step_of = [&](int t, int r0, int h, const f16* sq, const f16* sg, bool plain) {
+        using Rows = Ring<2 * KS, 3>;
+        using Cols = Ring<DT, 3>;
         const int tf = r0 / group, m0 = r0 - tf * group;
-#pragma unroll
-        for (int rb2 = 0; rb2 < 2; ++rb2) {
-            floatx4 s[KB], dp[KB];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) s[kb] = dp[kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const half8 qf = fr.row(sq, 32 * h + 16 * rb2, ks), gf = fr.row(sg, 32 * h + 16 * rb2, ks);
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    s[kb] = mfma16(qf, kf[kb][ks], s[kb]);
-                    dp[kb] = mfma16(gf, vf[kb][ks], dp[kb]);
-                }
-            }
-            float2 st4[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) st4[j] = sst[t & 1][32 * h + 16 * rb2 + 4 * g + j];
+        half8 qf[Rows::SLOTS], gf[Rows::SLOTS], qt[Cols::SLOTS], gt[Cols::SLOTS], p[KB], ds[KB];
+        floatx4 s[2][KB], dp[2][KB];
+        auto row = [&](auto i, auto slot) {
+            qf[slot] = fr.row(sq, 32 * h + 16 * (i / KS), i % KS);
+            gf[slot] = fr.row(sg, 32 * h + 16 * (i / KS), i % KS);
+        };
+        auto col = [&](auto i, auto slot) {
+            gt[slot] = fr.col(sg, 32 * h, i);
+            qt[slot] = fr.col(sq, 32 * h, i);
+        };
+        Rows::template start<2>(row);
+        Rows::template run<2 * KB, 2>(row, [&](auto i, auto slot) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
+                const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                s[i / KS][kb] = mfma16(qf[slot], kf[kb][i % KS], i % KS ? s[i / KS][kb] : zero);
+                dp[i / KS][kb] = mfma16(gf[slot], vf[kb][i % KS], i % KS ? dp[i / KS][kb] : zero);
+            }
+        });
+        if (!plain) {  // workgroup-uniform: hidden scores to -inf, hidden dP to D
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 32 * h + 16 * rb + 4 * g + j, pos = tf + by_group(m0 + r);
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) {
+                        const int key = k0 + (wave * KB + kb) * 16 + l16;
+                        const bool see = (r0 + r < rb_end) & (key <= pos) & ((key > pos - a.window) | (key < a.sinks));
+                        s[rb][kb][j] = see ? s[rb][kb][j] : -INFINITY;
+                        dp[rb][kb][j] = see ? dp[rb][kb][j] : 0.0f;
+                    }
+                }
+            for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sg, 32 * h, d), wild2(fr.col(sq, 32 * h, d), wild));
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            u32x4 pu, du;
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
                 float e[4], f[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][j], c2, -st4[j].x));
-                    f[j] = e[j] * (dp[kb][j] - st4[j].y);
-                    if constexpr (MASK) {
-                        const int r = 32 * h + 16 * rb2 + 4 * g + j, pos = tf + by_group(m0 + r);
-                        const int key = k0 + (wave * KB + kb) * 16 + l16;
-                        const bool see = (r0 + r < rb) & (key <= pos) & ((key > pos - a.window) | (key < a.sinks));
-                        e[j] = see ? e[j] : 0.0f;
-                        f[j] = see ? f[j] : 0.0f;
-                    }
+                    const float2 st4 = sst[t & 1][32 * h + 16 * rb + 4 * g + j];
+                    e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][kb][j], c2, -st4.x));
+                    f[j] = e[j] * (dp[rb][kb][j] - st4.y);
                 }
-                u32x4 pu = as_u32x4(p[kb]), du = as_u32x4(ds[kb]);
-                pu[2 * rb2] = pack_h2(e[0], e[1]);
-                pu[2 * rb2 + 1] = pack_h2(e[2], e[3]);
-                du[2 * rb2] = pack_h2(f[0], f[1]);
-                du[2 * rb2 + 1] = pack_h2(f[2], f[3]);
-                p[kb] = as_half8(pu);
-                ds[kb] = as_half8(du);
+                pu[2 * rb] = pack_h2(e[0], e[1]);
+                pu[2 * rb + 1] = pack_h2(e[2], e[3]);
+                du[2 * rb] = pack_h2(f[0], f[1]);
+                du[2 * rb + 1] = pack_h2(f[2], f[3]);
             }
+            p[kb] = as_half8(pu);
+            ds[kb] = as_half8(du);
         }
+        Cols::template start<4>(col);
+        Cols::template run<2 * KB, 4>(col, [&](auto i, auto slot) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                gv[i][kb] = mfma16(gt[slot], p[kb], gv[i][kb]);
+                gk[i][kb] = mfma16(qt[slot], ds[kb], gk[i][kb]);
+            }
+        });
     };
     for (int t = 0; t < nt; ++t) {
         if (threadIdx.x < QT) sst[t & 1][threadIdx.x] = st;
@@ -1075,25 +1112,10 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, KvGrad<DH>::NWV / 4) void win
         // every query of the tile sees every key of the block: the first query the last key, the last query the first
         // key outside the sinks
         const int tf = r0 / group, tl = (r0 + QT - 1) / group;
-        const bool plain = (r0 + QT <= rb) & (klast <= tf) & ((klast < a.sinks) | (max(k0, a.sinks) > tl - a.window));
+        const bool plain = (r0 + QT <= rb_end) & (klast <= tf) & ((klast < a.sinks) | (max(k0, a.sinks) > tl - a.window));
 #pragma unroll
         for (int h = 0; h < QT / 32; ++h) {
-            half8 p[KB], ds[KB];
-            if (plain) {
-                scores(t, r0, h, sq, sg, p, ds, std::false_type{});
-            } else {
-                scores(t, r0, h, sq, sg, p, ds, std::true_type{});
-                for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sq, 32 * h, d), wild2(fr.col(sg, 32 * h, d), wild));
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const half8 gt = fr.col(sg, 32 * h, d), qt = fr.col(sq, 32 * h, d);
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    gv[d][kb] = mfma16(gt, p[kb], gv[d][kb]);
-                    gk[d][kb] = mfma16(qt, ds[kb], gk[d][kb]);
-                }
-            }
+            step_of(t, r0, h, sq, sg, plain);
         }
     }
     bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
@@ -1248,7 +1270,7 @@ Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
     };
     // long parts, as few as fill the chip (and fewer than 2^24)
     int64_t q = full == blocks ? std::max<int64_t>(1, span / 4) : span;
-    while (q > 1 && items(q) * heads < 768) q /= 2;
+    while (q > 1 && items(q) * heads < 500) q /= 2;
     while (items(q) * heads > (1 << 24) && q < blocks) q *= 2;
     Parts p{};
     p.q = (int)q;
