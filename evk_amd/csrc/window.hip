@@ -983,19 +983,21 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
     uint32_t off[Dma::PER];
 #pragma unroll
     for (int i = 0; i < Dma::PER; ++i) off[i] = offset(i, 0);
-    auto load = [&](int r0, f16* sq, f16* sg) {
-        const int t0 = r0 / group, m0 = r0 - t0 * group, rows = min(QT, rb_end - r0);
+    // tile at flat row r0, row m0 of position t0
+    const uint32_t whole = (uint32_t)(by_group(QT - 1) * a.H + (QT - 1 - by_group(QT - 1) * group) + 1) * a.dh * 2;
+    auto load = [&](int r0, int t0, int m0, f16* sq, f16* sg) {
         const int64_t base = (qb0 + (int64_t)t0 * a.H) * a.dh;
-        // up to the end of the last row
-        const int tl = by_group(m0 + rows - 1);
+        if (m0 == 0 && r0 + QT <= rb_end) {
+            dma.go(wave_rsrc(a.q + base, whole), off, sq);
+            dma.go(wave_rsrc(a.dO + base, whole), off, sg);
+            return;
+        }
+        const int rows = min(QT, rb_end - r0), tl = by_group(m0 + rows - 1);  // up to the end of the last row
         const uint32_t span = (uint32_t)(tl * a.H + (m0 + rows - 1 - tl * group) + 1) * a.dh * 2;
         uint32_t o[Dma::PER];
+        // rows past the last one may lie before its end in memory (other heads' rows of the same position)
 #pragma unroll
-        for (int i = 0; i < Dma::PER; ++i) {
-            o[i] = m0 ? offset(i, m0) : off[i];
-            // rows past the last one may lie before its end in memory (other heads' rows of the same position)
-            if (rows < QT) o[i] = oob_or(dma.row(i) < rows, o[i]);
-        }
+        for (int i = 0; i < Dma::PER; ++i) o[i] = oob_or(dma.row(i) < rows, offset(i, m0));
         dma.go(wave_rsrc(a.q + base, span), o, sq);
         dma.go(wave_rsrc(a.dO + base, span), o, sg);
     };
@@ -1004,7 +1006,7 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
         if (threadIdx.x < QT) st = r0 + (int)threadIdx.x < rb_end ? stats[(int64_t)bc * NR + r0 + threadIdx.x] : float2{0.0f, 0.0f};
     };
     if (nt > 0) {
-        load(ra, smem, smem + TILE);
+        load(ra, ta, 0, smem, smem + TILE);
         load_stats(ra);
     }
     half8 kf[KB][KS], vf[KB][KS];
@@ -1029,10 +1031,9 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
     const float c2 = a.scale * kLog2e;
     half2_t wild = {(f16)0.0f, (f16)0.0f};
     // 32 rows of a tile
-    auto step_of = [&](int t, int r0, int h, const f16* sq, const f16* sg, bool plain) {
+    auto step_of = [&](int t, int r0, int tf, int m0, int h, const f16* sq, const f16* sg, bool plain) {
         using Rows = Ring<2 * KS, 3>;
         using Cols = Ring<DT, 3>;
-        const int tf = r0 / group, m0 = r0 - tf * group;
         half8 qf[Rows::SLOTS], gf[Rows::SLOTS], qt[Cols::SLOTS], gt[Cols::SLOTS], p[KB], ds[KB];
         floatx4 s[2][KB], dp[2][KB];
         auto row = [&](auto i, auto slot) {
@@ -1097,6 +1098,7 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
             }
         });
     };
+    int t0 = ta, m0 = 0;
     for (int t = 0; t < nt; ++t) {
         if (threadIdx.x < QT) sst[t & 1][threadIdx.x] = st;
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
@@ -1104,18 +1106,21 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
         f16* const sq = smem + (t & 1) * 2 * TILE;
         f16* const sg = sq + TILE;
         const int r0 = ra + t * QT;
+        const int gone = __builtin_amdgcn_readfirstlane(by_group(m0 + QT)), tf = t0, mf = m0;  // positions up to the next tile
+        t0 += gone;
+        m0 += QT - gone * group;
         if (t + 1 < nt) {
             f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
-            load(r0 + QT, nx, nx + TILE);
+            load(r0 + QT, t0, m0, nx, nx + TILE);
             load_stats(r0 + QT);
         }
-        // every query of the tile sees every key of the block: the first query the last key, the last query the first
-        // key outside the sinks
-        const int tf = r0 / group, tl = (r0 + QT - 1) / group;
+        // every query of the tile sees every key of the block: the first query the last key, the last query (before
+        // row m0 of position t0) the first key outside the sinks
+        const int tl = m0 ? t0 : t0 - 1;
         const bool plain = (r0 + QT <= rb_end) & (klast <= tf) & ((klast < a.sinks) | (max(k0, a.sinks) > tl - a.window));
 #pragma unroll
         for (int h = 0; h < QT / 32; ++h) {
-            step_of(t, r0, h, sq, sg, plain);
+            step_of(t, r0, tf, mf, h, sq, sg, plain);
         }
     }
     bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
