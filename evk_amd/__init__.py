@@ -117,8 +117,7 @@ SIGNATURES = {
                                                                         C.c_void_p]),
     "evkhip_window_attention_bwd_workspace": (C.c_uint64, [C.c_uint32] * 7),
     "evkhip_window_attention_bwd": (C.c_int, [TP] * 8 + [C.c_void_p] + [C.c_uint32] * 3 + [C.c_void_p, C.c_uint64, C.c_void_p]),
-    "evkhip_gated_linear_workspace": (C.c_uint64, [C.c_uint64, C.c_uint32, C.c_uint32]),
-    "evkhip_gated_linear": (C.c_int, [TP] * 4 + [C.c_int, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "evkhip_gated_linear": (C.c_int, [TP] * 4 + [C.c_int, C.c_void_p]),
     "evkhip_gated_linear_backward_workspace": (C.c_uint64, [C.c_uint64, C.c_uint32, C.c_uint32]),
     "evkhip_gated_linear_backward": (C.c_int, [TP] * 6 + [C.c_int, C.c_int, C.c_void_p, C.c_uint64, C.c_void_p]),
     "evkhip_model_weight_elems": (C.c_uint64, [C.POINTER(ModelCfg)]),
@@ -449,87 +448,116 @@ def greedy_sample(logits, out_tokens, position, token_base, token_count, stream=
 # from torch's allocator, in the order of the current stream, and so needs
 # `stream` to be that stream.
 
-def _H(t, ref) -> Optional[bytes]:
-    """Descriptor of an fp16 tensor on ref's device (None: an argument left out)."""
+_F16 = None
+
+
+def _first(t) -> int:
+    """Device of a call's first tensor, which has to be fp16 on the current one."""
+    global _torch, _F16
+    if _F16 is None:
+        import torch
+        _torch, _F16 = torch, torch.float16
+    if t.dtype is not _F16:
+        raise ValueError(f"evk_amd ops take float16 tensors, got {t.dtype}")
+    dev = t.get_device()
+    if dev < 0 or dev != _torch.cuda.current_device():
+        raise ValueError(f"tensors on {t.device}: not the current GPU")
+    return dev
+
+
+def _H(t, dev) -> Optional[bytes]:
+    """Descriptor of an fp16 tensor on device `dev` (None: an argument left out)."""
     if t is None:
         return None
-    if t.dtype is not ref.dtype or t.device != ref.device:
-        raise ValueError(f"expected {ref.dtype} on {ref.device}, got {t.dtype} on {t.device}")
+    if t.dtype is not _F16 or t.get_device() != dev:
+        raise ValueError(f"expected float16 on cuda:{dev}, got {t.dtype} on {t.device}")
     return _D(t)
 
 
-def _ref(t):
-    """The tensor that a call's others are held against: fp16 on the current device."""
-    global _torch
-    if _torch is None:
-        import torch
-        _torch = torch
-    if t.dtype is not _torch.float16:
-        raise ValueError(f"evk_amd ops take float16 tensors, got {t.dtype}")
-    if not t.is_cuda or t.get_device() != _torch.cuda.current_device():
-        raise ValueError(f"tensors on {t.device}: not the current GPU")
-    return t
-
-
-def _P(t, ref, dtype, count) -> Optional[int]:
+def _P(t, dev, dtype, count) -> Optional[int]:
     """Address of a contiguous tensor of `count` values of another type (None: left out)."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.device != ref.device or not t.is_contiguous() or t.numel() != count:
-        raise ValueError(f"expected {count} contiguous {dtype} values on {ref.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or t.numel() != count:
+        raise ValueError(f"expected {count} contiguous {dtype} values on cuda:{dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-def _workspace(workspace, need, ref, stream):
+_NEEDS = {}  # bytes of workspace by entry point and sizes
+
+
+def _need(name, *sizes) -> int:
+    key = (name, *sizes)
+    n = _NEEDS.get(key)
+    if n is None:
+        if len(_NEEDS) > 4096:
+            _NEEDS.clear()
+        n = _NEEDS[key] = int(getattr(lib(), name)(*sizes))
+    return n
+
+
+def _workspace(workspace, need, dev, stream):
     """(tensor, address, bytes) of a call's workspace; the tensor is kept until the call has been made."""
     if workspace is None:
         if need == 0:
             return None, None, 0
         if stream is not None and int(stream) != _stream():
             raise ValueError(f"a call on another stream than the current one needs a workspace of {need} bytes")
-        workspace = _torch.empty(need, dtype=_torch.uint8, device=ref.device)
-    elif not workspace.is_contiguous() or workspace.device != ref.device:
+        workspace = _torch.empty(need, dtype=_torch.uint8, device=dev)
+    elif not workspace.is_contiguous() or workspace.get_device() != dev:
         raise ValueError("the workspace is a contiguous tensor on the operands' device")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _shape3(t, name):
-    if t.dim() != 3:
-        raise ValueError(f"{name} has 3 dimensions, got {tuple(t.shape)}")
-    return t.shape
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name} has 3 dimensions, got {tuple(shape)}")
+    return shape
+
+
+def _at_least(least, **values):
+    for name, v in values.items():
+        if v < least:
+            raise ValueError(f"{name} is {v}, at least {least} is needed")
 
 
 def qkv_norm_rope(qkv, q, k, v, head_dim, q_weight=None, k_weight=None, eps=1e-4, rotary_base=10000.0, position_offset=0,
                   offsets=None, stream=None):
     """Norm and rotation of each query and key head of qkv (B, N, (H + 2 KV) head_dim) into q (B, N, H head_dim) and the
     rows position_offset + t (or offsets[b] + t, int32) of k and v (B, rows, KV head_dim)."""
-    r = _ref(qkv)
-    _check(_calls.evkhip_qkv_norm_rope(_D(r), _H(q_weight, r), _H(k_weight, r), _H(q, r), _H(k, r), _H(v, r), int(head_dim),
-                                       float(eps), float(rotary_base), int(position_offset),
-                                       None if offsets is None else _P(offsets, r, _torch.int32, r.shape[0]), _stream(stream)))
+    dev = _first(qkv)
+    if head_dim < 1 or position_offset < 0:
+        _at_least(1, head_dim=head_dim)
+        _at_least(0, position_offset=position_offset)
+    _check(_calls.evkhip_qkv_norm_rope(_D(qkv), _H(q_weight, dev), _H(k_weight, dev), _H(q, dev), _H(k, dev), _H(v, dev),
+                                       head_dim, eps, rotary_base, position_offset,
+                                       None if offsets is None else _P(offsets, dev, _torch.int32, qkv.shape[0]),
+                                       _stream(stream)))
     return q, k, v
 
 
 def qkv_norm_rope_backward(qkv, dq, dk, dv, dqkv, head_dim, q_weight=None, k_weight=None, dq_weight=None, dk_weight=None,
                            eps=1e-4, rotary_base=10000.0, position_offset=0, accumulate=False, workspace=None, stream=None):
     """Gradient of qkv_norm_rope: dqkv is written, dq_weight and dk_weight are written or, with accumulate, added to."""
-    r = _ref(qkv)
+    dev = _first(qkv)
+    _at_least(1, head_dim=head_dim)
+    _at_least(0, position_offset=position_offset)
     need = 0
     if dq_weight is not None or dk_weight is not None:
         b, n, _ = _shape3(qkv, "qkv")
-        need = lib().evkhip_qkv_norm_rope_backward_workspace(b * n, int(head_dim))
-    ws, wp, wn = _workspace(workspace, need, r, stream)
-    _check(_calls.evkhip_qkv_norm_rope_backward(_D(r), _H(q_weight, r), _H(k_weight, r), _H(dq, r), _H(dk, r), _H(dv, r),
-                                                _H(dqkv, r), _H(dq_weight, r), _H(dk_weight, r), int(head_dim), float(eps),
-                                                float(rotary_base), int(position_offset), int(accumulate), wp, wn,
-                                                _stream(stream)))
+        need = _need("evkhip_qkv_norm_rope_backward_workspace", b * n, head_dim)
+    ws, wp, wn = _workspace(workspace, need, dev, stream)
+    _check(_calls.evkhip_qkv_norm_rope_backward(_D(qkv), _H(q_weight, dev), _H(k_weight, dev), _H(dq, dev), _H(dk, dev),
+                                                _H(dv, dev), _H(dqkv, dev), _H(dq_weight, dev), _H(dk_weight, dev), head_dim,
+                                                eps, rotary_base, position_offset, int(accumulate), wp, wn, _stream(stream)))
     return dqkv
 
 
 def window_attention_workspace(q, k, head_dim, window=0, sinks=0) -> int:
     """Bytes of workspace of window_attention for these q and k."""
     (b, n, d), (_, rows, dk) = _shape3(q, "q"), _shape3(k, "k")
-    return lib().evkhip_window_attention_workspace(b, n, rows, d // head_dim, dk // head_dim, head_dim, window, sinks)
+    return _need("evkhip_window_attention_workspace", b, n, rows, d // head_dim, dk // head_dim, head_dim, window, sinks)
 
 
 def window_attention(q, k, v, o, head_dim, window=0, sinks=0, position_offset=0, offsets=None, lse=None, workspace=None,
@@ -537,30 +565,29 @@ def window_attention(q, k, v, o, head_dim, window=0, sinks=0, position_offset=0,
     """Causal attention of q (B, N, H head_dim) over the rows of k, v (B, rows, KV head_dim) that are among the last
     `window` (0: all) up to the query's position position_offset + t (or offsets[b] + t, int32), or among the first
     `sinks`.  lse: optional (B, H, N) fp32."""
-    r = _ref(q)
-    head_dim, window, sinks = int(head_dim), int(window), int(sinks)
-    if head_dim <= 0 or window < 0 or sinks < 0 or position_offset < 0:
-        raise ValueError("head_dim is positive; window, sinks and position_offset are not negative")
-    ws, wp, wn = _workspace(workspace, window_attention_workspace(q, k, head_dim, window, sinks), r, stream)
-    n = r.shape[0] * r.shape[1] * (r.shape[2] // head_dim)
-    _check(_calls.evkhip_window_attention(_D(r), _H(k, r), _H(v, r), _H(o, r), head_dim, window, sinks, int(position_offset),
-                                          None if offsets is None else _P(offsets, r, _torch.int32, r.shape[0]),
-                                          None if lse is None else _P(lse, r, _torch.float32, n), wp, wn, _stream(stream)))
+    dev = _first(q)
+    if head_dim < 1 or window < 0 or sinks < 0 or position_offset < 0:
+        _at_least(1, head_dim=head_dim)
+        _at_least(0, window=window, sinks=sinks, position_offset=position_offset)
+    ws, wp, wn = _workspace(workspace, window_attention_workspace(q, k, head_dim, window, sinks), dev, stream)
+    _check(_calls.evkhip_window_attention(_D(q), _H(k, dev), _H(v, dev), _H(o, dev), head_dim, window, sinks, position_offset,
+                                          None if offsets is None else _P(offsets, dev, _torch.int32, q.shape[0]),
+                                          None if lse is None else _P(lse, dev, _torch.float32, q.numel() // head_dim), wp, wn,
+                                          _stream(stream)))
     return o
 
 
 def window_attention_bwd(q, k, v, o, dO, dQ, dK, dV, lse, head_dim, window=0, sinks=0, workspace=None, stream=None):
     """Gradient of window_attention over a whole sequence (as many rows as queries) from its o and lse."""
-    r = _ref(q)
-    head_dim, window, sinks = int(head_dim), int(window), int(sinks)
-    if head_dim <= 0 or window < 0 or sinks < 0:
-        raise ValueError("head_dim is positive; window and sinks are not negative")
+    dev = _first(q)
+    _at_least(1, head_dim=head_dim)
+    _at_least(0, window=window, sinks=sinks)
     (b, n, d), (_, _, dk) = _shape3(q, "q"), _shape3(k, "k")
-    need = lib().evkhip_window_attention_bwd_workspace(b, n, d // head_dim, dk // head_dim, head_dim, window, sinks)
-    ws, wp, wn = _workspace(workspace, need, r, stream)
-    _check(_calls.evkhip_window_attention_bwd(_D(r), _H(k, r), _H(v, r), _H(o, r), _H(dO, r), _H(dQ, r), _H(dK, r), _H(dV, r),
-                                              _P(lse, r, _torch.float32, b * n * (d // head_dim)), head_dim, window, sinks,
-                                              wp, wn, _stream(stream)))
+    need = _need("evkhip_window_attention_bwd_workspace", b, n, d // head_dim, dk // head_dim, head_dim, window, sinks)
+    ws, wp, wn = _workspace(workspace, need, dev, stream)
+    _check(_calls.evkhip_window_attention_bwd(_D(q), _H(k, dev), _H(v, dev), _H(o, dev), _H(dO, dev), _H(dQ, dev), _H(dK, dev),
+                                              _H(dV, dev), _P(lse, dev, _torch.float32, q.numel() // head_dim), head_dim, window,
+                                              sinks, wp, wn, _stream(stream)))
     return dQ, dK, dV
 
 
@@ -573,26 +600,22 @@ def _activation(name) -> int:
     return ACTIVATIONS[name]
 
 
-def gated_linear(x, w, h, gate_up=None, activation="silu", workspace=None, stream=None):
+def gated_linear(x, w, h, gate_up=None, activation="silu", stream=None):
     """h (..., F) = act(x w[0]) * (x w[1]), x (..., D), w (2, D, F).  gate_up (2, ..., F), where given, receives both
     products for the backward pass."""
-    r = _ref(x)
-    d, f = _shape3(w, "w")[1:]
-    need = lib().evkhip_gated_linear_workspace(x.numel() // d if d else 0, d, f)
-    ws, wp, wn = _workspace(workspace, need, r, stream)
-    _check(_calls.evkhip_gated_linear(_D(r), _H(w, r), _H(h, r), _H(gate_up, r), _activation(activation), wp, wn,
-                                      _stream(stream)))
+    dev = _first(x)
+    _check(_calls.evkhip_gated_linear(_D(x), _H(w, dev), _H(h, dev), _H(gate_up, dev), _activation(activation), _stream(stream)))
     return h
 
 
 def gated_linear_backward(x, w, gate_up, dh, dx=None, dw=None, activation="silu", accumulate=False, workspace=None,
                           stream=None):
     """Gradient of gated_linear: dx is written, dw written or, with accumulate, added to (either may be left out)."""
-    r = _ref(x)
+    dev = _first(x)
     d, f = _shape3(w, "w")[1:]
-    need = lib().evkhip_gated_linear_backward_workspace(x.numel() // d if d else 0, d, f)
-    ws, wp, wn = _workspace(workspace, need, r, stream)
-    _check(_calls.evkhip_gated_linear_backward(_D(r), _H(w, r), _H(gate_up, r), _H(dh, r), _H(dx, r), _H(dw, r),
+    need = _need("evkhip_gated_linear_backward_workspace", x.numel() // d if d else 0, d, f)
+    ws, wp, wn = _workspace(workspace, need, dev, stream)
+    _check(_calls.evkhip_gated_linear_backward(_D(x), _H(w, dev), _H(gate_up, dev), _H(dh, dev), _H(dx, dev), _H(dw, dev),
                                                _activation(activation), int(accumulate), wp, wn, _stream(stream)))
     return dx, dw
 

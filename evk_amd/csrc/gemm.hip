@@ -190,6 +190,12 @@ DEV void wait_vmcnt(int n) {
 // of B, joined in the epilogue (C = act(A B0) * A B1); a tile holds BN / 2
 // columns of each.  GEMM_PAIR: the sum of two products, A0 B0 + A1 B1 (each
 // second operand behind the first one), whose K tiles follow each other.
+DEV float glu_of(float a, float b, int act) {
+    if (act == EVKHIP_ACT_SILU) return silu_f(a) * b;
+    if (act == EVKHIP_ACT_GELU) return gelu_fast(a) * b;
+    return (a < 0.0f ? 0.0f : a) * b;
+}
+
 template <int BM, int BN, bool TA, bool TB, int NWV, int KG, int NST, bool RAG, int KIND = GEMM_ONE>
 __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int tiles_m, int tiles_n) {
     constexpr bool GLU = KIND == GEMM_GLU, PAIR = KIND == GEMM_PAIR;
@@ -467,9 +473,7 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
             write_out(p.gate_up + (int64_t)M * N);
             wave_lds();
         }
-        if (p.act == EVKHIP_ACT_SILU) stage2([](float a, float b) { return silu_f(a) * b; });
-        else if (p.act == EVKHIP_ACT_GELU) stage2([](float a, float b) { return gelu_fast(a) * b; });
-        else stage2([](float a, float b) { return (a < 0.0f ? 0.0f : a) * b; });
+        stage2([&](float a, float b) { return glu_of(a, b, p.act); });
         write_out(Cp);
         return;
     }
@@ -819,6 +823,109 @@ __global__ __launch_bounds__(256) void gemv_mf(GemmArgs p, float* __restrict__ p
     gemv_finish_m16(p, part, cnt, c0);
 }
 
+// ---- gated linear unit of few rows: C (M, N) = act(A B0) * (A B1), M <= 16 MB ----
+// Bandwidth-bound on both matrices, each read once.  A workgroup owns NC
+// columns of both; its NW waves take every NW-th step of 32 K rows, each through
+// a ring of LG_ST stages in LDS that only it uses (32 rows of NC columns of the
+// gate's matrix and NC of the other one, and the rows of A), filled by LDS-direct
+// loads LG_ST - 1 steps ahead, without a barrier; the waves' sums meet in LDS, in
+// the order of the waves.  16 x 4096 x 11008: 39.6 us = 4.6 TB/s (56 on the tiles
+// for many rows); 64 rows 50.9 (67.7).
+template <int NC, int MB, int NW, int LG_ST>
+__global__ __launch_bounds__(64 * NW) void glu_skinny(GemmArgs p) {
+    constexpr int W = 2 * NC, CPR = W / 8, RPI = 64 / CPR;                  // halves and chunks of a row, rows of a load
+    constexpr int B_EL = 32 * W, A_EL = 16 * 32, STAGE = B_EL + MB * A_EL;  // halves
+    constexpr int LPS = 32 / RPI + MB, NB = W / 16;                         // loads a step, column blocks
+    constexpr int RING = LG_ST * STAGE * 2 > MB * 16 * W * 4 ? LG_ST * STAGE : MB * 16 * W * 2;  // or the wave's sums
+    __shared__ __attribute__((aligned(1024))) f16 smem[NW * RING];
+    const int M = p.M, N = p.N, K = p.K;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4, trow = l16 >> 2, tcol = (l16 & 3) * 4;
+    const int n0 = xcd_tile(blockIdx.x, gridDim.x) * NC;
+    f16* const ring = smem + wave * RING;
+    const __amdgpu_buffer_rsrc_t ares = buf_rsrc(p.A, (uint32_t)((int64_t)M * K * 2));
+    const __amdgpu_buffer_rsrc_t bres = buf_rsrc(p.B, (uint32_t)((int64_t)K * N * 4));
+    // slots: chunk c of a B row r at c ^ bswz(r) (transposed reads of rows 0 .. 3 and 8 .. 11 together), of an A row at
+    // c ^ aswz(r) (16-byte reads of 16 rows)
+    auto bswz = [](int r) { return 2 * (W == 64 ? (r >> 1 & 1) | (r >> 2 & 2) : (r & 3) | (r >> 1 & 4)); };
+    auto aswz = [](int r) { return 2 * (r >> 2 & 1); };
+    auto load = [&](int step) {  // past the end: zeros, without touching memory
+        f16* const st = ring + step / NW % LG_ST * STAGE;
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+            const int r = RPI * i + lane / CPR, ch = (lane % CPR) ^ bswz(r), k = step * 32 + r, col = n0 + ch % (NC / 8) * 8;
+            dma16(bres, oob_or(k < K && col < N, (uint32_t)((((int64_t)(ch / (NC / 8)) * K + k) * N + col) * 2)), lds_addr(st + i * 512));
+        }
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+            const int r = lane / 4, ch = (lane % 4) ^ aswz(r), k = step * 32 + ch * 8, m = 16 * mb + r;
+            dma16(ares, oob_or(k < K && m < M, (uint32_t)(((int64_t)m * K + k) * 2)), lds_addr(st + B_EL + mb * A_EL));
+        }
+    };
+    floatx4 acc[MB][NB];  // the gate's column blocks, the other matrix's
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[mb][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int steps = (K + 31) / 32;
+#pragma unroll
+    for (int i = 0; i < LG_ST - 1; ++i) load(wave + i * NW);
+    constexpr int LEFT = (LG_ST - 2) * LPS;  // loads of younger steps once step `step` is there
+    static_assert(LEFT < 64, "vmcnt");
+    for (int step = wave; step < steps; step += NW) {
+        __builtin_amdgcn_s_waitcnt((LEFT & 15) | (LEFT >> 4 << 14) | 0x0f70);  // vmcnt(LEFT)
+        const f16* st = ring + step / NW % LG_ST * STAGE;
+        half8 bf[NB], af[MB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            auto at = [&](int r) {
+                const int c = 2 * j + (tcol >> 3);
+                return st + r * W + ((c ^ bswz(r)) << 3 | (tcol & 7));
+            };
+            bf[j] = cat4(lds_read_tr(at(8 * g + trow)), lds_read_tr(at(8 * g + trow + 4)));
+        }
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+            af[mb] = *reinterpret_cast<const half8*>(st + B_EL + mb * A_EL + l16 * 32 + ((g ^ aswz(l16)) << 3));
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the fragments are read before a later step's rows arrive
+        load(step + (LG_ST - 1) * NW);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[mb][j] = mfma16(af[mb], bf[j], acc[mb][j]);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): nothing arrives in the ring any more
+    // D: column 16 j + l16 of the W, row 4 g + e
+    float* const sums = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[(16 * mb + 4 * g + e) * W + 16 * j + l16] = acc[mb][j][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MB * 16 * (NC / 4); i += 64 * NW) {
+        const int m = i / (NC / 4), c = i % (NC / 4) * 4, col = n0 + c;
+        if (m >= M || col >= N) continue;  // N % 8 == 0: the four columns are whole
+        floatx4 ga = {0.0f, 0.0f, 0.0f, 0.0f}, up = ga;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float* q = reinterpret_cast<const float*>(smem + w * RING) + m * W + c;
+            ga += *reinterpret_cast<const floatx4*>(q);
+            up += *reinterpret_cast<const floatx4*>(q + NC);
+        }
+        float h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = glu_of(ga[e], up[e], p.act);
+        const int64_t at = (int64_t)m * N + col;
+        *reinterpret_cast<uint2*>(p.C + at) = uint2{pack_h2(h[0], h[1]), pack_h2(h[2], h[3])};
+        if (p.gate_up) {
+            *reinterpret_cast<uint2*>(p.gate_up + at) = uint2{pack_h2(ga[0], ga[1]), pack_h2(ga[2], ga[3])};
+            *reinterpret_cast<uint2*>(p.gate_up + (int64_t)M * N + at) = uint2{pack_h2(up[0], up[1]), pack_h2(up[2], up[3])};
+        }
+    }
+}
+
 // ---- short K, any alignment: one thread per element of C.  Launch-bound up
 // to a few thousand elements; a chain of K loads of each operand otherwise ----
 __global__ __launch_bounds__(256) void gemm_short(GemmArgs p, int ta, int tb) {
@@ -1076,7 +1183,29 @@ int noalloc_scratch(GemvScratch* out) {
 int glu_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st) {
     const bool direct = vec_ok && (int64_t)a.M * a.K * 2 < INT32_MAX && (int64_t)a.K * a.N * 4 < INT32_MAX &&
                         (int64_t)a.M * a.N < INT32_MAX;
-    const hipError_t e = launch_kind_plan<GEMM_GLU>(a, direct, st);
+    hipError_t e;
+    if (direct && a.M <= 64) {
+        auto go = [&](auto nc, auto mb, auto nw, auto st_) {
+            constexpr int NC = decltype(nc)::value, MB = decltype(mb)::value, NW = decltype(nw)::value, ST = decltype(st_)::value;
+            hipLaunchKernelGGL((glu_skinny<NC, MB, NW, ST>), dim3((unsigned)((a.N + NC - 1) / NC)), dim3(64 * NW), 0, st, a);
+        };
+        using I1 = std::integral_constant<int, 1>;
+        using I2 = std::integral_constant<int, 2>;
+        using I3 = std::integral_constant<int, 3>;
+        using I4 = std::integral_constant<int, 4>;
+        using I8 = std::integral_constant<int, 8>;
+        using C32 = std::integral_constant<int, 32>;
+        using C64 = std::integral_constant<int, 64>;
+        // 32 columns of each matrix while every workgroup has a CU of its own, else 64, whose rows are whole 128-byte
+        // lines (16 x 4096, us with 32 and 64: 5632 columns 31.2, 35.3; 8192 39.0, 40.6; 11008 55.0, 39.6)
+        const bool narrow = (a.N + 31) / 32 <= device_cu_count();
+        if (a.M <= 16) narrow ? go(C32{}, I1{}, I8{}, I4{}) : go(C64{}, I1{}, I4{}, I4{});
+        else if (a.M <= 32) narrow ? go(C32{}, I2{}, I8{}, I3{}) : go(C64{}, I2{}, I4{}, I3{});
+        else narrow ? go(C32{}, I4{}, I8{}, I2{}) : go(C64{}, I4{}, I4{}, I3{});
+        e = hipGetLastError();
+    } else {
+        e = launch_kind_plan<GEMM_GLU>(a, direct, st);
+    }
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "gated_linear launch");
 }
 

@@ -370,10 +370,8 @@ int evkhip_window_attention_bwd(const evkhip_tensor* q, const evkhip_tensor* k, 
 #define EVKHIP_ACT_SILU 0
 #define EVKHIP_ACT_GELU 1 /* the tanh form of evkhip_gelu */
 #define EVKHIP_ACT_RELU 2
-uint64_t evkhip_gated_linear_workspace(uint64_t tokens, uint32_t d, uint32_t f);
 int evkhip_gated_linear(const evkhip_tensor* x, const evkhip_tensor* w, const evkhip_tensor* h,
-                        const evkhip_tensor* gate_up, int activation, void* workspace, uint64_t workspace_bytes,
-                        void* stream);
+                        const evkhip_tensor* gate_up, int activation, void* stream);
 
 /* Its gradient from the forward's gate_up: dx (as x) is written; dw (as w) is
  * written, or added to with accumulate.  Either may be NULL (not wanted).  The
