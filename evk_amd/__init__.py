@@ -460,9 +460,14 @@ def _first(t) -> int:
     if t.dtype is not _F16:
         raise ValueError(f"evk_amd ops take float16 tensors, got {t.dtype}")
     dev = t.get_device()
-    if dev < 0 or dev != _torch.cuda.current_device():
+    if dev < 0 or dev != _torch._C._cuda_getDevice():
         raise ValueError(f"tensors on {t.device}: not the current GPU")
     return dev
+
+
+def _on(stream, dev) -> int:
+    """A call's stream: the one given, or the current one (the device is in use, so torch has its streams)."""
+    return _torch._C._cuda_getCurrentRawStream(dev) if stream is None else int(stream)
 
 
 def _H(t, dev) -> Optional[bytes]:
@@ -471,7 +476,13 @@ def _H(t, dev) -> Optional[bytes]:
         return None
     if t.dtype is not _F16 or t.get_device() != dev:
         raise ValueError(f"expected float16 on cuda:{dev}, got {t.dtype} on {t.device}")
-    return _D(t)
+    shape = t.shape
+    if t.is_contiguous():
+        try:
+            return _PACK[len(shape)](t.data_ptr(), len(shape), *shape)
+        except (struct.error, IndexError):
+            pass
+    return _D(t)  # refuses it
 
 
 def _P(t, dev, dtype, count) -> Optional[int]:
@@ -530,10 +541,10 @@ def qkv_norm_rope(qkv, q, k, v, head_dim, q_weight=None, k_weight=None, eps=1e-4
     if head_dim < 1 or position_offset < 0:
         _at_least(1, head_dim=head_dim)
         _at_least(0, position_offset=position_offset)
-    _check(_calls.evkhip_qkv_norm_rope(_D(qkv), _H(q_weight, dev), _H(k_weight, dev), _H(q, dev), _H(k, dev), _H(v, dev),
+    _check(_calls.evkhip_qkv_norm_rope(_H(qkv, dev), _H(q_weight, dev), _H(k_weight, dev), _H(q, dev), _H(k, dev), _H(v, dev),
                                        head_dim, eps, rotary_base, position_offset,
                                        None if offsets is None else _P(offsets, dev, _torch.int32, qkv.shape[0]),
-                                       _stream(stream)))
+                                       _on(stream, dev)))
     return q, k, v
 
 
@@ -548,9 +559,9 @@ def qkv_norm_rope_backward(qkv, dq, dk, dv, dqkv, head_dim, q_weight=None, k_wei
         b, n, _ = _shape3(qkv, "qkv")
         need = _need("evkhip_qkv_norm_rope_backward_workspace", b * n, head_dim)
     ws, wp, wn = _workspace(workspace, need, dev, stream)
-    _check(_calls.evkhip_qkv_norm_rope_backward(_D(qkv), _H(q_weight, dev), _H(k_weight, dev), _H(dq, dev), _H(dk, dev),
+    _check(_calls.evkhip_qkv_norm_rope_backward(_H(qkv, dev), _H(q_weight, dev), _H(k_weight, dev), _H(dq, dev), _H(dk, dev),
                                                 _H(dv, dev), _H(dqkv, dev), _H(dq_weight, dev), _H(dk_weight, dev), head_dim,
-                                                eps, rotary_base, position_offset, int(accumulate), wp, wn, _stream(stream)))
+                                                eps, rotary_base, position_offset, int(accumulate), wp, wn, _on(stream, dev)))
     return dqkv
 
 
@@ -570,10 +581,10 @@ def window_attention(q, k, v, o, head_dim, window=0, sinks=0, position_offset=0,
         _at_least(1, head_dim=head_dim)
         _at_least(0, window=window, sinks=sinks, position_offset=position_offset)
     ws, wp, wn = _workspace(workspace, window_attention_workspace(q, k, head_dim, window, sinks), dev, stream)
-    _check(_calls.evkhip_window_attention(_D(q), _H(k, dev), _H(v, dev), _H(o, dev), head_dim, window, sinks, position_offset,
+    _check(_calls.evkhip_window_attention(_H(q, dev), _H(k, dev), _H(v, dev), _H(o, dev), head_dim, window, sinks, position_offset,
                                           None if offsets is None else _P(offsets, dev, _torch.int32, q.shape[0]),
                                           None if lse is None else _P(lse, dev, _torch.float32, q.numel() // head_dim), wp, wn,
-                                          _stream(stream)))
+                                          _on(stream, dev)))
     return o
 
 
@@ -585,9 +596,9 @@ def window_attention_bwd(q, k, v, o, dO, dQ, dK, dV, lse, head_dim, window=0, si
     (b, n, d), (_, _, dk) = _shape3(q, "q"), _shape3(k, "k")
     need = _need("evkhip_window_attention_bwd_workspace", b, n, d // head_dim, dk // head_dim, head_dim, window, sinks)
     ws, wp, wn = _workspace(workspace, need, dev, stream)
-    _check(_calls.evkhip_window_attention_bwd(_D(q), _H(k, dev), _H(v, dev), _H(o, dev), _H(dO, dev), _H(dQ, dev), _H(dK, dev),
+    _check(_calls.evkhip_window_attention_bwd(_H(q, dev), _H(k, dev), _H(v, dev), _H(o, dev), _H(dO, dev), _H(dQ, dev), _H(dK, dev),
                                               _H(dV, dev), _P(lse, dev, _torch.float32, q.numel() // head_dim), head_dim, window,
-                                              sinks, wp, wn, _stream(stream)))
+                                              sinks, wp, wn, _on(stream, dev)))
     return dQ, dK, dV
 
 
@@ -604,7 +615,7 @@ def gated_linear(x, w, h, gate_up=None, activation="silu", stream=None):
     """h (..., F) = act(x w[0]) * (x w[1]), x (..., D), w (2, D, F).  gate_up (2, ..., F), where given, receives both
     products for the backward pass."""
     dev = _first(x)
-    _check(_calls.evkhip_gated_linear(_D(x), _H(w, dev), _H(h, dev), _H(gate_up, dev), _activation(activation), _stream(stream)))
+    _check(_calls.evkhip_gated_linear(_H(x, dev), _H(w, dev), _H(h, dev), _H(gate_up, dev), _activation(activation), _on(stream, dev)))
     return h
 
 
@@ -615,8 +626,8 @@ def gated_linear_backward(x, w, gate_up, dh, dx=None, dw=None, activation="silu"
     d, f = _shape3(w, "w")[1:]
     need = _need("evkhip_gated_linear_backward_workspace", x.numel() // d if d else 0, d, f)
     ws, wp, wn = _workspace(workspace, need, dev, stream)
-    _check(_calls.evkhip_gated_linear_backward(_D(x), _H(w, dev), _H(gate_up, dev), _H(dh, dev), _H(dx, dev), _H(dw, dev),
-                                               _activation(activation), int(accumulate), wp, wn, _stream(stream)))
+    _check(_calls.evkhip_gated_linear_backward(_H(x, dev), _H(w, dev), _H(gate_up, dev), _H(dh, dev), _H(dx, dev), _H(dw, dev),
+                                               _activation(activation), int(accumulate), wp, wn, _on(stream, dev)))
     return dx, dw
 
 

@@ -1,0 +1,301 @@
+"""GPU: the grouped-query block's operators as programs use them: a block's
+training step and its decoding against 64 bits, streams, captured graphs, calls
+at the same time, caches past 2 GiB."""
+import math
+
+import pytest
+import torch
+
+import evk_amd as evk
+from test_gpu_block import F16, F64, H, Rng, close, empty, seen, window_want
+
+pytestmark = pytest.mark.gpu
+
+
+class Block:
+    """One grouped-query block on evk_amd's operators: weights, and the activations of a forward pass."""
+
+    def __init__(self, dev, r, d, heads, kv, dh, f, window, sinks, act):
+        self.dev, self.d, self.heads, self.kv, self.dh, self.f = dev, d, heads, kv, dh, f
+        self.window, self.sinks, self.act = window, sinks, act
+        wide = (heads + 2 * kv) * dh
+        self.w = dict(qkv=r(d, wide, std=d ** -0.5), q=r(dh, mean=1.0, std=0.1), k=r(dh, mean=1.0, std=0.1),
+                      o=r(heads * dh, d, std=(heads * dh) ** -0.5), gu=r(2, d, f, std=d ** -0.5), down=r(f, d, std=f ** -0.5))
+
+    def forward(self, x, kc=None, vc=None, p0=0, offsets=None):
+        """x (B, N, d) -> (B, N, d); rows into the caches kc, vc (B, rows, kv dh), or into tensors of their own."""
+        b, n, d = x.shape
+        w, e = self.w, lambda *s: torch.empty(*s, dtype=F16, device=self.dev)  # noqa: E731
+        a = dict(x=x, xn=e(b, n, d), qkv=e(b, n, w["qkv"].shape[1]), q=e(b, n, self.heads * self.dh), att=e(b, n, self.heads * self.dh),
+                 lse=torch.empty(b, self.heads, n, device=self.dev), y=e(b, n, d), x1=e(b, n, d), x1n=e(b, n, d), gu=e(2, b, n, self.f),
+                 h=e(b, n, self.f), z=e(b, n, d), out=e(b, n, d))
+        a["k"], a["v"] = (e(b, n, self.kv * self.dh), e(b, n, self.kv * self.dh)) if kc is None else (kc, vc)
+        evk.rms_norm(x, a["xn"])
+        evk.matmul(a["xn"], w["qkv"], a["qkv"])
+        evk.qkv_norm_rope(a["qkv"], a["q"], a["k"], a["v"], self.dh, w["q"], w["k"], 1e-4, 10000.0, p0, offsets)
+        evk.window_attention(a["q"], a["k"], a["v"], a["att"], self.dh, self.window, self.sinks, p0, offsets, a["lse"])
+        evk.matmul(a["att"], w["o"], a["y"])
+        evk.add(x, a["y"], a["x1"])
+        evk.rms_norm(a["x1"], a["x1n"])
+        evk.gated_linear(a["x1n"], w["gu"], a["h"], a["gu"], self.act)
+        evk.matmul(a["h"], w["down"], a["z"])
+        evk.add(a["x1"], a["z"], a["out"])
+        return a
+
+    def backward(self, a, dout):
+        """Gradients of x and of every weight."""
+        w, like = self.w, torch.empty_like
+        b, n, d = dout.shape
+        flat = lambda t: t.view(b * n, -1)  # noqa: E731
+        g = {k: like(v) for k, v in w.items()}
+        dh, dx1n, datt, dxn, dqkv = like(a["h"]), like(a["x1n"]), like(a["att"]), like(a["xn"]), like(a["qkv"])
+        dq, dk, dv = like(a["q"]), like(a["k"]), like(a["v"])
+        evk.matmul(flat(a["h"]), flat(dout), g["down"], transpose_a=True)
+        evk.matmul(flat(dout), w["down"], flat(dh), transpose_b=True)
+        evk.gated_linear_backward(a["x1n"], w["gu"], a["gu"], dh, dx1n, g["gu"], self.act)
+        dx1 = dout.clone()
+        evk.rms_norm_backward(a["x1"], dx1n, dx1)  # adds to the residual's gradient
+        evk.matmul(flat(a["att"]), flat(dx1), g["o"], transpose_a=True)
+        evk.matmul(flat(dx1), w["o"], flat(datt), transpose_b=True)
+        evk.window_attention_bwd(a["q"], a["k"], a["v"], a["att"], datt, dq, dk, dv, a["lse"], self.dh, self.window, self.sinks)
+        evk.qkv_norm_rope_backward(a["qkv"], dq, dk, dv, dqkv, self.dh, w["q"], w["k"], g["q"], g["k"])
+        evk.matmul(flat(a["xn"]), flat(dqkv), g["qkv"], transpose_a=True)
+        evk.matmul(flat(dqkv), w["qkv"], flat(dxn), transpose_b=True)
+        dx = dx1.clone()
+        evk.rms_norm_backward(a["x"], dxn, dx)
+        return dx, g
+
+    def exact(self, x, w):
+        """The block in 64 bits on tensors that autograd follows."""
+        b, n, d = x.shape
+        norm = lambda t: t / torch.sqrt(t.square().mean(-1, keepdim=True) + 1e-4)  # noqa: E731
+        hq = self.heads * self.dh
+        qkv = norm(x).reshape(b * n, d) @ w["qkv"]
+        heads = qkv.view(b, n, self.heads + 2 * self.kv, self.dh)
+        ang = torch.arange(n, device=self.dev, dtype=F64)[:, None, None] * 10000.0 ** (-torch.arange(0, self.dh, 2, device=self.dev, dtype=F64) / self.dh)
+        c, s = torch.cos(ang), torch.sin(ang)
+
+        def turned(t):
+            p, q = t[..., 0::2], t[..., 1::2]
+            return torch.stack([p * c - q * s, p * s + q * c], -1).flatten(-2)
+
+        q = turned(norm(heads[:, :, :self.heads]) * w["q"])
+        k = turned(norm(heads[:, :, self.heads:self.heads + self.kv]) * w["k"])
+        v = heads[:, :, self.heads + self.kv:]
+        m = seen(torch.arange(n, device=self.dev), n, self.window, self.sinks)
+        att = []
+        for i in range(b):
+            for hd in range(self.heads):
+                to = hd // (self.heads // self.kv)
+                sc = (q[i, :, hd] @ k[i, :, to].t() * self.dh ** -0.5).masked_fill(~m, -math.inf)
+                att.append(torch.softmax(sc, 1) @ v[i, :, to])
+        att = torch.stack(att).view(b, self.heads, n, self.dh).transpose(1, 2).reshape(b * n, hq)
+        x1 = x + (att @ w["o"]).view(b, n, d)
+        xn = norm(x1).reshape(b * n, d)
+        g, u = xn @ w["gu"][0], xn @ w["gu"][1]
+        h = (torch.nn.functional.silu(g) if self.act == "silu" else g * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3))) * u
+        return x1 + (h @ w["down"]).view(b, n, d)
+
+
+def rel(got, want):
+    return float((got.to(F64) - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("b,n,d,heads,kv,dh,f,window,sinks,act", [(2, 150, 256, 8, 2, 32, 384, 40, 4, "silu"), (1, 97, 200, 3, 1, 64, 136, 0, 0, "gelu"),
+                                                                  (2, 260, 384, 6, 6, 64, 512, 64, 1, "silu")])
+def test_block_training_step(dev, b, n, d, heads, kv, dh, f, window, sinks, act):
+    """A block forward and backward.  Every gradient has at most about 30 roundings to fp16 behind it, each off by at most
+    H of its tensor's norm; added in quadrature 5.5 H, and the softmax and the norms pass on at most three times as much."""
+    r = Rng(dev, 60 + n)
+    blk = Block(dev, r, d, heads, kv, dh, f, window, sinks, act)
+    x, dout = r(b, n, d), r(b, n, d)
+    a = blk.forward(x)
+    dx, g = blk.backward(a, dout)
+    x64 = x.to(F64).requires_grad_(True)
+    w64 = {k: t.to(F64).requires_grad_(True) for k, t in blk.w.items()}
+    out = blk.exact(x64, w64)
+    want = torch.autograd.grad(out, [x64, *w64.values()], dout.to(F64))
+    assert rel(a["out"], out.detach()) <= 16 * H
+    assert rel(dx, want[0]) <= 16 * H
+    for k, t in zip(w64, want[1:]):
+        assert rel(g[k], t) <= 16 * H, k
+
+
+def test_block_decodes_what_it_computes_at_once(dev):
+    """A prompt in two chunks and then single tokens, each sequence at its own length, against the whole sequence."""
+    b, n, rows = 3, 90, 120
+    r = Rng(dev, 71)
+    blk = Block(dev, r, 192, 6, 2, 32, 256, 24, 3, "silu")
+    x = r(b, n, 192)
+    whole = blk.forward(x)["out"]
+    lengths = [50, 64, 80]
+    kc, vc = (torch.full((b, rows, 2 * 32), math.nan, dtype=F16, device=dev) for _ in range(2))
+    for i, m in enumerate(lengths):
+        k1, v1 = kc[i:i + 1], vc[i:i + 1]
+        first = blk.forward(x[i:i + 1, :31].contiguous(), k1, v1)["out"]
+        second = blk.forward(x[i:i + 1, 31:m].contiguous(), k1, v1, p0=31)["out"]
+        # the same sums in another order and with other roundings of P: sqrt(2 * 30) H at most of the norm
+        assert rel(torch.cat([first, second], 1), whole[i:i + 1, :m].to(F64)) <= 8 * H
+    for step in range(10):
+        at = torch.tensor([m + step for m in lengths], dtype=torch.int32, device=dev)
+        tok = torch.stack([x[i, int(at[i])] for i in range(b)])[:, None]
+        out = blk.forward(tok.contiguous(), kc, vc, offsets=at)["out"]
+        want = torch.stack([whole[i, int(at[i])] for i in range(b)])[:, None]
+        assert rel(out, want.to(F64)) <= 8 * H, step
+    assert torch.isnan(kc[0, 60:]).all() and not torch.isnan(kc[0, :60]).any()
+
+
+def steps(dev):
+    """Calls of every entry point on static tensors: [(name, inputs, outputs, call)]."""
+    r = Rng(dev, 81)
+    b, n, h, kv, dh, rows, f = 2, 130, 4, 2, 64, 2100, 256
+    wide = (h + 2 * kv) * dh
+    qkv, wq, wk = r(b, n, wide), r(dh, mean=1.0), r(dh, mean=1.0)
+    q, k, v = empty(dev, b, n, h * dh), empty(dev, b, n, kv * dh), empty(dev, b, n, kv * dh)
+    o, lse, do = empty(dev, b, n, h * dh), torch.zeros(b, h, n, device=dev), r(b, n, h * dh)
+    dq, dk, dv = empty(dev, b, n, h * dh), empty(dev, b, n, kv * dh), empty(dev, b, n, kv * dh)
+    dqkv, dwq, dwk = empty(dev, b, n, wide), empty(dev, dh), empty(dev, dh)
+    kc, vc, q1, o1 = r(1, rows, kv * dh), r(1, rows, kv * dh), r(1, 1, h * dh), empty(dev, 1, 1, h * dh)
+    off = torch.tensor([rows - 1], dtype=torch.int32, device=dev)
+    x, w, hh, gu = r(70, 128), r(2, 128, f, std=0.1), empty(dev, 70, f), empty(dev, 2, 70, f)
+    x1, h1 = r(3, 128), empty(dev, 3, f)
+    dh_, dx, dw = r(70, f), empty(dev, 70, 128), empty(dev, 2, 128, f)
+
+    def call():
+        evk.qkv_norm_rope(qkv, q, k, v, dh, wq, wk)
+        evk.window_attention(q, k, v, o, dh, 40, 3, lse=lse)
+        evk.window_attention_bwd(q, k, v, o, do, dq, dk, dv, lse, dh, 40, 3)
+        evk.qkv_norm_rope_backward(qkv, dq, dk, dv, dqkv, dh, wq, wk, dwq, dwk)
+        evk.window_attention(q1, kc, vc, o1, dh, 0, 0, 0, off)  # split over workgroups
+        evk.gated_linear(x, w, hh, gu)
+        evk.gated_linear_backward(x, w, gu, dh_, dx, dw)
+        evk.gated_linear(x1, w, h1)
+
+    ins = [qkv, do, kc, vc, q1, x, w, dh_, x1]
+    outs = [q, k, v, o, lse, dq, dk, dv, dqkv, dwq, dwk, o1, hh, gu, dx, dw, h1]
+    assert evk.window_attention_workspace(q1, kc, dh) > 0
+    return ins, outs, call
+
+
+def test_other_stream(dev):
+    ins, outs, call = steps(dev)
+    call()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in outs]
+    for t in outs:
+        t.fill_(9.0)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    for t, w in zip(outs, want):
+        assert torch.equal(t, w)
+
+
+def test_streams_at_once(dev):
+    """The same calls on two streams at the same time, on tensors and workspaces of their own."""
+    sets = [steps(dev) for _ in range(2)]
+    for _, _, call in sets:
+        call()
+    torch.cuda.synchronize()
+    want = [[t.clone() for t in outs] for _, outs, _ in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        for (_, outs, call), s in zip(sets, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                call()
+    torch.cuda.synchronize()
+    for (_, outs, _), w in zip(sets, want):
+        for t, x in zip(outs, w):
+            assert torch.equal(t, x)
+
+
+def test_two_graphs(dev):
+    """Two captured graphs, replayed in turn with eager calls, allocations and new inputs between the replays."""
+    sets = [steps(dev) for _ in range(2)]
+    graphs = []
+    s = torch.cuda.Stream()
+    for _, _, call in sets:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call()
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call()
+        graphs.append(g)
+    r = Rng(dev, 5)
+    other = steps(dev)[2]
+    for it in range(4):
+        for (ins, outs, call), g in zip(sets, graphs):
+            for t in ins:
+                t.copy_(r(*t.shape, std=0.5 if it % 2 else 1.0))
+            for t in outs:
+                t.fill_(3.0)
+            junk = torch.full((1 << 20,), math.nan, device=dev)  # what a released workspace would be taken by
+            other()
+            g.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in outs]
+            call()
+            torch.cuda.synchronize()
+            for t, w in zip(got, outs):
+                assert torch.equal(t, w)
+            del junk
+
+
+def test_explicit_workspace_and_stream(dev):
+    r = Rng(dev, 91)
+    q, kc, vc = r(1, 1, 256), r(1, 5000, 128), r(1, 5000, 128)
+    o, o2 = torch.empty_like(q), torch.empty_like(q)
+    evk.window_attention(q, kc, vc, o, 64, 0, 0, 4999)
+    need = evk.window_attention_workspace(q, kc, 64)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="workspace"):
+        evk.window_attention(q, kc, vc, o2, 64, 0, 0, 4999, stream=s.cuda_stream)
+    with pytest.raises(evk.EvkError, match="workspace"):
+        evk.window_attention(q, kc, vc, o2, 64, 0, 0, 4999, workspace=torch.empty(need - 1, dtype=torch.uint8, device=dev))
+    evk.window_attention(q, kc, vc, o2, 64, 0, 0, 4999, workspace=torch.full((need,), 255, dtype=torch.uint8, device=dev), stream=s.cuda_stream)
+    s.synchronize()
+    assert torch.equal(o, o2)
+
+
+@pytest.mark.parametrize("n,sinks", [(1, 4), (1, 0), (20, 70), (600, 70), (600, 64), (600, 0)])
+def test_cache_past_2_gib(dev, n, sinks):
+    """One sequence whose rows of K pass 2 GiB, queries at its end: the sinks and the window lie that far apart."""
+    h, kv, dh, window, rows = 32, 8, 128, 200, 1_100_000
+    tail = n + window
+    assert rows * kv * dh * 2 > 2 ** 31
+    r = Rng(dev, 95)
+    q = r(1, n, h * dh)
+    k, v = (torch.empty(1, rows, kv * dh, dtype=F16, device=dev) for _ in range(2))
+    for t in (k, v):
+        t[:, sinks:rows - tail] = math.nan  # seen by nobody
+        t[:, :sinks], t[:, rows - tail:] = r(1, sinks, kv * dh), r(1, tail, kv * dh)
+    o, lse = torch.empty_like(q), torch.empty(1, h, n, device=dev)
+    evk.window_attention(q, k, v, o, dh, window, sinks, rows - n, lse=lse)
+    # the rows that count, and positions moved down with them
+    kk, vv = (torch.cat([t[:, :sinks], t[:, rows - tail:]], 1) for t in (k, v))
+    w = window_want(q, kk, vv, h, kv, dh, [sinks + window], window, sinks)
+    close(o, w["o"], w["o_t"], "o")
+    close(lse, w["lse"], w["lse_t"], "lse", norm=None)
+
+
+def test_rows_into_a_cache_past_4_gib(dev):
+    """Cache rows whose elements lie past 2^32 bytes."""
+    b, n, kv, dh, rows = 2, 3, 8, 128, 1_200_000
+    r = Rng(dev, 96)
+    qkv = r(b, n, 3 * kv * dh)
+    q = empty(dev, b, n, kv * dh)
+    k, v = (torch.zeros(b, rows, kv * dh, dtype=F16, device=dev) for _ in range(2))
+    assert k.numel() * 2 > 2 ** 32
+    off = torch.tensor([5, rows - n], dtype=torch.int32, device=dev)
+    evk.qkv_norm_rope(qkv, q, k, v, dh, offsets=off)
+    for s in range(b):
+        at = int(off[s])
+        assert torch.equal(v[s, at:at + n], qkv[s, :, 2 * kv * dh:])
+        assert (k[s, at:at + n] != 0).any(1).all()
+        assert int((k[s] != 0).any(1).sum()) == n and int((v[s] != 0).any(1).sum()) == n
