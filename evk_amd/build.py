@@ -23,7 +23,7 @@ ARCH = os.environ.get("EVK_OFFLOAD_ARCH", "gfx950")
 
 KERNEL_SOURCES = ["capi.hip", "gemm.hip", "flash.hip", "flash_wide.hip", "decode_ops.hip", "model.hip", "decode_persist.hip",
                   "kv_step.hip", "train_ops.hip", "capi_block.hip", "qkv_rope.hip", "window.hip"]
-API_SOURCES = ["evk_runtime.cpp", "evk_ai.cpp"]
+API_SOURCES = ["evk_runtime.cpp", "evk_ai.cpp", "evk_block.cpp"]
 
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
@@ -83,8 +83,8 @@ def build(verbose: bool = False) -> None:
                   "-L", HERE, "-levk", "-levkhip", "-Wl,-rpath,$ORIGIN/.."])
             os.replace(exe + ".tmp", exe)
 
-        with cf.ThreadPoolExecutor(max_workers=2) as ex:
-            list(ex.map(program, ["api_tests", "kv_decoder_tool"]))
+        with cf.ThreadPoolExecutor(max_workers=3) as ex:
+            list(ex.map(program, ["api_tests", "kv_decoder_tool", "block_tests"]))
     if verbose:
         print("built", kern)
 

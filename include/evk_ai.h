@@ -395,6 +395,41 @@ void rms_norm(Tensor& input, Tensor& output, float eps = 1e-4f);
 // tensor = 0 (evk_ai.h:602).
 void zero(Tensor& tensor);
 
+// ---- operators of a grouped-query block (no reference counterparts); 32-bit
+// values (offsets, lse) lie in the storage of fp16 tensors of twice as many
+// elements, as for flash_attention ----
+
+// Norm and rotation of each query and key head of qkv (B, N, (H + 2 KV) *
+// head_dim): q (B, N, H * head_dim); k, v (B, rows, KV * head_dim), whose rows
+// position_offset + t (or offsets[b] + t, B int32 values) take token t.
+// Weights: head_dim values, nullptr for ones.
+void qkv_norm_rope(Tensor& qkv, Tensor& q, Tensor& k, Tensor& v, uint32_t head_dim, Tensor* q_weight = nullptr,
+                   Tensor* k_weight = nullptr, float eps = 1e-4f, float rotary_base = 10000.0f, uint32_t position_offset = 0,
+                   Tensor* offsets = nullptr);
+// dqkv is written; the weights' gradients (nullptr: not wanted) are written or,
+// with accumulate, added to.
+void qkv_norm_rope_backward(Tensor& qkv, Tensor& dq, Tensor& dk, Tensor& dv, Tensor& dqkv, uint32_t head_dim,
+                            Tensor* q_weight = nullptr, Tensor* k_weight = nullptr, Tensor* dq_weight = nullptr,
+                            Tensor* dk_weight = nullptr, float eps = 1e-4f, float rotary_base = 10000.0f,
+                            uint32_t position_offset = 0, bool accumulate = false);
+
+// Causal attention over the last `window` rows (0: all) up to the query's
+// position and the first `sinks` rows; q, o (B, N, H * head_dim), k, v (B, rows,
+// KV * head_dim).  N = 1 is a decode step.  lse: B * H * N fp32 values.
+void window_attention(Tensor& q, Tensor& k, Tensor& v, Tensor& o, uint32_t head_dim, uint32_t window = 0, uint32_t sinks = 0,
+                      uint32_t position_offset = 0, Tensor* offsets = nullptr, Tensor* lse = nullptr);
+// Over a whole sequence (rows == N), from the forward's o and lse.
+void window_attention_bwd(Tensor& q, Tensor& k, Tensor& v, Tensor& o, Tensor& dO, Tensor& dQ, Tensor& dK, Tensor& dV, Tensor& lse,
+                          uint32_t head_dim, uint32_t window = 0, uint32_t sinks = 0);
+
+// h (..., F) = act(x w[0]) * (x w[1]), x (..., D), w (2, D, F); gate_up
+// (2, ..., F) receives both products for the backward pass.
+enum class Activation { Silu = 0, Gelu = 1, Relu = 2 };
+void gated_linear(Tensor& x, Tensor& w, Tensor& h, Tensor* gate_up = nullptr, Activation activation = Activation::Silu);
+// dx is written, dw written or, with accumulate, added to; nullptr: not wanted.
+void gated_linear_backward(Tensor& x, Tensor& w, Tensor& gate_up, Tensor& dh, Tensor* dx, Tensor* dw,
+                           Activation activation = Activation::Silu, bool accumulate = false);
+
 // ---- training ops (evk_ai.h:476-614).  *_backward ops accumulate into
 // their grad_in, as the reference's shaders do. ----
 
@@ -690,6 +725,68 @@ struct Graph {
             evk::ai::add(q.grad(), dq, q.grad());
             evk::ai::add(k.grad(), dk, k.grad());
             evk::ai::add(v.grad(), dv, v.grad());
+        };
+        return out;
+    }
+
+    // Queries, keys and values of qkv (B, N, (heads + 2 kv_heads) * head_dim),
+    // normalised per head and rotated; weights of head_dim values, or nullptr.
+    struct Heads {
+        Tensor &q, &k, &v;
+    };
+    Heads qkv_norm_rope(Tensor& qkv, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, Tensor* q_weight = nullptr,
+                        Tensor* k_weight = nullptr, float eps = 1e-4f, float rotary_base = 10000.0f) {
+        assert(qkv.shape.rank() == 3 && "qkv_norm_rope: (B, N, (heads + 2 kv_heads) * head_dim)");
+        const uint32_t B = qkv.shape[0], N = qkv.shape[1];
+        Tensor& dqkv = node(qkv.shape);
+        Tensor& q = node(Shape({B, N, heads * head_dim}));
+        Tensor& k = node(Shape({B, N, kv_heads * head_dim}));
+        Tensor& v = node(Shape({B, N, kv_heads * head_dim}));
+        q.forward_fn = [&qkv, &q, &k, &v, head_dim, q_weight, k_weight, eps, rotary_base]() {
+            evk::ai::qkv_norm_rope(qkv, q, k, v, head_dim, q_weight, k_weight, eps, rotary_base);
+        };
+        // the backward functions run in reverse: q's after those of every node that reads q, k or v
+        q.backward_fn = [&qkv, &q, &k, &v, &dqkv, head_dim, q_weight, k_weight, eps, rotary_base]() {
+            evk::ai::qkv_norm_rope_backward(qkv, q.grad(), k.grad(), v.grad(), dqkv, head_dim, q_weight, k_weight,
+                                            q_weight ? &q_weight->grad() : nullptr, k_weight ? &k_weight->grad() : nullptr, eps,
+                                            rotary_base, 0, true);
+            evk::ai::add(qkv.grad(), dqkv, qkv.grad());
+        };
+        return {q, k, v};
+    }
+
+    // Causal attention over the last `window` positions (0: all) and the first
+    // `sinks`: q (B, N, H * head_dim), k, v (B, N, KV * head_dim).
+    Tensor& window_attention(Tensor& q, Tensor& k, Tensor& v, uint32_t head_dim, uint32_t window = 0, uint32_t sinks = 0) {
+        assert(q.shape.rank() == 3 && k.shape.rank() == 3 && v.shape.rank() == 3 && "window_attention: (B, N, D)");
+        Tensor& lse = node(Shape({q.shape[0], q.shape[2] / head_dim, q.shape[1], 2}));  // fp32 log-sum-exp per row
+        Tensor& dq = node(q.shape);
+        Tensor& dk = node(k.shape);
+        Tensor& dv = node(v.shape);
+        Tensor& out = node(q.shape);
+        out.forward_fn = [&q, &k, &v, &out, &lse, head_dim, window, sinks]() {
+            evk::ai::window_attention(q, k, v, out, head_dim, window, sinks, 0, nullptr, &lse);
+        };
+        out.backward_fn = [&q, &k, &v, &out, &lse, &dq, &dk, &dv, head_dim, window, sinks]() {
+            evk::ai::window_attention_bwd(q, k, v, out, out.grad(), dq, dk, dv, lse, head_dim, window, sinks);
+            evk::ai::add(q.grad(), dq, q.grad());
+            evk::ai::add(k.grad(), dk, k.grad());
+            evk::ai::add(v.grad(), dv, v.grad());
+        };
+        return out;
+    }
+
+    // act(x w[0]) * (x w[1]): x (T, D) or (B, N, D), w (2, D, F).
+    Tensor& gated_linear(Tensor& x, Tensor& w, evk::ai::Activation activation = evk::ai::Activation::Silu) {
+        assert((x.shape.rank() == 2 || x.shape.rank() == 3) && w.shape.rank() == 3 && "gated_linear: x (.., D), w (2, D, F)");
+        const uint32_t F = w.shape[2], T = x.shape.count() / x.shape[x.shape.rank() - 1];
+        Tensor& gate_up = node(Shape({2, T, F}));
+        Tensor& dx = node(x.shape);
+        Tensor& out = node(x.shape.rank() == 2 ? Shape({T, F}) : Shape({x.shape[0], x.shape[1], F}));
+        out.forward_fn = [&x, &w, &out, &gate_up, activation]() { evk::ai::gated_linear(x, w, out, &gate_up, activation); };
+        out.backward_fn = [&x, &w, &out, &gate_up, &dx, activation]() {
+            evk::ai::gated_linear_backward(x, w, gate_up, out.grad(), &dx, &w.grad(), activation, true);
+            evk::ai::add(x.grad(), dx, x.grad());
         };
         return out;
     }
