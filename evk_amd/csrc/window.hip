@@ -271,7 +271,7 @@ struct Frag {
 };
 
 // buf_rsrc of values that are the same in the whole wave, wherever they were computed
-DEV __amdgpu_buffer_rsrc_t wave_rsrc(const f16* base, uint32_t bytes) {
+DEV __amdgpu_buffer_rsrc_t wave_rsrc(const void* base, uint32_t bytes) {
     const uint64_t p = (uint64_t)base;
     const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)p), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32));
     return buf_rsrc((const void*)(hi << 32 | lo), (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
@@ -289,8 +289,9 @@ struct TileDma {
     DEV int row(int i) const { return (wave * PER + i) * RPI + lane / G::CPR; }
     DEV int chunk(int i) const { return (lane % G::CPR) ^ swz<G::W>(row(i)); }
     DEV void go(__amdgpu_buffer_rsrc_t res, const uint32_t (&off)[PER], f16* lds) const {
+        const uint32_t at = lds_addr(lds) + wave * PER * 1024;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) dma16(res, off[i], lds_addr(lds + (wave * PER + i) * 512));
+        for (int i = 0; i < PER; ++i) dma16(res, off[i], at + i * 1024);
     }
 };
 
@@ -770,15 +771,35 @@ __global__ __launch_bounds__(64) void window_join(WindowArgs a, int splits, cons
     if (__any(bad)) fwd_row(a, at, lds, lane);
 }
 
+// dS is rounded to fp16 for its products.  |dS| <= P |dO| (|V| + |O|), so that
+// output gradients as small as those of a mean over a batch would leave it a
+// few bits of fp16's subnormals.  P therefore carries a power of two that
+// leaves the sums at the end: for dQ one for each query, which makes its dO
+// about as long as 1; for dK and dV one for all queries of a sum, by the longest
+// (each wave of window_dq leaves its rows'), so that dO is about 4 long, within
+// what fp16 holds of P itself: 2^12 P is at most 4096, and P / 4 loses nothing
+// down to 2^-12.
+constexpr int LONG = 2, MOST = 12, LEAST = -2;
+constexpr int K_LEAST = -24;  // of rows that are zero
+DEV float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+DEV int length_exponent(float squares) {  // |x| < 2^k
+    return squares > 0.0f ? (__builtin_amdgcn_frexp_expf(squares) + 1) >> 1 : K_LEAST;
+}
+
 // Backward, dQ and the rows' statistics.  Workgroup as in the forward:
 //   S^T = K Q^T, dP^T = V dO^T, P = 2^(S c - lse), dS = P (dP - D),
 //   dQ^T += K^T dS^T (K^T by transposed reads of the same tile),
-// dS rounded to fp16 for the product.  Stores (lse log2 e, D) of every row,
-// flat by key head, for the kernel of dK and dV.
-template <int DH, int QB>
-__global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a, int tiles, float2* stats) {
+// Stores -lse / scale and -D of every row, flat by key head (`rows` of each),
+// and the largest length exponent of each wave's rows for the kernel of dK and dV.
+template <int DH>
+struct DqGeo {
+    static constexpr int QB = DH <= 128 ? 2 : 1, ROWS = 64 * QB;
+    static int tiles(int64_t nr) { return (int)((nr + ROWS - 1) / ROWS); }
+};
+template <int DH>
+__global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a, int tiles, float* stats, int64_t rows, int* tops) {
     using G = Geo<DH>;
-    constexpr int KS = G::KS, DT = G::DT, W = G::W, TILE = BK * W, ROWS = 64 * QB;
+    constexpr int KS = G::KS, DT = G::DT, W = G::W, QB = DqGeo<DH>::QB, TILE = BK * W, ROWS = DqGeo<DH>::ROWS;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
@@ -794,14 +815,15 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
     half8 qf[QB][KS], gf[QB][KS];
     int qp[QB];
     float lse2[QB], dsum[QB];
+    int lift[QB], top = K_LEAST;
     const int64_t q0 = ((int64_t)b * a.N * a.H + c * group) * a.dh;
     auto row_at = [&](int r) { return q0 + ((int64_t)(r / group) * a.H + r % group) * a.dh; };
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int r = min(wr0 + 16 * q + l16, NR - 1);
         qp[q] = r / group;
-        lse2[q] = a.lse[((int64_t)b * a.H + c * group + r % group) * a.N + r / group] * kLog2e;
-        float sum = 0.0f;
+        const float lse = a.lse[((int64_t)b * a.H + c * group + r % group) * a.N + r / group];
+        float sum = 0.0f, squares = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             half8 of = {};
@@ -813,11 +835,22 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
                 of = *reinterpret_cast<const half8*>(a.o + src);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += (float)gf[q][ks][i] * (float)of[i];
+            for (int i = 0; i < 8; ++i) {
+                sum += (float)gf[q][ks][i] * (float)of[i];
+                squares += (float)gf[q][ks][i] * (float)gf[q][ks][i];
+            }
         }
         dsum[q] = query_sum(sum);
-        if (g == 0 && wr0 + 16 * q + l16 < NR) stats[(int64_t)bc * NR + r] = float2{lse2[q], dsum[q]};
+        if (g == 0 && wr0 + 16 * q + l16 < NR) {
+            stats[(int64_t)bc * NR + r] = -lse / a.scale;
+            stats[rows + (int64_t)bc * NR + r] = -dsum[q];
+        }
+        lift[q] = length_exponent(query_sum(squares));
+        lse2[q] = lse * kLog2e + (float)lift[q];  // into P
+        top = max(top, lift[q]);
     }
+    top = (int)wave_max((float)top);
+    if (lane == 0) tops[((int64_t)bc * tiles + tile) * 4 + wave] = top;
     const float c2 = a.scale * kLog2e;
     floatx4 acc[DT][QB];
 #pragma unroll
@@ -885,11 +918,12 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
         const int r = wr0 + 16 * q + l16;
         if (r >= NR) continue;
         f16* dst = a.out + row_at(r);
+        const float back = __builtin_ldexpf(a.scale, lift[q]);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
             if (16 * d + 4 * g < a.dh)
-                *reinterpret_cast<uint2*>(dst + 16 * d + 4 * g) = uint2{pack_h2(acc[d][q][0] * a.scale, acc[d][q][1] * a.scale),
-                                                                        pack_h2(acc[d][q][2] * a.scale, acc[d][q][3] * a.scale)};
+                *reinterpret_cast<uint2*>(dst + 16 * d + 4 * g) =
+                    uint2{pack_h2(acc[d][q][0] * back, acc[d][q][1] * back), pack_h2(acc[d][q][2] * back, acc[d][q][3] * back)};
     }
     static_assert(4 * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
     const bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
@@ -902,8 +936,9 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
 // Backward, dK and dV.  Workgroup: NWV waves of 16 KB rows (keys) of one key head
 // and one part of the queries that see any of them; Q and dO come in tiles of
 // QT flat rows through two LDS stages.
-//   S = Q K^T and dP = dO V^T (a lane: one key, rows 4 g + j of a 16-row
-//   block), P and dS are then the B operands of dV^T += dO^T P and
+//   S = Q K^T - lse / scale and dP = dO V^T - D (a lane: one key, rows 4 g + j
+//   of a 16-row block; the rows' terms are what the sums start from),
+//   P = 2^(S c), dS = P dP, which are then the B operands of dV^T += dO^T P and
 //   dK^T += Q^T dS, whose A operands are transposed reads of the same tiles.
 // The sum over the heads of a group is part of the sum over rows.
 //
@@ -948,21 +983,24 @@ struct KvGrad {
     static constexpr int KEYS = 16 * KB * NWV, QT = Geo<DH>::W >= 128 ? 32 : 64;
 };
 template <int DH>
-__global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void window_dkdv(WindowArgs a, Parts pt, const float2* stats, float* ws) {
+__global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void window_dkdv(WindowArgs a, Parts pt, const float* stats, int64_t rows, const int* tops, int tiles, float* ws) {
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, KB = KvGrad<DH>::KB, NWV = KvGrad<DH>::NWV, KEYS = KvGrad<DH>::KEYS;
     constexpr int QT = KvGrad<DH>::QT, TILE = QT * W;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
-    __shared__ float2 sst[2][QT];
+    __shared__ __attribute__((aligned(1024))) float sst[2][2][256];  // -lse / scale and -D of a tile's rows; a wave's load fills 1 KB
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const Frag<DH> fr(lane);
     const int at = xcd_tile(blockIdx.x, gridDim.x);
-    const int bc = at / pt.items, c = bc % a.KV, b = bc / a.KV, item = at % pt.items;
+    auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // quotients come in vector registers
+    const int bc = uni(at / pt.items), c = uni(bc % a.KV), b = uni(bc / a.KV), item = uni(at % pt.items);
     int blk, part;
     pt.find(item, &blk, &part);
-    const int nparts = pt.parts_of(blk);
-    const int group = a.H / a.KV, NR = a.N * group;
+    blk = uni(blk);
+    part = uni(part);
+    const int nparts = uni(pt.parts_of(blk));
+    const int group = uni(a.H / a.KV), NR = a.N * group;
     const int k0 = blk * KEYS, klast = min(k0 + KEYS, a.N) - 1;
     // queries of this part: flat rows [ra, rb_end)
     const int64_t unit = (int64_t)pt.q * KEYS;
@@ -977,17 +1015,20 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
     using Dma = TileDma<DH, QT, NWV>;
     const Dma dma{wave, lane};
     auto offset = [&](int i, int m0) {
+        Dma dma{wave, lane};
+        // formed for every tile: kept, they were spilled (DH 128 holds 168 registers) and a reload waits for the loads before it
+        if constexpr (DH == 128) asm volatile("" : "+v"(dma.lane));
         const int m = m0 + dma.row(i), t = by_group(m);
         return oob_or(dma.chunk(i) * 8 < a.dh, (uint32_t)((t * a.H + (m - t * group)) * a.dh + dma.chunk(i) * 8) * 2);
     };
-    uint32_t off[Dma::PER];
-#pragma unroll
-    for (int i = 0; i < Dma::PER; ++i) off[i] = offset(i, 0);
     // tile at flat row r0, row m0 of position t0
-    const uint32_t whole = (uint32_t)(by_group(QT - 1) * a.H + (QT - 1 - by_group(QT - 1) * group) + 1) * a.dh * 2;
+    const uint32_t whole = (uint32_t)uni((by_group(QT - 1) * a.H + (QT - 1 - by_group(QT - 1) * group) + 1) * a.dh * 2);
     auto load = [&](int r0, int t0, int m0, f16* sq, f16* sg) {
         const int64_t base = (qb0 + (int64_t)t0 * a.H) * a.dh;
         if (m0 == 0 && r0 + QT <= rb_end) {
+            uint32_t off[Dma::PER];
+#pragma unroll
+            for (int i = 0; i < Dma::PER; ++i) off[i] = offset(i, 0);
             dma.go(wave_rsrc(a.q + base, whole), off, sq);
             dma.go(wave_rsrc(a.dO + base, whole), off, sg);
             return;
@@ -1001,13 +1042,18 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
         dma.go(wave_rsrc(a.q + base, span), o, sq);
         dma.go(wave_rsrc(a.dO + base, span), o, sg);
     };
-    float2 st = {0.0f, 0.0f};
-    auto load_stats = [&](int r0) {
-        if (threadIdx.x < QT) st = r0 + (int)threadIdx.x < rb_end ? stats[(int64_t)bc * NR + r0 + threadIdx.x] : float2{0.0f, 0.0f};
+    auto load_stats = [&](int r0, int stage) {
+        // whole lanes: up to three values past the rows are the other array's or the exponents', and masked
+        if (wave < 2)
+            dma16(wave_rsrc(stats + (wave ? rows : 0) + (int64_t)bc * NR + r0, (uint32_t)(min(QT, rb_end - r0) + 3) / 4 * 16),
+                  (uint32_t)lane * 16, lds_addr(reinterpret_cast<const f16*>(sst)) + (2 * stage + wave) * 1024);
     };
+    int top = K_LEAST;
     if (nt > 0) {
         load(ra, ta, 0, smem, smem + TILE);
-        load_stats(ra);
+        load_stats(ra, 0);
+        constexpr int ROWS = DqGeo<DH>::ROWS / 4;  // of an entry
+        for (int i = ra / ROWS + lane; i <= (rb_end - 1) / ROWS; i += 64) top = max(top, (tops + (int64_t)bc * tiles * 4)[i]);
     }
     half8 kf[KB][KS], vf[KB][KS];
     const int64_t kv_ld = (int64_t)a.KV * a.dh, kv0 = (int64_t)b * a.R * kv_ld + (int64_t)c * a.dh;
@@ -1029,6 +1075,8 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) gk[d][kb] = gv[d][kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     const float c2 = a.scale * kLog2e;
+    const int lift = __builtin_amdgcn_readfirstlane(min(max(LONG - (int)wave_max((float)top), LEAST), MOST));
+    const float lift_s = (float)lift / c2;  // in S
     half2_t wild = {(f16)0.0f, (f16)0.0f};
     // 32 rows of a tile
     auto step_of = [&](int t, int r0, int tf, int m0, int h, const f16* sq, const f16* sg, bool plain) {
@@ -1044,16 +1092,21 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
             gt[slot] = fr.col(sg, 32 * h, i);
             qt[slot] = fr.col(sq, 32 * h, i);
         };
+        floatx4 x0[2], y0[2];
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            x0[rb] = *reinterpret_cast<const floatx4*>(&sst[t & 1][0][32 * h + 16 * rb + 4 * g]) + lift_s;
+            y0[rb] = *reinterpret_cast<const floatx4*>(&sst[t & 1][1][32 * h + 16 * rb + 4 * g]);
+        }
         Rows::template start<2>(row);
         Rows::template run<2 * KB, 2>(row, [&](auto i, auto slot) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-                const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                s[i / KS][kb] = mfma16(qf[slot], kf[kb][i % KS], i % KS ? s[i / KS][kb] : zero);
-                dp[i / KS][kb] = mfma16(gf[slot], vf[kb][i % KS], i % KS ? dp[i / KS][kb] : zero);
+                s[i / KS][kb] = mfma16(qf[slot], kf[kb][i % KS], i % KS ? s[i / KS][kb] : x0[i / KS]);
+                dp[i / KS][kb] = mfma16(gf[slot], vf[kb][i % KS], i % KS ? dp[i / KS][kb] : y0[i / KS]);
             }
         });
-        if (!plain) {  // workgroup-uniform: hidden scores to -inf, hidden dP to D
+        if (!plain) {  // workgroup-uniform: hidden scores to -inf, hidden dP to 0
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
@@ -1077,9 +1130,8 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
                 float e[4], f[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 st4 = sst[t & 1][32 * h + 16 * rb + 4 * g + j];
-                    e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][kb][j], c2, -st4.x));
-                    f[j] = e[j] * (dp[rb][kb][j] - st4.y);
+                    e[j] = __builtin_amdgcn_exp2f(s[rb][kb][j] * c2);
+                    f[j] = e[j] * dp[rb][kb][j];
                 }
                 pu[2 * rb] = pack_h2(e[0], e[1]);
                 pu[2 * rb + 1] = pack_h2(e[2], e[3]);
@@ -1100,7 +1152,6 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
     };
     int t0 = ta, m0 = 0;
     for (int t = 0; t < nt; ++t) {
-        if (threadIdx.x < QT) sst[t & 1][threadIdx.x] = st;
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
         __syncthreads();                     // everyone's; the other stage is free
         f16* const sq = smem + (t & 1) * 2 * TILE;
@@ -1112,7 +1163,7 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
         if (t + 1 < nt) {
             f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
             load(r0 + QT, t0, m0, nx, nx + TILE);
-            load_stats(r0 + QT);
+            load_stats(r0 + QT, (t + 1) & 1);
         }
         // every query of the tile sees every key of the block: the first query the last key, the last query (before
         // row m0 of position t0) the first key outside the sinks
@@ -1124,6 +1175,7 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
         }
     }
     bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
+    const float back_v = exp2i(-lift), back_k = a.scale * back_v;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
         if (nparts > 1) {
@@ -1131,8 +1183,8 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
             float* dst = ws + ((int64_t)bc * pt.slots + item) * (2 * KEYS * DH) + ((wave * KB + kb) * 16 + l16) * (2 * DH);
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                *reinterpret_cast<floatx4*>(dst + 16 * d + 4 * g) = gk[d][kb];
-                *reinterpret_cast<floatx4*>(dst + DH + 16 * d + 4 * g) = gv[d][kb];
+                *reinterpret_cast<floatx4*>(dst + 16 * d + 4 * g) = gk[d][kb] * back_k;
+                *reinterpret_cast<floatx4*>(dst + DH + 16 * d + 4 * g) = gv[d][kb] * back_v;
             }
             continue;
         }
@@ -1142,10 +1194,9 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
 #pragma unroll
         for (int d = 0; d < DT; ++d)
             if (16 * d + 4 * g < a.dh) {
-                *reinterpret_cast<uint2*>(a.dK + dst + 16 * d + 4 * g) =
-                    uint2{pack_h2(gk[d][kb][0] * a.scale, gk[d][kb][1] * a.scale), pack_h2(gk[d][kb][2] * a.scale, gk[d][kb][3] * a.scale)};
-                *reinterpret_cast<uint2*>(a.dV + dst + 16 * d + 4 * g) =
-                    uint2{pack_h2(gv[d][kb][0], gv[d][kb][1]), pack_h2(gv[d][kb][2], gv[d][kb][3])};
+                const floatx4 k = gk[d][kb] * back_k, v = gv[d][kb] * back_v;
+                *reinterpret_cast<uint2*>(a.dK + dst + 16 * d + 4 * g) = uint2{pack_h2(k[0], k[1]), pack_h2(k[2], k[3])};
+                *reinterpret_cast<uint2*>(a.dV + dst + 16 * d + 4 * g) = uint2{pack_h2(v[0], v[1]), pack_h2(v[2], v[3])};
             }
     }
     if (nparts > 1) again = false;  // window_dkdv_join looks at the sums
@@ -1177,7 +1228,7 @@ __global__ __launch_bounds__(64) void window_dkdv_join(WindowArgs a, Parts pt, i
     for (int i = 0; i < PER; ++i) {
         bad |= !(fabsf(v[i]) < INFINITY);
         const int d = lane % 32 * PER + i;
-        if (d < a.dh) (is_k ? a.dK : a.dV)[row * a.dh + d] = (f16)(is_k ? v[i] * a.scale : v[i]);
+        if (d < a.dh) (is_k ? a.dK : a.dV)[row * a.dh + d] = (f16)v[i];
     }
     if (__any(bad)) dkdv_row(a, row, lds, lane);
 }
@@ -1288,12 +1339,22 @@ Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
 }
 }  // namespace
 
+// The backward workspace: the rows' statistics, the length exponents of waves' rows, the parts' sums, each a multiple of
+// 16 bytes.
+namespace {
+uint64_t window_stats_rows(int B, int N, int H) { return ((uint64_t)B * N * H + 3) / 4 * 4; }  // of each of two
+uint64_t window_tops_bytes(int B, int N, int H, int KV, int dh) {
+    const int64_t nr = (int64_t)N * (H / KV);
+    return (uint64_t)B * KV * (dh <= 128 ? DqGeo<128>::tiles(nr) : DqGeo<256>::tiles(nr)) * 4 * sizeof(int);
+}
+}  // namespace
+
 uint64_t window_bwd_workspace(int B, int N, int H, int KV, int dh, int window, int sinks) {
     if (dh % 8) return 0;
     const Parts p = parts_for(B, N, KV, dh, window, sinks);
     uint64_t part = 0;
     (void)by_head64(dh, [&](auto dhc) { part = KvGrad<decltype(dhc)::value>::KEYS * 2 * decltype(dhc)::value * sizeof(float); });
-    return ((uint64_t)B * N * H + 1) / 2 * 2 * sizeof(float2) + (uint64_t)B * KV * p.slots * part;
+    return 2 * window_stats_rows(B, N, H) * sizeof(float) + window_tops_bytes(B, N, H, KV, dh) + (uint64_t)B * KV * p.slots * part;
 }
 
 int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
@@ -1302,20 +1363,22 @@ int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
     const int64_t rows = (int64_t)a.B * a.N * a.H, kv_rows = (int64_t)a.B * a.R * a.KV;
     hipError_t e;
     if (mfma_ok(a)) {
-        // stats first: 8 bytes a row, rounded up so that the sums behind them are aligned
-        float2* const stats = (float2*)ws;
-        float* const sums = (float*)(stats + (rows + 1) / 2 * 2);
+        const int64_t nr = (int64_t)a.N * (a.H / a.KV);
+        const int64_t srows = (int64_t)window_stats_rows(a.B, a.N, a.H);
+        float* const stats = (float*)ws;
+        int* const tops = (int*)(stats + 2 * srows);
+        float* const sums = (float*)((char*)tops + window_tops_bytes(a.B, a.N, a.H, a.KV, a.dh));
         e = by_head(a.dh, [&](auto dhc) {
-            constexpr int DH = decltype(dhc)::value, QB = DH <= 128 ? 2 : 1;
-            const int64_t nr = (int64_t)a.N * (a.H / a.KV);
-            const int tiles = (int)((nr + 64 * QB - 1) / (64 * QB));
-            hipLaunchKernelGGL((window_dq<DH, QB>), dim3((unsigned)((int64_t)tiles * a.B * a.KV)), dim3(256), 0, st, a, tiles, stats);
+            constexpr int DH = decltype(dhc)::value;
+            const int tiles = DqGeo<DH>::tiles(nr);
+            hipLaunchKernelGGL(window_dq<DH>, dim3((unsigned)((int64_t)tiles * a.B * a.KV)), dim3(256), 0, st, a, tiles, stats, srows, tops);
         });
         const Parts p = parts_for(a.B, a.N, a.KV, a.dh, a.window, a.sinks);
         if (e == hipSuccess)
             e = by_head64(a.dh, [&](auto dhc) {
                 constexpr int DH = decltype(dhc)::value, KEYS = KvGrad<DH>::KEYS;
-                hipLaunchKernelGGL(window_dkdv<DH>, dim3((unsigned)(p.items * a.B * a.KV)), dim3(64 * KvGrad<DH>::NWV), 0, st, a, p, stats, sums);
+                hipLaunchKernelGGL(window_dkdv<DH>, dim3((unsigned)(p.items * a.B * a.KV)), dim3(64 * KvGrad<DH>::NWV), 0, st, a, p, stats, srows, tops,
+                                   DqGeo<DH>::tiles(nr), sums);
                 const int joined = p.rest > 1 ? p.blocks : p.full;
                 if (p.slots > 0 && joined > 0)
                     hipLaunchKernelGGL((window_dkdv_join<DH, KEYS>), dim3((unsigned)((int64_t)joined * KEYS * a.B * a.KV)), dim3(64), 0, st, a,

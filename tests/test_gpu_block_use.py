@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import evk_amd as evk
-from test_gpu_block import F16, F64, H, Rng, close, empty, seen, window_want
+from test_gpu_block import F16, F32, F64, H, Rng, close, empty, seen, window_want
 
 pytestmark = pytest.mark.gpu
 
@@ -299,3 +299,37 @@ def test_rows_into_a_cache_past_4_gib(dev):
         assert torch.equal(v[s, at:at + n], qkv[s, :, 2 * kv * dh:])
         assert (k[s, at:at + n] != 0).any(1).all()
         assert int((k[s] != 0).any(1).sum()) == n and int((v[s] != 0).any(1).sum()) == n
+
+
+@pytest.mark.parametrize("size", [2.0 ** -13, 2.0 ** -6, 4000.0])
+@pytest.mark.parametrize("dh,h,kv,n,window", [(64, 4, 2, 300, 100), (128, 4, 1, 200, 0), (40, 2, 2, 150, 0), (256, 2, 1, 130, 50)])
+def test_window_attention_bwd_gradient_sizes(dev, dh, h, kv, n, window, size):
+    """Output gradients as small as those of a mean over a batch, and as large as loss scaling makes them: the scores'
+    gradients pass fp16 on their way into the products, and must neither vanish nor overflow there."""
+    g = torch.Generator(device=dev).manual_seed(dh)
+    rnd = lambda std, heads: torch.empty(1, n, heads * dh, dtype=F16, device=dev).normal_(0, std, generator=g)
+    q, k, v, do = rnd(0.25, h), rnd(0.25, kv), rnd(1.0, kv), rnd(size, h)
+    o, lse = torch.empty_like(q), torch.empty(1, h, n, dtype=F32, device=dev)
+    evk.window_attention(q, k, v, o, dh, window, 3, lse=lse)
+    got = [torch.empty_like(t) for t in (q, k, v)]
+    evk.window_attention_bwd(q, k, v, o, do, *got, lse, dh, window, 3)
+
+    heads = lambda t, m: t.view(n, m, dh).transpose(0, 1).double()
+    Q, K, V, G = heads(q, h), heads(k, kv).repeat_interleave(h // kv, 0), heads(v, kv).repeat_interleave(h // kv, 0), heads(do, h)
+    i, j = torch.arange(n, device=dev)[:, None], torch.arange(n, device=dev)[None]
+    see = (j <= i) & ((j > i - (window or n)) | (j < 3))
+    P = torch.softmax((Q @ K.transpose(1, 2) / dh ** 0.5).masked_fill(~see, -torch.inf), -1)
+    dP = G @ V.transpose(1, 2)
+    # D from the rounded output, as the operator takes it
+    dS = P * (dP - (G * heads(o, h)).sum(-1, keepdim=True)) / dh ** 0.5
+    share = lambda t: t.view(kv, h // kv, n, dh).sum(1)
+    want = [dS @ K, share(dS.transpose(1, 2) @ Q), share(P.transpose(1, 2) @ G)]
+    for what, a, w in zip(("dQ", "dK", "dV"), got, want):
+        a = heads(a, a.shape[2] // dh)
+        assert torch.isfinite(a).all(), what
+        # roundings of P or dS and of the result (each at most half a step of the norm), the result's subnormals, and P's
+        # (products in fp16 of probabilities below 2^-14, off by 2^-25 each, at most the norm of G's columns)
+        tol = 2 * 2.0 ** -11 * w.norm() + 2.0 ** -25 * w.numel() ** 0.5
+        if what == "dV":
+            tol = tol + 2.0 ** -25 * n ** 0.5 * (h // kv) * G.norm()
+        assert (a - w).norm() <= tol, f"{what}: off by {float((a - w).norm() / w.norm()):.3g} of the norm, {float(tol / w.norm()):.3g} allowed"
