@@ -449,6 +449,7 @@ def greedy_sample(logits, out_tokens, position, token_base, token_count, stream=
 # `stream` to be that stream.
 
 _F16 = None
+_U32 = (1 << 32) - 1
 
 
 def _first(t) -> int:
@@ -529,8 +530,8 @@ def _shape3(t, name):
 
 def _at_least(least, **values):
     for name, v in values.items():
-        if v < least:
-            raise ValueError(f"{name} is {v}, at least {least} is needed")
+        if not least <= v <= _U32:
+            raise ValueError(f"{name} is {v}, at least {least} and at most 2^32 - 1 is needed")
 
 
 def qkv_norm_rope(qkv, q, k, v, head_dim, q_weight=None, k_weight=None, eps=1e-4, rotary_base=10000.0, position_offset=0,
@@ -538,7 +539,7 @@ def qkv_norm_rope(qkv, q, k, v, head_dim, q_weight=None, k_weight=None, eps=1e-4
     """Norm and rotation of each query and key head of qkv (B, N, (H + 2 KV) head_dim) into q (B, N, H head_dim) and the
     rows position_offset + t (or offsets[b] + t, int32) of k and v (B, rows, KV head_dim)."""
     dev = _first(qkv)
-    if head_dim < 1 or position_offset < 0:
+    if not (1 <= head_dim <= _U32 and 0 <= position_offset <= _U32):
         _at_least(1, head_dim=head_dim)
         _at_least(0, position_offset=position_offset)
     _check(_calls.evkhip_qkv_norm_rope(_H(qkv, dev), _H(q_weight, dev), _H(k_weight, dev), _H(q, dev), _H(k, dev), _H(v, dev),
@@ -577,7 +578,7 @@ def window_attention(q, k, v, o, head_dim, window=0, sinks=0, position_offset=0,
     `window` (0: all) up to the query's position position_offset + t (or offsets[b] + t, int32), or among the first
     `sinks`.  lse: optional (B, H, N) fp32."""
     dev = _first(q)
-    if head_dim < 1 or window < 0 or sinks < 0 or position_offset < 0:
+    if not (1 <= head_dim <= _U32 and 0 <= window <= _U32 and 0 <= sinks <= _U32 and 0 <= position_offset <= _U32):
         _at_least(1, head_dim=head_dim)
         _at_least(0, window=window, sinks=sinks, position_offset=position_offset)
     ws, wp, wn = _workspace(workspace, window_attention_workspace(q, k, head_dim, window, sinks), dev, stream)

@@ -80,7 +80,7 @@ int head_shapes(const char* op, const evkhip_tensor* q, const evkhip_tensor* k, 
     *s = {q->dims[0], q->dims[1], k->dims[1], q->dims[2] / dh, k->dims[2] / dh};
     EVK_RETURN_IF(s->H % s->KV, EVKHIP_ERR_SHAPE, "%s: %u query heads do not share %u key heads evenly", op, s->H, s->KV);
     EVK_RETURN_IF((uint64_t)s->B * s->N * s->H > kMaxRows || (uint64_t)s->B * s->R * s->KV > kMaxRows || s->R > kMaxRows ||
-                      s->N > kMaxRows,
+                      s->N > kMaxRows || (uint64_t)s->H + 2 * s->KV > kMaxRows,
                   EVKHIP_ERR_UNSUPPORTED, "%s: more than 2^30 rows", op);
     return EVKHIP_OK;
 }
@@ -272,6 +272,7 @@ int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, cons
     CHECK(check_tensor(o, op, 3, 3));
     EVK_RETURN_IF(!same_dims(q, o), EVKHIP_ERR_SHAPE, "%s: o must match q", op);
     CHECK(check_positions(op, s, position_offset, offsets));
+    EVK_RETURN_IF((uintptr_t)lse & 3, EVKHIP_ERR_INVALID_ARG, "%s: lse is not 4-byte aligned", op);
     const uint64_t need = evkhip_window_attention_workspace(s.B, s.N, s.R, s.H, s.KV, head_dim, window, sinks);
     CHECK(check_workspace(op, workspace, workspace_bytes, need));
     CHECK(check_apart(op, {bytes_of("o", o), {"lse", lse, (uint64_t)s.B * s.H * s.N * sizeof(float)}, {"the workspace", workspace, need}},
@@ -313,6 +314,7 @@ int evkhip_window_attention_bwd(const evkhip_tensor* q, const evkhip_tensor* k, 
     }
     EVK_RETURN_IF(s.R != s.N, EVKHIP_ERR_SHAPE, "%s: %u queries over %u rows; the gradient takes a whole sequence", op, s.N, s.R);
     EVK_RETURN_IF(!lse && s.B && s.N, EVKHIP_ERR_INVALID_ARG, "%s: null lse", op);
+    EVK_RETURN_IF((uintptr_t)lse & 3, EVKHIP_ERR_INVALID_ARG, "%s: lse is not 4-byte aligned", op);
     const uint64_t need = evkhip_window_attention_bwd_workspace(s.B, s.N, s.H, s.KV, head_dim, window, sinks);
     CHECK(check_workspace(op, workspace, workspace_bytes, need));
     CHECK(check_apart(op, {bytes_of("dQ", dQ), bytes_of("dK", dK), bytes_of("dV", dV), {"the workspace", workspace, need}},

@@ -293,4 +293,10 @@ inline uint64_t batch_of(const evkhip_tensor* t, uint32_t inner) {  // Shape::ba
 }
 int check_tensor(const evkhip_tensor* t, const char* name, uint32_t min_rank, uint32_t max_rank);
 bool aligned16(const void* p);
+// A launch holds less than 2^32 threads.
+inline int check_grid(const char* op, int64_t workgroups, int threads) {
+    EVK_RETURN_IF(workgroups > (int64_t)UINT32_MAX / threads, EVKHIP_ERR_UNSUPPORTED, "%s: %lld workgroups of %d threads", op,
+                  (long long)workgroups, threads);
+    return EVKHIP_OK;
+}
 }  // namespace evkhip

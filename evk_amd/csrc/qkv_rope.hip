@@ -258,6 +258,8 @@ uint64_t qkv_rope_bwd_workspace(uint64_t tokens, int dh) { return (uint64_t)bwd_
 
 int qkv_rope_forward(const QkvRopeArgs& a, hipStream_t st) {
     const int64_t tokens = (int64_t)a.B * a.N;
+    const int rc = check_grid("qkv_norm_rope", (std::max<int64_t>(tokens, 8192) + 3) / 4, 256);
+    if (rc != EVKHIP_OK) return rc;
     const Turns tn = turns_of(a.base, a.dh);
     const hipError_t e = by_lanes(a.dh, [&](auto lph) {
         constexpr int LPH = decltype(lph)::value;

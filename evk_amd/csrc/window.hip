@@ -1288,6 +1288,10 @@ int window_forward(const WindowArgs& args, void* ws, hipStream_t st) {
     const int64_t nr = (int64_t)a.N * (a.H / a.KV), heads = (int64_t)a.B * a.KV;
     const int splits = fwd_splits(a.B, a.N, a.R, a.H, a.KV, a.dh, a.window, a.sinks);
     hipError_t e;
+    int rc = mfma_ok(a) ? splits ? check_grid("window_attention", (nr + 15) / 16 * heads * splits, 512) : EVKHIP_OK
+                        : check_grid("window_attention", rows, 64);
+    if (rc == EVKHIP_OK && mfma_ok(a) && splits > 1) rc = check_grid("window_attention", nr * heads, 64);
+    if (rc != EVKHIP_OK) return rc;
     if (!mfma_ok(a)) {
         hipLaunchKernelGGL(window_fwd_rows, dim3((unsigned)rows), dim3(64), 0, st, a);
         e = hipGetLastError();
@@ -1362,6 +1366,9 @@ int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
     a.big = (int64_t)a.R * a.KV * a.dh * 2 >= INT32_MAX;
     const int64_t rows = (int64_t)a.B * a.N * a.H, kv_rows = (int64_t)a.B * a.R * a.KV;
     hipError_t e;
+    // the widest launch of either path: a wave for each key (rounded up to blocks of 64) or query row
+    const int rc = check_grid("window_attention_bwd", mfma_ok(a) ? (int64_t)a.B * a.KV * ((a.N + 63) / 64 * 64) : std::max(rows, kv_rows), 64);
+    if (rc != EVKHIP_OK) return rc;
     if (mfma_ok(a)) {
         const int64_t nr = (int64_t)a.N * (a.H / a.KV);
         const int64_t srows = (int64_t)window_stats_rows(a.B, a.N, a.H);

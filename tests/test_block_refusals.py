@@ -234,3 +234,30 @@ def test_python_wrappers_refuse():
     with pytest.raises(ValueError, match="workspace"):
         evk._workspace(None, 64, 0, 12345)
     assert evk._workspace(None, 0, 0, 12345) == (None, None, 0)
+
+
+def test_more_rows_than_a_launch_holds(L):
+    """Sizes below the 2^30 rows of the checks whose launches would pass 2^32 threads."""
+    m = Mem()
+    n = 1 << 26
+    assert rope(L, m, qkv=(n, 1, 6), q=(n, 1, 2), k=(n, 1, 2), dh=2) == UNSUPPORTED
+    assert window(L, m, q=(n, 1, 8), k=(n, 1, 8), dh=8) == UNSUPPORTED  # single tokens
+    assert window(L, m, q=(n, 1, 3), k=(n, 1, 3), dh=3) == UNSUPPORTED  # row by row
+    need = L.evkhip_window_attention_bwd_workspace(n, 1, 1, 1, 8, 4, 1)
+    t = [m(n, 1, 8) for _ in range(8)]
+    assert L.evkhip_window_attention_bwd(*[b(x) for x in t], 1 << 50, 8, 4, 1, 1 << 51, need, None) == UNSUPPORTED
+    assert b"workgroups" in L.evkhip_last_error()
+
+
+def test_lse_alignment(L):
+    m = Mem()
+    q, k = m(2, 5, 256), m(2, 9, 128)
+    args = [b(x) for x in (q, k, m(2, 9, 128), m(2, 5, 256))]
+    assert L.evkhip_window_attention(*args, 64, 4, 1, 0, None, (1 << 42) + 2, None, 0, None) == INVALID
+    assert b"lse" in L.evkhip_last_error()
+
+
+@pytest.mark.parametrize("name,value", [("window", 1 << 32), ("sinks", -1), ("position_offset", (1 << 32) + 3)])
+def test_python_sizes_are_not_cut_to_32_bits(name, value):
+    with pytest.raises(ValueError, match=name):
+        evk._at_least(0, **{name: value})
