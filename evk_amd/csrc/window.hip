@@ -791,15 +791,10 @@ DEV int length_exponent(float squares) {  // |x| < 2^k
 //   dQ^T += K^T dS^T (K^T by transposed reads of the same tile),
 // Stores -lse / scale and -D of every row, flat by key head (`rows` of each),
 // and the largest length exponent of each wave's rows for the kernel of dK and dV.
-template <int DH>
-struct DqGeo {
-    static constexpr int QB = DH <= 128 ? 2 : 1, ROWS = 64 * QB;
-    static int tiles(int64_t nr) { return (int)((nr + ROWS - 1) / ROWS); }
-};
-template <int DH>
+template <int DH, int QB>
 __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a, int tiles, float* stats, int64_t rows, int* tops) {
     using G = Geo<DH>;
-    constexpr int KS = G::KS, DT = G::DT, W = G::W, QB = DqGeo<DH>::QB, TILE = BK * W, ROWS = DqGeo<DH>::ROWS;
+    constexpr int KS = G::KS, DT = G::DT, W = G::W, TILE = BK * W, ROWS = 64 * QB;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
@@ -983,7 +978,7 @@ struct KvGrad {
     static constexpr int KEYS = 16 * KB * NWV, QT = Geo<DH>::W >= 128 ? 32 : 64;
 };
 template <int DH>
-__global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void window_dkdv(WindowArgs a, Parts pt, const float* stats, int64_t rows, const int* tops, int tiles, float* ws) {
+__global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void window_dkdv(WindowArgs a, Parts pt, const float* stats, int64_t rows, const int* tops, int tops_n, int tops_lg, float* ws) {
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, KB = KvGrad<DH>::KB, NWV = KvGrad<DH>::NWV, KEYS = KvGrad<DH>::KEYS;
     constexpr int QT = KvGrad<DH>::QT, TILE = QT * W;
@@ -1052,8 +1047,8 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
     if (nt > 0) {
         load(ra, ta, 0, smem, smem + TILE);
         load_stats(ra, 0);
-        constexpr int ROWS = DqGeo<DH>::ROWS / 4;  // of an entry
-        for (int i = ra / ROWS + lane; i <= (rb_end - 1) / ROWS; i += 64) top = max(top, (tops + (int64_t)bc * tiles * 4)[i]);
+        // an entry for every 2^tops_lg rows, tops_n a key head
+        for (int i = (ra >> tops_lg) + lane; i <= (rb_end - 1) >> tops_lg; i += 64) top = max(top, (tops + (int64_t)bc * tops_n)[i]);
     }
     half8 kf[KB][KS], vf[KB][KS];
     const int64_t kv_ld = (int64_t)a.KV * a.dh, kv0 = (int64_t)b * a.R * kv_ld + (int64_t)c * a.dh;
@@ -1261,12 +1256,23 @@ hipError_t by_head(int dh, F&& f) {
 }  // namespace
 
 namespace {
+// Blocks of 16 queries of a wave in window_fwd and window_dq: two, each LDS read
+// serving both, where that gives every CU more than one workgroup (forward of 8
+// heads over 2 of 128 values, window 512, us with one and two: 252 workgroups of
+// two 18.7 and 20.0, 378 30.0 and 27.7, 1008 56.4 and 50.5); 256 values leave no
+// registers for two.
+int query_blocks(int64_t rows, int64_t heads, int dh) { return dh <= 128 && heads * ((rows + 127) / 128) > 256 ? 2 : 1; }
+
 // How the forward of a shape runs: 16-row tiles with the list split `splits`
-// ways, or (splits 0) tiles of 128 rows.
+// ways (window_split), or (splits 0) tiles of 64 rows and more (window_fwd).
+// The latter from 65 such tiles on (us, window_fwd and window_split: 4 x 300
+// queries of 4 heads over 1 of 256 values, 76 tiles, 13.5 and 23.1; 1 x 256 of
+// 16 over 4 of 128, 64 tiles, 18.9 and 24.4 with a window of 1024, 104.2 and
+// 84.4 over 8192 rows; 32 tiles 18.7 and 14.4, 104.3 and 51.5).
 int fwd_splits(int B, int N, int R, int H, int KV, int dh, int window, int sinks) {
-    const int64_t rows = (int64_t)N * (H / KV), heads = (int64_t)B * KV, wide = dh <= 128 ? 128 : 64;
+    const int64_t rows = (int64_t)N * (H / KV), heads = (int64_t)B * KV;
     const int64_t tiles = heads * ((rows + 15) / 16);
-    if (rows > 64 && heads * ((rows + wide - 1) / wide) >= 128) return 0;
+    if (rows > 64 && heads * ((rows + 63) / 64) > 64) return 0;
     const int64_t waves = dh <= 128 ? 8 : 4;
     const int64_t list = std::min<int64_t>(R, (int64_t)window + sinks + 16), steps = (list + 31) / 32;
     return (int)std::max<int64_t>(1, std::min((steps + 4 * waves - 1) / (4 * waves), 512 / tiles));
@@ -1297,9 +1303,16 @@ int window_forward(const WindowArgs& args, void* ws, hipStream_t st) {
         e = hipGetLastError();
     } else if (splits == 0) {
         e = by_head(a.dh, [&](auto dhc) {
-            constexpr int DH = decltype(dhc)::value, QB = DH <= 128 ? 2 : 1;
-            const int tiles = (int)((nr + 64 * QB - 1) / (64 * QB));
-            hipLaunchKernelGGL((window_fwd<DH, QB>), dim3((unsigned)(tiles * heads)), dim3(256), 0, st, a, tiles);
+            constexpr int DH = decltype(dhc)::value;
+            auto go = [&](auto qb) {
+                constexpr int QB = decltype(qb)::value;
+                const int tiles = (int)((nr + 64 * QB - 1) / (64 * QB));
+                hipLaunchKernelGGL((window_fwd<DH, QB>), dim3((unsigned)(tiles * heads)), dim3(256), 0, st, a, tiles);
+            };
+            if constexpr (DH <= 128) {
+                if (query_blocks(nr, heads, a.dh) == 2) return go(std::integral_constant<int, 2>{});
+            }
+            go(std::integral_constant<int, 1>{});
         });
     } else {
         e = by_head(a.dh, [&](auto dhc) {
@@ -1348,8 +1361,8 @@ Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
 namespace {
 uint64_t window_stats_rows(int B, int N, int H) { return ((uint64_t)B * N * H + 3) / 4 * 4; }  // of each of two
 uint64_t window_tops_bytes(int B, int N, int H, int KV, int dh) {
-    const int64_t nr = (int64_t)N * (H / KV);
-    return (uint64_t)B * KV * (dh <= 128 ? DqGeo<128>::tiles(nr) : DqGeo<256>::tiles(nr)) * 4 * sizeof(int);
+    const int64_t nr = (int64_t)N * (H / KV), per = 64 * query_blocks(nr, (int64_t)B * KV, dh);
+    return (uint64_t)B * KV * ((nr + per - 1) / per) * 4 * sizeof(int);
 }
 }  // namespace
 
@@ -1371,21 +1384,28 @@ int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
     if (rc != EVKHIP_OK) return rc;
     if (mfma_ok(a)) {
         const int64_t nr = (int64_t)a.N * (a.H / a.KV);
+        const int qb = query_blocks(nr, (int64_t)a.B * a.KV, a.dh), tiles = (int)((nr + 64 * qb - 1) / (64 * qb));
         const int64_t srows = (int64_t)window_stats_rows(a.B, a.N, a.H);
         float* const stats = (float*)ws;
         int* const tops = (int*)(stats + 2 * srows);
         float* const sums = (float*)((char*)tops + window_tops_bytes(a.B, a.N, a.H, a.KV, a.dh));
         e = by_head(a.dh, [&](auto dhc) {
             constexpr int DH = decltype(dhc)::value;
-            const int tiles = DqGeo<DH>::tiles(nr);
-            hipLaunchKernelGGL(window_dq<DH>, dim3((unsigned)((int64_t)tiles * a.B * a.KV)), dim3(256), 0, st, a, tiles, stats, srows, tops);
+            const dim3 grid((unsigned)((int64_t)tiles * a.B * a.KV));
+            if constexpr (DH <= 128) {
+                if (qb == 2) {
+                    hipLaunchKernelGGL((window_dq<DH, 2>), grid, dim3(256), 0, st, a, tiles, stats, srows, tops);
+                    return;
+                }
+            }
+            hipLaunchKernelGGL((window_dq<DH, 1>), grid, dim3(256), 0, st, a, tiles, stats, srows, tops);
         });
         const Parts p = parts_for(a.B, a.N, a.KV, a.dh, a.window, a.sinks);
         if (e == hipSuccess)
             e = by_head64(a.dh, [&](auto dhc) {
                 constexpr int DH = decltype(dhc)::value, KEYS = KvGrad<DH>::KEYS;
                 hipLaunchKernelGGL(window_dkdv<DH>, dim3((unsigned)(p.items * a.B * a.KV)), dim3(64 * KvGrad<DH>::NWV), 0, st, a, p, stats, srows, tops,
-                                   DqGeo<DH>::tiles(nr), sums);
+                                   tiles * 4, qb == 2 ? 5 : 4, sums);
                 const int joined = p.rest > 1 ? p.blocks : p.full;
                 if (p.slots > 0 && joined > 0)
                     hipLaunchKernelGGL((window_dkdv_join<DH, KEYS>), dim3((unsigned)((int64_t)joined * KEYS * a.B * a.KV)), dim3(64), 0, st, a,

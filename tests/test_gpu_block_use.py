@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import evk_amd as evk
+import test_gpu_block as gb
 from test_gpu_block import F16, F32, F64, H, Rng, close, empty, seen, window_want
 
 pytestmark = pytest.mark.gpu
@@ -333,3 +334,18 @@ def test_window_attention_bwd_gradient_sizes(dev, dh, h, kv, n, window, size):
         if what == "dV":
             tol = tol + 2.0 ** -25 * n ** 0.5 * (h // kv) * G.norm()
         assert (a - w).norm() <= tol, f"{what}: off by {float((a - w).norm() / w.norm()):.3g} of the norm, {float(tol / w.norm()):.3g} allowed"
+
+
+WIDE = [  # b, n, heads, kv: workgroups of 64 rows (a few to every compute unit), and of 128 where there are more
+    (2, 300, 16, 8), (1, 1100, 12, 4), (8, 300, 16, 16), (3, 701, 24, 8),
+]
+
+
+@pytest.mark.parametrize("dh", [32, 40, 64, 96, 128, 256])
+@pytest.mark.parametrize("b,n,h,kv", WIDE)
+def test_window_attention_many_rows(dev, b, n, h, kv, dh):
+    """Grids of hundreds of workgroups, forward and backward, with rows that some query of a tile does not see at both
+    ends of its list; a chunk of a longer sequence in the forward."""
+    gb.test_window_attention(dev, b, n, h, kv, dh, n, 0, 100, 5, False)
+    gb.test_window_attention(dev, b, n, h, kv, dh, n + 90, 77, 0, 0, False)
+    gb.test_window_attention_bwd(dev, b, n, h, kv, dh, n, 0, 100, 5, False)
