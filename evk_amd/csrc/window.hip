@@ -736,39 +736,51 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
     }
 }
 
-// The states of one query row's splits, a wave each, in their order.  What is
-// not finite may be a hidden NaN's work: that row is computed again.
+// The states of one query row's splits (at most JOIN_MOST): each thread weighs
+// one, then each of NW waves adds every NW-th one's sums, and theirs are
+// added in order.  What is not finite may be a hidden NaN's work: that row is
+// computed again.
+constexpr int JOIN_MOST = 256;  // CUs
 template <int DH>
-__global__ __launch_bounds__(64) void window_join(WindowArgs a, int splits, const float* ws) {
-    constexpr int PER = (DH + 63) / 64;
+__global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int splits, const float* ws) {
+    constexpr int NW = 4, PER = DH < 64 ? 1 : DH / 64 + (DH % 64 ? 1 : 0);
     __shared__ RowLds lds;
-    const int lane = threadIdx.x, group = a.H / a.KV, NR = a.N * group;
+    __shared__ float part[NW][64 * PER], weight[JOIN_MOST], red[2][NW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.H / a.KV, NR = a.N * group;
     const int row = blockIdx.x % NR, bc = blockIdx.x / NR, c = bc % a.KV, b = bc / a.KV;
     const float* src = ws + (int64_t)blockIdx.x * splits * (DH + 4);
-    float m = -INFINITY;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, src[s * (DH + 4)]);
-    float l = 0.0f, o[PER] = {};
-    for (int s = 0; s < splits; ++s) {
-        const float* p = src + s * (DH + 4);
-        const float f = p[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[0] - m);
-        l += f * p[1];
+    const float mine = tid < splits ? src[tid * (DH + 4)] : -INFINITY;
+    float l = tid < splits ? src[tid * (DH + 4) + 1] : 0.0f, m = wave_max(mine);
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, red[0][w]);
+    const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - m);
+    weight[tid] = f;
+    l = wave_sum(f * l);
+    if (lane == 0) red[1][wave] = l;
+    __syncthreads();
+    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    float o[PER] = {};
+#pragma unroll 8
+    for (int s = wave; s < splits; s += NW)
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (lane * PER + i < DH) o[i] += f * p[4 + lane * PER + i];
-    }
+            if (lane + 64 * i < DH) o[i] += weight[s] * src[s * (DH + 4) + 4 + lane + 64 * i];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) part[wave][lane + 64 * i] = o[i];
+    __syncthreads();
     const int64_t at = ((int64_t)b * a.N + row / group) * a.H + c * group + row % group;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     bool bad = !(fabsf(l) < INFINITY);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int d = lane * PER + i;
-        if (d >= a.dh) continue;
-        bad |= !(fabsf(o[i]) < INFINITY);
-        a.out[at * a.dh + d] = (f16)(o[i] * inv);
+    for (int d = tid; d < a.dh; d += 256) {
+        const float v = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
+        bad |= !(fabsf(v) < INFINITY);
+        a.out[at * a.dh + d] = (f16)(v * inv);
     }
-    if (a.lse && lane == 0)
+    if (a.lse && tid == 0)
         a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
-    if (__any(bad)) fwd_row(a, at, lds, lane);
+    if (__syncthreads_or(bad) && wave == 0) fwd_row(a, at, lds, lane);
 }
 
 // dS is rounded to fp16 for its products.  |dS| <= P |dO| (|V| + |O|), so that
@@ -1275,7 +1287,12 @@ int fwd_splits(int B, int N, int R, int H, int KV, int dh, int window, int sinks
     if (rows > 64 && heads * ((rows + 63) / 64) > 64) return 0;
     const int64_t waves = dh <= 128 ? 8 : 4;
     const int64_t list = std::min<int64_t>(R, (int64_t)window + sinks + 16), steps = (list + 31) / 32;
-    return (int)std::max<int64_t>(1, std::min((steps + 4 * waves - 1) / (4 * waves), 512 / tiles));
+    // One workgroup of `waves` steps at a time up to four of them; longer lists split down to one, as far as every
+    // workgroup has a CU of its own (single tokens, us with one and four steps a wave: 8 heads over 1 of 128 values,
+    // 65536 rows 15.1 and 18.4; 32 over 8, 8192 rows 12.0 and 18.7; 17 steps of 12 over 4 of 64 values 6.4, split 8.7;
+    // 512 workgroups for 256: 64 sequences of 8 over 1, 4096 rows 30.3, 27.4).
+    if (steps <= 4 * waves) return 1;
+    return (int)std::max<int64_t>(1, std::min((steps + waves - 1) / waves, JOIN_MOST / tiles));
 }
 }  // namespace
 
@@ -1296,7 +1313,7 @@ int window_forward(const WindowArgs& args, void* ws, hipStream_t st) {
     hipError_t e;
     int rc = mfma_ok(a) ? splits ? check_grid("window_attention", (nr + 15) / 16 * heads * splits, 512) : EVKHIP_OK
                         : check_grid("window_attention", rows, 64);
-    if (rc == EVKHIP_OK && mfma_ok(a) && splits > 1) rc = check_grid("window_attention", nr * heads, 64);
+    if (rc == EVKHIP_OK && mfma_ok(a) && splits > 1) rc = check_grid("window_attention", nr * heads, 256);
     if (rc != EVKHIP_OK) return rc;
     if (!mfma_ok(a)) {
         hipLaunchKernelGGL(window_fwd_rows, dim3((unsigned)rows), dim3(64), 0, st, a);
@@ -1321,7 +1338,7 @@ int window_forward(const WindowArgs& args, void* ws, hipStream_t st) {
             hipLaunchKernelGGL(window_split<DH>, dim3((unsigned)(tiles * splits * heads)), dim3(64 * SplitGeo<DH>::NW), 0, st, a, tiles, splits,
                                (float*)ws);
             if (splits > 1)
-                hipLaunchKernelGGL(window_join<DH>, dim3((unsigned)(nr * heads)), dim3(64), 0, st, a, splits, (const float*)ws);
+                hipLaunchKernelGGL(window_join<DH>, dim3((unsigned)(nr * heads)), dim3(256), 0, st, a, splits, (const float*)ws);
         });
     }
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "window_attention launch");
