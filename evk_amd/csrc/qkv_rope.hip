@@ -16,6 +16,12 @@
 // same in every head, are formed once.  Far positions lose the angle in 32
 // bits: turns are counted in 64 (p times the frequency that the host computed)
 // and only their fraction goes on in 32.
+//
+// Forward of 8192 tokens of 32 + 8 + 8 heads of 128 values: 42.7 us, 4.7 TB/s
+// (a copy of 1 GiB runs at 5.2); of 7996 tokens of 12 + 4 + 4 heads of 64 11.4
+// us, 3.6 TB/s, the sines' instructions beside the loads; 16 single tokens 4.0,
+// a launch.  Gradient of the 7996 tokens 15.7 us, 3.9 TB/s, and 4.0 for the
+// weights' sums.
 #include "kernels.h"
 
 #include <algorithm>
@@ -27,8 +33,8 @@ namespace evkhip {
 namespace {
 
 // Turns per position of pair i: base^(-2 i / dh) / (2 pi).  A lane multiplies
-// its first pair's from the powers of two in i (a table of every pair in the
-// kernel's arguments is read past the caches: 17 us instead of LATER).
+// its first pair's from the powers of two in i, so that any head size is a few
+// arguments.
 struct Turns {
     double unit;  // pair 0
     double r[7];  // ratio of pairs 2^k apart
@@ -74,7 +80,8 @@ DEV void store_n(f16* p, int n, const float* x) {
 
 // What a lane knows of its token: the turned pairs' cosines and sines.  The
 // hardware's take turns; over a turn they are within 1.25e-7 of the exact ones
-// (measured), half a step of fp16 being 4.9e-4.
+// (measured), half a step of fp16 being 4.9e-4.  By the library's functions the
+// 7996 tokens above took 17 us.
 struct Angles {
     float cs[4], sn[4];
     DEV void set(const Turns& tn, int i0, int p) {
@@ -250,6 +257,8 @@ hipError_t by_lanes(int dh, F&& f) {
     return hipGetLastError();
 }
 
+// 7996 tokens, us of the pass and of the weights' sums: 512 workgroups 18.8 and
+// 4.1, 1024 15.8 and 3.9, 2048 15.8 and 7.7
 int bwd_groups(uint64_t tokens) { return (int)std::min<uint64_t>((tokens + 3) / 4, 1024); }
 
 }  // namespace
@@ -264,7 +273,10 @@ int qkv_rope_forward(const QkvRopeArgs& a, hipStream_t st) {
     const hipError_t e = by_lanes(a.dh, [&](auto lph) {
         constexpr int LPH = decltype(lph)::value;
         const int groups = (a.H + 2 * a.KV + 64 / LPH - 1) / (64 / LPH);
-        int splits = 1;  // enough waves for the chip, else as few as hold a token's angles once
+        // A wave for a part of a token's heads up to 4096 waves, past that one for the token, which forms its angles
+        // once (us, split and not: 1 token of 32 + 8 + 8 heads of 128 values 2.7 and 7.2, 64 tokens 2.9 and 8.4, 200
+        // tokens 3.6 and 8.5; 1500 tokens of 12 + 4 + 4 heads of 64 4.9 and 4.5).
+        int splits = 1;
         while (splits < groups && tokens * splits < 4096) splits = std::min(groups, splits * 2);
         const int per = (groups + splits - 1) / splits;
         splits = (groups + per - 1) / per;

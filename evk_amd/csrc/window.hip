@@ -48,7 +48,9 @@ DEV int position_of(const WindowArgs& a, int b, int t) {
 // ---------------------------------------------------------------------------
 // One wave per query row (or per K, V row), any head size and alignment.
 // Latency-bound chains of scalar loads: the path of head sizes and pointers
-// that the MFMA kernels do not take.
+// that the MFMA kernels do not take (1000 queries of 8 heads over 2 of 100
+// values, window 512: 187 us, backward 3.7 ms), and of the few rows whose
+// tiles hold a hidden NaN.
 // ---------------------------------------------------------------------------
 constexpr int SMAX = 256;  // largest head size
 
@@ -488,7 +490,12 @@ struct Softmax {
 
 // Forward.  Workgroup: 4 waves of 16 QB rows of one key head; K and V tiles in
 // two LDS stages, filled by LDS-direct loads while the tile before is used; one
-// barrier a tile.
+// barrier a tile.  Bound by the MFMA and the softmax's instructions beside it:
+// 8192 queries of 16 heads over 4 of 128 values, window 1024 and 4 sinks, 80 us
+// = 811 TFLOP/s of the visible pairs (whole tiles are 6% more); 97 us before the
+// tiles' rows were placed without bank conflicts and read ahead of the MFMAs.
+// Workgroups of eight waves, reads further ahead and a priority for waves in
+// their products changed nothing.
 //
 // The product of a probability of 0 and a NaN or an infinity is NaN, so a tile
 // that some query does not wholly see is looked at for such values in V; a wave
@@ -597,9 +604,13 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
 // straight into A operands, V through the wave's own LDS slot, no barrier
 // before the end: what counts is that every wave has its loads in flight.  A
 // long list is split over workgroups as well, whose states window_join adds.
+// Bound by memory: 64 sequences' tokens of 32 heads over 8 of 128 values, window
+// 1024, 53 us for 254 MB = 4.8 TB/s; 32 over 8, 131072 rows 108 us = 5.0 TB/s; a
+// lone token of 12 heads over 4 of 64, window 512, 6.5, a launch and two loads'
+// latencies.
 template <int DH>
 struct SplitGeo {
-    static constexpr int NW = DH <= 128 ? 8 : 4;  // waves
+    static constexpr int NW = DH <= 128 ? 8 : 4;  // waves; 256 values take the registers of two
 };
 
 template <int DH>
@@ -803,6 +814,8 @@ DEV int length_exponent(float squares) {  // |x| < 2^k
 //   dQ^T += K^T dS^T (K^T by transposed reads of the same tile),
 // Stores -lse / scale and -D of every row, flat by key head (`rows` of each),
 // and the largest length exponent of each wave's rows for the kernel of dK and dV.
+// Bound as the forward is, with three products for two: 2 x 1999 queries of 8
+// heads over 2 of 128 values, window 512, 25 us (504 workgroups, two for a CU).
 template <int DH, int QB>
 __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a, int tiles, float* stats, int64_t rows, int* tops) {
     using G = Geo<DH>;
@@ -947,13 +960,17 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
 //   of a 16-row block; the rows' terms are what the sums start from),
 //   P = 2^(S c), dS = P dP, which are then the B operands of dV^T += dO^T P and
 //   dK^T += Q^T dS, whose A operands are transposed reads of the same tiles.
-// The sum over the heads of a group is part of the sum over rows.
+// The sum over the heads of a group is part of the sum over rows.  Four products
+// for the forward's two, over the same pairs as window_dq: 47.5 us at its size,
+// 310 TFLOP/s; 168 registers hold three workgroups a CU.  32 keys a wave, tiles of
+// 64 rows and eight waves were no faster.
 //
 // Parts: the queries from the first key's position to the last one that sees
 // the block are cut every `unit` positions (KEYS times Parts::q).  A block with
 // one part writes dK and dV; the others (the sinks' blocks, which every later
 // query sees, and all where the grid would not fill the chip otherwise) leave
-// 32-bit sums that window_dkdv_join adds in the order of the parts.
+// 32-bit sums that window_dkdv_join adds in the order of the parts (11.4 us for
+// 45 MB there).
 struct Parts {
     int q;       // key blocks' lengths of queries per part
     int blocks;  // key blocks of a sequence
@@ -1358,7 +1375,9 @@ Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
         };
         return sum(blocks) - sum(blocks - full) + (blocks - full) * ((span + q - 1) / q);
     };
-    // long parts, as few as fill the chip (and fewer than 2^24)
+    // long parts, as few as make 500 workgroups, two for a CU (2 x 1999 queries of 8 heads over 2 of 128 values, window
+    // 512, the whole backward: 250 97 us, 500 84, 1000 97; one sequence of 4000, no window: 245, 203, 208), and fewer
+    // than 2^24
     int64_t q = full == blocks ? std::max<int64_t>(1, span / 4) : span;
     while (q > 1 && items(q) * heads < 500) q /= 2;
     while (items(q) * heads > (1 << 24) && q < blocks) q *= 2;
