@@ -569,6 +569,8 @@ def qkv_norm_rope_backward(qkv, dq, dk, dv, dqkv, head_dim, q_weight=None, k_wei
 def window_attention_workspace(q, k, head_dim, window=0, sinks=0) -> int:
     """Bytes of workspace of window_attention for these q and k."""
     (b, n, d), (_, rows, dk) = _shape3(q, "q"), _shape3(k, "k")
+    if head_dim < 1:
+        _at_least(1, head_dim=head_dim)
     return _need("evkhip_window_attention_workspace", b, n, rows, d // head_dim, dk // head_dim, head_dim, window, sinks)
 
 

@@ -946,7 +946,15 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
                     uint2{pack_h2(acc[d][q][0] * back, acc[d][q][1] * back), pack_h2(acc[d][q][2] * back, acc[d][q][3] * back)};
     }
     static_assert(4 * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
-    const bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
+    // a hidden NaN, or a dS past fp16 (values of V in the thousands and more)
+    bool bad = !((float)wild[0] == 0.0f && (float)wild[1] == 0.0f);
+#pragma unroll
+    for (int q = 0; q < QB; ++q)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bad |= !(fabsf(acc[d][q][j]) < INFINITY);
+    const bool again = __any(bad);
     if (!__syncthreads_or(again) || !again) return;
 #pragma unroll 1
     for (int r = wr0; r < min(wr0 + 16 * QB, NR); ++r)
@@ -979,13 +987,13 @@ struct Parts {
     int items;   // parts of one key head
     int slots;   // of them with sums in the workspace, the first ones
     __host__ __device__ __forceinline__ int parts_of(int i) const { return i < full ? (blocks - i + q - 1) / q : rest; }
-    __host__ __device__ __forceinline__ int sum(int n) const {  // of ceil(m / q) for m = 1 .. n
-        const int k = n / q;
+    __host__ __device__ __forceinline__ int64_t sum(int64_t n) const {  // of ceil(m / q) for m = 1 .. n
+        const int64_t k = n / q;
         return q * k * (k + 1) / 2 + (n - q * k) * (k + 1);
     }
-    __host__ __device__ __forceinline__ int before(int i) const {  // parts before block i
+    __host__ __device__ __forceinline__ int64_t before(int i) const {  // parts before block i
         const int f = i < full ? i : full;
-        return sum(blocks) - sum(blocks - f) + (i - f) * rest;
+        return sum(blocks) - sum(blocks - f) + (int64_t)(i - f) * rest;
     }
     // the block and the part that item `it` is: the first blocks in groups of q of equally many parts
     DEV void find(int it, int* blk, int* part) const {
@@ -1198,7 +1206,15 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
             step_of(t, r0, tf, mf, h, sq, sg, plain);
         }
     }
-    bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
+    // a hidden NaN, or a dS past fp16 (values of V in the thousands and more)
+    bool bad = !((float)wild[0] == 0.0f && (float)wild[1] == 0.0f);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bad |= !(fabsf(gk[d][kb][j]) < INFINITY) | !(fabsf(gv[d][kb][j]) < INFINITY);
+    bool again = __any(bad);
     const float back_v = exp2i(-lift), back_k = a.scale * back_v;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -1264,21 +1280,24 @@ bool mfma_ok(const WindowArgs& a) {
     // a tile's rows behind one descriptor
     return (int64_t)a.KV * a.dh * 2 * (BK + 1) < INT32_MAX && (int64_t)a.H * a.dh * 2 * 260 < INT32_MAX;
 }
+// The DH that serves a head size, from `least` on
+uint64_t head_width(int dh, int least) {
+    return dh <= 32 && least <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : dh <= 128 ? 128 : 256;
+}
 template <class F>
 hipError_t by_head64(int dh, F&& f) {
-    if (dh <= 64) f(std::integral_constant<int, 64>{});
-    else if (dh <= 96) f(std::integral_constant<int, 96>{});
-    else if (dh <= 128) f(std::integral_constant<int, 128>{});
-    else f(std::integral_constant<int, 256>{});
+    switch (head_width(dh, 64)) {
+        case 64: f(std::integral_constant<int, 64>{}); break;
+        case 96: f(std::integral_constant<int, 96>{}); break;
+        case 128: f(std::integral_constant<int, 128>{}); break;
+        default: f(std::integral_constant<int, 256>{}); break;
+    }
     return hipGetLastError();
 }
 template <class F>
 hipError_t by_head(int dh, F&& f) {
-    if (dh <= 32) f(std::integral_constant<int, 32>{});
-    else if (dh <= 64) f(std::integral_constant<int, 64>{});
-    else if (dh <= 96) f(std::integral_constant<int, 96>{});
-    else if (dh <= 128) f(std::integral_constant<int, 128>{});
-    else f(std::integral_constant<int, 256>{});
+    if (head_width(dh, 32) > 32) return by_head64(dh, f);
+    f(std::integral_constant<int, 32>{});
     return hipGetLastError();
 }
 
@@ -1316,9 +1335,7 @@ int fwd_splits(int B, int N, int R, int H, int KV, int dh, int window, int sinks
 uint64_t window_fwd_workspace(int B, int N, int R, int H, int KV, int dh, int window, int sinks) {
     if (dh % 8) return 0;
     const int splits = fwd_splits(B, N, R, H, KV, dh, window, sinks);
-    uint64_t row = 0;
-    (void)by_head(dh, [&](auto dhc) { row = (decltype(dhc)::value + 4) * sizeof(float); });
-    return splits > 1 ? (uint64_t)B * N * H * splits * row : 0;
+    return splits > 1 ? (uint64_t)B * N * H * splits * (head_width(dh, 32) + 4) * sizeof(float) : 0;
 }
 
 int window_forward(const WindowArgs& args, void* ws, hipStream_t st) {
@@ -1369,11 +1386,8 @@ Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
     // queries that see a block, in key blocks' lengths: the window, or every later one
     const int64_t span = full == blocks ? blocks : std::min(blocks, ((int64_t)window + keys - 2) / keys + 1);
     auto items = [&](int64_t q) {
-        auto sum = [&](int64_t n) {
-            const int64_t k = n / q;
-            return q * k * (k + 1) / 2 + (n - q * k) * (k + 1);
-        };
-        return sum(blocks) - sum(blocks - full) + (blocks - full) * ((span + q - 1) / q);
+        const Parts p{(int)q, (int)blocks, (int)full, (int)((span + q - 1) / q), 0, 0};
+        return p.before((int)blocks);
     };
     // long parts, as few as make 500 workgroups, two for a CU (2 x 1999 queries of 8 heads over 2 of 128 values, window
     // 512, the whole backward: 250 97 us, 500 84, 1000 97; one sequence of 4000, no window: 245, 203, 208), and fewer
@@ -1405,8 +1419,8 @@ uint64_t window_tops_bytes(int B, int N, int H, int KV, int dh) {
 uint64_t window_bwd_workspace(int B, int N, int H, int KV, int dh, int window, int sinks) {
     if (dh % 8) return 0;
     const Parts p = parts_for(B, N, KV, dh, window, sinks);
-    uint64_t part = 0;
-    (void)by_head64(dh, [&](auto dhc) { part = KvGrad<decltype(dhc)::value>::KEYS * 2 * decltype(dhc)::value * sizeof(float); });
+    static_assert(KvGrad<64>::KEYS == KvGrad<256>::KEYS, "one length of key blocks");
+    const uint64_t part = KvGrad<64>::KEYS * 2 * head_width(dh, 64) * sizeof(float);
     return 2 * window_stats_rows(B, N, H) * sizeof(float) + window_tops_bytes(B, N, H, KV, dh) + (uint64_t)B * KV * p.slots * part;
 }
 

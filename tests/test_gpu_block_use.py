@@ -349,3 +349,59 @@ def test_window_attention_many_rows(dev, b, n, h, kv, dh):
     gb.test_window_attention(dev, b, n, h, kv, dh, n, 0, 100, 5, False)
     gb.test_window_attention(dev, b, n, h, kv, dh, n + 90, 77, 0, 0, False)
     gb.test_window_attention_bwd(dev, b, n, h, kv, dh, n, 0, 100, 5, False)
+
+
+@pytest.mark.parametrize("dh,h,kv,n", [(128, 4, 2, 150), (64, 2, 2, 2000), (256, 1, 1, 70)])
+def test_window_attention_bwd_large_values(dev, dh, h, kv, n):
+    """Values near fp16's largest, and output gradients that point along them: the scores' gradients pass 65504 though no
+    gradient that is asked for does."""
+    r = Rng(dev, dh)
+    q, k = r(1, n, h * dh, std=0.02), r(1, n, kv * dh, std=0.02)
+    v = r(1, n, kv * dh, std=40000.0).clamp_(-60000, 60000)
+    do = v.view(1, n, kv, 1, dh).expand(1, n, kv, h // kv, dh).float()
+    do = (do / do.norm(dim=-1, keepdim=True)).reshape(1, n, h * dh).half()
+    got = gb.window_grads(q, k, v, do, dh, h, 2, 0)
+    w = window_want(q, k, v, h, kv, dh, [0], 2, 0, do)
+    P = 0.5  # two rows of nearly equal scores
+    assert float((do.view(n, h, dh).double() * v.view(n, kv, 1, dh).expand(n, kv, h // kv, dh).reshape(n, h, dh).double()).sum(-1).max()) * P * P > 65504
+    for g, x in zip(got, ("dq", "dk", "dv")):
+        close(g, w[x], w[x + "_t"], x, norm=None)
+
+
+def test_window_attention_bwd_millions_of_positions(dev):
+    """Enough key blocks that the number of their parts, summed, passes 32 bits; the sinks' blocks are joined from parts."""
+    n, dh, window, sinks = 3_200_000, 8, 64, 200
+    r = Rng(dev, 5)
+    q, k, v, do = (r(1, n, dh) for _ in range(4))
+    o, lse = torch.empty_like(q), torch.empty(1, 1, n, device=dev)
+    evk.window_attention(q, k, v, o, dh, window, sinks, lse=lse)
+    dq, dk, dv = (empty(dev, 1, n, dh) for _ in range(3))
+    evk.window_attention_bwd(q, k, v, o, do, dq, dk, dv, lse, dh, window, sinks)
+    Q, K, V, G, O = (t[0].double() for t in (q, k, v, do, o))  # noqa: E741
+    D = (G * O).sum(1)
+    for j in (0, 63, 64, 130, 199, 200, 255, 1_500_000, n - 65, n - 1):
+        first, last = j, n if j < sinks else min(n, j + window)
+        s = Q[first:last] @ K[j] * dh ** -0.5
+        p = torch.exp(s - lse[0, 0, first:last].double())
+        ds = p * (G[first:last] @ V[j] - D[first:last]) * dh ** -0.5
+        for what, g, want, mag in (("dk", dk[0, j], ds @ Q[first:last], (ds.abs() @ Q[first:last].abs())),
+                                   ("dv", dv[0, j], p @ G[first:last], (p.abs() @ G[first:last].abs()))):
+            # P and dS rounded, their exponent's and the sums' errors in 32 bits (a part adds a few hundred thousand
+            # rows, 32 by 32, in order: the error of a term is at most half a step of the sum so far), the result's
+            terms = last - first
+            tol = (H + 2.0 ** -18 + (terms / 32 + 100) * gb.E) * mag + H * want.abs() + gb.T * (1 + terms * 2.0 ** -10)
+            assert ((g.double() - want).abs() <= tol).all(), (what, j, g, want, tol)
+
+
+def test_empty_cache(dev):
+    """No row in the cache: nothing is written, nothing is seen."""
+    b, n, h, kv, dh = 2, 3, 4, 2, 64
+    r = Rng(dev, 1)
+    off = torch.zeros(b, dtype=torch.int32, device=dev)
+    x, q = r(b, n, (h + 2 * kv) * dh), empty(dev, b, n, h * dh)
+    k, v = torch.empty(b, 0, kv * dh, dtype=F16, device=dev), torch.empty(b, 0, kv * dh, dtype=F16, device=dev)
+    evk.qkv_norm_rope(x, q, k, v, dh, offsets=off)
+    o, lse = empty(dev, b, n, h * dh), torch.zeros(b, h, n, device=dev)
+    evk.window_attention(q, k, v, o, dh, 4, 1, offsets=off, lse=lse)
+    assert (o == 0).all() and (lse == -math.inf).all()
+    assert torch.isfinite(q).all() and (q != 7.0).any()
