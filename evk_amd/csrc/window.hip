@@ -1379,7 +1379,7 @@ int window_forward(const WindowArgs& args, void* ws, hipStream_t st) {
 }
 
 namespace {
-Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
+Parts parts_for(int B, int N, int H, int KV, int dh, int window, int sinks) {
     const int64_t keys = dh <= 128 ? KvGrad<128>::KEYS : KvGrad<256>::KEYS, heads = (int64_t)B * KV;
     const int64_t blocks = (N + keys - 1) / keys;
     const int64_t full = window >= N ? blocks : std::min<int64_t>(blocks, ((int64_t)sinks + keys - 1) / keys);
@@ -1390,10 +1390,11 @@ Parts parts_for(int B, int N, int KV, int dh, int window, int sinks) {
         return p.before((int)blocks);
     };
     // long parts, as few as make 500 workgroups, two for a CU (2 x 1999 queries of 8 heads over 2 of 128 values, window
-    // 512, the whole backward: 250 97 us, 500 84, 1000 97; one sequence of 4000, no window: 245, 203, 208), and fewer
-    // than 2^24
+    // 512, the whole backward: 250 97 us, 500 84, 1000 97; one sequence of 4000, no window: 245, 203, 208), none of
+    // under 128 rows (one sequence of 4000, 2 heads over 1 of 64 values, window 512: 50.1 us, with this limit 40.0;
+    // 2000, one head of 128, no window: 67.5, 58.9), and fewer than 2^24
     int64_t q = full == blocks ? std::max<int64_t>(1, span / 4) : span;
-    while (q > 1 && items(q) * heads < 500) q /= 2;
+    while (q > 1 && items(q) * heads < 500 && q * keys * (H / KV) > 256) q /= 2;
     while (items(q) * heads > (1 << 24) && q < blocks) q *= 2;
     Parts p{};
     p.q = (int)q;
@@ -1418,7 +1419,7 @@ uint64_t window_tops_bytes(int B, int N, int H, int KV, int dh) {
 
 uint64_t window_bwd_workspace(int B, int N, int H, int KV, int dh, int window, int sinks) {
     if (dh % 8) return 0;
-    const Parts p = parts_for(B, N, KV, dh, window, sinks);
+    const Parts p = parts_for(B, N, H, KV, dh, window, sinks);
     static_assert(KvGrad<64>::KEYS == KvGrad<256>::KEYS, "one length of key blocks");
     const uint64_t part = KvGrad<64>::KEYS * 2 * head_width(dh, 64) * sizeof(float);
     return 2 * window_stats_rows(B, N, H) * sizeof(float) + window_tops_bytes(B, N, H, KV, dh) + (uint64_t)B * KV * p.slots * part;
@@ -1450,7 +1451,7 @@ int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
             }
             hipLaunchKernelGGL((window_dq<DH, 1>), grid, dim3(256), 0, st, a, tiles, stats, srows, tops);
         });
-        const Parts p = parts_for(a.B, a.N, a.KV, a.dh, a.window, a.sinks);
+        const Parts p = parts_for(a.B, a.N, a.H, a.KV, a.dh, a.window, a.sinks);
         if (e == hipSuccess)
             e = by_head64(a.dh, [&](auto dhc) {
                 constexpr int DH = decltype(dhc)::value, KEYS = KvGrad<DH>::KEYS;
