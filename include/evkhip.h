@@ -305,6 +305,8 @@ int evkhip_embed_backward(const evkhip_tensor* grad_out, const evkhip_tensor* in
  * workspaces do not overlap may run at the same time, and a captured call uses
  * the workspace it was captured with.  Outputs may not overlap inputs, each
  * other or the workspace (EVKHIP_ERR_INVALID_ARG).
+ * More than 2^30 rows of heads, or a launch of more than 2^32 threads, are
+ * EVKHIP_ERR_UNSUPPORTED.  No atomics: results repeat bit for bit.
  * ------------------------------------------------------------------------- */
 
 /* Norms of queries and keys for each head with the position rotation, the
