@@ -84,11 +84,11 @@ DEV void store_n(f16* p, int n, const float* x) {
 // 7996 tokens above took 17 us.
 struct Angles {
     float cs[4], sn[4];
-    DEV void set(const Turns& tn, int i0, int p) {
+    DEV void set(const Turns& tn, int i0, int64_t p) {
         double f = tn.unit;
 #pragma unroll
         for (int k = 2; k < 7; ++k) f *= (i0 >> (k + 1)) & 1 ? tn.r[k] : 1.0;
-        const double p0 = f * p, p1 = p0 * tn.r[0];
+        const double p0 = f * (double)p, p1 = p0 * tn.r[0];
         const double t[4] = {p0, p1, p0 * tn.r[1], p1 * tn.r[1]};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -117,8 +117,7 @@ __global__ __launch_bounds__(256) void qkv_rope_k(QkvRopeArgs a, Turns tn, int p
     const int b = (int)(token / a.N), t = (int)(token % a.N);
     const int g0 = (int)(w % splits) * per, g1 = min(g0 + per, (HT + HPW - 1) / HPW);
     const int i0 = (lane % LPH) * 8, n = min(8, dh - i0);
-    const int64_t p64 = (int64_t)(a.offsets ? a.offsets[b] : a.p0) + t;
-    const int p = (int)(p64 < INT32_MAX ? p64 : INT32_MAX);
+    const int64_t p = (int64_t)(a.offsets ? a.offsets[b] : a.p0) + t;  // past 2^31 for the last offsets
     Angles ang;
     ang.set(tn, i0, p);
     float wq[8], wk[8];
