@@ -17,6 +17,7 @@ using namespace evkhip;
 namespace {
 
 constexpr uint32_t kMaxRows = 1u << 30;  // positions, rows, tokens: 32-bit arithmetic with room
+static_assert(kMaxRows <= WINDOW_MOST, "no window");
 
 bool same_dims(const evkhip_tensor* a, const evkhip_tensor* b) {
     if (a->rank != b->rank) return false;
@@ -101,6 +102,7 @@ int check_norm(const char* op, float eps, float base) {
 }
 
 int clamp_int(uint32_t v) { return v > (uint32_t)INT32_MAX ? INT32_MAX : (int)v; }
+int window_rows(uint32_t window) { return (int)(window && window < WINDOW_MOST ? window : WINDOW_MOST); }
 
 // Whether the call takes these sizes; those that it refuses need no workspace.
 bool window_sizes(uint32_t B, uint32_t N, uint32_t R, uint32_t H, uint32_t KV, uint32_t dh) {
@@ -116,7 +118,8 @@ WindowArgs window_args(const Heads& s, uint32_t dh, uint32_t window, uint32_t si
     a.KV = (int)s.KV;
     a.R = (int)s.R;
     a.dh = (int)dh;
-    a.window = window ? clamp_int(window) : INT32_MAX;
+    a.window = window_rows(window);
+    a.far = window ? (int64_t)window - a.window : 1LL << 40;
     a.sinks = clamp_int(sinks);
     a.scale = 1.0f / sqrtf((float)dh);
     return a;
@@ -259,7 +262,7 @@ uint64_t evkhip_window_attention_workspace(uint32_t batch, uint32_t n, uint32_t 
                                            uint32_t kv_heads, uint32_t head_dim, uint32_t window, uint32_t sinks) {
     if (!window_sizes(batch, n, rows, heads, kv_heads, head_dim)) return 0;
     return window_fwd_workspace((int)batch, (int)n, (int)rows, (int)heads, (int)kv_heads, (int)head_dim,
-                                window ? clamp_int(window) : INT32_MAX, clamp_int(sinks));
+                                window_rows(window), clamp_int(sinks));
 }
 
 int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,
@@ -293,7 +296,7 @@ uint64_t evkhip_window_attention_bwd_workspace(uint32_t batch, uint32_t n, uint3
                                                uint32_t head_dim, uint32_t window, uint32_t sinks) {
     if (!window_sizes(batch, n, n, heads, kv_heads, head_dim)) return 0;
     return window_bwd_workspace((int)batch, (int)n, (int)heads, (int)kv_heads, (int)head_dim,
-                                window ? clamp_int(window) : INT32_MAX, clamp_int(sinks));
+                                window_rows(window), clamp_int(sinks));
 }
 
 int evkhip_window_attention_bwd(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,

@@ -169,6 +169,7 @@ uint64_t qkv_rope_bwd_workspace(uint64_t tokens, int dh);
 int qkv_rope_backward(const QkvRopeArgs& a, float* part, hipStream_t st);  // part: that workspace, or null
 
 // ---- window.hip ----
+constexpr uint32_t WINDOW_MOST = 1u << 30;  // no cache holds more rows
 struct WindowArgs {
     const f16 *q, *k, *v;   // (B, N, H dh), (B, R, KV dh) twice
     const f16 *o, *dO;      // backward
@@ -176,7 +177,8 @@ struct WindowArgs {
     float* lse;             // (B, H, N), null where the forward's caller wants none
     const int* offsets;     // (B) positions of the first queries, or null: p0
     int B, N, H, KV, R, dh, p0;
-    int window, sinks;      // window: INT32_MAX for none
+    int window, sinks;      // window: at most WINDOW_MOST
+    int64_t far;            // rows by which the caller's window is longer; 2^40 for no window
     float scale;
     int big;                // MFMA kernels: a sequence's rows of K pass 2 GiB
 };

@@ -39,9 +39,14 @@ DEV Span span_of(int p, const WindowArgs& a) {
     v.s = min(a.sinks, v.lo);
     return v;
 }
-// Position of query t of sequence b, -1 for any that sees nothing.
+// Position of query t of sequence b, -1 for any that sees nothing.  Windows
+// longer than any cache (R <= 2^30 = WINDOW_MOST) run as ones of 2^30 rows, with
+// positions moved down by the difference (`far`) where the window starts past
+// row 0, so that neither a position nor the end of its window passes 32 bits;
+// other positions past 2^31 - 1 see what that one sees, the sinks.
 DEV int position_of(const WindowArgs& a, int b, int t) {
-    const int64_t p = (int64_t)(a.offsets ? a.offsets[b] : a.p0) + t;
+    int64_t p = (int64_t)(a.offsets ? a.offsets[b] : a.p0) + t;
+    if (a.far) p = max(min(p, (int64_t)a.R - 1), p - a.far);
     return (int)(p < 0 ? -1 : p < INT32_MAX ? p : INT32_MAX);
 }
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import evk_amd as evk
-from test_gpu_block import H, T, Rng, close, empty, rope_want
+from test_gpu_block import H, T, Rng, close, empty, rope_want, window_want
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +27,20 @@ def test_qkv_norm_rope_far_positions(dev):
     # formula in 64 bits
     close(q.view(b, n, h, dh), y[:, :, :h], H * y[:, :, :h].abs() + (2.0 ** -20 + 8 * 2.0 ** -22) * size[:, :, :h] + T, "q")
     assert (k[:2] == 7.0).all() and (v[:2] == 7.0).all(), "rows that the cache does not have"
+
+
+@pytest.mark.parametrize("dh,h,kv", [(64, 4, 2), (128, 4, 1), (256, 2, 1), (33, 2, 1)])
+@pytest.mark.parametrize("n,rows", [(1, 40), (3, 700), (70, 90)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (0, 3), (2 ** 31 - 5, 0), (2 ** 31 + 1, 2), (2 ** 32 - 1, 0), (50, 2)])
+def test_window_attention_far_positions(dev, dh, h, kv, n, rows, window, sinks):
+    """Positions next to 2^31 and past it: no window shows every row, a window as long as that cuts where it should."""
+    b = 3
+    r = Rng(dev, 22 + dh + n)
+    q, k, v = r(b, n, h * dh), r(b, rows, kv * dh), r(b, rows, kv * dh)
+    off = torch.tensor([2 ** 31 - 1, 2 ** 31 - 2 - n // 2, rows - n], dtype=torch.int32, device=dev)
+    o, lse = empty(dev, b, n, h * dh), torch.full((b, h, n), 7.0, device=dev)
+    evk.window_attention(q, k, v, o, dh, window, sinks, 0, off, lse)
+    w = window_want(q, k, v, h, kv, dh, off.tolist(), window, sinks)
+    none = torch.isinf(w["lse"])
+    close(o, w["o"], w["o_t"], "o")
+    close(lse, w["lse"], torch.where(none, torch.zeros_like(w["lse"]), w["lse_t"]), "lse", norm=None)
