@@ -5,7 +5,8 @@
 // Query t of sequence b stands at position p = p0 + t and sees the rows
 //   [0, s) and [lo, hi)   with hi = min(p + 1, rows), lo = max(0, p - W + 1),
 //                              s = min(sinks, lo)
-// of its K and V; a query that sees nothing (p < 0) has O = 0, LSE = -inf.
+// of its K and V; a query that sees nothing (p < 0) has O = 0, LSE = -inf.  One
+// whose scores are all -inf has no softmax: O = NaN, LSE = -inf.
 //   S = Q K^T / sqrt(Dh), P = exp(S - LSE), O = P V
 //   backward: D = rowsum(dO * O), dS = P (dO V^T - D),
 //             dQ = dS K / sqrt(Dh), dK = dS^T Q / sqrt(Dh), dV = P^T dO,
@@ -92,7 +93,7 @@ DEV void fwd_row(const WindowArgs& a, int64_t row, RowLds& s, int lane) {
         const float sc = lane < n ? dot_row(a.k + kv0 + j, s.x, dh) * a.scale * kLog2e : -INFINITY;
         const float m_new = fmaxf(m, wave_max(sc));
         const float keep = m == -INFINITY ? 0.0f : exp2f(m - m_new);
-        const float e = lane < n ? exp2f(sc - m_new) : 0.0f;
+        const float e = lane < n ? exp2f(sc - (m_new == -INFINITY ? 0.0f : m_new)) : 0.0f;
         l = l * keep + wave_sum(e);
         m = m_new;
         s.p[lane] = e;
@@ -584,7 +585,9 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int r = wr0 + 16 * q + l16;
-        const float l = query_sum(sm.l[q]), inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float l = query_sum(sm.l[q]);
+        const bool none = span_of(qp[q], a).count() == 0;
+        const float inv = none ? 0.0f : 1.0f / l;
         if (r >= NR) continue;
         f16* dst = a.out + row_at(r);
 #pragma unroll
@@ -593,7 +596,7 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
                 *reinterpret_cast<uint2*>(dst + 16 * d + 4 * g) =
                     uint2{pack_h2(sm.o[d][q][0] * inv, sm.o[d][q][1] * inv), pack_h2(sm.o[d][q][2] * inv, sm.o[d][q][3] * inv)};
         if (a.lse && g == 0)
-            a.lse[((int64_t)b * a.H + c * group + r % group) * a.N + r / group] = l == 0.0f ? -INFINITY : (sm.m[q] + log2f(l)) * kLn2;
+            a.lse[((int64_t)b * a.H + c * group + r % group) * a.N + r / group] = none ? -INFINITY : (sm.m[q] + log2f(l)) * kLn2;
     }
     static_assert(4 * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
     const bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
@@ -737,11 +740,12 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
             continue;
         }
         const int64_t at_row = ((int64_t)b * a.N + row / group) * a.H + c * group + row % group;
-        const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+        const bool none = span_of(position_of(a, b, row / group), a).count() == 0;
+        const float inv = none ? 0.0f : 1.0f / ls;
         if (d < a.dh)
             *reinterpret_cast<uint2*>(a.out + at_row * a.dh + d) = uint2{pack_h2(o[0] * inv, o[1] * inv), pack_h2(o[2] * inv, o[3] * inv)};
         if (a.lse && d == 0)
-            a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = ls == 0.0f ? -INFINITY : (m + log2f(ls)) * kLn2;
+            a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = none ? -INFINITY : (m + log2f(ls)) * kLn2;
     }
     if (splits > 1 || !any_again) return;
     __syncthreads();
@@ -787,7 +791,8 @@ __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int split
     for (int i = 0; i < PER; ++i) part[wave][lane + 64 * i] = o[i];
     __syncthreads();
     const int64_t at = ((int64_t)b * a.N + row / group) * a.H + c * group + row % group;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const bool none = span_of(position_of(a, b, row / group), a).count() == 0;
+    const float inv = none ? 0.0f : 1.0f / l;
     bool bad = !(fabsf(l) < INFINITY);
     for (int d = tid; d < a.dh; d += 256) {
         const float v = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
@@ -795,7 +800,7 @@ __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int split
         a.out[at * a.dh + d] = (f16)(v * inv);
     }
     if (a.lse && tid == 0)
-        a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = none ? -INFINITY : (m + log2f(l)) * kLn2;
     if (__syncthreads_or(bad) && wave == 0) fwd_row(a, at, lds, lane);
 }
 

@@ -345,8 +345,9 @@ int evkhip_qkv_norm_rope_backward(const evkhip_tensor* qkv, const evkhip_tensor*
  * position_offset is 0), and sees the rows j <= p with j > p - window or
  * j < sinks; window 0 shows every row up to p.  Rows that a query does not see
  * do not reach its output, whatever they hold.  A query that sees no row (an
- * offset below 0) has output 0 and log-sum-exp -inf.  lse: NULL or fp32
- * (B,H,N).  N == 1 is a decode step.  head_dim up to 256. */
+ * offset below 0) has output 0 and log-sum-exp -inf; one whose scores are all
+ * -inf has output NaN (it has no softmax) and log-sum-exp -inf.  lse: NULL or
+ * fp32 (B,H,N).  N == 1 is a decode step.  head_dim up to 256. */
 uint64_t evkhip_window_attention_workspace(uint32_t batch, uint32_t n, uint32_t rows, uint32_t heads,
                                            uint32_t kv_heads, uint32_t head_dim, uint32_t window, uint32_t sinks);
 int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,

@@ -2,11 +2,13 @@
 next to 2^31, scores that are all -inf, NaN and infinities beside finite rows, long
 contexts, gradients of every size.  Tolerances as in test_gpu_block.py: H is half
 a step of fp16, T of its subnormals, E of 32 bits."""
+import math
+
 import pytest
 import torch
 
 import evk_amd as evk
-from test_gpu_block import H, T, Rng, close, empty, rope_want, window_want
+from test_gpu_block import F64, H, T, Rng, close, empty, rope_want, seen, window_want
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +46,73 @@ def test_window_attention_far_positions(dev, dh, h, kv, n, rows, window, sinks):
     none = torch.isinf(w["lse"])
     close(o, w["o"], w["o_t"], "o")
     close(lse, w["lse"], torch.where(none, torch.zeros_like(w["lse"]), w["lse_t"]), "lse", norm=None)
+
+
+# ---------------------------------------------------------------------------
+# scores of -inf
+# ---------------------------------------------------------------------------
+def plain_want(q, k, v, h, kv, dh, p0, window, sinks):
+    """o and lse by the definition in 64 bits, whatever visible rows hold (hidden rows of v have to be finite)."""
+    b, n, _ = q.shape
+    o, lse = [], []
+    for s in range(b):
+        m = seen(p0 + torch.arange(n, device=q.device), k.shape[1], window, sinks)
+        for hd in range(h):
+            at, to = slice(hd * dh, hd * dh + dh), slice(hd // (h // kv) * dh, hd // (h // kv) * dh + dh)
+            sc = torch.where(m, q[s, :, at].to(F64) @ k[s, :, to].to(F64).t() * dh ** -0.5, torch.full((), -math.inf, dtype=F64, device=q.device))
+            o.append(torch.softmax(sc, 1) @ v[s, :, to].to(F64))
+            lse.append(torch.logsumexp(sc, 1))
+    return torch.stack(o).view(b, h, n, dh).transpose(1, 2).reshape(b, n, h * dh), torch.stack(lse).view(b, h, n)
+
+
+HEADS = [(64, 4, 2), (128, 4, 1), (256, 2, 1), (80, 2, 2), (33, 2, 1)]
+
+
+@pytest.mark.parametrize("dh,h,kv", HEADS)
+@pytest.mark.parametrize("b,n,rows,p0,window", [(1, 1, 1, 0, 0), (2, 1, 30, 20, 1), (1, 20, 20, 0, 1), (1, 150, 150, 0, 70), (9, 300, 300, 0, 70),
+                                               (1, 1, 20000, 19999, 0), (1, 2, 20000, 19990, 0)])
+def test_window_attention_scores_of_minus_infinity(dev, dh, h, kv, b, n, rows, p0, window):
+    """K that overflowed in its leading rows: a query that sees no other row has no softmax (NaN, log-sum-exp -inf), one
+    that sees a finite score too has that of the finite ones."""
+    r = Rng(dev, 30 + dh)
+    q, k, v = r(b, n, h * dh), r(b, rows, kv * dh), r(b, rows, kv * dh)
+    q.view(b, n, h, dh)[..., 0] = 1.0
+    for lead in sorted({min(rows, 80), rows - 3, rows} - {0}):
+        if lead <= 0:
+            continue
+        kk = k.clone()
+        kk.view(b, rows, kv, dh)[:, :lead, :, 0] = -math.inf
+        o, lse = empty(dev, b, n, h * dh), torch.full((b, h, n), 7.0, device=dev)
+        evk.window_attention(q, kk, v, o, dh, window, 0, p0, lse=lse)
+        ow, lw = plain_want(q, kk, v, h, kv, dh, p0, window, 0)
+        # what remains is the softmax of the finite rows, with the roundings of any other
+        t = window_want(q, k, v, h, kv, dh, [p0] * b, window, 0)
+        few = 2 * (2 * H + 2.0 ** -16) * v.abs().max().to(F64)  # as o_t, whatever weights the finite rows have
+        close(o, ow, t["o_t"] + few, f"o, {lead} rows", norm=None)
+        close(lse, lw, t["lse_t"] + 2.0 ** -19, f"lse, {lead} rows", norm=None)
+        sees = seen(p0 + torch.arange(n, device=dev), rows, window, 0)
+        dead = ~sees[:, lead:].any(1)
+        assert torch.isnan(o[:, dead]).all() and torch.isfinite(o[:, ~dead]).all()
+
+
+@pytest.mark.parametrize("dh,h,kv", HEADS)
+def test_window_attention_bwd_scores_of_minus_infinity(dev, dh, h, kv):
+    """The gradients of a query without a softmax are NaN; rows that no such query sees keep theirs."""
+    b, n, window = 1, 200, 20
+    r = Rng(dev, 33 + dh)
+    q, k, v, do = r(b, n, h * dh), r(b, n, kv * dh), r(b, n, kv * dh), r(b, n, h * dh)
+    q.view(b, n, h, dh)[..., 0] = 1.0
+    k.view(b, n, kv, dh)[:, :40, :, 0] = -math.inf
+    o, lse = torch.empty_like(q), torch.empty(b, h, n, device=dev)
+    evk.window_attention(q, k, v, o, dh, window, 0, lse=lse)
+    dq, dk, dv = (torch.empty_like(t) for t in (q, k, v))
+    evk.window_attention_bwd(q, k, v, o, do, dq, dk, dv, lse, dh, window, 0)
+    assert torch.isnan(dq[:, :40]).all()
+    far = 40 + window  # queries from here on see finite rows only
+    assert torch.isnan(dk[:, :40]).any(-1).all() and torch.isnan(dv[:, :40]).any(-1).all()
+    fin = k.clone()
+    fin.view(b, n, kv, dh)[:, :40, :, 0] = -100.0
+    w = window_want(q, fin, v, h, kv, dh, [0], window, 0, do)
+    close(dq[:, far:], w["dq"][:, far:], w["dq_t"][:, far:], "dq")
+    for g, x in ((dk, "dk"), (dv, "dv")):
+        close(g[:, far:], w[x][:, far:], w[x + "_t"][:, far:], x)
