@@ -804,30 +804,43 @@ __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int split
     if (__syncthreads_or(bad) && wave == 0) fwd_row(a, at, lds, lane);
 }
 
-// dS is rounded to fp16 for its products.  |dS| <= P |dO| (|V| + |O|), so that
-// output gradients as small as those of a mean over a batch would leave it a
-// few bits of fp16's subnormals.  P therefore carries a power of two that
-// leaves the sums at the end: for dQ one for each query, which makes its dO
-// about as long as 1; for dK and dV one for all queries of a sum, by the longest
-// (each wave of window_dq leaves its rows'), so that dO is about 4 long, within
-// what fp16 holds of P itself: 2^12 P is at most 4096, and P / 4 loses nothing
-// down to 2^-12.
-constexpr int LONG = 2, MOST = 12, LEAST = -2;
-constexpr int K_LEAST = -24;  // of rows that are zero
+// P and dS are rounded to fp16 for their products, which has 30 powers of two
+// above its subnormals: P of a flat row of n is 1 / n, dS follows the lengths of
+// the output's gradient.  Both therefore carry powers of two that leave the sums
+// at the end.
+//   dV: P is at most 1 and carries 2^P_LIFT: full precision down to 2^-29.
+//   dK: |dS| <= P |dO| (|V| + |O|), Cauchy-Schwarz.  Each wave bounds that by its
+//       own keys' V and by the largest |dO| and |dO| |O| among its queries, which
+//       window_dq leaves, and takes that bound to 2^DS_TOP: nothing overflows.
+//   dQ: |dS| <= |dO| max |V_i - V_j| / 4, and V is not known before it is read: a
+//       query's dO is made shorter than 1 and dS lifted by 2^DQ_LIFT.  A query
+//       whose sums overflow (V longer than some hundreds, along dO) is done again
+//       with DQ_STEP less, and once more: at 2^-4 no V of fp16 overflows.
+// One power for both products of dK and dV, set by |dO| alone, and none for dS
+// in dQ, lost bits from 16k rows on (131072 rows of one head of 64, no window: the
+// later half of dQ off by 4.8 H of its norm and that of dV by 14, H half a step of
+// fp16; now 0.6 both, at any length).
+constexpr int P_LIFT = 15, DS_TOP = 14, DQ_LIFT = 10, DQ_STEP = 7;
+constexpr int K_LEAST = -24;  // of rows that are zero, or not finite (those spoil what they are part of at any power)
 DEV float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+typedef short short2_t __attribute__((ext_vector_type(2)));  // a pair of exponents
+DEV short2_t max_xor(short2_t v, int o) {
+    return __builtin_elementwise_max(v, __builtin_bit_cast(short2_t, __shfl_xor(__builtin_bit_cast(int, v), o, 64)));
+}
 DEV int length_exponent(float squares) {  // |x| < 2^k
-    return squares > 0.0f ? (__builtin_amdgcn_frexp_expf(squares) + 1) >> 1 : K_LEAST;
+    return (squares > 0.0f) & (squares < INFINITY) ? (__builtin_amdgcn_frexp_expf(squares) + 1) >> 1 : K_LEAST;
 }
 
 // Backward, dQ and the rows' statistics.  Workgroup as in the forward:
 //   S^T = K Q^T, dP^T = V dO^T, P = 2^(S c - lse), dS = P (dP - D),
 //   dQ^T += K^T dS^T (K^T by transposed reads of the same tile),
 // Stores -lse / scale and -D of every row, flat by key head (`rows` of each),
-// and the largest length exponent of each wave's rows for the kernel of dK and dV.
+// and the largest length exponents of dO and of dO times O among each wave's rows
+// for the kernel of dK and dV.
 // Bound as the forward is, with three products for two: 2 x 1999 queries of 8
 // heads over 2 of 128 values, window 512, 25 us (504 workgroups, two for a CU).
 template <int DH, int QB>
-__global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a, int tiles, float* stats, int64_t rows, int* tops) {
+__global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a, int tiles, float* stats, int64_t rows, short2_t* tops) {
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, TILE = BK * W, ROWS = 64 * QB;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
@@ -845,7 +858,8 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
     half8 qf[QB][KS], gf[QB][KS];
     int qp[QB];
     float lse2[QB], dsum[QB];
-    int lift[QB], top = K_LEAST;
+    int lift[QB];
+    short2_t top = {K_LEAST, 2 * K_LEAST};
     const int64_t q0 = ((int64_t)b * a.N * a.H + c * group) * a.dh;
     auto row_at = [&](int r) { return q0 + ((int64_t)(r / group) * a.H + r % group) * a.dh; };
 #pragma unroll
@@ -853,107 +867,138 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
         const int r = min(wr0 + 16 * q + l16, NR - 1);
         qp[q] = r / group;
         const float lse = a.lse[((int64_t)b * a.H + c * group + r % group) * a.N + r / group];
-        float sum = 0.0f, squares = 0.0f;
+        half8 of[KS];
+        const int64_t src = row_at(r) + 8 * g;
+        const f16 *q_at = a.q + src, *g_at = a.dO + src, *o_at = a.o + src;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            half8 of = {};
-            qf[q][ks] = gf[q][ks] = half8{};
+            qf[q][ks] = gf[q][ks] = of[ks] = half8{};
             if (32 * ks + 8 * g < a.dh) {
-                const int64_t src = row_at(r) + 32 * ks + 8 * g;
-                qf[q][ks] = *reinterpret_cast<const half8*>(a.q + src);
-                gf[q][ks] = *reinterpret_cast<const half8*>(a.dO + src);
-                of = *reinterpret_cast<const half8*>(a.o + src);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                sum += (float)gf[q][ks][i] * (float)of[i];
-                squares += (float)gf[q][ks][i] * (float)gf[q][ks][i];
+                qf[q][ks] = *reinterpret_cast<const half8*>(q_at + 32 * ks);
+                gf[q][ks] = *reinterpret_cast<const half8*>(g_at + 32 * ks);
+                of[ks] = *reinterpret_cast<const half8*>(o_at + 32 * ks);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);  // every load out before the first sum waits
+        float sum = 0.0f, squares = 0.0f, o_squares = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sum += (float)gf[q][ks][i] * (float)of[ks][i];
+                squares += (float)gf[q][ks][i] * (float)gf[q][ks][i];
+                o_squares += (float)of[ks][i] * (float)of[ks][i];
+            }
         dsum[q] = query_sum(sum);
         if (g == 0 && wr0 + 16 * q + l16 < NR) {
             stats[(int64_t)bc * NR + r] = -lse / a.scale;
             stats[rows + (int64_t)bc * NR + r] = -dsum[q];
         }
-        lift[q] = length_exponent(query_sum(squares));
+        const int kg = length_exponent(query_sum(squares)), ko = length_exponent(query_sum(o_squares));
+        lift[q] = kg - DQ_LIFT;
         lse2[q] = lse * kLog2e + (float)lift[q];  // into P
-        top = max(top, lift[q]);
+        top = __builtin_elementwise_max(top, short2_t{(short)kg, (short)(kg + ko)});
     }
-    top = (int)wave_max((float)top);
+    for (int o = 32; o > 0; o >>= 1) top = max_xor(top, o);
     if (lane == 0) tops[((int64_t)bc * tiles + tile) * 4 + wave] = top;
     const float c2 = a.scale * kLog2e;
     floatx4 acc[DT][QB];
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int q = 0; q < QB; ++q) acc[d][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     half2_t wild = {(f16)0.0f, (f16)0.0f};
-    for (int t = 0; t < nt; ++t) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
-        __syncthreads();                     // everyone's; the other stage is free
-        f16* const sk = smem + (t & 1) * 2 * TILE;
-        f16* const sv = sk + TILE;
-        if (t + 1 < nt) {
-            f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
-            kv.load(list, (t + 1) * BK, nx, nx + TILE);
+    auto store = [&] {
+        int at_lane = lane;
+        asm volatile("" : "+v"(at_lane));  // places formed here, not kept from before the loop
+        const int l16 = at_lane & 15, g = at_lane >> 4;
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+            const int r = wr0 + 16 * q + l16;
+            if (r >= NR) continue;
+            f16* dst = a.out + row_at(r);
+            const float back = __builtin_ldexpf(a.scale, lift[q]);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                if (16 * d + 4 * g < a.dh)
+                    *reinterpret_cast<uint2*>(dst + 16 * d + 4 * g) =
+                        uint2{pack_h2(acc[d][q][0] * back, acc[d][q][1] * back), pack_h2(acc[d][q][2] * back, acc[d][q][3] * back)};
         }
-        using Rows = Ring<2 * KS, 2>;
-        using Cols = Ring<DT, 2>;
-        half8 kf[Rows::SLOTS], vf[Rows::SLOTS], kt[Cols::SLOTS];
-#pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-            auto row = [&](auto i, auto slot) {
-                kf[slot] = fr.row(sk, 32 * k2 + 16 * (i / KS), i % KS);
-                vf[slot] = fr.row(sv, 32 * k2 + 16 * (i / KS), i % KS);
-            };
-            auto col = [&](auto i, auto slot) { kt[slot] = fr.col(sk, 32 * k2, i); };
-            floatx4 s[2][QB], dp[2][QB];
-            Rows::template start<2>(row);
-            Rows::template run<2 * QB, 2>(row, [&](auto i, auto slot) {
-#pragma unroll
-                for (int q = 0; q < QB; ++q) {
-                    const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                    s[i / KS][q] = mfma16(kf[slot], qf[q][i % KS], i % KS ? s[i / KS][q] : zero);
-                    dp[i / KS][q] = mfma16(vf[slot], gf[q][i % KS], i % KS ? dp[i / KS][q] : zero);
-                }
-            });
-            const bool plain = list.plain(a, t * BK + 32 * k2, 32);  // workgroup-uniform
-            half8 ds[QB];
-#pragma unroll
-            for (int q = 0; q < QB; ++q) {
-                float e[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][q][i % 4], c2, -lse2[q]));
-                    e[i] = p * (dp[i / 4][q][i % 4] - dsum[q]);
-                }
-                if (!plain) {
-                    const Seen see(a, list, qp[q]);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) e[i] = see(t * BK + 32 * k2 + 16 * (i / 4) + 4 * g + i % 4) ? e[i] : 0.0f;
-                }
-                ds[q] = as_half8(u32x4{pack_h2(e[0], e[1]), pack_h2(e[2], e[3]), pack_h2(e[4], e[5]), pack_h2(e[6], e[7])});
-            }
-            if (!plain)
-                for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sk, 32 * k2, d), wild);
-            Cols::template start<2>(col);
-            Cols::template run<QB, 2>(col, [&](auto i, auto slot) {
-#pragma unroll
-                for (int q = 0; q < QB; ++q) acc[i][q] = mfma16(kt[slot], ds[q], acc[i][q]);
-            });
-        }
-    }
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        const int r = wr0 + 16 * q + l16;
-        if (r >= NR) continue;
-        f16* dst = a.out + row_at(r);
-        const float back = __builtin_ldexpf(a.scale, lift[q]);
+    };
+    for (int left = DQ_LIFT;; left -= DQ_STEP) {
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-            if (16 * d + 4 * g < a.dh)
-                *reinterpret_cast<uint2*>(dst + 16 * d + 4 * g) =
-                    uint2{pack_h2(acc[d][q][0] * back, acc[d][q][1] * back), pack_h2(acc[d][q][2] * back, acc[d][q][3] * back)};
+#pragma unroll
+            for (int q = 0; q < QB; ++q) acc[d][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < nt; ++t) {
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
+            __syncthreads();                     // everyone's; the other stage is free
+            f16* const sk = smem + (t & 1) * 2 * TILE;
+            f16* const sv = sk + TILE;
+            if (t + 1 < nt) {
+                f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
+                kv.load(list, (t + 1) * BK, nx, nx + TILE);
+            }
+            using Rows = Ring<2 * KS, 2>;
+            using Cols = Ring<DT, 2>;
+            half8 kf[Rows::SLOTS], vf[Rows::SLOTS], kt[Cols::SLOTS];
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) {
+                auto row = [&](auto i, auto slot) {
+                    kf[slot] = fr.row(sk, 32 * k2 + 16 * (i / KS), i % KS);
+                    vf[slot] = fr.row(sv, 32 * k2 + 16 * (i / KS), i % KS);
+                };
+                auto col = [&](auto i, auto slot) { kt[slot] = fr.col(sk, 32 * k2, i); };
+                floatx4 s[2][QB], dp[2][QB];
+                Rows::template start<2>(row);
+                Rows::template run<2 * QB, 2>(row, [&](auto i, auto slot) {
+#pragma unroll
+                    for (int q = 0; q < QB; ++q) {
+                        const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                        s[i / KS][q] = mfma16(kf[slot], qf[q][i % KS], i % KS ? s[i / KS][q] : zero);
+                        dp[i / KS][q] = mfma16(vf[slot], gf[q][i % KS], i % KS ? dp[i / KS][q] : zero);
+                    }
+                });
+                const bool plain = list.plain(a, t * BK + 32 * k2, 32);  // workgroup-uniform
+                half8 ds[QB];
+#pragma unroll
+                for (int q = 0; q < QB; ++q) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][q][i % 4], c2, -lse2[q]));
+                        e[i] = p * (dp[i / 4][q][i % 4] - dsum[q]);
+                    }
+                    if (!plain) {
+                        const Seen see(a, list, qp[q]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) e[i] = see(t * BK + 32 * k2 + 16 * (i / 4) + 4 * g + i % 4) ? e[i] : 0.0f;
+                    }
+                    ds[q] = as_half8(u32x4{pack_h2(e[0], e[1]), pack_h2(e[2], e[3]), pack_h2(e[4], e[5]), pack_h2(e[6], e[7])});
+                }
+                if (!plain)
+                    for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sk, 32 * k2, d), wild);
+                Cols::template start<2>(col);
+                Cols::template run<QB, 2>(col, [&](auto i, auto slot) {
+#pragma unroll
+                    for (int q = 0; q < QB; ++q) acc[i][q] = mfma16(kt[slot], ds[q], acc[i][q]);
+                });
+            }
+        }
+        store();
+        if (left < 0) break;
+        // sums past fp16 of queries whose own terms are finite
+        bool over = false;
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+            bool mine = false;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mine |= !(fabsf(acc[d][q][j]) < INFINITY);
+            mine = query_max(mine ? 1.0f : 0.0f) > 0.0f && fabsf(dsum[q]) < INFINITY && fabsf(lse2[q]) < INFINITY;
+            lift[q] += mine ? DQ_STEP : 0;
+            lse2[q] += mine ? (float)DQ_STEP : 0.0f;
+            over |= mine;
+        }
+        if (!__syncthreads_or(over)) break;
+        kv.load(list, 0, smem, smem + TILE);
     }
     static_assert(4 * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
     // a hidden NaN, or a dS past fp16 (values of V in the thousands and more)
@@ -1025,7 +1070,7 @@ struct KvGrad {
     static constexpr int KEYS = 16 * KB * NWV, QT = Geo<DH>::W >= 128 ? 32 : 64;
 };
 template <int DH>
-__global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void window_dkdv(WindowArgs a, Parts pt, const float* stats, int64_t rows, const int* tops, int tops_n, int tops_lg, float* ws) {
+__global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void window_dkdv(WindowArgs a, Parts pt, const float* stats, int64_t rows, const short2_t* tops, int tops_n, int tops_lg, float* ws) {
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, KB = KvGrad<DH>::KB, NWV = KvGrad<DH>::NWV, KEYS = KvGrad<DH>::KEYS;
     constexpr int QT = KvGrad<DH>::QT, TILE = QT * W;
@@ -1090,12 +1135,13 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
             dma16(wave_rsrc(stats + (wave ? rows : 0) + (int64_t)bc * NR + r0, (uint32_t)(min(QT, rb_end - r0) + 3) / 4 * 16),
                   (uint32_t)lane * 16, lds_addr(reinterpret_cast<const f16*>(sst)) + (2 * stage + wave) * 1024);
     };
-    int top = K_LEAST;
+    short2_t top = {K_LEAST, 2 * K_LEAST}, v_top = {K_LEAST, 0};
     if (nt > 0) {
         load(ra, ta, 0, smem, smem + TILE);
         load_stats(ra, 0);
         // an entry for every 2^tops_lg rows, tops_n a key head
-        for (int i = (ra >> tops_lg) + lane; i <= (rb_end - 1) >> tops_lg; i += 64) top = max(top, (tops + (int64_t)bc * tops_n)[i]);
+        for (int i = (ra >> tops_lg) + lane; i <= (rb_end - 1) >> tops_lg; i += 64)
+            top = __builtin_elementwise_max(top, (tops + (int64_t)bc * tops_n)[i]);
     }
     half8 kf[KB][KS], vf[KB][KS];
     const int64_t kv_ld = (int64_t)a.KV * a.dh, kv0 = (int64_t)b * a.R * kv_ld + (int64_t)c * a.dh;
@@ -1110,6 +1156,12 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
                 vf[kb][ks] = *reinterpret_cast<const half8*>(a.v + src + 32 * ks + 8 * g);
             }
         }
+        float squares = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) squares += (float)vf[kb][ks][i] * (float)vf[kb][ks][i];
+        v_top.x = max((int)v_top.x, length_exponent(query_sum(squares)));
     }
     floatx4 gk[DT][KB], gv[DT][KB];
 #pragma unroll
@@ -1117,8 +1169,14 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) gk[d][kb] = gv[d][kb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     const float c2 = a.scale * kLog2e;
-    const int lift = __builtin_amdgcn_readfirstlane(min(max(LONG - (int)wave_max((float)top), LEAST), MOST));
-    const float lift_s = (float)lift / c2;  // in S
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        top = max_xor(top, o);
+        if (o < 16) v_top = max_xor(v_top, o);  // the lanes of a key hold the same
+    }
+    // |dS| < P 2^(DS_TOP - lift)
+    const int lift = __builtin_amdgcn_readfirstlane(DS_TOP - 1 - max(top.x + v_top.x, (int)top.y));  // -27 .. 61
+    const float lift_ds = exp2i(lift - P_LIFT);
     half2_t wild = {(f16)0.0f, (f16)0.0f};
     // 32 rows of a tile
     auto step_of = [&](int t, int r0, int tf, int m0, int h, const f16* sq, const f16* sg, bool plain) {
@@ -1137,7 +1195,7 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
         floatx4 x0[2], y0[2];
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
-            x0[rb] = *reinterpret_cast<const floatx4*>(&sst[t & 1][0][32 * h + 16 * rb + 4 * g]) + lift_s;
+            x0[rb] = *reinterpret_cast<const floatx4*>(&sst[t & 1][0][32 * h + 16 * rb + 4 * g]);
             y0[rb] = *reinterpret_cast<const floatx4*>(&sst[t & 1][1][32 * h + 16 * rb + 4 * g]);
         }
         Rows::template start<2>(row);
@@ -1172,8 +1230,8 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
                 float e[4], f[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    e[j] = __builtin_amdgcn_exp2f(s[rb][kb][j] * c2);
-                    f[j] = e[j] * dp[rb][kb][j];
+                    e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][kb][j], c2, (float)P_LIFT));
+                    f[j] = e[j] * lift_ds * dp[rb][kb][j];
                 }
                 pu[2 * rb] = pack_h2(e[0], e[1]);
                 pu[2 * rb + 1] = pack_h2(e[2], e[3]);
@@ -1225,7 +1283,7 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
 #pragma unroll
             for (int j = 0; j < 4; ++j) bad |= !(fabsf(gk[d][kb][j]) < INFINITY) | !(fabsf(gv[d][kb][j]) < INFINITY);
     bool again = __any(bad);
-    const float back_v = exp2i(-lift), back_k = a.scale * back_v;
+    const float back_v = exp2i(-P_LIFT), back_k = a.scale * exp2i(-lift);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
         if (nparts > 1) {
@@ -1423,7 +1481,7 @@ namespace {
 uint64_t window_stats_rows(int B, int N, int H) { return ((uint64_t)B * N * H + 3) / 4 * 4; }  // of each of two
 uint64_t window_tops_bytes(int B, int N, int H, int KV, int dh) {
     const int64_t nr = (int64_t)N * (H / KV), per = 64 * query_blocks(nr, (int64_t)B * KV, dh);
-    return (uint64_t)B * KV * ((nr + per - 1) / per) * 4 * sizeof(int);
+    return (uint64_t)B * KV * ((nr + per - 1) / per) * 4 * sizeof(short2_t);
 }
 }  // namespace
 
@@ -1448,7 +1506,7 @@ int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
         const int qb = query_blocks(nr, (int64_t)a.B * a.KV, a.dh), tiles = (int)((nr + 64 * qb - 1) / (64 * qb));
         const int64_t srows = (int64_t)window_stats_rows(a.B, a.N, a.H);
         float* const stats = (float*)ws;
-        int* const tops = (int*)(stats + 2 * srows);
+        short2_t* const tops = (short2_t*)(stats + 2 * srows);
         float* const sums = (float*)((char*)tops + window_tops_bytes(a.B, a.N, a.H, a.KV, a.dh));
         e = by_head(a.dh, [&](auto dhc) {
             constexpr int DH = decltype(dhc)::value;

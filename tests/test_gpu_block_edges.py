@@ -116,3 +116,71 @@ def test_window_attention_bwd_scores_of_minus_infinity(dev, dh, h, kv):
     close(dq[:, far:], w["dq"][:, far:], w["dq_t"][:, far:], "dq")
     for g, x in ((dk, "dk"), (dv, "dv")):
         close(g[:, far:], w[x][:, far:], w[x + "_t"][:, far:], x)
+
+
+# ---------------------------------------------------------------------------
+# long contexts: probabilities of 2^-16 and less, and gradients of very different sizes
+# ---------------------------------------------------------------------------
+def bwd64(q, k, v, o, do, h, dh, window=0, chunk=4096):
+    """Gradients of one sequence with one key head in 64 bits, a chunk of queries at a time; D from the forward's rounded
+    o, as the operator takes it."""
+    n = q.shape[1]
+    K, V = k[0].to(F64), v[0].to(F64)
+    dq, dk, dv = [], torch.zeros_like(K), torch.zeros_like(V)
+    for t0 in range(0, n, chunk):
+        t1 = min(n, t0 + chunk)
+        j0 = max(0, t0 - window + 1) if window else 0
+        p, j = torch.arange(t0, t1, device=q.device)[:, None], torch.arange(j0, t1, device=q.device)[None]
+        m = (j <= p) & (j > p - window) if window else j <= p
+        row = []
+        for hd in range(h):
+            Q, G, O = (x[0, t0:t1, hd * dh:hd * dh + dh].to(F64) for x in (q, do, o))  # noqa: E741
+            P = torch.softmax((Q @ K[j0:t1].t() * dh ** -0.5).masked_fill(~m, -math.inf), 1)
+            dS = P * (G @ V[j0:t1].t() - (G * O).sum(1, keepdim=True)) * dh ** -0.5
+            row.append(dS @ K[j0:t1])
+            dk[j0:t1] += dS.t() @ Q
+            dv[j0:t1] += P.t() @ G
+        dq.append(torch.cat(row, 1))
+    return torch.cat(dq)[None], dk[None], dv[None]
+
+
+def grads(q, k, v, do, dh, h, window):
+    o, lse = torch.empty_like(q), torch.empty(1, h, q.shape[1], device=q.device)
+    evk.window_attention(q, k, v, o, dh, window, 0, lse=lse)
+    out = [torch.empty_like(t) for t in (q, k, v)]
+    evk.window_attention_bwd(q, k, v, o, do, *out, lse, dh, window, 0)
+    return o, out
+
+
+@pytest.mark.parametrize("n,h,dh,size", [(65536, 1, 128, 1.0), (65536, 2, 64, 1.0), (131072, 1, 64, 4000.0), (65536, 1, 64, 2.0 ** -10), (40000, 1, 256, 1.0)])
+def test_window_attention_bwd_long_context(dev, n, h, dh, size):
+    """Nearly flat attention over all of a long context: P and dS of 1 / n keep the bits that fp16 has."""
+    r = Rng(dev, 60)
+    q, k, v, do = r(1, n, h * dh, std=0.3), r(1, n, dh), r(1, n, dh), r(1, n, h * dh, std=size)
+    o, got = grads(q, k, v, do, dh, h, 0)
+    want = bwd64(q, k, v, o, do, h, dh)
+    for what, g, w in zip(("dq", "dk", "dv"), got, want):
+        g = g.to(F64)
+        for part in (slice(0, n // 8), slice(n // 8, n // 2), slice(n // 2, n - 2048), slice(n - 2048, n)):
+            a, b = g[:, part], w[:, part]
+            # 2 H for the roundings of P or dS, of O in D and of the result, and the result's own subnormals
+            tol = 2 * H * b.norm() + T * b.numel() ** 0.5
+            assert (a - b).norm() <= tol, f"{what} {part}: off by {float((a - b).norm() / b.norm() / H):.2f} H of the norm"
+
+
+@pytest.mark.parametrize("dh,h,n,window", [(128, 2, 4096, 512), (64, 1, 6000, 0), (40, 3, 3000, 256), (256, 1, 2000, 300)])
+def test_window_attention_bwd_gradients_of_two_sizes(dev, dh, h, n, window):
+    """Short output gradients (2^-12 of the long ones) in the same parts of a key block's queries: the gradients that they
+    alone make keep their bits."""
+    r = Rng(dev, 65)
+    q, k, v, do = r(1, n, h * dh, std=0.3), r(1, n, dh), r(1, n, dh), r(1, n, h * dh)
+    short = torch.arange(n, device=dev) >= n // 2 + 37
+    do[:, ~short] *= 256.0
+    do[:, short] *= 2.0 ** -4
+    o, got = grads(q, k, v, do, dh, h, window)
+    want = bwd64(q, k, v, o, do, h, dh, window)
+    for what, g, w in zip(("dq", "dk", "dv"), got, want):
+        for part in (~short, short):  # keys from there on are seen by the short ones alone
+            a, b = g[:, part].to(F64), w[:, part]
+            tol = 2 * H * b.norm() + T * b.numel() ** 0.5
+            assert (a - b).norm() <= tol, f"{what}: off by {float((a - b).norm() / b.norm() / H):.2f} H of the norm"
