@@ -55,8 +55,7 @@ DEV int position_of(const WindowArgs& a, int b, int t) {
 // One wave per query row (or per K, V row), any head size and alignment.
 // Latency-bound chains of scalar loads: the path of head sizes and pointers
 // that the MFMA kernels do not take (1000 queries of 8 heads over 2 of 100
-// values, window 512: 187 us, backward 3.7 ms), and of the few rows whose
-// tiles hold a hidden NaN.
+// values, window 512: 187 us, backward 3.7 ms).
 // ---------------------------------------------------------------------------
 constexpr int SMAX = 256;  // largest head size
 
@@ -379,6 +378,14 @@ struct KvTiles {
     }
 };
 
+// This wave's loads have arrived, and no access moves ahead of that.  The builtin
+// tells the compiler as much, which otherwise waits in the loop for registers
+// that were loaded before it, and so for the loads into LDS.
+DEV void wait_loads() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
 // N steps, each of M MFMAs on fragments that R LDS reads brought: the reads of
 // step i + AHEAD go out before the MFMAs of step i (read(i, slot) into slot
 // i % (AHEAD + 1) of a ring, use(i, slot)).  start() requests the first ones,
@@ -428,12 +435,140 @@ struct SmallDiv {
     DEV int operator()(int n) const { return (int)(((float)n + 0.5f) * inv); }
 };
 
+// Hidden rows.  The MFMA's product of a weight of 0 and a NaN or an infinity is
+// NaN, and the rows of a tile that some of its columns (queries; keys in the
+// kernel of dK and dV) do not see may hold either: stale cache rows, padding, a
+// gradient that overflowed.  In tiles that are not seen whole, the wave that
+// loads a row looks at it and leaves zeros in LDS where it finds such a value;
+// the columns that do see the row add it at the end, from memory and in 32 bits,
+// unless their sums are NaN by then.  So it reaches those alone, and what it
+// costs goes by the rows at the ends of a list, not by pairs: 4096 queries of 8
+// heads over 2 of 128 values, window 512, both directions 111 us, with one
+// infinite row of dO 129, an infinity in every hundredth value of dO 497, a third
+// of all rows NaN 382.
+
 // NaN or infinity among the values: a product with 0 is 0 for every other one
 DEV half2_t wild2(const half8& x, half2_t w) {
     const half2_t z = {(f16)0.0f, (f16)0.0f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) w = __builtin_elementwise_fma(half2_t{x[2 * i], x[2 * i + 1]}, z, w);
     return w;
+}
+
+DEV bool is_wild(half2_t w) { return !((float)w[0] == 0.0f && (float)w[1] == 0.0f); }
+DEV bool wild_row(const f16* p, int n) {  // n a multiple of 8
+    half2_t w = {(f16)0.0f, (f16)0.0f};
+    for (int i = 0; i < n; i += 8) w = wild2(*reinterpret_cast<const half8*>(p + i), w);
+    return is_wild(w);
+}
+// This wave's part of a tile in LDS, with zeros for the rows that hold a NaN or
+// an infinity; their bits, the part's first row lowest.
+template <class Dma>
+DEV uint32_t clean_rows(const Dma& dma, f16* tile) {
+    constexpr int CPR = Dma::G::CPR, RPI = Dma::RPI;
+    int lane = dma.lane;
+    asm volatile("" : "+v"(lane));  // addresses formed here, not kept through the kernel
+    uint32_t rows = 0;
+#pragma unroll
+    for (int i = 0; i < Dma::PER; ++i) {
+        u32x4* const p = reinterpret_cast<u32x4*>(tile + ((dma.wave * Dma::PER + i) * 64 + lane) * 8);
+        const uint64_t hit = __ballot(is_wild(wild2(as_half8(*p), half2_t{(f16)0.0f, (f16)0.0f})));
+        if (!hit) continue;
+        constexpr uint64_t ROW = (1ull << CPR) - 1;
+        if (hit >> (lane / CPR * CPR) & ROW) *p = u32x4{0u, 0u, 0u, 0u};
+        for (int k = 0; k < RPI; ++k) rows |= (hit >> (k * CPR) & ROW ? 1u : 0u) << (i * RPI + k);
+    }
+    return rows;
+}
+// What follows runs for such rows only, a few loads at a time and from places
+// formed on the spot: kept from the kernel's start, they would cost every call
+// the registers.
+//
+// products of the columns' operands (values 32 ks + 8 g and on) and a row, in each column's four lanes
+template <int KS, int QB>
+DEV void row_dot(float (&v)[QB], const half8 (&x)[QB][KS], const f16* row, int dh, int g) {
+    asm volatile("" : "+v"(g));
+#pragma unroll
+    for (int q = 0; q < QB; ++q) v[q] = 0.0f;
+#pragma unroll
+    for (int k0 = 0; k0 < KS; k0 += 4) {
+        u32x4 y[4];
+#pragma unroll
+        for (int k = 0; k < 4 && k0 + k < KS; ++k) y[k] = *reinterpret_cast<const u32x4*>(row + min(32 * (k0 + k) + 8 * g, dh - 8));
+#pragma unroll
+        for (int k = 0; k < 4 && k0 + k < KS; ++k) {
+            const half8 r = as_half8(32 * (k0 + k) + 8 * g < dh ? y[k] : u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+            for (int q = 0; q < QB; ++q) {
+                u32x4 u = as_u32x4(x[q][k0 + k]);
+                asm volatile("" : "+v"(u));  // else converted once, for the lengths at the start, and kept
+                const half8 c = as_half8(u);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[q] = __builtin_fmaf((float)c[i], (float)r[i], v[q]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int q = 0; q < QB; ++q) v[q] = query_sum(v[q]);
+}
+// acc[d][q] += w[q] row, for the columns that see it (and what nobody stores: values past dh)
+template <int DT, int QB>
+DEV void add_row(floatx4 (&acc)[DT][QB], const float (&w)[QB], const bool (&sees)[QB], const f16* row, int dh, int g) {
+    asm volatile("" : "+v"(g));
+#pragma unroll
+    for (int d0 = 0; d0 < DT; d0 += 8) {
+        half4 v[8];
+#pragma unroll
+        for (int d = 0; d < 8 && d0 + d < DT; ++d) v[d] = *reinterpret_cast<const half4*>(row + min(16 * (d0 + d) + 4 * g, dh - 4));
+#pragma unroll
+        for (int d = 0; d < 8 && d0 + d < DT; ++d)
+#pragma unroll
+            for (int q = 0; q < QB; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float o = acc[d0 + d][q][j];
+                    acc[d0 + d][q][j] = sees[q] ? __builtin_fmaf(w[q], (float)v[d][j], o) : o;
+                }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// Columns whose sums in this lane are all NaN, which nothing that is added changes
+template <int DT, int QB>
+DEV void spoilt(bool (&nan)[QB], const floatx4 (&acc)[DT][QB]) {
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        nan[q] = true;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) nan[q] &= acc[d][q][j] != acc[d][q][j];
+    }
+}
+template <int QB>
+DEV bool any_open(const bool (&sees)[QB], const bool (&nan)[QB]) {
+    bool open = false;
+#pragma unroll
+    for (int q = 0; q < QB; ++q) open |= sees[q] & !nan[q];
+    return __any(open);
+}
+// f(entry, row) for the entries of the list's tiles of `len`, from tile t0 in
+// steps of dt, that are not seen whole and whose rows of x (a row every ld
+// values) hold a NaN or an infinity
+template <class F>
+DEV void each_wild(const WindowArgs& a, const List& list, const f16* x, int64_t ld, int len, int t0, int t1, int dt, int lane, F&& f) {
+#pragma unroll 1
+    for (int t = t0; t < t1; t += dt) {
+        if (list.plain(a, t * len, len)) continue;
+        const int i = t * len + lane;
+        const bool is_row = (lane < len) & (i < list.n) & ((i < list.s) | (i >= list.sl));
+        uint64_t m = __ballot(is_row && wild_row(x + (int64_t)list.row(is_row ? i : 0) * ld, a.dh));
+#pragma unroll 1
+        for (; m; m &= m - 1) {
+            const int e = t * len + __builtin_ctzll(m);
+            f(e, (int64_t)list.row(e));
+        }
+    }
 }
 
 // The running softmax state of QB blocks of 16 queries (a lane: query l16 of
@@ -492,6 +627,20 @@ struct Softmax {
             }
         }
     }
+    // V's row of entry e, whose probability the sums l already hold
+    DEV void add_row(const WindowArgs& a, const List& list, int e, const f16* k, const f16* v, const half8 (&qf)[QB][Geo<DH>::KS], const int (&qp)[QB],
+                     float c2, int g) {
+        float w[QB];
+        bool sees[QB], nan[QB];
+#pragma unroll
+        for (int q = 0; q < QB; ++q) sees[q] = Seen(a, list, qp[q])(e);
+        spoilt(nan, o);
+        if (!any_open(sees, nan)) return;
+        row_dot(w, qf, k, a.dh, g);
+#pragma unroll
+        for (int q = 0; q < QB; ++q) w[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[q], c2, m[q] == -INFINITY ? 0.0f : -m[q]));
+        ::evkhip::add_row(o, w, sees, v, a.dh, g);
+    }
 };
 
 // Forward.  Workgroup: 4 waves of 16 QB rows of one key head; K and V tiles in
@@ -502,10 +651,6 @@ struct Softmax {
 // tiles' rows were placed without bank conflicts and read ahead of the MFMAs.
 // Workgroups of eight waves, reads further ahead and a priority for waves in
 // their products changed nothing.
-//
-// The product of a probability of 0 and a NaN or an infinity is NaN, so a tile
-// that some query does not wholly see is looked at for such values in V; a wave
-// that meets one computes its rows again at the end, row by row.
 template <int DH, int QB>
 __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a, int tiles) {
     using G = Geo<DH>;
@@ -540,12 +685,14 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
     }
     const float c2 = a.scale * kLog2e;
     Softmax<DH, QB> sm;
-    half2_t wild = {(f16)0.0f, (f16)0.0f};
+    uint32_t wild = 0;
     for (int t = 0; t < nt; ++t) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
-        __syncthreads();                     // everyone's; the other stage is free
         f16* const sk = smem + (t & 1) * 2 * TILE;
         f16* const sv = sk + TILE;
+        const bool plain = list.plain(a, t * BK, BK);  // workgroup-uniform
+        wait_loads();  // this wave's part of tile t is in LDS
+        if (!plain) wild |= clean_rows(kv.dma, sv);
+        __syncthreads();  // everyone's; the other stage is free
         if (t + 1 < nt) {
             f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
             kv.load(list, (t + 1) * BK, nx, nx + TILE);
@@ -562,7 +709,7 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
             for (int q = 0; q < QB; ++q)
                 s[i / KS][q] = mfma16(kf[slot], qf[q][i % KS], i % KS ? s[i / KS][q] : floatx4{0.0f, 0.0f, 0.0f, 0.0f});
         });
-        if (!list.plain(a, t * BK, BK)) {  // workgroup-uniform
+        if (!plain) {
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
                 const Seen see(a, list, qp[q]);
@@ -572,7 +719,6 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
                     for (int j = 0; j < 4; ++j)
                         s[kb][q][j] = see(t * BK + 16 * kb + 4 * g + j) ? s[kb][q][j] : -INFINITY;
             }
-            for (int i = 0; i < 2 * DT; ++i) wild = wild2(fr.col(sv, i & 1 ? 32 : 0, i / 2), wild);
         }
         half8 p[2][QB];
         sm.template probs<4>(s, c2, p);
@@ -581,6 +727,10 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
 #pragma unroll
             for (int q = 0; q < QB; ++q) sm.o[i % DT][q] = mfma16(vf[slot], p[i / DT][q], sm.o[i % DT][q]);
         });
+    }
+    if (__syncthreads_or(wild)) {
+        const int64_t ld = (int64_t)a.KV * a.dh;
+        each_wild(a, list, kv.v, ld, BK, 0, nt, 1, lane, [&](int e, int64_t row) { sm.add_row(a, list, e, kv.k + row * ld, kv.v + row * ld, qf, qp, c2, g); });
     }
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
@@ -598,12 +748,6 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
         if (a.lse && g == 0)
             a.lse[((int64_t)b * a.H + c * group + r % group) * a.N + r / group] = none ? -INFINITY : (sm.m[q] + log2f(l)) * kLn2;
     }
-    static_assert(4 * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
-    const bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
-    if (!__syncthreads_or(again) || !again) return;
-#pragma unroll 1
-    for (int r = wr0; r < min(wr0 + 16 * QB, NR); ++r)
-        fwd_row(a, ((int64_t)b * a.N + r / group) * a.H + c * group + r % group, reinterpret_cast<RowLds*>(smem)[wave], lane);
 }
 
 // Forward for few query rows (single tokens, short prompts): a workgroup takes
@@ -626,8 +770,7 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, NW = SplitGeo<DH>::NW, VPER = 32 * G::CPR / 64, OW = DH + 4;
     constexpr int SLOT = 32 * W * 2, STATE = 16 * OW * 4;  // bytes of a wave's V, then of its state
-    constexpr int EACH = SLOT > STATE ? SLOT : STATE;
-    constexpr int BYTES = NW * (EACH > (int)sizeof(RowLds) ? EACH : (int)sizeof(RowLds));
+    constexpr int BYTES = NW * (SLOT > STATE ? SLOT : STATE);
     __shared__ __attribute__((aligned(16))) char smem[BYTES];
     __shared__ float sm_m[NW][16], sm_l[NW][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -668,7 +811,7 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
         load_k(step);
         load_v(step);
     }
-    const int r = min(R0 + l16, NR - 1), qp = position_of(a, b, r / group);
+    const int r = min(R0 + l16, NR - 1), qp[1] = {position_of(a, b, r / group)};
     const int64_t q_at = ((int64_t)b * a.N + r / group) * a.H + c * group + r % group;  // row of q
     half8 qf[1][KS];
 #pragma unroll
@@ -678,8 +821,17 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
     }
     const float c2 = a.scale * kLog2e;
     Softmax<DH, 1> sm;
-    half2_t wild = {(f16)0.0f, (f16)0.0f};
+    uint64_t wild = 0;
     for (; step < c1; step += NW) {
+        const bool plain = list.plain(a, 32 * step, 32);
+        if (!plain) {
+#pragma unroll
+            for (int i = 0; i < VPER; ++i) {
+                const uint64_t hit = __ballot(is_wild(wild2(as_half8(vr[i]), half2_t{(f16)0.0f, (f16)0.0f})));
+                if (hit >> (lane / G::CPR * G::CPR) & ((1ull << G::CPR) - 1)) vr[i] = u32x4{0u, 0u, 0u, 0u};
+                wild |= hit;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < VPER; ++i) *reinterpret_cast<u32x4*>(slot + (lane + 64 * i) * 8) = vr[i];
         if (step + NW < c1) load_v(step + NW);
@@ -694,23 +846,23 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
             for (int ks = 0; ks < KS; ++ks) s[kb][0] = mfma16(as_half8(kr[kb][ks]), qf[0][ks], s[kb][0]);
         }
         if (step + NW < c1) load_k(step + NW);
-        if (!list.plain(a, 32 * step, 32)) {
-            const Seen see(a, list, qp);
+        if (!plain) {
+            const Seen see(a, list, qp[0]);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[kb][0][j] = see(32 * step + 16 * kb + 4 * g + j) ? s[kb][0][j] : -INFINITY;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) wild = wild2(vf[d], wild);
         }
         half8 p[1][1];
         sm.template probs<2>(s, c2, p);
 #pragma unroll
         for (int d = 0; d < DT; ++d) sm.o[d][0] = mfma16(vf[d], p[0][0], sm.o[d][0]);
     }
-    const bool again = __any(!((float)wild[0] == 0.0f && (float)wild[1] == 0.0f));
-    // the states, one row of OW floats a query; the slots have been read
-    const int any_again = __syncthreads_or(again);
+    if (wild)
+        each_wild(a, list, a.v + kv0, ld, 32, c0 + wave, c1, NW, lane,
+                  [&](int e, int64_t row) { sm.add_row(a, list, e, a.k + kv0 + row * ld, a.v + kv0 + row * ld, qf, qp, c2, g); });
+    // the states, one row of OW floats a query, once the slots have been read
+    __syncthreads();
     float* const st = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int d = 0; d < DT; ++d) *reinterpret_cast<floatx4*>(st + (wave * 16 + l16) * OW + 16 * d + 4 * g) = sm.o[d][0];
@@ -747,24 +899,15 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
         if (a.lse && d == 0)
             a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = none ? -INFINITY : (m + log2f(ls)) * kLn2;
     }
-    if (splits > 1 || !any_again) return;
-    __syncthreads();
-#pragma unroll 1
-    for (int q = wave; q < 16 && R0 + q < NR; q += NW) {
-        const int row = R0 + q;
-        fwd_row(a, ((int64_t)b * a.N + row / group) * a.H + c * group + row % group, reinterpret_cast<RowLds*>(smem)[wave], lane);
-    }
 }
 
 // The states of one query row's splits (at most JOIN_MOST): each thread weighs
 // one, then each of NW waves adds every NW-th one's sums, and theirs are
-// added in order.  What is not finite may be a hidden NaN's work: that row is
-// computed again.
+// added in order.
 constexpr int JOIN_MOST = 256;  // CUs
 template <int DH>
 __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int splits, const float* ws) {
     constexpr int NW = 4, PER = DH < 64 ? 1 : DH / 64 + (DH % 64 ? 1 : 0);
-    __shared__ RowLds lds;
     __shared__ float part[NW][64 * PER], weight[JOIN_MOST], red[2][NW];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.H / a.KV, NR = a.N * group;
     const int row = blockIdx.x % NR, bc = blockIdx.x / NR, c = bc % a.KV, b = bc / a.KV;
@@ -793,15 +936,10 @@ __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int split
     const int64_t at = ((int64_t)b * a.N + row / group) * a.H + c * group + row % group;
     const bool none = span_of(position_of(a, b, row / group), a).count() == 0;
     const float inv = none ? 0.0f : 1.0f / l;
-    bool bad = !(fabsf(l) < INFINITY);
-    for (int d = tid; d < a.dh; d += 256) {
-        const float v = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
-        bad |= !(fabsf(v) < INFINITY);
-        a.out[at * a.dh + d] = (f16)(v * inv);
-    }
+    for (int d = tid; d < a.dh; d += 256)
+        a.out[at * a.dh + d] = (f16)(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
     if (a.lse && tid == 0)
         a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = none ? -INFINITY : (m + log2f(l)) * kLn2;
-    if (__syncthreads_or(bad) && wave == 0) fwd_row(a, at, lds, lane);
 }
 
 // P and dS are rounded to fp16 for their products, which has 30 powers of two
@@ -838,12 +976,14 @@ DEV int length_exponent(float squares) {  // |x| < 2^k
 // and the largest length exponents of dO and of dO times O among each wave's rows
 // for the kernel of dK and dV.
 // Bound as the forward is, with three products for two: 2 x 1999 queries of 8
-// heads over 2 of 128 values, window 512, 25 us (504 workgroups, two for a CU).
+// heads over 2 of 128 values, window 512, 26.5 us (504 workgroups, two for a CU).
 template <int DH, int QB>
 __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a, int tiles, float* stats, int64_t rows, short2_t* tops) {
     using G = Geo<DH>;
     constexpr int KS = G::KS, DT = G::DT, W = G::W, TILE = BK * W, ROWS = 64 * QB;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
+    __shared__ uint32_t zeroed[2][4];  // rows of a tile that clean_rows has made zeros, 16 of each wave
+    static_assert(BK == 64, "16 rows a wave");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const Frag<DH> fr(lane);
@@ -903,7 +1043,7 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
     if (lane == 0) tops[((int64_t)bc * tiles + tile) * 4 + wave] = top;
     const float c2 = a.scale * kLog2e;
     floatx4 acc[DT][QB];
-    half2_t wild = {(f16)0.0f, (f16)0.0f};
+    uint32_t wild = 0;
     auto store = [&] {
         int at_lane = lane;
         asm volatile("" : "+v"(at_lane));  // places formed here, not kept from before the loop
@@ -927,10 +1067,16 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
 #pragma unroll
             for (int q = 0; q < QB; ++q) acc[d][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         for (int t = 0; t < nt; ++t) {
-            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
-            __syncthreads();                     // everyone's; the other stage is free
             f16* const sk = smem + (t & 1) * 2 * TILE;
             f16* const sv = sk + TILE;
+            wait_loads();  // this wave's part of tile t is in LDS
+            const bool whole = list.plain(a, t * BK, BK);
+            if (!whole) {
+                const uint32_t hit = clean_rows(kv.dma, sk);
+                if (lane == 0) zeroed[t & 1][wave] = hit;
+                wild |= hit;
+            }
+            __syncthreads();  // everyone's; the other stage is free
             if (t + 1 < nt) {
                 f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
                 kv.load(list, (t + 1) * BK, nx, nx + TILE);
@@ -955,7 +1101,8 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
                         dp[i / KS][q] = mfma16(vf[slot], gf[q][i % KS], i % KS ? dp[i / KS][q] : zero);
                     }
                 });
-                const bool plain = list.plain(a, t * BK + 32 * k2, 32);  // workgroup-uniform
+                // workgroup-uniform: every query sees these rows, and all of them are here
+                const bool plain = list.plain(a, t * BK + 32 * k2, 32) && (whole || __builtin_amdgcn_readfirstlane(zeroed[t & 1][2 * k2] | zeroed[t & 1][2 * k2 + 1]) == 0);
                 half8 ds[QB];
 #pragma unroll
                 for (int q = 0; q < QB; ++q) {
@@ -968,12 +1115,13 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
                     if (!plain) {
                         const Seen see(a, list, qp[q]);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) e[i] = see(t * BK + 32 * k2 + 16 * (i / 4) + 4 * g + i % 4) ? e[i] : 0.0f;
+                        for (int i = 0; i < 8; ++i) {
+                            const bool zero = zeroed[t & 1][2 * k2 + i / 4] >> (4 * g + i % 4) & 1;
+                            e[i] = see(t * BK + 32 * k2 + 16 * (i / 4) + 4 * g + i % 4) & !zero ? e[i] : 0.0f;
+                        }
                     }
                     ds[q] = as_half8(u32x4{pack_h2(e[0], e[1]), pack_h2(e[2], e[3]), pack_h2(e[4], e[5]), pack_h2(e[6], e[7])});
                 }
-                if (!plain)
-                    for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sk, 32 * k2, d), wild);
                 Cols::template start<2>(col);
                 Cols::template run<QB, 2>(col, [&](auto i, auto slot) {
 #pragma unroll
@@ -982,38 +1130,41 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
             }
         }
         store();
-        if (left < 0) break;
         // sums past fp16 of queries whose own terms are finite
         bool over = false;
+        if (left >= 0) {
 #pragma unroll
-        for (int q = 0; q < QB; ++q) {
-            bool mine = false;
+            for (int q = 0; q < QB; ++q) {
+                bool mine = false;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+                for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mine |= !(fabsf(acc[d][q][j]) < INFINITY);
-            mine = query_max(mine ? 1.0f : 0.0f) > 0.0f && fabsf(dsum[q]) < INFINITY && fabsf(lse2[q]) < INFINITY;
-            lift[q] += mine ? DQ_STEP : 0;
-            lse2[q] += mine ? (float)DQ_STEP : 0.0f;
-            over |= mine;
+                    for (int j = 0; j < 4; ++j) mine |= !(fabsf(acc[d][q][j]) < INFINITY);
+                mine = query_max(mine ? 1.0f : 0.0f) > 0.0f && fabsf(dsum[q]) < INFINITY && fabsf(lse2[q]) < INFINITY;
+                lift[q] += mine ? DQ_STEP : 0;
+                lse2[q] += mine ? (float)DQ_STEP : 0.0f;
+                over |= mine;
+            }
         }
+        if (!__syncthreads_or(over | (wild != 0))) return;
         if (!__syncthreads_or(over)) break;
         kv.load(list, 0, smem, smem + TILE);
     }
-    static_assert(4 * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
-    // a hidden NaN, or a dS past fp16 (values of V in the thousands and more)
-    bool bad = !((float)wild[0] == 0.0f && (float)wild[1] == 0.0f);
+    const int64_t ld = (int64_t)a.KV * a.dh;
+    each_wild(a, list, kv.k, ld, BK, 0, nt, 1, lane, [&](int i, int64_t row) {
+        float ds[QB], dp[QB];
+        bool sees[QB], nan[QB];
 #pragma unroll
-    for (int q = 0; q < QB; ++q)
+        for (int q = 0; q < QB; ++q) sees[q] = Seen(a, list, qp[q])(i);
+        spoilt(nan, acc);
+        if (!any_open(sees, nan)) return;
+        row_dot(ds, qf, kv.k + row * ld, a.dh, g);
+        row_dot(dp, gf, kv.v + row * ld, a.dh, g);
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) bad |= !(fabsf(acc[d][q][j]) < INFINITY);
-    const bool again = __any(bad);
-    if (!__syncthreads_or(again) || !again) return;
-#pragma unroll 1
-    for (int r = wr0; r < min(wr0 + 16 * QB, NR); ++r)
-        dq_row(a, ((int64_t)b * a.N + r / group) * a.H + c * group + r % group, reinterpret_cast<RowLds*>(smem)[wave], lane);
+        for (int q = 0; q < QB; ++q) ds[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(ds[q], c2, -lse2[q])) * (dp[q] - dsum[q]);
+        add_row(acc, ds, sees, kv.k + row * ld, a.dh, g);
+    });
+    store();
 }
 
 // Backward, dK and dV.  Workgroup: NWV waves of 16 KB rows (keys) of one key head
@@ -1024,8 +1175,8 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
 //   P = 2^(S c), dS = P dP, which are then the B operands of dV^T += dO^T P and
 //   dK^T += Q^T dS, whose A operands are transposed reads of the same tiles.
 // The sum over the heads of a group is part of the sum over rows.  Four products
-// for the forward's two, over the same pairs as window_dq: 47.5 us at its size,
-// 310 TFLOP/s; 168 registers hold three workgroups a CU.  32 keys a wave, tiles of
+// for the forward's two, over the same pairs as window_dq: 47 us at its size,
+// 313 TFLOP/s; 168 registers hold three workgroups a CU.  32 keys a wave, tiles of
 // 64 rows and eight waves were no faster.
 //
 // Parts: the queries from the first key's position to the last one that sees
@@ -1177,7 +1328,7 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
     // |dS| < P 2^(DS_TOP - lift)
     const int lift = __builtin_amdgcn_readfirstlane(DS_TOP - 1 - max(top.x + v_top.x, (int)top.y));  // -27 .. 61
     const float lift_ds = exp2i(lift - P_LIFT);
-    half2_t wild = {(f16)0.0f, (f16)0.0f};
+    uint32_t wild = 0;
     // 32 rows of a tile
     auto step_of = [&](int t, int r0, int tf, int m0, int h, const f16* sq, const f16* sg, bool plain) {
         using Rows = Ring<2 * KS, 3>;
@@ -1220,7 +1371,6 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
                         dp[rb][kb][j] = see ? dp[rb][kb][j] : 0.0f;
                     }
                 }
-            for (int d = 0; d < DT; ++d) wild = wild2(fr.col(sg, 32 * h, d), wild2(fr.col(sq, 32 * h, d), wild));
         }
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -1251,38 +1401,78 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
         });
     };
     int t0 = ta, m0 = 0;
+    // every query of the tile at flat row r0 (position tf; the next tile is at row mn of position tn) sees every key of the
+    // block: the first query the last key, the last query (before the next tile) the first key outside the sinks
+    auto plain_at = [&](int r0, int tf, int tn, int mn) {
+        const int tl = mn ? tn : tn - 1;
+        return (r0 + QT <= rb_end) & (klast <= tf) & ((klast < a.sinks) | (max(k0, a.sinks) > tl - a.window));
+    };
     for (int t = 0; t < nt; ++t) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of tile t is in LDS
-        __syncthreads();                     // everyone's; the other stage is free
         f16* const sq = smem + (t & 1) * 2 * TILE;
         f16* const sg = sq + TILE;
         const int r0 = ra + t * QT;
         const int gone = __builtin_amdgcn_readfirstlane(by_group(m0 + QT)), tf = t0, mf = m0;  // positions up to the next tile
         t0 += gone;
         m0 += QT - gone * group;
+        const bool plain = plain_at(r0, tf, t0, m0);
+        wait_loads();  // this wave's part of tile t is in LDS
+        if (!plain) wild |= clean_rows(dma, sq) | clean_rows(dma, sg);
+        __syncthreads();  // everyone's; the other stage is free
         if (t + 1 < nt) {
             f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
             load(r0 + QT, t0, m0, nx, nx + TILE);
             load_stats(r0 + QT, (t + 1) & 1);
         }
-        // every query of the tile sees every key of the block: the first query the last key, the last query (before
-        // row m0 of position t0) the first key outside the sinks
-        const int tl = m0 ? t0 : t0 - 1;
-        const bool plain = (r0 + QT <= rb_end) & (klast <= tf) & ((klast < a.sinks) | (max(k0, a.sinks) > tl - a.window));
 #pragma unroll
         for (int h = 0; h < QT / 32; ++h) {
             step_of(t, r0, tf, mf, h, sq, sg, plain);
         }
     }
-    // a hidden NaN, or a dS past fp16 (values of V in the thousands and more)
-    bool bad = !((float)wild[0] == 0.0f && (float)wild[1] == 0.0f);
+    if (__syncthreads_or(wild)) {
+#pragma unroll 1
+        for (int t = 0; t < nt; ++t) {
+            const int r0 = ra + t * QT;
+            if (plain_at(r0, r0 / group, (r0 + QT) / group, (r0 + QT) % group)) continue;
+            const int rl = r0 + lane;
+            auto at_row = [&](int r) { return (qb0 + (int64_t)(r / group) * a.H + r % group) * a.dh; };
+            const bool is_row = (lane < QT) & (rl < rb_end);
+            const uint64_t mq = __ballot(is_row && wild_row(a.q + at_row(is_row ? rl : r0), a.dh));
+            const uint64_t mg = __ballot(is_row && wild_row(a.dO + at_row(is_row ? rl : r0), a.dh));
+#pragma unroll 1
+            for (uint64_t m = mq | mg; m; m &= m - 1) {
+                const int i = __builtin_ctzll(m), r = r0 + i, pos = r / group;
+                const f16 *qr = a.q + at_row(r), *gr = a.dO + at_row(r);
+                float p[KB], ds[KB];
+                bool sees[KB], nan_k[KB], nan_v[KB];
+                spoilt(nan_k, gk);
+                spoilt(nan_v, gv);
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+                for (int kb = 0; kb < KB; ++kb) {
+                    const int key = k0 + (wave * KB + kb) * 16 + l16;
+                    sees[kb] = (key <= pos) & ((key > pos - a.window) | (key < a.sinks));
+                    nan_k[kb] &= nan_v[kb];
+                }
+                if (!any_open(sees, nan_k)) continue;
+                const float x0 = stats[(int64_t)bc * NR + r], y0 = stats[rows + (int64_t)bc * NR + r];
+                row_dot(p, kf, qr, a.dh, g);
+                row_dot(ds, vf, gr, a.dh, g);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+                for (int kb = 0; kb < KB; ++kb) {
+                    p[kb] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[kb] + x0, c2, (float)P_LIFT));
+                    ds[kb] = p[kb] * lift_ds * (ds[kb] + y0);
+                }
+                if (mq >> i & 1) add_row(gk, ds, sees, qr, a.dh, g);
+                if (mg >> i & 1) {
+                    add_row(gv, p, sees, gr, a.dh, g);
+                } else {  // q is not finite, and dO is in the sums, with a weight from zeros in q's place
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bad |= !(fabsf(gk[d][kb][j]) < INFINITY) | !(fabsf(gv[d][kb][j]) < INFINITY);
-    bool again = __any(bad);
+                    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) gv[d][kb] += sees[kb] ? p[kb] * 0.0f : 0.0f;
+                }
+            }
+        }
+    }
     const float back_v = exp2i(-P_LIFT), back_k = a.scale * exp2i(-lift);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -1307,20 +1497,12 @@ __global__ __launch_bounds__(64 * KvGrad<DH>::NWV, DH <= 128 ? 3 : 1) void windo
                 *reinterpret_cast<uint2*>(a.dV + dst + 16 * d + 4 * g) = uint2{pack_h2(v[0], v[1]), pack_h2(v[2], v[3])};
             }
     }
-    if (nparts > 1) again = false;  // window_dkdv_join looks at the sums
-    static_assert(NWV * sizeof(RowLds) <= sizeof(smem), "a wave's rows");
-    if (!__syncthreads_or(again) || !again) return;
-#pragma unroll 1
-    for (int j = k0 + wave * 16 * KB; j < min(k0 + (wave + 1) * 16 * KB, a.N); ++j)
-        dkdv_row(a, ((int64_t)b * a.R + j) * a.KV + c, reinterpret_cast<RowLds*>(smem)[wave], lane);
 }
 
-// The sums of the parts of one key, a wave each.  A sum that is not finite may
-// be a hidden NaN's work: that key is computed again, row by row.
+// The sums of the parts of one key, a wave each.
 template <int DH, int KEYS>
 __global__ __launch_bounds__(64) void window_dkdv_join(WindowArgs a, Parts pt, int blocks, const float* ws) {
     constexpr int PER = 2 * DH / 64;
-    __shared__ RowLds lds;
     const int lane = threadIdx.x, j = blockIdx.x % (blocks * KEYS), bc = blockIdx.x / (blocks * KEYS);
     const int blk = j / KEYS, nparts = pt.parts_of(blk), c = bc % a.KV, b = bc / a.KV;
     if (nparts < 2 || j >= a.N) return;
@@ -1331,14 +1513,11 @@ __global__ __launch_bounds__(64) void window_dkdv_join(WindowArgs a, Parts pt, i
         for (int i = 0; i < PER; ++i) v[i] += src[(int64_t)p * (2 * KEYS * DH) + i];
     const int64_t row = ((int64_t)b * a.R + j) * a.KV + c;
     const bool is_k = lane < 32;
-    bool bad = false;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        bad |= !(fabsf(v[i]) < INFINITY);
         const int d = lane % 32 * PER + i;
         if (d < a.dh) (is_k ? a.dK : a.dV)[row * a.dh + d] = (f16)v[i];
     }
-    if (__any(bad)) dkdv_row(a, row, lds, lane);
 }
 
 // The MFMA kernels' shapes

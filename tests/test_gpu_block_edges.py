@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import evk_amd as evk
-from test_gpu_block import F64, H, T, Rng, close, empty, rope_want, seen, window_want
+from test_gpu_block import F16, F64, H, T, Rng, close, empty, rope_want, seen, window_want
 
 pytestmark = pytest.mark.gpu
 
@@ -184,3 +184,80 @@ def test_window_attention_bwd_gradients_of_two_sizes(dev, dh, h, n, window):
             a, b = g[:, part].to(F64), w[:, part]
             tol = 2 * H * b.norm() + T * b.numel() ** 0.5
             assert (a - b).norm() <= tol, f"{what}: off by {float((a - b).norm() / b.norm() / H):.2f} H of the norm"
+
+
+# ---------------------------------------------------------------------------
+# NaN and infinities beside finite rows
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dh,h,kv", HEADS)
+@pytest.mark.parametrize("what", ["q", "k", "v", "do"])
+@pytest.mark.parametrize("b,n,window,sinks", [(1, 300, 40, 3), (3, 700, 90, 0), (1, 333, 0, 0)])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_window_attention_bwd_single_wild_rows(dev, dh, h, kv, what, b, n, window, sinks, value):
+    """One row of q, k, v or dO that is not finite, in the middle: outputs and gradients that it takes no part in are those
+    without it, the others say so."""
+    at = n // 2 + 5
+    r = Rng(dev, 40 + dh + n)
+    t = dict(q=r(b, n, h * dh), k=r(b, n, kv * dh), v=r(b, n, kv * dh), do=r(b, n, h * dh))
+    w = window_want(t["q"], t["k"], t["v"], h, kv, dh, [0] * b, window, sinks, t["do"])
+    t[what][0, at] = value
+    q, k, v, do = t["q"], t["k"], t["v"], t["do"]
+    o, lse = torch.empty_like(q), torch.empty(b, h, n, device=dev)
+    evk.window_attention(q, k, v, o, dh, window, sinks, lse=lse)
+    dq, dk, dv = (torch.empty_like(x) for x in (q, k, v))
+    evk.window_attention_bwd(q, k, v, o, do, dq, dk, dv, lse, dh, window, sinks)
+    m = seen(torch.arange(n, device=dev), n, window, sinks)
+    rows = torch.zeros(b, n, dtype=torch.bool, device=dev)  # queries whose gradient is touched
+    rows[0] = m[:, at] if what in "kv" else torch.arange(n, device=dev) == at
+    keys = torch.zeros(b, n, dtype=torch.bool, device=dev)  # keys that such a query sees
+    keys[0] = (m & rows[0][:, None]).any(0)
+    outs = rows if what != "do" else torch.zeros_like(rows)
+    close(o[~outs], w["o"][~outs], w["o_t"][~outs], "o")
+    if outs.any():
+        assert not torch.isfinite(o[outs].float()).all(-1).any()
+    close(dq[~rows], w["dq"][~rows], w["dq_t"][~rows], "dq", norm=4 * H)
+    assert not torch.isfinite(dq[rows].float()).all(-1).any(), "dq"
+    for g, x in ((dk, "dk"), (dv, "dv")):
+        close(g[~keys], w[x][~keys], w[x + "_t"][~keys], x, norm=4 * H)
+        if not (what in "kv" and x == "dv"):  # P of a row that overflowed may be 0 for the others
+            assert not torch.isfinite(g[keys].float()).all(-1).any(), x
+
+
+def passes_us(f, n=5):
+    f()
+    best = math.inf
+    for _ in range(n):
+        a, e = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        e.record()
+        e.synchronize()
+        best = min(best, a.elapsed_time(e) * 1e3)
+    return best
+
+
+@pytest.mark.parametrize("where", ["do", "k", "q", "do everywhere"])
+@pytest.mark.parametrize("dh,h,kv,n,window", [(128, 8, 2, 4096, 512), (64, 4, 1, 8192, 0)])
+def test_window_attention_bwd_overflow_costs_no_more(dev, dh, h, kv, n, window, where):
+    """A gradient that overflowed (the step that loss scaling skips) must not send its rows and keys through scalar code:
+    at most three passes where one serves, and as much again.  With an infinity in every row, the rows of the tiles that
+    are not seen whole are added one by one, whose number does not grow with the pairs of a key."""
+    r = Rng(dev, 50)
+    t = dict(q=r(1, n, h * dh), k=r(1, n, kv * dh), v=r(1, n, kv * dh), do=r(1, n, h * dh))
+    q, k, v, do = t.values()
+    o, lse = torch.empty_like(q), torch.empty(1, h, n, device=dev)
+    g = [torch.empty_like(x) for x in (q, k, v)]
+    ws = torch.empty(1 << 28, dtype=torch.uint8, device=dev)
+
+    def step():
+        evk.window_attention(q, k, v, o, dh, window, 0, lse=lse, workspace=ws)
+        evk.window_attention_bwd(q, k, v, o, do, *g, lse, dh, window, 0, workspace=ws)
+
+    clean = passes_us(step)
+    if where == "do everywhere":
+        t["do"][0, :, 5] = torch.where(torch.arange(n, device=dev) % 3 == 0, math.inf, -math.inf).to(F16)
+    else:
+        t[where][0, n // 2 + 3, 5] = math.inf
+    wild = passes_us(step, 2)
+    assert not torch.isfinite(g[1].float()).all()
+    assert wild <= (20 if where == "do everywhere" else 6) * clean + 50, f"{wild:.0f} us with an infinity, {clean:.0f} without"
