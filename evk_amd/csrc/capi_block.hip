@@ -365,7 +365,7 @@ int evkhip_gated_linear(const evkhip_tensor* x, const evkhip_tensor* w, const ev
 
 uint64_t evkhip_gated_linear_backward_workspace(uint64_t tokens, uint32_t d, uint32_t f) {
     (void)d;
-    return 2 * tokens * f * sizeof(f16);  // the gradients of both products
+    return glu_bwd_workspace(tokens * f);
 }
 
 int evkhip_gated_linear_backward(const evkhip_tensor* x, const evkhip_tensor* w, const evkhip_tensor* gate_up,
@@ -396,7 +396,8 @@ int evkhip_gated_linear_backward(const evkhip_tensor* x, const evkhip_tensor* w,
         return EVKHIP_OK;
     }
     f16* dgu = (f16*)workspace;
-    CHECK(glu_bwd_launch((const f16*)gate_up->data, (const f16*)dh->data, dgu, (int64_t)(s.T * s.F), activation, st));
+    GemmBack back;
+    CHECK(glu_bwd_launch((const f16*)gate_up->data, (const f16*)dh->data, dgu, (int64_t)(s.T * s.F), activation, &back, st));
     const bool rows_ok = s.D % 8 == 0 && s.F % 8 == 0;
     if (dw) {  // dw[i] (+)= x^T dgu[i]
         GemmArgs a{};
@@ -409,7 +410,8 @@ int evkhip_gated_linear_backward(const evkhip_tensor* x, const evkhip_tensor* w,
         a.sB = (int64_t)(s.T * s.F);
         a.sC = (int64_t)s.D * s.F;
         a.acc = accumulate ? 1 : 0;
-        CHECK(gemm_dispatch(a, 2, true, false, rows_ok && aligned16(x->data) && aligned16(dw->data), st));
+        a.back = back;
+        CHECK(scaled_dispatch(a, 2, rows_ok && aligned16(x->data) && aligned16(dw->data), st));
     }
     if (dx) {  // dx = dgu[0] w[0]^T + dgu[1] w[1]^T
         GemmArgs a{};
@@ -419,6 +421,7 @@ int evkhip_gated_linear_backward(const evkhip_tensor* x, const evkhip_tensor* w,
         a.M = (int)s.T;
         a.N = (int)s.D;
         a.K = (int)s.F;
+        a.back = back;
         CHECK(pair_dispatch(a, rows_ok && aligned16(w->data) && aligned16(dx->data), st));
     }
     return EVKHIP_OK;

@@ -195,6 +195,7 @@ DEV int xcd_tile(int w, int total) {
     return x * (total / 8) + min(x, total % 8) + w / 8;
 }
 
+DEV float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
 DEV float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
@@ -250,6 +251,15 @@ DEV float gelu_fast(float x) {
 // x / (1 + e^-x) on the hardware exponential and reciprocal
 DEV float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x)); }
 DEV float silu_f(float x) { return x * sigmoid_fast(x); }
+
+// What the gradients of a gated linear unit's products do not exceed, so far: |dh u act'(g)| <= 1.13 |dh u| and
+// |dh act(g)| <= |dh g| for silu, gelu and relu; values that are not finite are left out.  And the power of two that takes
+// it to 2^14 .. 2^15.
+DEV float glu_top(float top, float g, float u, float dh) {
+    const float x = fabsf(1.13f * dh * u), y = fabsf(dh * g);
+    return fmaxf(top, fmaxf(x < INFINITY ? x : 0.0f, y < INFINITY ? y : 0.0f));
+}
+DEV int glu_lift(float top) { return top > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; }
 
 // 16-byte accesses at any fp16 address
 DEV half8 ld_h8(const f16* p) {

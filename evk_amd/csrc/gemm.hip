@@ -190,7 +190,8 @@ DEV void wait_vmcnt(int n) {
 // of B, joined in the epilogue (C = act(A B0) * A B1); a tile holds BN / 2
 // columns of each, so A is read once for both and neither product passes memory.
 // GEMM_PAIR: the sum of two products, A0 B0 + A1 B1 (each second operand behind
-// the first one), whose K tiles follow each other: no partial C.  Bound by the
+// the first one), whose K tiles follow each other: no partial C.  It and
+// GEMM_SCALED, otherwise a product, store their sums times GemmArgs::back.  Bound by the
 // MFMA's feeding like the plain product: 6001 x 4096 x 2 x 11008 957 us = 1131
 // TFLOP/s (a large product of the library's reaches 1187); 2560 x 768 x 2 x 2048
 // with the kept products 33 us (160 tiles on 256 CUs), its pair 26 us.
@@ -200,9 +201,17 @@ DEV float glu_of(float a, float b, int act) {
     return (a < 0.0f ? 0.0f : a) * b;
 }
 
+// Every lane of the wave has to be here.
+DEV float back_of(const GemmBack& b) {
+    if (b.factor) return *b.factor;
+    float top = 0.0f;
+    for (int i = threadIdx.x & 63; i < b.n; i += 64) top = glu_top(top, (float)b.gate_up[i], (float)b.gate_up[b.n + i], (float)b.dh[i]);
+    return exp2i(-glu_lift(wave_max(top)));
+}
+
 template <int BM, int BN, bool TA, bool TB, int NWV, int KG, int NST, bool RAG, int KIND = GEMM_ONE>
 __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int tiles_m, int tiles_n) {
-    constexpr bool GLU = KIND == GEMM_GLU, PAIR = KIND == GEMM_PAIR;
+    constexpr bool GLU = KIND == GEMM_GLU, PAIR = KIND == GEMM_PAIR, SCALED = KIND == GEMM_PAIR || KIND == GEMM_SCALED;
     static_assert(!GLU || (!TA && !TB), "rows of A against both matrices as they are");
     constexpr int WGN = NWV / 2;  // waves along N (2 along M)
     constexpr int BK = MB_K, WM = BM / 2, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
@@ -480,6 +489,13 @@ __global__ __launch_bounds__(64 * NWV * KG, 1) void gemm_mfma(GemmArgs p, int ti
         stage2([&](float a, float b) { return glu_of(a, b, p.act); });
         write_out(Cp);
         return;
+    }
+    if constexpr (SCALED) {
+        const float back = back_of(p.back);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] *= back;
     }
     auto stage = [&](auto&& f) {  // LDS tile = fp16(f(sum, what it holds))
 #pragma unroll
@@ -932,8 +948,11 @@ __global__ __launch_bounds__(64 * NW) void glu_skinny(GemmArgs p) {
 
 // ---- short K, any alignment: one thread per element of C.  Launch-bound up
 // to a few thousand elements; a chain of K loads of each operand otherwise ----
+template <int KIND>
 __global__ __launch_bounds__(256) void gemm_short(GemmArgs p, int ta, int tb) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    float back = 1.0f;
+    if constexpr (KIND == GEMM_SCALED) back = back_of(p.back);
     if (i >= (int64_t)p.M * p.N) return;
     const int bz = blockIdx.y, row = (int)(i / p.N), col = (int)(i % p.N);
     const f16* a = p.A + (int64_t)bz * p.sA + (ta ? (int64_t)row : (int64_t)row * p.K);
@@ -942,6 +961,7 @@ __global__ __launch_bounds__(256) void gemm_short(GemmArgs p, int ta, int tb) {
     float v = 0.0f;
 #pragma unroll 4
     for (int k = 0; k < p.K; ++k) v += (float)a[k * step_a] * (float)b[k * step_b];
+    if constexpr (KIND == GEMM_SCALED) v *= back;
     f16* c = p.C + (int64_t)bz * p.sC + i;
     *c = (f16)(p.acc ? v + (float)*c : v);
 }
@@ -1039,11 +1059,11 @@ int choose_plan(const GemmArgs& a, int batch, unsigned allowed) {
     return best;
 }
 
-template <int PLAN, bool TA, bool TB, bool RAG>
+template <int PLAN, bool TA, bool TB, bool RAG, int KIND = GEMM_ONE>
 hipError_t launch_mfma(const GemmArgs& a, int batch, hipStream_t st) {
     constexpr GemmPlan P = kPlans[PLAN];
     const int tm = (a.M + P.bm - 1) / P.bm, tn = (a.N + P.bn - 1) / P.bn;
-    hipLaunchKernelGGL((gemm_mfma<P.bm, P.bn, TA, TB, P.waves, P.kg, RAG ? 2 : P.stages, RAG>),
+    hipLaunchKernelGGL((gemm_mfma<P.bm, P.bn, TA, TB, P.waves, P.kg, RAG ? 2 : P.stages, RAG, KIND>),
                        dim3((unsigned)(tm * tn), 1, batch), dim3(64 * P.waves * P.kg), 0, st, a, tm, tn);
     return hipGetLastError();
 }
@@ -1220,6 +1240,35 @@ int pair_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st) {
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "gated_linear_backward launch");
 }
 
+int scaled_dispatch(const GemmArgs& a, int batch, bool vec_ok, hipStream_t st) {
+    if (a.M == 0 || a.N == 0) return EVKHIP_OK;
+    hipError_t e;
+    const bool direct = vec_ok && (int64_t)a.M * a.K * 2 < INT32_MAX && (int64_t)a.K * a.N * 2 < INT32_MAX &&
+                        (int64_t)a.M * a.N < INT32_MAX;
+    if (!vec_ok && short_k_wins(a, batch, false)) {
+        const dim3 grid((unsigned)(((int64_t)a.M * a.N + 255) / 256), batch);
+        hipLaunchKernelGGL(gemm_short<GEMM_SCALED>, grid, dim3(256), 0, st, a, 1, 0);
+        e = hipGetLastError();
+    } else if (direct) {
+        switch (choose_plan(a, batch, kColPlans)) {
+            case 0: e = launch_mfma<0, true, false, false, GEMM_SCALED>(a, batch, st); break;
+            case 1: e = launch_mfma<1, true, false, false, GEMM_SCALED>(a, batch, st); break;
+            case 2: e = launch_mfma<2, true, false, false, GEMM_SCALED>(a, batch, st); break;
+            case 3: e = launch_mfma<3, true, false, false, GEMM_SCALED>(a, batch, st); break;
+            case 4: e = launch_mfma<4, true, false, false, GEMM_SCALED>(a, batch, st); break;
+            case 5: e = launch_mfma<5, true, false, false, GEMM_SCALED>(a, batch, st); break;
+            default: e = launch_mfma<6, true, false, false, GEMM_SCALED>(a, batch, st); break;
+        }
+    } else {
+        switch (choose_plan(a, batch, kRagPlans)) {
+            case 1: e = launch_mfma<1, true, false, true, GEMM_SCALED>(a, batch, st); break;
+            case 4: e = launch_mfma<4, true, false, true, GEMM_SCALED>(a, batch, st); break;
+            default: e = launch_mfma<6, true, false, true, GEMM_SCALED>(a, batch, st); break;
+        }
+    }
+    return e == hipSuccess ? EVKHIP_OK : check_hip(e, "gated_linear_backward launch");
+}
+
 int gemm_dispatch(const GemmArgs& a, int batch, bool ta, bool tb, bool vec_ok, hipStream_t st,
                   const GemvScratch* fixed) {
     if (a.M == 0 || a.N == 0) return EVKHIP_OK;
@@ -1275,7 +1324,7 @@ int gemm_dispatch(const GemmArgs& a, int batch, bool ta, bool tb, bool vec_ok, h
                         (int64_t)a.M * a.N < INT32_MAX;
     if (!vec_ok && a.epi == GEMM_STORE && short_k_wins(a, batch, tb)) {
         const dim3 grid((unsigned)(((int64_t)a.M * a.N + 255) / 256), batch);
-        hipLaunchKernelGGL(gemm_short, grid, dim3(256), 0, st, a, (int)ta, (int)tb);
+        hipLaunchKernelGGL(gemm_short<GEMM_ONE>, grid, dim3(256), 0, st, a, (int)ta, (int)tb);
         e = hipGetLastError();
     } else if (direct) {
         e = launch_plan(choose_plan(a, batch, ta ? kColPlans : kRowPlans), a, batch, ta, tb, st);

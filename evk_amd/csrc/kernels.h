@@ -13,6 +13,14 @@ struct QkvDest {
     f16 *kc, *vc;        // cache rows 0..M-1: (M, d)
     int dh;              // head size, a multiple of 8
 };
+// A power of two that a product's store takes back: *factor, or, where that is
+// null, what the n values of a gated linear unit make it (glu_top).
+constexpr int GLU_FEW = 256;
+struct GemmBack {
+    const float* factor;
+    const f16 *gate_up, *dh;
+    int n;
+};
 struct GemmArgs {
     const f16* A;
     const f16* B;
@@ -24,18 +32,22 @@ struct GemmArgs {
     QkvDest qkv;         // GEMM_QKV (C is not written)
     f16* gate_up;        // glu_dispatch: both products, (2, M, N), or null
     int act;             // glu_dispatch: EVKHIP_ACT_*
+    GemmBack back;       // pair_dispatch, scaled_dispatch
 };
 // Ops folded into the store of a product, with the roundings of the separate
 // ops: C = fp16(C + fp16(A B)), C = fp16(gelu(fp16(A B))), and rope of the q
 // and k columns of fp16(A B), regrouped per head and into the cache (A and B
 // row-major, N % 24 == 0).
 enum { GEMM_STORE = 0, GEMM_RESIDUAL = 1, GEMM_GELU = 2, GEMM_QKV = 3 };
-// gemm_mfma's forms: one product, a gated linear unit, a sum of two products
-enum { GEMM_ONE = 0, GEMM_GLU = 1, GEMM_PAIR = 2 };
+// gemm_mfma's forms: one product, a gated linear unit, a sum of two products, one
+// product (the latter two times GemmArgs::back)
+enum { GEMM_ONE = 0, GEMM_GLU = 1, GEMM_PAIR = 2, GEMM_SCALED = 3 };
 // C (M, N) = act(A B[0]) * (A B[1]): A (M, K), B (2, K, N).
 int glu_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st);
-// C (M, N) = A[0] B[0]^T + A[1] B[1]^T: A (2, M, K), B (2, N, K).
+// C (M, N) = (A[0] B[0]^T + A[1] B[1]^T) back: A (2, M, K), B (2, N, K).
 int pair_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st);
+// C (+)= A^T B back, A (K, M), `batch` of them with strides as in gemm_dispatch.
+int scaled_dispatch(const GemmArgs& a, int batch, bool vec_ok, hipStream_t st);
 // Caller-provided split-K scratch of the skinny (M <= 16) path: partials and
 // arrival counters.  With it, gemm_dispatch allocates nothing.
 struct GemvScratch {
@@ -144,7 +156,9 @@ int cross_entropy_launch(const f16* logits, const uint16_t* tgt, f16* grad, f16*
                          bool vec, hipStream_t st);
 int sum_batch_launch(const f16* in, f16* out, int batch, int64_t per_batch, hipStream_t st);
 int causal_mask_launch(f16* scores, int64_t batch, int N, hipStream_t st);
-int glu_bwd_launch(const f16* gate_up, const f16* dh, f16* dgu, int64_t n, int act, hipStream_t st);
+// Gradients of a gated linear unit's products, (2, n) at the start of `ws` (glu_bwd_workspace bytes), times 1 / *out.
+uint64_t glu_bwd_workspace(uint64_t n);
+int glu_bwd_launch(const f16* gate_up, const f16* dh, void* ws, int64_t n, int act, GemmBack* out, hipStream_t st);
 int position_add_launch(const f16* in, const f16* pos, f16* out, int B, int64_t per_batch, hipStream_t st);
 int position_add_bwd_launch(const f16* gout, f16* gin, f16* gpos, int B, int64_t per_batch, hipStream_t st);
 int rope_bwd_launch(const f16* gout, f16* gin, int B, int S, int E, float base, hipStream_t st);

@@ -44,9 +44,11 @@ DEV half8 ld_stream(const half8* p) {
 DEV void st_stream(half8* p, const half8& v) {
     __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(p));
 }
+template <bool STREAM = true>
 DEV void ld8(const f16* p, int64_t i0, int64_t n, bool vec, float (&v)[8]) {
     if (vec && i0 + 8 <= n) {
-        const half8 h = ld_stream(reinterpret_cast<const half8*>(p + i0));
+        const half8* at = reinterpret_cast<const half8*>(p + i0);
+        const half8 h = STREAM ? ld_stream(at) : *at;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (float)h[e];
     } else {
@@ -153,23 +155,68 @@ DEV float act_of(float g, int act, float* grad) {
 }
 // Gradients of both products of a gated linear unit, h = act(g) u: dg = dh u
 // act'(g), du = dh act(g), from the g and u that the forward kept.  They are the
-// operands of two fp16 products each and so rounded to fp16 here, once.
-// Memory-bound: 2560 x 2048 12.2 us, 4.3 TB/s; a pass of its own, since each
-// value is an operand of D / 128 tiles of either product.
-__global__ __launch_bounds__(EW_NT) void glu_bwd_k(const f16* gate_up, const f16* dh, f16* dgu, int64_t n, int act,
-                                                   bool vec) {
+// operands of two fp16 products each and so rounded to fp16 here, once, times
+// the power of two that takes a bound of them (glu_top) to 2^14 .. 2^15 and that
+// the products' stores take back: neither a loss scale nor a mean over a batch
+// leaves fp16's 30 powers of two.
+// Memory-bound, two passes: 2560 x 2048 7.8 us for the bound (512 workgroups 10.5,
+// 2560 8.3 and 2.4 more to read their parts) and 10.6 for the values, 4.9 TB/s; a
+// pass of its own, since each value is an operand of D / 128 tiles of either
+// product.
+//
+// Parts of the bound in tops[0 .. gridDim.x), for more values than one workgroup holds.
+__global__ __launch_bounds__(EW_NT) void glu_top_k(const f16* gate_up, const f16* dh, float* tops, int64_t n, bool vec) {
+    float top = 0.0f;
+    for (int64_t i0 = first8(); i0 < n; i0 += (int64_t)gridDim.x * EW_NT * 8) {
+        float g[8], u[8], h[8];
+        ld8<false>(gate_up, i0, n, vec, g);
+        ld8<false>(gate_up + n, i0, n, vec, u);
+        ld8<false>(dh, i0, n, vec, h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = glu_top(top, g[e], u[e], h[e]);
+    }
+    __shared__ float red[EW_NT / 64];
+    top = wave_max(top);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) tops[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+// count: workgroups of glu_top_k, a multiple of 4; 0 where this is one workgroup, which finds the bound itself.
+// The factor that takes the power back goes to *back (null: the products find it, too).
+__global__ __launch_bounds__(EW_NT) void glu_bwd_k(const f16* gate_up, const f16* dh, f16* dgu, const float* tops, int count, float* back,
+                                                   int64_t n, int act, bool vec) {
     const int64_t i0 = first8();
+    float g[8] = {}, u[8] = {}, h[8] = {}, top = 0.0f;
+    if (i0 < n) {
+        ld8(gate_up, i0, n, vec, g);
+        ld8(gate_up + n, i0, n, vec, u);
+        ld8(dh, i0, n, vec, h);
+    }
+    if (count) {
+        for (int i = threadIdx.x % 64 * 4; i < count; i += 256) {
+            const floatx4 t = *reinterpret_cast<const floatx4*>(tops + i);
+            top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), top);
+        }
+        top = wave_max(top);
+    } else {
+        __shared__ float red[EW_NT / 64];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = glu_top(top, g[e], u[e], h[e]);
+        top = wave_max(top);
+        if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    }
+    const int lift = glu_lift(top);
+    if (back && blockIdx.x == 0 && threadIdx.x == 0) *back = exp2i(-lift);
     if (i0 >= n) return;
-    float g[8], u[8], h[8];
-    ld8(gate_up, i0, n, vec, g);
-    ld8(gate_up + n, i0, n, vec, u);
-    ld8(dh, i0, n, vec, h);
+    const float up = exp2i(lift);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         float da;
         const float a = act_of(g[e], act, &da);
-        g[e] = h[e] * u[e] * da;
-        u[e] = h[e] * a;
+        g[e] = h[e] * u[e] * da * up;
+        u[e] = h[e] * a * up;
     }
     st8(dgu, i0, n, vec, g);
     st8(dgu + n, i0, n, vec, u);
@@ -817,10 +864,37 @@ int gelu_bwd_launch(const f16* gout, const f16* in, f16* gin, int64_t n, bool ve
     hipLaunchKernelGGL(gelu_bwd_k, dim3(ew_grid8(n)), dim3(EW_NT), 0, st, gout, in, gin, n, vec);
     return launched("gelu_backward launch");
 }
-int glu_bwd_launch(const f16* gate_up, const f16* dh, f16* dgu, int64_t n, int act, hipStream_t st) {
-    if (n == 0) return EVKHIP_OK;
+namespace {
+// Workgroups of glu_top_k: none up to a workgroup's values, whose gradients' kernel is one workgroup.
+int glu_top_groups(uint64_t n) {
+    return n <= EW_NT * 8 ? 0 : (int)std::min<uint64_t>(((n + EW_NT * 8 - 1) / (EW_NT * 8) + 3) / 4 * 4, 1024);
+}
+uint64_t glu_grads_bytes(uint64_t n) { return (2 * n * sizeof(f16) + 15) / 16 * 16; }
+}  // namespace
+
+// Both gradients, then 16 bytes for the factor and the bound's parts; up to GLU_FEW values the products find the
+// factor themselves.
+uint64_t glu_bwd_workspace(uint64_t n) {
+    return n <= GLU_FEW ? 2 * n * sizeof(f16) : glu_grads_bytes(n) + 16 + glu_top_groups(n) * sizeof(float);
+}
+int glu_bwd_launch(const f16* gate_up, const f16* dh, void* ws, int64_t n, int act, GemmBack* out, hipStream_t st) {
+    f16* const dgu = (f16*)ws;
+    *out = GemmBack{nullptr, gate_up, dh, (int)n};
     const bool vec = n % 8 == 0 && aligned16(gate_up) && aligned16(dh) && aligned16(dgu);
-    hipLaunchKernelGGL(glu_bwd_k, dim3(ew_grid8(n)), dim3(EW_NT), 0, st, gate_up, dh, dgu, n, act, vec);
+    const int groups = glu_top_groups(n);
+    float* back = nullptr;
+    float* tops = nullptr;
+    if (n > GLU_FEW) {
+        back = (float*)((char*)ws + glu_grads_bytes(n));
+        tops = back + 4;
+        *out = GemmBack{back, nullptr, nullptr, 0};
+    }
+    if (groups) {
+        hipLaunchKernelGGL(glu_top_k, dim3(groups), dim3(EW_NT), 0, st, gate_up, dh, tops, n, vec);
+        const int rc = launched("gated_linear_backward launch");
+        if (rc != EVKHIP_OK) return rc;
+    }
+    hipLaunchKernelGGL(glu_bwd_k, dim3(ew_grid8(n)), dim3(EW_NT), 0, st, gate_up, dh, dgu, tops, groups, back, n, act, vec);
     return launched("gated_linear_backward launch");
 }
 int sgd_launch(f16* param, const f16* grad, float lr, int64_t n, bool vec, hipStream_t st) {

@@ -960,7 +960,6 @@ __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int split
 // fp16; now 0.6 both, at any length).
 constexpr int P_LIFT = 15, DS_TOP = 14, DQ_LIFT = 10, DQ_STEP = 7;
 constexpr int K_LEAST = -24;  // of rows that are zero, or not finite (those spoil what they are part of at any power)
-DEV float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
 typedef short short2_t __attribute__((ext_vector_type(2)));  // a pair of exponents
 DEV short2_t max_xor(short2_t v, int o) {
     return __builtin_elementwise_max(v, __builtin_bit_cast(short2_t, __shfl_xor(__builtin_bit_cast(int, v), o, 64)));

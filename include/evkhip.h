@@ -378,7 +378,9 @@ int evkhip_gated_linear(const evkhip_tensor* x, const evkhip_tensor* w, const ev
 
 /* Its gradient from the forward's gate_up: dx (as x) is written; dw (as w) is
  * written, or added to with accumulate.  Either may be NULL (not wanted).  The
- * gradients of both products pass through fp16 once. */
+ * gradients of both products are rounded to fp16 once, times a power of two for
+ * the call (by the largest |dh u| and |dh g|) that dx and dw take back, so that
+ * their size does not matter; those below 2^-28 of the largest lose bits. */
 uint64_t evkhip_gated_linear_backward_workspace(uint64_t tokens, uint32_t d, uint32_t f);
 int evkhip_gated_linear_backward(const evkhip_tensor* x, const evkhip_tensor* w, const evkhip_tensor* gate_up,
                                  const evkhip_tensor* dh, const evkhip_tensor* dx, const evkhip_tensor* dw,

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import evk_amd as evk
-from test_gpu_block import F16, F64, H, T, Rng, close, empty, rope_want, seen, window_want
+from test_gpu_block import E, F16, F64, H, T, Rng, act64, close, empty, rope_want, seen, window_want
 
 pytestmark = pytest.mark.gpu
 
@@ -261,3 +261,68 @@ def test_window_attention_bwd_overflow_costs_no_more(dev, dh, h, kv, n, window, 
     wild = passes_us(step, 2)
     assert not torch.isfinite(g[1].float()).all()
     assert wild <= (20 if where == "do everywhere" else 6) * clean + 50, f"{wild:.0f} us with an infinity, {clean:.0f} without"
+
+
+# ---------------------------------------------------------------------------
+# gated_linear: gradients of every size, an infinite gate
+# ---------------------------------------------------------------------------
+SIZES = [  # dh, up, x and w: std
+    (2.0 ** -17, 1.0, 4.0, 4.0), (2.0 ** -13, 1.0, 2.0, 2.0), (4000.0, 30.0, 2.0 ** -10, 2.0 ** -10), (10000.0, 200.0, 2.0 ** -14, 2.0 ** -14),
+]
+
+
+@pytest.mark.parametrize("size,up,sx,sw", SIZES)
+@pytest.mark.parametrize("t,d,f,odd", [(1, 64, 128, False), (3, 40, 56, False), (37, 520, 200, False), (600, 768, 1024, False), (1500, 96, 640, False),
+                                       (50, 33, 77, True), (300, 100, 201, False), (5, 33, 77, True), (20, 64, 96, False),
+                                       (2, 300, 128, False), (1, 24, 257, False)])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_gated_linear_backward_gradient_sizes(dev, t, d, f, odd, act, size, up, sx, sw):
+    """Gradients as small as a mean over a batch makes them and as large as loss scaling does: the products' gradients
+    neither vanish nor overflow on their way into dx and dw."""
+    r = Rng(dev, 9000 + t + f)
+    x, w = r(t, d, odd=odd, std=sx), r(2, d, f, std=sw, odd=odd)
+    gu, dh = torch.stack([r(t, f), r(t, f, std=up)]), r(t, f, std=size)
+    if odd:
+        gu, dh = empty(dev, 2, t, f, odd=True).copy_(gu), empty(dev, t, f, odd=True).copy_(dh)
+    X, W, G = x.to(F64), w.to(F64), dh.to(F64)
+    a, da = act64(gu[0].to(F64), act)
+    dgu = torch.stack([G * gu[1].to(F64) * da, G * a])
+    # rounded to fp16 with what bounds them, |dh u| and |dh g| (1.13 being the steepest slope), at 2^14 at least, so that
+    # subnormals are off by 2^-39 of that; the functions to 2^-20
+    most = max(float((G * gu[1].to(F64)).abs().max()) * 1.13, float((G * gu[0].to(F64)).abs().max()))
+    edgu = H * dgu.abs() + 2.0 ** -39 * most + 2.0 ** -19 * torch.stack([(G * gu[1].to(F64)).abs(), G.abs()]) * (1 + gu[0].to(F64).abs())
+    dx = dgu[0] @ W[0].t() + dgu[1] @ W[1].t()
+    mag = dgu[0].abs() @ W[0].abs().t() + dgu[1].abs() @ W[1].abs().t()
+    dx_t = edgu[0] @ W[0].abs().t() + edgu[1] @ W[1].abs().t() + (2 * f + 2) * E * mag + H * dx.abs() + T
+    dw = torch.stack([X.t() @ dgu[0], X.t() @ dgu[1]])
+    dw_t = torch.stack([X.abs().t() @ (edgu[i] + (t + 2) * E * dgu[i].abs()) for i in range(2)]) + H * dw.abs() + T
+    assert dx.abs().max() < 60000 and dw.abs().max() < 60000
+    gx, gw = empty(dev, t, d, odd=odd), empty(dev, 2, d, f, odd=odd)
+    evk.gated_linear_backward(x, w, gu, dh, gx, gw, act)
+    for g, want, tol, what in ((gx, dx, dx_t, "dx"), (gw, dw, dw_t, "dw")):
+        close(g, want, tol, what, norm=None)
+        # two roundings, and the result's own subnormals
+        assert (g.to(F64) - want).norm() <= 2 * H * want.norm() + T * want.numel() ** 0.5, what
+    more = gw.clone()
+    evk.gated_linear_backward(x, w, gu, dh, None, more, act, True)
+    close(more, 2 * dw, 2 * dw_t + H * (2 * dw).abs() + T, "dw added to", norm=None)
+
+
+@pytest.mark.parametrize("t,f", [(1, 64), (40, 200)])
+def test_gated_linear_backward_wild_values(dev, t, f):
+    """A row of the gradient that overflowed stays in its own row of dx; the others keep their bits."""
+    r = Rng(dev, 70)
+    d = 64
+    x, w, gu, dh = r(t + 1, d), r(2, d, f, std=0.1), r(2, t + 1, f), r(t + 1, f)
+    clean, dx = torch.empty(t + 1, d, dtype=F16, device=dev), torch.empty(t + 1, d, dtype=F16, device=dev)
+    evk.gated_linear_backward(x, w, gu, dh, clean)
+    dh[t, 1] = math.inf
+    gu[1, t, 3] = math.nan
+    dw = torch.empty_like(w)
+    evk.gated_linear_backward(x, w, gu, dh, dx, dw)
+    assert not torch.isfinite(dx[t].float()).any()
+    if t > 1:
+        close(dx[:t], clean[:t].to(F64), 2 * H * clean[:t].abs().to(F64) + T, "dx")
+    hit = torch.zeros(f, dtype=torch.bool, device=dev)
+    hit[1] = hit[3] = True
+    assert torch.isfinite(dw[:, :, ~hit]).all() and not torch.isfinite(dw[0][:, hit].float()).any()
