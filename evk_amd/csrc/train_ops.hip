@@ -139,19 +139,25 @@ __global__ __launch_bounds__(EW_NT) void gelu_bwd_k(const f16* gout, const f16* 
     st8(gin, i0, n, vec, a);
 }
 
-// Activation of a gated linear unit and its slope
+// Activation of a gated linear unit and its slope.  A gate past fp16 was kept as
+// an infinity: its slope is 1 above and 0 below, as of the largest finite gates,
+// and the activation as infinite above and 0 below.
 DEV float act_of(float g, int act, float* grad) {
+    float a, d;
     if (act == EVKHIP_ACT_SILU) {
         const float sg = sigmoid_fast(g);
-        *grad = sg * (1.0f + g * (1.0f - sg));
-        return g * sg;
+        d = sg * (1.0f + g * (1.0f - sg));
+        a = g * sg;
+    } else if (act == EVKHIP_ACT_GELU) {
+        d = gelu_grad(g);
+        a = gelu_fast(g);
+    } else {
+        d = g > 0.0f ? 1.0f : 0.0f;
+        a = g < 0.0f ? 0.0f : g;
     }
-    if (act == EVKHIP_ACT_GELU) {
-        *grad = gelu_grad(g);
-        return gelu_fast(g);
-    }
-    *grad = g > 0.0f ? 1.0f : 0.0f;
-    return g < 0.0f ? 0.0f : g;
+    const bool inf = fabsf(g) == INFINITY;
+    *grad = inf ? __builtin_amdgcn_fmed3f(g, 0.0f, 1.0f) : d;
+    return inf ? fmaxf(g, 0.0f) : a;
 }
 // Gradients of both products of a gated linear unit, h = act(g) u: dg = dh u
 // act'(g), du = dh act(g), from the g and u that the forward kept.  They are the
@@ -159,10 +165,9 @@ DEV float act_of(float g, int act, float* grad) {
 // the power of two that takes a bound of them (glu_top) to 2^14 .. 2^15 and that
 // the products' stores take back: neither a loss scale nor a mean over a batch
 // leaves fp16's 30 powers of two.
-// Memory-bound, two passes: 2560 x 2048 7.8 us for the bound (512 workgroups 10.5,
-// 2560 8.3 and 2.4 more to read their parts) and 10.6 for the values, 4.9 TB/s; a
-// pass of its own, since each value is an operand of D / 128 tiles of either
-// product.
+// Memory-bound, two passes: 2560 x 2048 7.8 us for the bound (512 workgroups
+// 10.5, 2560 8.3) and 10.4 for the values, 5.0 TB/s; a pass of its own, since each
+// value is an operand of D / 128 tiles of either product.
 //
 // Parts of the bound in tops[0 .. gridDim.x), for more values than one workgroup holds.
 __global__ __launch_bounds__(EW_NT) void glu_top_k(const f16* gate_up, const f16* dh, float* tops, int64_t n, bool vec) {
@@ -193,20 +198,19 @@ __global__ __launch_bounds__(EW_NT) void glu_bwd_k(const f16* gate_up, const f16
         ld8(dh, i0, n, vec, h);
     }
     if (count) {
-        for (int i = threadIdx.x % 64 * 4; i < count; i += 256) {
+        for (int i = threadIdx.x * 4; i < count; i += EW_NT * 4) {
             const floatx4 t = *reinterpret_cast<const floatx4*>(tops + i);
             top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), top);
         }
-        top = wave_max(top);
     } else {
-        __shared__ float red[EW_NT / 64];
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = glu_top(top, g[e], u[e], h[e]);
-        top = wave_max(top);
-        if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     }
+    __shared__ float red[EW_NT / 64];
+    top = wave_max(top);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const int lift = glu_lift(top);
     if (back && blockIdx.x == 0 && threadIdx.x == 0) *back = exp2i(-lift);
     if (i0 >= n) return;

@@ -377,7 +377,8 @@ int evkhip_gated_linear(const evkhip_tensor* x, const evkhip_tensor* w, const ev
                         const evkhip_tensor* gate_up, int activation, void* stream);
 
 /* Its gradient from the forward's gate_up: dx (as x) is written; dw (as w) is
- * written, or added to with accumulate.  Either may be NULL (not wanted).  The
+ * written, or added to with accumulate.  Either may be NULL (not wanted).  A
+ * gate past fp16, kept as an infinity, has slope 1 above and 0 below.  The
  * gradients of both products are rounded to fp16 once, times a power of two for
  * the call (by the largest |dh u| and |dh g|) that dx and dw take back, so that
  * their size does not matter; those below 2^-28 of the largest lose bits. */

@@ -326,3 +326,37 @@ def test_gated_linear_backward_wild_values(dev, t, f):
     hit = torch.zeros(f, dtype=torch.bool, device=dev)
     hit[1] = hit[3] = True
     assert torch.isfinite(dw[:, :, ~hit]).all() and not torch.isfinite(dw[0][:, hit].float()).any()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_gated_linear_infinite_gate(dev, act):
+    """A gate past fp16, kept as an infinity: its slope is 1 above and 0 below; the second product's gradient is infinite
+    above and 0 below."""
+    t, d, f = 3, 64, 128
+    r = Rng(dev, 71)
+    x, w, dh = r(t, d), r(2, d, f, std=0.1), r(t, f)
+    gu = r(2, t, f)
+    gu[0, 0, 5], gu[0, 1, 6] = math.inf, -math.inf
+    gu[1, 0, 5], gu[1, 1, 6] = 1.0, 1.0
+    dw = torch.empty_like(w)
+    evk.gated_linear_backward(x, w, gu, dh, dw=dw, activation=act)
+    gc = gu.to(F64).clamp(-60000, 60000)
+    a, da = act64(gc[0], act)
+    X, G = x.to(F64), dh.to(F64)
+    dgu = torch.stack([G * gc[1] * da, G * a])
+    assert abs(float(da[0, 5]) - 1) < 1e-9 and abs(float(da[1, 6])) < 1e-9
+    edgu = H * dgu.abs() + T + 2.0 ** -19 * torch.stack([(G * gc[1]).abs(), G.abs()]) * (1 + gc[0].abs().clamp(max=100.0))
+    want = torch.stack([X.t() @ dgu[0], X.t() @ dgu[1]])
+    tol = torch.stack([X.abs().t() @ (edgu[i] + (t + 2) * E * dgu[i].abs()) for i in range(2)]) + H * want.abs() + T
+    close(dw[0], want[0], tol[0], "dw of the gate", norm=None)
+    up = torch.ones(f, dtype=torch.bool, device=dev)
+    up[5] = False
+    close(dw[1][:, up], want[1][:, up], tol[1][:, up], "dw of the second product", norm=None)
+    assert not torch.isfinite(dw[1][:, 5].float()).any()
+    # forward: sums past fp16 but within 32 bits
+    big = torch.full((t, d), 60000.0, dtype=F16, device=dev)
+    one = torch.zeros(2, d, f, dtype=F16, device=dev)
+    one[0, 0, 0], one[0, 0, 1], one[1, 0, :2] = 60000.0, -60000.0, 2.0 ** -18
+    h, keep = torch.empty(t, f, dtype=F16, device=dev), torch.empty(2, t, f, dtype=F16, device=dev)
+    evk.gated_linear(big, one, h, keep, act)
+    assert torch.isinf(keep[0, :, :2]).all() and torch.isinf(h[:, 0]).all() and (h[:, 1] == 0).all()
