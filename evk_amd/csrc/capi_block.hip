@@ -396,34 +396,35 @@ int evkhip_gated_linear_backward(const evkhip_tensor* x, const evkhip_tensor* w,
         return EVKHIP_OK;
     }
     f16* dgu = (f16*)workspace;
-    GemmBack back;
-    CHECK(glu_bwd_launch((const f16*)gate_up->data, (const f16*)dh->data, dgu, (int64_t)(s.T * s.F), activation, &back, st));
     const bool rows_ok = s.D % 8 == 0 && s.F % 8 == 0;
+    GemmArgs gw{}, gx{};
+    const bool gw_ok = rows_ok && aligned16(x->data) && dw && aligned16(dw->data);
+    const bool gx_ok = rows_ok && aligned16(w->data) && dx && aligned16(dx->data);
     if (dw) {  // dw[i] (+)= x^T dgu[i]
-        GemmArgs a{};
-        a.A = (const f16*)x->data;
-        a.B = dgu;
-        a.C = (f16*)dw->data;
-        a.M = (int)s.D;
-        a.N = (int)s.F;
-        a.K = (int)s.T;
-        a.sB = (int64_t)(s.T * s.F);
-        a.sC = (int64_t)s.D * s.F;
-        a.acc = accumulate ? 1 : 0;
-        a.back = back;
-        CHECK(scaled_dispatch(a, 2, rows_ok && aligned16(x->data) && aligned16(dw->data), st));
+        gw.A = (const f16*)x->data;
+        gw.B = dgu;
+        gw.C = (f16*)dw->data;
+        gw.M = (int)s.D;
+        gw.N = (int)s.F;
+        gw.K = (int)s.T;
+        gw.sB = (int64_t)(s.T * s.F);
+        gw.sC = (int64_t)s.D * s.F;
+        gw.acc = accumulate ? 1 : 0;
+        CHECK(scaled_dispatch(gw, 2, gw_ok, st, true));
     }
     if (dx) {  // dx = dgu[0] w[0]^T + dgu[1] w[1]^T
-        GemmArgs a{};
-        a.A = dgu;
-        a.B = (const f16*)w->data;
-        a.C = (f16*)dx->data;
-        a.M = (int)s.T;
-        a.N = (int)s.D;
-        a.K = (int)s.F;
-        a.back = back;
-        CHECK(pair_dispatch(a, rows_ok && aligned16(w->data) && aligned16(dx->data), st));
+        gx.A = dgu;
+        gx.B = (const f16*)w->data;
+        gx.C = (f16*)dx->data;
+        gx.M = (int)s.T;
+        gx.N = (int)s.D;
+        gx.K = (int)s.F;
+        CHECK(pair_dispatch(gx, gx_ok, st, true));
     }
+    CHECK(glu_bwd_launch((const f16*)gate_up->data, (const f16*)dh->data, dgu, (int64_t)(s.T * s.F), activation, &gw.back, st));
+    gx.back = gw.back;
+    if (dw) CHECK(scaled_dispatch(gw, 2, gw_ok, st));
+    if (dx) CHECK(pair_dispatch(gx, gx_ok, st));
     return EVKHIP_OK;
 }
 

@@ -1110,11 +1110,20 @@ hipError_t launch_kind(const GemmArgs& a, hipStream_t st) {
 }
 
 template <int KIND>
-hipError_t launch_kind_plan(const GemmArgs& a, bool direct, hipStream_t st) {
+int kind_plan(const GemmArgs& a, bool direct) {
     GemmArgs as = a;
     if (KIND == GEMM_GLU) as.N = 2 * a.N;
     else as.K = 2 * a.K;
-    const int plan = choose_plan(as, 1, direct ? kRowPlans : kRagPlans);
+    return choose_plan(as, 1, direct ? kRowPlans : kRagPlans);
+}
+// Whether one launch holds the plan's tiles of C, `columns` wide.
+int check_plan(const char* op, const GemmPlan& p, const GemmArgs& a, int columns) {
+    return check_grid(op, (int64_t)((a.M + p.bm - 1) / p.bm) * ((a.N + columns - 1) / columns), 64 * p.waves * p.kg);
+}
+
+template <int KIND>
+hipError_t launch_kind_plan(const GemmArgs& a, bool direct, hipStream_t st) {
+    const int plan = kind_plan<KIND>(a, direct);
     if (!direct) {
         switch (plan) {
             case 1: return launch_kind<1, true, KIND>(a, st);
@@ -1228,24 +1237,37 @@ int glu_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st) {
         else narrow ? go(C32{}, I4{}, I8{}, I2{}) : go(C64{}, I4{}, I4{}, I3{});
         e = hipGetLastError();
     } else {
+        const GemmPlan& p = kPlans[kind_plan<GEMM_GLU>(a, direct)];
+        const int rc = check_plan("gated_linear", p, a, p.bn / 2);
+        if (rc != EVKHIP_OK) return rc;
         e = launch_kind_plan<GEMM_GLU>(a, direct, st);
     }
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "gated_linear launch");
 }
 
-int pair_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st) {
+int pair_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st, bool check_only) {
     const bool direct = vec_ok && (int64_t)a.M * a.K * 2 < INT32_MAX && (int64_t)a.K * a.N * 2 < INT32_MAX &&
                         (int64_t)a.M * a.N < INT32_MAX;
+    if (check_only) {
+        const GemmPlan& p = kPlans[kind_plan<GEMM_PAIR>(a, direct)];
+        return check_plan("gated_linear_backward", p, a, p.bn);
+    }
     const hipError_t e = launch_kind_plan<GEMM_PAIR>(a, direct, st);
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "gated_linear_backward launch");
 }
 
-int scaled_dispatch(const GemmArgs& a, int batch, bool vec_ok, hipStream_t st) {
+int scaled_dispatch(const GemmArgs& a, int batch, bool vec_ok, hipStream_t st, bool check_only) {
     if (a.M == 0 || a.N == 0) return EVKHIP_OK;
     hipError_t e;
     const bool direct = vec_ok && (int64_t)a.M * a.K * 2 < INT32_MAX && (int64_t)a.K * a.N * 2 < INT32_MAX &&
                         (int64_t)a.M * a.N < INT32_MAX;
-    if (!vec_ok && short_k_wins(a, batch, false)) {
+    const bool by_element = !vec_ok && short_k_wins(a, batch, false);
+    if (check_only) {
+        if (by_element) return check_grid("gated_linear_backward", ((int64_t)a.M * a.N + 255) / 256, 256);
+        const GemmPlan& p = kPlans[choose_plan(a, batch, direct ? kColPlans : kRagPlans)];
+        return check_plan("gated_linear_backward", p, a, p.bn);
+    }
+    if (by_element) {
         const dim3 grid((unsigned)(((int64_t)a.M * a.N + 255) / 256), batch);
         hipLaunchKernelGGL(gemm_short<GEMM_SCALED>, grid, dim3(256), 0, st, a, 1, 0);
         e = hipGetLastError();

@@ -45,9 +45,10 @@ enum { GEMM_ONE = 0, GEMM_GLU = 1, GEMM_PAIR = 2, GEMM_SCALED = 3 };
 // C (M, N) = act(A B[0]) * (A B[1]): A (M, K), B (2, K, N).
 int glu_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st);
 // C (M, N) = (A[0] B[0]^T + A[1] B[1]^T) back: A (2, M, K), B (2, N, K).
-int pair_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st);
+// check_only: only whether a launch holds it.
+int pair_dispatch(const GemmArgs& a, bool vec_ok, hipStream_t st, bool check_only = false);
 // C (+)= A^T B back, A (K, M), `batch` of them with strides as in gemm_dispatch.
-int scaled_dispatch(const GemmArgs& a, int batch, bool vec_ok, hipStream_t st);
+int scaled_dispatch(const GemmArgs& a, int batch, bool vec_ok, hipStream_t st, bool check_only = false);
 // Caller-provided split-K scratch of the skinny (M <= 16) path: partials and
 // arrival counters.  With it, gemm_dispatch allocates nothing.
 struct GemvScratch {

@@ -883,6 +883,8 @@ uint64_t glu_bwd_workspace(uint64_t n) {
 }
 int glu_bwd_launch(const f16* gate_up, const f16* dh, void* ws, int64_t n, int act, GemmBack* out, hipStream_t st) {
     f16* const dgu = (f16*)ws;
+    const int fits = check_grid("gated_linear_backward", (n + 8 * EW_NT - 1) / (8 * EW_NT), EW_NT);
+    if (fits != EVKHIP_OK) return fits;
     *out = GemmBack{nullptr, gate_up, dh, (int)n};
     const bool vec = n % 8 == 0 && aligned16(gate_up) && aligned16(dh) && aligned16(dgu);
     const int groups = glu_top_groups(n);

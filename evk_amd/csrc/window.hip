@@ -1591,8 +1591,10 @@ int window_forward(const WindowArgs& args, void* ws, hipStream_t st) {
     const int64_t nr = (int64_t)a.N * (a.H / a.KV), heads = (int64_t)a.B * a.KV;
     const int splits = fwd_splits(a.B, a.N, a.R, a.H, a.KV, a.dh, a.window, a.sinks);
     hipError_t e;
-    int rc = mfma_ok(a) ? splits ? check_grid("window_attention", (nr + 15) / 16 * heads * splits, 512) : EVKHIP_OK
-                        : check_grid("window_attention", rows, 64);
+    const int fwd_rows = 64 * query_blocks(nr, heads, a.dh);
+    int rc = !mfma_ok(a) ? check_grid("window_attention", rows, 64)
+             : splits    ? check_grid("window_attention", (nr + 15) / 16 * heads * splits, 512)
+                         : check_grid("window_attention", (nr + fwd_rows - 1) / fwd_rows * heads, 256);
     if (rc == EVKHIP_OK && mfma_ok(a) && splits > 1) rc = check_grid("window_attention", nr * heads, 256);
     if (rc != EVKHIP_OK) return rc;
     if (!mfma_ok(a)) {
@@ -1641,7 +1643,7 @@ Parts parts_for(int B, int N, int H, int KV, int dh, int window, int sinks) {
     // 2000, one head of 128, no window: 67.5, 58.9), and fewer than 2^24
     int64_t q = full == blocks ? std::max<int64_t>(1, span / 4) : span;
     while (q > 1 && items(q) * heads < 500 && q * keys * (H / KV) > 256) q /= 2;
-    while (items(q) * heads > (1 << 24) && q < blocks) q *= 2;
+    while (items(q) * heads >= (1 << 24) && q < blocks) q *= 2;
     Parts p{};
     p.q = (int)q;
     p.blocks = (int)blocks;
@@ -1676,8 +1678,10 @@ int window_backward(const WindowArgs& args, void* ws, hipStream_t st) {
     a.big = (int64_t)a.R * a.KV * a.dh * 2 >= INT32_MAX;
     const int64_t rows = (int64_t)a.B * a.N * a.H, kv_rows = (int64_t)a.B * a.R * a.KV;
     hipError_t e;
-    // the widest launch of either path: a wave for each key (rounded up to blocks of 64) or query row
-    const int rc = check_grid("window_attention_bwd", mfma_ok(a) ? (int64_t)a.B * a.KV * ((a.N + 63) / 64 * 64) : std::max(rows, kv_rows), 64);
+    // the widest launches of either path: a wave for each key (rounded up to blocks of 64) or query row, four for a tile
+    const int64_t group = a.H / a.KV, heads = (int64_t)a.B * a.KV, dq_rows = 64 * query_blocks(a.N * group, heads, a.dh);
+    int rc = check_grid("window_attention_bwd", mfma_ok(a) ? heads * ((a.N + 63) / 64 * 64) : std::max(rows, kv_rows), 64);
+    if (rc == EVKHIP_OK && mfma_ok(a)) rc = check_grid("window_attention_bwd", (a.N * group + dq_rows - 1) / dq_rows * heads, 256);
     if (rc != EVKHIP_OK) return rc;
     if (mfma_ok(a)) {
         const int64_t nr = (int64_t)a.N * (a.H / a.KV);
