@@ -191,10 +191,11 @@ DEV void wait_vmcnt(int n) {
 // columns of each, so A is read once for both and neither product passes memory.
 // GEMM_PAIR: the sum of two products, A0 B0 + A1 B1 (each second operand behind
 // the first one), whose K tiles follow each other: no partial C.  It and
-// GEMM_SCALED, otherwise a product, store their sums times GemmArgs::back.  Bound by the
-// MFMA's feeding like the plain product: 6001 x 4096 x 2 x 11008 957 us = 1131
-// TFLOP/s (a large product of the library's reaches 1187); 2560 x 768 x 2 x 2048
-// with the kept products 33 us (160 tiles on 256 CUs), its pair 26 us.
+// GEMM_SCALED, otherwise a product, store their sums times GemmArgs::back.  Bound
+// by the MFMA's feeding like the plain product: 6001 x 4096 x 2 x 11008 970-990 us
+// call after call = 1093-1115 TFLOP/s (a large product of the library's reaches
+// 1187; under a profiler, at its clocks, 1056-1311 us); 2560 x 768 x 2 x 2048 with
+// the kept products 33 us (160 tiles on 256 CUs), its pair 27 us.
 DEV float glu_of(float a, float b, int act) {
     if (act == EVKHIP_ACT_SILU) return silu_f(a) * b;
     if (act == EVKHIP_ACT_GELU) return gelu_fast(a) * b;

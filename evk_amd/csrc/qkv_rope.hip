@@ -19,9 +19,9 @@
 //
 // Forward of 8192 tokens of 32 + 8 + 8 heads of 128 values: 42.7 us, 4.7 TB/s
 // (a copy of 1 GiB runs at 5.2); of 7996 tokens of 12 + 4 + 4 heads of 64 11.4
-// us, 3.6 TB/s, the sines' instructions beside the loads; 16 single tokens 4.0,
-// a launch.  Gradient of the 7996 tokens 15.7 us, 3.9 TB/s, and 4.0 for the
-// weights' sums.
+// us, 3.6 TB/s, a wave's groups of heads one after another with no load ahead; 16
+// single tokens 4.0, a launch.  Gradient of the 7996 tokens 15.9 us, 3.9 TB/s, and
+// 3.8 for the weights' sums.
 #include "kernels.h"
 
 #include <algorithm>

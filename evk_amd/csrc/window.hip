@@ -646,9 +646,10 @@ struct Softmax {
 // Forward.  Workgroup: 4 waves of 16 QB rows of one key head; K and V tiles in
 // two LDS stages, filled by LDS-direct loads while the tile before is used; one
 // barrier a tile.  Bound by the MFMA and the softmax's instructions beside it:
-// 8192 queries of 16 heads over 4 of 128 values, window 1024 and 4 sinks, 80 us
-// = 811 TFLOP/s of the visible pairs (whole tiles are 6% more); 97 us before the
-// tiles' rows were placed without bank conflicts and read ahead of the MFMAs.
+// 8192 queries of 16 heads over 4 of 128 values, window 1024 and 4 sinks, 82-84
+// us call after call = 770-790 TFLOP/s of the visible pairs (whole tiles are 6%
+// more; 86-90 us under a profiler, at its clocks); 97 us before the tiles' rows
+// were placed without bank conflicts and read ahead of the MFMAs.
 // Workgroups of eight waves, reads further ahead and a priority for waves in
 // their products changed nothing.
 template <int DH, int QB>
@@ -758,7 +759,7 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
 // long list is split over workgroups as well, whose states window_join adds.
 // Bound by memory: 64 sequences' tokens of 32 heads over 8 of 128 values, window
 // 1024, 53 us for 254 MB = 4.8 TB/s; 32 over 8, 131072 rows 108 us = 5.0 TB/s; a
-// lone token of 12 heads over 4 of 64, window 512, 6.5, a launch and two loads'
+// lone token of 12 heads over 4 of 64, window 512, 6.8, a launch and two loads'
 // latencies.
 template <int DH>
 struct SplitGeo {
@@ -1182,7 +1183,7 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
 // the block are cut every `unit` positions (KEYS times Parts::q).  A block with
 // one part writes dK and dV; the others (the sinks' blocks, which every later
 // query sees, and all where the grid would not fill the chip otherwise) leave
-// 32-bit sums that window_dkdv_join adds in the order of the parts (11.4 us for
+// 32-bit sums that window_dkdv_join adds in the order of the parts (11.8 us for
 // 45 MB there).
 struct Parts {
     int q;       // key blocks' lengths of queries per part
