@@ -947,7 +947,8 @@ __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int split
 // above its subnormals: P of a flat row of n is 1 / n, dS follows the lengths of
 // the output's gradient.  Both therefore carry powers of two that leave the sums
 // at the end.
-//   dV: P is at most 1 and carries 2^P_LIFT: full precision down to 2^-29.
+//   dV: P is at most 1, but for the error of its exponent (scores of millions),
+//       and carries 2^P_LIFT: full precision down to 2^-27.
 //   dK: |dS| <= P |dO| (|V| + |O|), Cauchy-Schwarz.  Each wave bounds that by its
 //       own keys' V and by the largest |dO| and |dO| |O| among its queries, which
 //       window_dq leaves, and takes that bound to 2^DS_TOP: nothing overflows.
@@ -959,7 +960,7 @@ __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int split
 // in dQ, lost bits from 16k rows on (131072 rows of one head of 64, no window: the
 // later half of dQ off by 4.8 H of its norm and that of dV by 14, H half a step of
 // fp16; now 0.6 both, at any length).
-constexpr int P_LIFT = 15, DS_TOP = 14, DQ_LIFT = 10, DQ_STEP = 7;
+constexpr int P_LIFT = 13, DS_TOP = 14, DQ_LIFT = 10, DQ_STEP = 7;
 constexpr int K_LEAST = -24;  // of rows that are zero, or not finite (those spoil what they are part of at any power)
 typedef short short2_t __attribute__((ext_vector_type(2)));  // a pair of exponents
 DEV short2_t max_xor(short2_t v, int o) {

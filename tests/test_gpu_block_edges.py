@@ -223,6 +223,33 @@ def test_window_attention_bwd_single_wild_rows(dev, dh, h, kv, what, b, n, windo
             assert not torch.isfinite(g[keys].float()).all(-1).any(), x
 
 
+@pytest.mark.parametrize("dh,h,kv", [(64, 4, 2), (128, 4, 1), (256, 2, 1), (40, 2, 2)])
+@pytest.mark.parametrize("n,window", [(200, 0), (700, 60)])
+def test_window_attention_bwd_wild_rows_beside_large_values(dev, dh, h, kv, n, window):
+    """Values near fp16's largest with output gradients along them, whose scores' gradients pass fp16, and a row of k, a row
+    of q and one of dO that are not finite."""
+    r = Rng(dev, 80 + dh)
+    q, k = r(1, n, h * dh, std=0.02), r(1, n, kv * dh, std=0.02)
+    v = r(1, n, kv * dh, std=20000.0).clamp_(-60000, 60000)
+    do = v.view(1, n, kv, 1, dh).expand(1, n, kv, h // kv, dh).float()
+    do = (do / do.norm(dim=-1, keepdim=True)).reshape(1, n, h * dh).half()
+    w = window_want(q, k, v, h, kv, dh, [0], window, 0, do)
+    j, t, u = n - 40, n - 25, n - 10
+    k[0, j, 1], q[0, t], do[0, u, :dh] = math.nan, math.nan, math.inf
+    o, lse = torch.empty_like(q), torch.empty(1, h, n, device=dev)
+    evk.window_attention(q, k, v, o, dh, window, 0, lse=lse)
+    dq, dk, dv = (torch.empty_like(x) for x in (q, k, v))
+    evk.window_attention_bwd(q, k, v, o, do, dq, dk, dv, lse, dh, window, 0)
+    m = seen(torch.arange(n, device=dev), n, window, 0)
+    rows = m[:, j].clone()
+    rows[t] = rows[u] = True
+    keys = (m & rows[:, None]).any(0)
+    assert not (window and (rows.all() or keys.all()))
+    close(dq[:, ~rows], w["dq"][:, ~rows], w["dq_t"][:, ~rows], "dq", norm=None)
+    for g, x in ((dk, "dk"), (dv, "dv")):
+        close(g[:, ~keys], w[x][:, ~keys], w[x + "_t"][:, ~keys], x, norm=None)
+
+
 def passes_us(f, n=5):
     f()
     best = math.inf
