@@ -223,6 +223,51 @@ def test_window_attention_bwd_single_wild_rows(dev, dh, h, kv, what, b, n, windo
             assert not torch.isfinite(g[keys].float()).all(-1).any(), x
 
 
+@pytest.mark.parametrize("dh,h,kv", HEADS)
+@pytest.mark.parametrize("b,n,window,sinks", [(1, 40, 9, 0), (1, 300, 40, 3), (5, 700, 90, 0), (1, 333, 0, 0)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_window_attention_single_wild_values(dev, dh, h, kv, b, n, window, sinks, value):
+    """One value of v, one of dO: the other columns of o and of dV are those without it, for queries and keys that take part
+    in the row and for those that do not; its own column says so where the row is seen, and only there."""
+    at, col, hd = n // 2 + 3, dh // 2 + 1, h - 1
+    c = hd // (h // kv)
+    r = Rng(dev, 90 + dh + n)
+    q, k, v, do = r(b, n, h * dh), r(b, n, kv * dh), r(b, n, kv * dh), r(b, n, h * dh)
+    w = window_want(q, k, v, h, kv, dh, [0] * b, window, sinks, do)
+    m = seen(torch.arange(n, device=dev), n, window, sinks)
+    v2 = v.clone()
+    v2[0, at, c * dh + col] = value
+    o, lse = torch.empty_like(q), torch.empty(b, h, n, device=dev)
+    evk.window_attention(q, k, v2, o, dh, window, sinks, lse=lse)
+    hit = torch.zeros(b, n, h, dh, dtype=torch.bool, device=dev)
+    hit[0, m[:, at], c * (h // kv):(c + 1) * (h // kv), col] = True
+    hit = hit.view(b, n, h * dh)
+    close(o[~hit], w["o"][~hit], w["o_t"][~hit], "o")
+    assert not torch.isfinite(o[hit].float()).any()
+    close(lse, w["lse"], w["lse_t"], "lse", norm=None)
+    do2 = do.clone()
+    do2[0, at, hd * dh + col] = value
+    evk.window_attention(q, k, v, o, dh, window, sinks, lse=lse)
+    dq, dk, dv = (torch.empty_like(x) for x in (q, k, v))
+    evk.window_attention_bwd(q, k, v, o, do2, dq, dk, dv, lse, dh, window, sinks)
+    hit = torch.zeros(b, n, kv, dh, dtype=torch.bool, device=dev)
+    hit[0, m[at], c, col] = True
+    hit = hit.view(b, n, kv * dh)
+    close(dv[~hit], w["dv"][~hit], w["dv_t"][~hit], "dv")
+    assert not torch.isfinite(dv[hit].float()).any()
+    rows = torch.zeros(b, n, h, dh, dtype=torch.bool, device=dev)
+    rows[0, at, hd] = True
+    rows = rows.view(b, n, h * dh)
+    close(dq[~rows], w["dq"][~rows], w["dq_t"][~rows], "dq", norm=4 * H)
+    assert not torch.isfinite(dq[rows].float()).any()
+    keys = torch.zeros(b, n, kv, dh, dtype=torch.bool, device=dev)
+    keys[0, m[at], c] = True
+    keys = keys.view(b, n, kv * dh)
+    close(dk[~keys], w["dk"][~keys], w["dk_t"][~keys], "dk", norm=4 * H)
+    # dP - D is an infinity where v and o have other signs in that column, else infinity less infinity
+    assert not torch.isfinite(dk[keys].float()).any()
+
+
 @pytest.mark.parametrize("dh,h,kv", [(64, 4, 2), (128, 4, 1), (256, 2, 1), (40, 2, 2)])
 @pytest.mark.parametrize("n,window", [(200, 0), (700, 60)])
 def test_window_attention_bwd_wild_rows_beside_large_values(dev, dh, h, kv, n, window):
