@@ -24,6 +24,8 @@ __all__ = [
     "model_weight_elems", "model_cache_elems", "model_packed_elems", "model_pack", "model_decode_packed",
     "qkv_norm_rope", "qkv_norm_rope_backward", "window_attention", "window_attention_bwd",
     "gated_linear", "gated_linear_backward",
+    "residual_norm", "residual_norm_backward", "prefix_attention", "prefix_attention_workspace",
+    "token_logprobs", "token_logprobs_backward",
     "EvkError",
 ]
 
@@ -109,6 +111,7 @@ SIGNATURES = {
                                        C.c_void_p]),
     "evkhip_embed_backward": (C.c_int, [TP, TP, TP, C.c_void_p]),
     "evkhip_qkv_norm_rope": (C.c_int, [TP] * 6 + [C.c_uint32, C.c_float, C.c_float, C.c_uint32, C.c_void_p, C.c_void_p]),
+    "evkhip_qkv_norm_rope_behind": (C.c_int, [TP] * 6 + [C.c_uint32, C.c_float, C.c_float, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p]),
     "evkhip_qkv_norm_rope_backward_workspace": (C.c_uint64, [C.c_uint64, C.c_uint32]),
     "evkhip_qkv_norm_rope_backward": (C.c_int, [TP] * 9 + [C.c_uint32, C.c_float, C.c_float, C.c_uint32, C.c_int,
                                                            C.c_void_p, C.c_uint64, C.c_void_p]),
@@ -120,6 +123,13 @@ SIGNATURES = {
     "evkhip_gated_linear": (C.c_int, [TP] * 4 + [C.c_int, C.c_void_p]),
     "evkhip_gated_linear_backward_workspace": (C.c_uint64, [C.c_uint64, C.c_uint32, C.c_uint32]),
     "evkhip_gated_linear_backward": (C.c_int, [TP] * 6 + [C.c_int, C.c_int, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "evkhip_residual_norm": (C.c_int, [TP] * 7 + [C.c_float, C.c_int, C.c_float, C.c_void_p]),
+    "evkhip_residual_norm_backward_workspace": (C.c_uint64, [C.c_uint64, C.c_uint64, C.c_uint32]),
+    "evkhip_residual_norm_backward": (C.c_int, [TP] * 12 + [C.c_float, C.c_int, C.c_float, C.c_int, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "evkhip_prefix_attention_workspace": (C.c_uint64, [C.c_uint32] * 7),
+    "evkhip_prefix_attention": (C.c_int, [TP] * 6 + [C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "evkhip_token_logprobs": (C.c_int, [TP, TP, C.c_void_p, C.c_void_p, TP, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p]),
+    "evkhip_token_logprobs_backward": (C.c_int, [TP, TP] + [C.c_void_p] * 4 + [TP, C.c_float, C.c_void_p]),
     "evkhip_model_weight_elems": (C.c_uint64, [C.POINTER(ModelCfg)]),
     "evkhip_model_cache_elems": (C.c_uint64, [C.POINTER(ModelCfg)]),
     "evkhip_model_prefill": (C.c_int, [C.POINTER(ModelCfg), C.c_void_p, C.c_void_p, C.c_void_p,
@@ -535,17 +545,18 @@ def _at_least(least, **values):
 
 
 def qkv_norm_rope(qkv, q, k, v, head_dim, q_weight=None, k_weight=None, eps=1e-4, rotary_base=10000.0, position_offset=0,
-                  offsets=None, stream=None):
+                  offsets=None, stream=None, first_position=0):
     """Norm and rotation of each query and key head of qkv (B, N, (H + 2 KV) head_dim) into q (B, N, H head_dim) and the
-    rows position_offset + t (or offsets[b] + t, int32) of k and v (B, rows, KV head_dim)."""
+    rows position_offset + t (or offsets[b] + t, int32) of k and v (B, rows, KV head_dim).  Row 0 stands at position
+    first_position: the length of a prefix that lies elsewhere."""
     dev = _first(qkv)
-    if not (1 <= head_dim <= _U32 and 0 <= position_offset <= _U32):
+    if not (1 <= head_dim <= _U32 and 0 <= position_offset <= _U32 and 0 <= first_position <= _U32):
         _at_least(1, head_dim=head_dim)
-        _at_least(0, position_offset=position_offset)
-    _check(_calls.evkhip_qkv_norm_rope(_H(qkv, dev), _H(q_weight, dev), _H(k_weight, dev), _H(q, dev), _H(k, dev), _H(v, dev),
-                                       head_dim, eps, rotary_base, position_offset,
-                                       None if offsets is None else _P(offsets, dev, _torch.int32, qkv.shape[0]),
-                                       _on(stream, dev)))
+        _at_least(0, position_offset=position_offset, first_position=first_position)
+    _check(_calls.evkhip_qkv_norm_rope_behind(_H(qkv, dev), _H(q_weight, dev), _H(k_weight, dev), _H(q, dev), _H(k, dev), _H(v, dev),
+                                              head_dim, eps, rotary_base, first_position, position_offset,
+                                              None if offsets is None else _P(offsets, dev, _torch.int32, qkv.shape[0]),
+                                              _on(stream, dev)))
     return q, k, v
 
 
@@ -632,6 +643,100 @@ def gated_linear_backward(x, w, gate_up, dh, dx=None, dw=None, activation="silu"
     _check(_calls.evkhip_gated_linear_backward(_H(x, dev), _H(w, dev), _H(gate_up, dev), _H(dh, dev), _H(dx, dev), _H(dw, dev),
                                                _activation(activation), int(accumulate), wp, wn, _on(stream, dev)))
     return dx, dw
+
+
+# ---------------------------------------------------------------------------
+# operators of a group of continuations of one prompt
+# ---------------------------------------------------------------------------
+# Types, devices and workspaces as for the block's operators; token ids are 16-bit
+# values in int16 or uint16 tensors, log-probabilities and entropies fp32.
+
+def residual_norm(x, y, s, h, post_weight=None, gate=None, pre_weight=None, residual_scale=1.0, post_norm=True, eps=1e-4, stream=None):
+    """s = residual_scale x + gate * norm(y) * post_weight (gate * y without post_norm), h = norm(s) * pre_weight; x, y, s, h
+    (..., D), weights (D), gate (D) or one for each of x's sequences (B, D).  y and s None: h = norm(x) * pre_weight."""
+    dev = _first(x)
+    _check(_calls.evkhip_residual_norm(_H(x, dev), _H(y, dev), _H(post_weight, dev), _H(gate, dev), _H(pre_weight, dev), _H(s, dev), _H(h, dev),
+                                       residual_scale, int(post_norm), eps, _on(stream, dev)))
+    return s, h
+
+
+def residual_norm_backward(x, y, ds, dh, dx, dy, post_weight=None, gate=None, pre_weight=None, dpost_weight=None, dgate=None,
+                           dpre_weight=None, residual_scale=1.0, post_norm=True, eps=1e-4, accumulate=False, workspace=None, stream=None):
+    """Gradient of residual_norm from ds (None: zeros) and dh: dx and dy are written, dpost_weight, dgate and dpre_weight
+    (None: not wanted) are written or, with accumulate, added to."""
+    dev = _first(x)
+    need = 0
+    if dpost_weight is not None or dgate is not None or dpre_weight is not None:
+        d = x.shape[-1] if x.dim() else 0
+        gates = gate.shape[0] if gate is not None and gate.dim() == 2 else 1
+        need = _need("evkhip_residual_norm_backward_workspace", x.numel() // d, gates, d) if 0 < d <= _U32 else 0
+    ws, wp, wn = _workspace(workspace, need, dev, stream)
+    _check(_calls.evkhip_residual_norm_backward(_H(x, dev), _H(y, dev), _H(post_weight, dev), _H(gate, dev), _H(pre_weight, dev), _H(ds, dev),
+                                                _H(dh, dev), _H(dx, dev), _H(dy, dev), _H(dpost_weight, dev), _H(dgate, dev),
+                                                _H(dpre_weight, dev), residual_scale, int(post_norm), eps, int(accumulate), wp, wn,
+                                                _on(stream, dev)))
+    return dx, dy
+
+
+def prefix_attention_workspace(q, prefix_k, k, head_dim) -> int:
+    """Bytes of workspace of prefix_attention for these q, prefix_k and k."""
+    (b, n, d), (_, rows, dk) = _shape3(q, "q"), _shape3(k, "k")
+    if prefix_k.dim() != 2:
+        raise ValueError(f"prefix_k has 2 dimensions, got {tuple(prefix_k.shape)}")
+    if not 1 <= head_dim <= _U32:
+        _at_least(1, head_dim=head_dim)
+    return _need("evkhip_prefix_attention_workspace", b, n, prefix_k.shape[0], rows, d // head_dim, dk // head_dim, head_dim)
+
+
+def prefix_attention(q, prefix_k, prefix_v, k, v, o, head_dim, position_offset=0, offsets=None, lse=None, workspace=None, stream=None):
+    """Attention of q (B, N, H head_dim) over the prefix (P, KV head_dim) that all sequences share and each one's own rows of
+    k, v (B, rows, KV head_dim) up to the query's, position_offset + t (or offsets[b] + t, int32).  lse: optional
+    (B, H, N) fp32."""
+    dev = _first(q)
+    if not 0 <= position_offset <= _U32:
+        _at_least(0, position_offset=position_offset)
+    ws, wp, wn = _workspace(workspace, prefix_attention_workspace(q, prefix_k, k, head_dim), dev, stream)
+    _check(_calls.evkhip_prefix_attention(_H(q, dev), _H(prefix_k, dev), _H(prefix_v, dev), _H(k, dev), _H(v, dev), _H(o, dev), head_dim,
+                                          position_offset, None if offsets is None else _P(offsets, dev, _torch.int32, q.shape[0]),
+                                          None if lse is None else _P(lse, dev, _torch.float32, q.numel() // head_dim), wp, wn,
+                                          _on(stream, dev)))
+    return o
+
+
+def _ids(t, dev) -> Optional[bytes]:
+    """Descriptor of a tensor of token ids on device `dev` (None: left out)."""
+    if t is None:
+        return None
+    if t.dtype not in (_torch.int16, _torch.uint16) or t.get_device() != dev:
+        raise ValueError(f"expected 16-bit token ids on cuda:{dev}, got {t.dtype} on {t.device}")
+    return _D(t)
+
+
+def _floats(t, dev, count) -> Optional[int]:
+    return None if t is None else _P(t, dev, _torch.float32, count)
+
+
+def token_logprobs(logits, tokens, logprobs, entropy=None, top_ids=None, top_logprobs=None, stats=None, input_scale=1.0, stream=None):
+    """Log-probabilities of `tokens` (one a row of logits (..., V)) under softmax(input_scale * logits), fp32; where given,
+    the rows' entropies, the K most likely ids (..., K) with their log-probabilities, and stats (rows, 2) for the gradient."""
+    dev = _first(logits)
+    rows = logits.numel() // logits.shape[-1] if logits.dim() and logits.shape[-1] else 0
+    alternatives = 0 if top_ids is None else top_ids.numel()
+    _check(_calls.evkhip_token_logprobs(_D(logits), _ids(tokens, dev), _floats(logprobs, dev, rows), _floats(entropy, dev, rows),
+                                        _ids(top_ids, dev), _floats(top_logprobs, dev, alternatives), _floats(stats, dev, 2 * rows),
+                                        input_scale, _on(stream, dev)))
+    return logprobs
+
+
+def token_logprobs_backward(logits, tokens, stats, dlogprobs, dlogits, entropy=None, dentropy=None, input_scale=1.0, stream=None):
+    """Gradient of token_logprobs from its stats, fp32 dlogprobs and, with the forward's entropy, dentropy (one of the two may
+    be None): dlogits is written."""
+    dev = _first(logits)
+    rows = logits.numel() // logits.shape[-1] if logits.dim() and logits.shape[-1] else 0
+    _check(_calls.evkhip_token_logprobs_backward(_D(logits), _ids(tokens, dev), _floats(stats, dev, 2 * rows), _floats(entropy, dev, rows),
+                                                 _floats(dlogprobs, dev, rows), _floats(dentropy, dev, rows), _H(dlogits, dev), input_scale,
+                                                 _on(stream, dev)))
+    return dlogits
 
 
 # ---------------------------------------------------------------------------

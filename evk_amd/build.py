@@ -22,7 +22,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("EVK_OFFLOAD_ARCH", "gfx950")
 
 KERNEL_SOURCES = ["capi.hip", "gemm.hip", "flash.hip", "flash_wide.hip", "decode_ops.hip", "model.hip", "decode_persist.hip",
-                  "kv_step.hip", "train_ops.hip", "capi_block.hip", "qkv_rope.hip", "window.hip"]
+                  "kv_step.hip", "train_ops.hip", "capi_block.hip", "qkv_rope.hip", "window.hip",
+                  "capi_group.hip", "residual_norm.hip", "token_logprobs.hip", "prefix.hip"]
 API_SOURCES = ["evk_runtime.cpp", "evk_ai.cpp", "evk_block.cpp"]
 
 HIP_FLAGS = [

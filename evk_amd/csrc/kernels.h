@@ -176,6 +176,7 @@ struct QkvRopeArgs {
     f16 *dqkv, *dwq, *dwk;    // as qkv; (dh) or null
     const int* offsets;    // (B) positions of the first tokens, or null: p0
     int B, N, H, KV, R, dh, p0;
+    int first;             // forward: position of row 0 of k and v
     float eps, base;
     int accumulate;        // dwq, dwk += instead of =
 };
@@ -201,6 +202,54 @@ uint64_t window_fwd_workspace(int B, int N, int R, int H, int KV, int dh, int wi
 int window_forward(const WindowArgs& a, void* ws, hipStream_t st);
 uint64_t window_bwd_workspace(int B, int N, int H, int KV, int dh, int window, int sinks);
 int window_backward(const WindowArgs& a, void* ws, hipStream_t st);  // R == N, p0 == 0
+
+// ---- prefix.hip ----
+struct PrefixArgs {
+    const f16 *q, *pk, *pv;  // (B, N, H dh), (P, KV dh) twice
+    const f16 *k, *v;        // (B, R, KV dh)
+    f16* out;                // as q
+    float* lse;              // (B, H, N) or null
+    const int* offsets;      // (B) own rows of the first queries, or null: p0
+    int B, N, H, KV, P, R, dh, p0;
+    float scale;
+};
+uint64_t prefix_workspace(int B, int N, int P, int R, int H, int KV, int dh);
+int prefix_forward(const PrefixArgs& a, void* ws, hipStream_t st);
+
+// ---- residual_norm.hip ----
+constexpr int RESIDUAL_NORM_MOST = 16384;  // values of a row
+struct ResidualNormArgs {
+    const f16 *x, *y;              // (rows, D); y null: x alone, normed
+    const f16 *wo, *gate, *wi;     // (D), (D) or (gates, D), (D); null: ones
+    f16 *s, *h;                    // as x
+    const f16 *ds, *dh;            // backward: as x; ds null: zeros
+    f16 *dx, *dy;
+    f16 *dwo, *dgate, *dwi;        // null: not wanted
+    int64_t rows, gate_rows;       // rows of one gate; 0: one gate (or none) for all
+    int D, post;
+    float scale, eps;
+    int accumulate;
+};
+int residual_norm_forward(const ResidualNormArgs& a, hipStream_t st);
+uint64_t residual_norm_bwd_workspace(uint64_t rows, uint64_t gates, int D);
+int residual_norm_backward(const ResidualNormArgs& a, float* part, hipStream_t st);  // part: that workspace, or null
+
+// ---- token_logprobs.hip ----
+constexpr uint32_t LOGPROBS_VOCAB = 65536, LOGPROBS_TOP = 32;
+struct TokenLogprobsArgs {
+    const f16* logits;       // (rows, V)
+    const uint16_t* tokens;  // (rows)
+    float *logprobs, *entropy, *stats;  // (rows), (rows) or null, (rows, 2) or null
+    uint16_t* top_ids;       // (rows, top) or null
+    float* top_logprobs;
+    const float *dlogprobs, *dentropy;  // backward: (rows) or null
+    f16* dlogits;
+    int64_t rows;
+    int V, top;
+    float scale;
+};
+int token_logprobs_forward(const TokenLogprobsArgs& a, hipStream_t st);
+int token_logprobs_backward(const TokenLogprobsArgs& a, hipStream_t st);
 
 // ---- model.hip ----
 void model_free_workspace();

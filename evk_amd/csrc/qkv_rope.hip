@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) void qkv_rope_k(QkvRopeArgs a, Turns tn, int p
     const int i0 = (lane % LPH) * 8, n = min(8, dh - i0);
     const int64_t p = (int64_t)(a.offsets ? a.offsets[b] : a.p0) + t;  // past 2^31 for the last offsets
     Angles ang;
-    ang.set(tn, i0, p);
+    ang.set(tn, i0, a.first + p);
     float wq[8], wk[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) wq[e] = wk[e] = 1.0f;

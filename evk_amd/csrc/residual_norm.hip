@@ -1,0 +1,353 @@
+// Norms after and before a block, with the block's gate and the residual scale,
+// in one pass, and its gradient (no counterpart in the reference, whose block
+// adds its products to the stream and norms them without weights, a pass each).
+//
+//   n = y q, q = 1 / sqrt(mean(y^2) + eps)      (post_norm; else n = y)
+//   s = a x + g (n wo)                          the stream behind the block
+//   u = s r, r = 1 / sqrt(mean(s^2) + eps),  h = u wi   what the next block reads
+// With c = dh wi and S = ds + r (c - u mean(c u)), the gradient of s:
+//   dx = a S,  dwi = sum dh u,  e = g wo S,  dy = q (e - n mean(e n))
+//   P = sum of S n over the rows of a gate:  dg = wo P,  dwo = sum over gates of g P
+// so that both gradients come from one sum.  Without y: s = x, which is not
+// written.
+//
+// Memory-bound: every value read once and written once.  A row lies in TPR
+// threads' registers, NV vectors of eight values each, at any alignment (the
+// last vector takes what is left); weights and gates stay in registers from row
+// to row.  The sums of a row are in 32 bits, as is everything between the loads
+// and the stores.
+#include "kernels.h"
+
+#include <algorithm>
+
+namespace evkhip {
+
+namespace {
+
+DEV half8 ld_part(const f16* p, int n) {  // n values, the rest zeros
+    half8 h = {};
+    if (n >= 8) {
+        h = ld_h8(p);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+            if (e < n) h[e] = p[e];
+    }
+    return h;
+}
+DEV void st_part(f16* p, int n, const float (&x)[8]) {
+    half8 h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = (f16)x[e];
+    if (n >= 8) {
+        st_h8(p, h);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+            if (e < n) p[e] = h[e];
+    }
+}
+DEV half8 ones() {
+    half8 h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = (f16)1.0f;
+    return h;
+}
+
+constexpr int threads_of(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// Sums over the TPR threads of a row.  Wider rows than a wave meet in LDS, in two
+// places in turn: who writes one again has passed the barrier of the other,
+// which everyone reaches after reading the first.
+template <int TPR>
+struct RowSum {
+    static constexpr int NW = TPR / 64;
+    int turn = 0;
+    template <int M>
+    DEV void operator()(float (&v)[M], float (*lds)[2][NW]) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) v[i] = wave_sum(v[i]);
+        if constexpr (NW > 1) {
+            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+            if (lane == 0)
+#pragma unroll
+                for (int i = 0; i < M; ++i) lds[turn][i][wave] = v[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < M; ++i) {
+                v[i] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) v[i] += lds[turn][i][w];
+            }
+            turn ^= 1;
+        }
+    }
+};
+
+// The stream behind the block, from a row's vectors: s, and n = y q
+template <bool Y, int NV>
+DEV void stream(const ResidualNormArgs& a, const half8 (&x)[NV], const half8 (&y)[NV], const half8 (&g)[NV], const half8 (&wo)[NV], float q,
+                float (&s)[NV][8]) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            s[v][e] = Y ? __builtin_fmaf(a.scale, (float)x[v][e], (float)y[v][e] * q * (float)wo[v][e] * (float)g[v][e]) : (float)x[v][e];
+}
+
+template <int TPR, int NV, bool Y>
+__global__ __launch_bounds__(threads_of(TPR)) void residual_norm_k(ResidualNormArgs a) {
+    constexpr int RPW = threads_of(TPR) / TPR;
+    __shared__ float red[2][2][TPR / 64];
+    const int t = threadIdx.x % TPR, D = a.D;
+    RowSum<TPR> sum;
+    int at[NV], n[NV];
+    half8 wi[NV], wo[NV], g[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        at[v] = 8 * (t + TPR * v);
+        n[v] = D - at[v];
+        wi[v] = a.wi ? ld_part(a.wi + at[v], n[v]) : ones();
+        wo[v] = a.wo ? ld_part(a.wo + at[v], n[v]) : ones();
+        g[v] = a.gate && !a.gate_rows ? ld_part(a.gate + at[v], n[v]) : ones();
+    }
+    for (int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR; row < a.rows; row += (int64_t)gridDim.x * RPW) {
+        const int64_t base = row * D;
+        half8 x[NV], y[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            x[v] = ld_part(a.x + base + at[v], n[v]);
+            if (Y) y[v] = ld_part(a.y + base + at[v], n[v]);
+        }
+        if (Y && a.gate_rows)
+#pragma unroll
+            for (int v = 0; v < NV; ++v) g[v] = ld_part(a.gate + row / a.gate_rows * D + at[v], n[v]);
+        float q = 1.0f, ss[1] = {0.0f};
+        if (Y && a.post) {
+            float yy[1] = {0.0f};
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) yy[0] += (float)y[v][e] * (float)y[v][e];
+            sum(yy, red);
+            q = rsqrtf(yy[0] / (float)D + a.eps);
+        }
+        float s[NV][8];
+        stream<Y>(a, x, y, g, wo, q, s);
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss[0] += s[v][e] * s[v][e];
+        sum(ss, red);
+        const float r = rsqrtf(ss[0] / (float)D + a.eps);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (Y) st_part(a.s + base + at[v], n[v], s[v]);
+            float h[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = s[v][e] * r * (float)wi[v][e];
+            st_part(a.h + base + at[v], n[v], h);
+        }
+    }
+}
+
+// The gradient.  A workgroup takes a run of rows of one gate (`parts` runs a
+// gate), keeps the columns' sums dh u and S n in registers and leaves them in the
+// workspace, one row of 2 D sums, which residual_norm_sums_k adds in a fixed
+// order.
+template <int TPR, int NV, bool Y>
+__global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualNormArgs a, int64_t rows_gate, int parts, float* part) {
+    constexpr int RPW = threads_of(TPR) / TPR;
+    __shared__ float red[2][2][TPR / 64];
+    __shared__ float cols[RPW > 1 ? RPW : 1][RPW > 1 ? 2 * TPR * NV * 8 : 1];
+    const int t = threadIdx.x % TPR, D = a.D;
+    const int64_t gate = blockIdx.x / parts, r0 = blockIdx.x % parts;
+    const int64_t first = gate * rows_gate + rows_gate * r0 / parts, end = gate * rows_gate + rows_gate * (r0 + 1) / parts;
+    RowSum<TPR> sum;
+    int at[NV], n[NV];
+    half8 wi[NV], wo[NV], g[NV];
+    float dwi[NV][8] = {}, dsn[NV][8] = {};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        at[v] = 8 * (t + TPR * v);
+        n[v] = D - at[v];
+        wi[v] = a.wi ? ld_part(a.wi + at[v], n[v]) : ones();
+        wo[v] = a.wo ? ld_part(a.wo + at[v], n[v]) : ones();
+        g[v] = a.gate ? ld_part(a.gate + (a.gate_rows ? gate * D : 0) + at[v], n[v]) : ones();
+    }
+    for (int64_t row = first + threadIdx.x / TPR; row < end; row += RPW) {
+        const int64_t base = row * D;
+        half8 x[NV], y[NV], ds[NV], dh[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            x[v] = ld_part(a.x + base + at[v], n[v]);
+            if (Y) y[v] = ld_part(a.y + base + at[v], n[v]);
+            dh[v] = ld_part(a.dh + base + at[v], n[v]);
+            ds[v] = half8{};
+            if (a.ds) ds[v] = ld_part(a.ds + base + at[v], n[v]);
+        }
+        float q = 1.0f;
+        if (Y && a.post) {
+            float yy[1] = {0.0f};
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) yy[0] += (float)y[v][e] * (float)y[v][e];
+            sum(yy, red);
+            q = rsqrtf(yy[0] / (float)D + a.eps);
+        }
+        float s[NV][8], sc[2] = {0.0f, 0.0f};
+        stream<Y>(a, x, y, g, wo, q, s);
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sc[0] += s[v][e] * s[v][e];
+                sc[1] += s[v][e] * ((float)dh[v][e] * (float)wi[v][e]);
+            }
+        sum(sc, red);
+        const float r = rsqrtf(sc[0] / (float)D + a.eps), back = sc[1] * r / (float)D;  // mean(c u)
+        float en[1] = {0.0f};
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float dx[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float u = s[v][e] * r, d = (float)dh[v][e];
+                dwi[v][e] += d * u;
+                const float S = (float)ds[v][e] + r * (d * (float)wi[v][e] - u * back);
+                s[v][e] = S;
+                dx[e] = (Y ? a.scale : 1.0f) * S;
+                if (Y) {
+                    const float m = (float)y[v][e] * q;
+                    dsn[v][e] += S * m;
+                    en[0] += S * (float)g[v][e] * (float)wo[v][e] * m;
+                }
+            }
+            st_part(a.dx + base + at[v], n[v], dx);
+        }
+        if (!Y) continue;
+        if (a.post) sum(en, red);
+        const float mean = a.post ? en[0] / (float)D : 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float dy[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dy[e] = q * (s[v][e] * (float)g[v][e] * (float)wo[v][e] - (float)y[v][e] * q * mean);
+            st_part(a.dy + base + at[v], n[v], dy);
+        }
+    }
+    if (!part) return;  // launch-uniform: neither weights nor gates have gradients
+    float* const dst = part + (int64_t)blockIdx.x * 2 * D;
+    if constexpr (RPW == 1) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < n[v]) {
+                    dst[at[v] + e] = dwi[v][e];
+                    if (Y) dst[D + at[v] + e] = dsn[v][e];
+                }
+    } else {
+        constexpr int W = TPR * NV * 8;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                cols[threadIdx.x / TPR][at[v] + e] = dwi[v][e];
+                cols[threadIdx.x / TPR][W + at[v] + e] = dsn[v][e];
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < (Y ? 2 : 1) * D; c += threads_of(TPR)) {
+            const int from = c < D ? c : W + c - D;
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < RPW; ++w) v += cols[w][from];
+            dst[c] = v;
+        }
+    }
+}
+
+// Sums over the runs: block (job, 16 columns), job 0 dwi, 1 dwo, 2 + b the
+// gradient of gate b.  64 threads a column take every 64th run, in order, and
+// their sums are added in order.
+__global__ __launch_bounds__(1024) void residual_norm_sums_k(ResidualNormArgs a, const float* part, int parts, int gates, int blocks) {
+    __shared__ float red[64][17];
+    const int x = threadIdx.x % 16, u = threadIdx.x / 16, job = blockIdx.x / blocks, c = blockIdx.x % blocks * 16 + x, D = a.D;
+    f16* const out = job == 0 ? a.dwi : job == 1 ? a.dwo : a.dgate ? a.dgate + (int64_t)(job - 2) * D : nullptr;
+    if (!out) return;
+    const int64_t r0 = job < 2 ? 0 : (int64_t)(job - 2) * parts, r1 = job < 2 ? (int64_t)gates * parts : r0 + parts;
+    const float* const src = part + (job ? D : 0) + c;
+    float v = 0.0f;
+    if (c < D)
+#pragma unroll 4
+        for (int64_t r = r0 + u; r < r1; r += 64) {
+            const float f = job == 1 && a.gate ? (float)a.gate[(a.gate_rows ? r / parts * D : 0) + c] : 1.0f;
+            v += f * src[r * 2 * D];
+        }
+    red[u][x] = v;
+    __syncthreads();
+    if (u || c >= D) return;
+    v = 0.0f;
+    for (int r = 0; r < 64; ++r) v += red[r][x];
+    if (job >= 2 && a.wo) v *= (float)a.wo[c];
+    out[c] = (f16)(a.accumulate ? v + (float)out[c] : v);
+}
+
+template <class F>
+void by_width(int D, F&& f) {
+    if (D <= 512) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    if (D <= 1024) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    if (D <= 2048) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
+    if (D <= 4096) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    if (D <= 8192) return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 2>{});
+    f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
+}
+static_assert(RESIDUAL_NORM_MOST == 1024 * 2 * 8, "the widest row");
+
+// Runs of rows of one gate
+int64_t runs(int64_t rows, int64_t gates, int D) {
+    const int64_t rows_gate = rows / gates;
+    return std::max<int64_t>(1, std::min((rows_gate + 3) / 4, (1024 + gates - 1) / gates));
+}
+
+}  // namespace
+
+uint64_t residual_norm_bwd_workspace(uint64_t rows, uint64_t gates, int D) {
+    return gates * runs((int64_t)rows, (int64_t)gates, D) * 2 * D * sizeof(float);
+}
+
+int residual_norm_forward(const ResidualNormArgs& a, hipStream_t st) {
+    by_width(a.D, [&](auto tpr, auto nv) {
+        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, NT = threads_of(TPR), RPW = NT / TPR;
+        const int64_t groups = std::min<int64_t>((a.rows + RPW - 1) / RPW, 1 << 20);
+        if (a.y) hipLaunchKernelGGL((residual_norm_k<TPR, NV, true>), dim3((unsigned)groups), dim3(NT), 0, st, a);
+        else hipLaunchKernelGGL((residual_norm_k<TPR, NV, false>), dim3((unsigned)groups), dim3(NT), 0, st, a);
+    });
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? EVKHIP_OK : check_hip(e, "residual_norm launch");
+}
+
+int residual_norm_backward(const ResidualNormArgs& a, float* part, hipStream_t st) {
+    const int64_t gates = a.gate_rows ? a.rows / a.gate_rows : 1, parts = runs(a.rows, gates, a.D);
+    const int blocks = (a.D + 15) / 16;
+    const int64_t jobs = 2 + (a.dgate ? gates : 0);
+    int rc = EVKHIP_OK;
+    by_width(a.D, [&](auto tpr, auto) { rc = check_grid("residual_norm_backward", gates * parts, threads_of(decltype(tpr)::value)); });
+    if (rc == EVKHIP_OK && part) rc = check_grid("residual_norm_backward", jobs * blocks, 1024);
+    if (rc != EVKHIP_OK) return rc;
+    by_width(a.D, [&](auto tpr, auto nv) {
+        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, NT = threads_of(TPR);
+        const dim3 grid((unsigned)(gates * parts));
+        if (a.y) hipLaunchKernelGGL((residual_norm_bwd_k<TPR, NV, true>), grid, dim3(NT), 0, st, a, a.rows / gates, (int)parts, part);
+        else hipLaunchKernelGGL((residual_norm_bwd_k<TPR, NV, false>), grid, dim3(NT), 0, st, a, a.rows / gates, (int)parts, part);
+    });
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && part) {
+        hipLaunchKernelGGL(residual_norm_sums_k, dim3((unsigned)(jobs * blocks)), dim3(1024), 0, st, a, part, (int)parts, (int)gates, blocks);
+        e = hipGetLastError();
+    }
+    return e == hipSuccess ? EVKHIP_OK : check_hip(e, "residual_norm_backward launch");
+}
+
+}  // namespace evkhip

@@ -326,6 +326,15 @@ int evkhip_qkv_norm_rope(const evkhip_tensor* qkv, const evkhip_tensor* q_weight
                          float eps, float rotary_base, uint32_t position_offset, const int32_t* offsets,
                          void* stream);
 
+/* The same with cache rows behind a prefix of first_position tokens that lies
+ * elsewhere (evkhip_prefix_attention): row p of k and v and the token that goes
+ * there stand at position first_position + p, and are turned by that angle.
+ * first_position at most 2^30. */
+int evkhip_qkv_norm_rope_behind(const evkhip_tensor* qkv, const evkhip_tensor* q_weight, const evkhip_tensor* k_weight,
+                                const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v, uint32_t head_dim,
+                                float eps, float rotary_base, uint32_t first_position, uint32_t position_offset,
+                                const int32_t* offsets, void* stream);
+
 /* Its gradient: dq (B,N,H*head_dim), dk and dv (B,N,KV*head_dim) in; dqkv (as
  * qkv) is written; dq_weight and dk_weight (head_dim, NULL: not wanted) are
  * written, or added to with accumulate (summed in 32 bits in a fixed order,
@@ -387,6 +396,75 @@ int evkhip_gated_linear_backward(const evkhip_tensor* x, const evkhip_tensor* w,
                                  const evkhip_tensor* dh, const evkhip_tensor* dx, const evkhip_tensor* dw,
                                  int activation, int accumulate, void* workspace, uint64_t workspace_bytes,
                                  void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Operators of a group of continuations of one prompt (no reference
+ * counterparts: its training program recomputes 16 sequences whole, norms
+ * without weights and has one mean loss).  Workspaces, overlaps, limits and
+ * repeatability as for the block's operators above.
+ * ------------------------------------------------------------------------- */
+
+/* Norms after and before a block with its gate and the residual scale, in one
+ * pass.  x (...,D) the stream, y (as x) the block's output:
+ *   s = residual_scale x + gate * norm(y) * post_weight    (post_norm; else gate * y)
+ *   h = norm(s) * pre_weight,  norm(t) = t / sqrt(mean(t^2) + eps) over a row
+ * h comes from the unrounded s.  s and h (as x) are written.  Weights (D), NULL:
+ * ones.  gate NULL (ones), (D), or (B,D) with one for each of x's B = dims[0]
+ * sequences.  y NULL is the norm before the first block: h = norm(x) *
+ * pre_weight; then s, gate and post_weight are NULL, residual_scale 1.  D up to
+ * 16384; residual_scale 0 or a magnitude from 2^-24 to 65504. */
+int evkhip_residual_norm(const evkhip_tensor* x, const evkhip_tensor* y, const evkhip_tensor* post_weight, const evkhip_tensor* gate,
+                         const evkhip_tensor* pre_weight, const evkhip_tensor* s, const evkhip_tensor* h, float residual_scale, int post_norm,
+                         float eps, void* stream);
+
+/* Its gradient from ds (of s, by what reads the stream later; NULL: zeros) and dh
+ * (of h): dx and dy (NULL without y) are written; dpost_weight, dgate and
+ * dpre_weight (as what they belong to, NULL: not wanted) are written, or added
+ * to with accumulate (summed in 32 bits in a fixed order, rounded once).  gates:
+ * B for a gate (B,D), else 1.  The workspace is needed for the latter three only. */
+uint64_t evkhip_residual_norm_backward_workspace(uint64_t rows, uint64_t gates, uint32_t d);
+int evkhip_residual_norm_backward(const evkhip_tensor* x, const evkhip_tensor* y, const evkhip_tensor* post_weight, const evkhip_tensor* gate,
+                                  const evkhip_tensor* pre_weight, const evkhip_tensor* ds, const evkhip_tensor* dh, const evkhip_tensor* dx,
+                                  const evkhip_tensor* dy, const evkhip_tensor* dpost_weight, const evkhip_tensor* dgate,
+                                  const evkhip_tensor* dpre_weight, float residual_scale, int post_norm, float eps, int accumulate,
+                                  void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Attention of sequences that share a prefix.  q, o (B,N,H*head_dim); prefix_k,
+ * prefix_v (P,KV*head_dim), one for all; k, v (B,rows,KV*head_dim), each
+ * sequence's own rows behind it; scale 1/sqrt(head_dim).  Query t of sequence b
+ * stands at own row p = position_offset + t, or offsets[b] + t (offsets: device
+ * int32 (B), then position_offset is 0), and sees the whole prefix and the own
+ * rows j <= p.  Own rows that a query does not see do not reach its output,
+ * whatever they hold.  A query that sees no row (P 0 and p below 0) has output 0
+ * and log-sum-exp -inf; one whose scores are all -inf has output NaN and
+ * log-sum-exp -inf.  lse: NULL or fp32 (B,H,N).  N == 1 is a decode step.
+ * head_dim up to 256. */
+uint64_t evkhip_prefix_attention_workspace(uint32_t batch, uint32_t n, uint32_t prefix, uint32_t rows, uint32_t heads, uint32_t kv_heads,
+                                           uint32_t head_dim);
+int evkhip_prefix_attention(const evkhip_tensor* q, const evkhip_tensor* prefix_k, const evkhip_tensor* prefix_v, const evkhip_tensor* k,
+                            const evkhip_tensor* v, const evkhip_tensor* o, uint32_t head_dim, uint32_t position_offset, const int32_t* offsets,
+                            float* lse, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Log-probabilities of given tokens.  logits (...,V), V up to 65536; tokens raw
+ * uint16, one a row; p = softmax(input_scale * logits) over a row:
+ *   logprobs[r] = log p[tokens[r]], 0 where the id is V or above (no token)
+ *   entropy[r]  = -sum p log p                           (NULL: not wanted)
+ *   top_ids (...,K) raw uint16, top_logprobs (rows,K): the K largest logits, the
+ *     lowest id first among equal ones, and their log p  (both NULL: not wanted)
+ *   stats (rows,2): what the gradient needs                (NULL: not wanted)
+ * All but top_ids are fp32.  Logits of -inf have p = 0.  A row that holds NaN or
+ * +inf, or nothing but -inf, has no distribution: its results are NaN; its
+ * alternatives go by the logits all the same, NaN above +inf.  K up to 32;
+ * input_scale from 2^-24 to 65504. */
+int evkhip_token_logprobs(const evkhip_tensor* logits, const evkhip_tensor* tokens, float* logprobs, float* entropy, const evkhip_tensor* top_ids,
+                          float* top_logprobs, float* stats, float input_scale, void* stream);
+
+/* Its gradient from the forward's stats (and entropy, with dentropy) and fp32
+ * dlogprobs, dentropy (rows; one may be NULL, zeros): dlogits (as logits) is
+ * written.  A row for which both are 0, or that has no token and no dentropy, is
+ * zeros, whatever its logits hold. */
+int evkhip_token_logprobs_backward(const evkhip_tensor* logits, const evkhip_tensor* tokens, const float* stats, const float* entropy,
+                                   const float* dlogprobs, const float* dentropy, const evkhip_tensor* dlogits, float input_scale, void* stream);
 
 /* ---------------------------------------------------------------------------
  * KV-cached greedy decode (the caller the single-query path exists for; the
