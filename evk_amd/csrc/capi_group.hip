@@ -98,7 +98,7 @@ int logits_shapes(const char* op, const evkhip_tensor* logits, const evkhip_tens
 
 // Whether the call takes these sizes; those that it refuses need no workspace.
 bool prefix_sizes(uint32_t B, uint32_t N, uint32_t P, uint32_t R, uint32_t H, uint32_t KV, uint32_t dh) {
-    return B && N && H && KV && H % KV == 0 && dh && dh <= 256 && N <= kMaxRows && R <= kMaxRows && P <= kMaxRows / KV &&
+    return B && N && H && KV && H % KV == 0 && dh && dh <= 256 && N <= kMaxRows && R <= kMaxRows && P <= kMaxRows / KV && (uint64_t)P + R <= kMaxRows &&
            (uint64_t)B * N <= kMaxRows / H && (uint64_t)B * R <= kMaxRows / KV && (uint64_t)H + 2 * KV <= kMaxRows;
 }
 
@@ -200,7 +200,7 @@ int evkhip_prefix_attention(const evkhip_tensor* q, const evkhip_tensor* prefix_
     EVK_RETURN_IF(!same_dims(prefix_k, prefix_v), EVKHIP_ERR_SHAPE, "%s: prefix_k and prefix_v differ", op);
     EVK_RETURN_IF(prefix_k->dims[1] != k->dims[2], EVKHIP_ERR_SHAPE, "%s: rows of %u values in the prefix, %u behind it", op, prefix_k->dims[1], k->dims[2]);
     const uint32_t P = prefix_k->dims[0];
-    EVK_RETURN_IF(P > kMaxRows / s.KV, EVKHIP_ERR_UNSUPPORTED, "%s: more than 2^30 rows", op);
+    EVK_RETURN_IF(P > kMaxRows / s.KV || (uint64_t)P + s.R > kMaxRows, EVKHIP_ERR_UNSUPPORTED, "%s: more than 2^30 rows", op);
     CHECK(check_positions(op, s, position_offset, offsets));
     CHECK(check_floats(op, "lse", lse));
     const uint64_t need = evkhip_prefix_attention_workspace(s.B, s.N, P, s.R, s.H, s.KV, head_dim);

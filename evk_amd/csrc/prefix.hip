@@ -8,18 +8,13 @@
 // One that sees nothing (P = 0, p < 0) has O = 0, LSE = -inf; one whose scores
 // are all -inf has no softmax: O = NaN, LSE = -inf.  Own rows that a query does
 // not see stay out of its sums, whatever they hold.
-#include "kernels.h"
+#include "attention_tiles.h"
 
 #include <algorithm>
-
-#include <math.h>
 
 namespace evkhip {
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // Own rows that query t of sequence b sees
 DEV int own_rows(const PrefixArgs& a, int b, int t) {
@@ -36,12 +31,6 @@ struct RowLds {
     float x[SMAX], p[64];
     const f16* v[64];
 };
-DEV void wave_sync() {  // the wave's LDS accesses before this are done
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 __global__ __launch_bounds__(64) void prefix_rows(PrefixArgs a) {
     __shared__ RowLds s;
     const int lane = threadIdx.x, dh = a.dh;
@@ -89,20 +78,330 @@ __global__ __launch_bounds__(64) void prefix_rows(PrefixArgs a) {
     if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = total ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
+// ---------------------------------------------------------------------------
+// MFMA kernels: head sizes that are multiples of 8 (zero-filled to DH = 32, 64,
+// 96, 128 or 256), 16-byte aligned pointers.
+//
+// The query side of a key head is a matrix of B N G rows (G = H / KV), row r
+// being query r / G (sequence r / G / N) of the group's head r % G.  Rows of all
+// sequences see the same prefix, so that a tile of them reads it once.
+// ---------------------------------------------------------------------------
+
+// Where a row of the matrix lies, and what it sees
+struct Rows {
+    int group;
+    int64_t q0;  // of head c
+    DEV Rows(const PrefixArgs& a, int c) : group(a.H / a.KV), q0((int64_t)c * group) {}
+    DEV int64_t row(const PrefixArgs& a, int r) const { return (int64_t)(r / group) * a.H + q0 + r % group; }  // of q
+    DEV int own(const PrefixArgs& a, int r) const { return own_rows(a, r / group / a.N, r / group % a.N); }
+    DEV int64_t lse(const PrefixArgs& a, int r) const {
+        return ((int64_t)(r / group / a.N) * a.H + q0 + r % group) * a.N + r / group % a.N;
+    }
+};
+
+// States of parts of a row's list: m, l, 2 unused, O
+template <int DH>
+DEV float* state_at(float* ws, int64_t row, int slots, int slot) {
+    return ws + (row * slots + slot) * (DH + 4);
+}
+
+// Tiles of 64 QB rows over the prefix and, where they are one sequence's, its own
+// rows behind it.  The prefix is padded to whole tiles of the list.
+struct TileWork {
+    int per, tiles;    // rows of one sequence (B N G: all of them together, over the prefix alone), tiles of them
+    int own;           // their own rows are part of the list
+    int splits, slots; // parts of the list; states of a row (0: none, the output is written)
+};
+template <int DH, int QB>
+DEV void tile_rows(const PrefixArgs& a, const TileWork& w, int item, float* ws, f16* smem) {
+    using G = Geo<DH>;
+    constexpr int KS = G::KS, DT = G::DT, TILE = BK * G::W, ROWS = 64 * QB;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const int split = item % w.splits, tile = w.tiles - 1 - item / w.splits % w.tiles, bc = item / w.splits / w.tiles, c = bc % a.KV, b = bc / a.KV;
+    const Rows rows(a, c);
+    const int R0 = b * w.per + tile * ROWS, end = (b + 1) * w.per, wr0 = R0 + wave * 16 * QB;
+    const int sl = w.own ? (a.P + BK - 1) / BK * BK : a.P;  // entries before the own rows
+    const int least = w.own ? __builtin_amdgcn_readfirstlane(rows.own(a, R0)) : 0;
+    const int most = w.own ? __builtin_amdgcn_readfirstlane(rows.own(a, min(R0 + ROWS, end) - 1)) : 0;
+    const int n = sl + most, nt = (n + BK - 1) / BK;
+    const int t0 = (int)((int64_t)nt * split / w.splits), t1 = (int)((int64_t)nt * (split + 1) / w.splits);
+    const uint32_t ld = (uint32_t)a.KV * a.dh * 2;
+    const int64_t own0 = (int64_t)b * a.R * a.KV * a.dh + (int64_t)c * a.dh;
+
+    TileDma<DH, BK, 4> dma{wave, lane};
+    uint32_t off[TileDma<DH, BK, 4>::PER];
+#pragma unroll
+    for (int i = 0; i < TileDma<DH, BK, 4>::PER; ++i) off[i] = oob_or(dma.chunk(i) * 8 < a.dh, dma.row(i) * ld + dma.chunk(i) * 16);
+    const auto k_row = [&](int e) { return (e < sl ? a.pk + (int64_t)c * a.dh + (int64_t)e * (ld / 2) : a.k + own0 + (int64_t)(e - sl) * (ld / 2)); };
+    const auto v_row = [&](int e) { return (e < sl ? a.pv + (int64_t)c * a.dh + (int64_t)e * (ld / 2) : a.v + own0 + (int64_t)(e - sl) * (ld / 2)); };
+    const auto load = [&](int t, f16* sk, f16* sv) {
+        const int i0 = t * BK;
+        const uint32_t span = (uint32_t)min((i0 < sl ? a.P : n) - i0, BK) * ld;  // what lies past it reads as zeros
+        dma.go(wave_rsrc(k_row(i0), span), off, sk);
+        dma.go(wave_rsrc(v_row(i0), span), off, sv);
+    };
+    if (t0 < t1) load(t0, smem, smem + TILE);
+
+    half8 qf[QB][KS];
+    int own[QB];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int r = min(wr0 + 16 * q + l16, end - 1);
+        own[q] = w.own ? rows.own(a, r) : 0;
+        const f16* src = a.q + rows.row(a, r) * a.dh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            qf[q][ks] = half8{};
+            if (32 * ks + 8 * g < a.dh) qf[q][ks] = *reinterpret_cast<const half8*>(src + 32 * ks + 8 * g);
+        }
+    }
+    const float c2 = a.scale * kLog2e;
+    Softmax<DH, QB> sm;
+    const auto plain = [&](int t) {
+        const int i1 = (t + 1) * BK;
+        return (i1 <= a.P) | ((i1 > sl) & (i1 <= sl + least));
+    };
+    const auto seen = [&](int q) { return [P = a.P, sl, last = sl + own[q]](int e) { return (e < P) | ((e >= sl) & (e < last)); }; };
+    const uint32_t wild = attend_tiles<DH, QB>(sm, qf, c2, smem, dma, t0, t1, load, plain, seen);
+    if (__syncthreads_or(wild))
+        each_wild(plain, [&](int e) { return ((e < a.P) | (e >= sl)) & (e < n) ? v_row(e) : nullptr; }, a.dh, BK, t0, t1, 1, lane, [&](int e) {
+            bool sees[QB];
+#pragma unroll
+            for (int q = 0; q < QB; ++q) sees[q] = seen(q)(e);
+            sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g);
+        });
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+        const int r = wr0 + 16 * q + l16;
+        const float l = query_sum(sm.l[q]);
+        if (r >= end) continue;
+        if (w.slots) {
+            float* dst = state_at<DH>(ws, rows.row(a, r), w.slots, split);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<floatx4*>(dst + 4 + 16 * d + 4 * g) = sm.o[d][q];
+            if (g == 0) dst[0] = sm.m[q], dst[1] = l;
+            continue;
+        }
+        const bool none = a.P + own[q] == 0;
+        const float inv = none ? 0.0f : 1.0f / l;
+        f16* dst = a.out + rows.row(a, r) * a.dh;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            if (16 * d + 4 * g < a.dh)
+                *reinterpret_cast<uint2*>(dst + 16 * d + 4 * g) =
+                    uint2{pack_h2(sm.o[d][q][0] * inv, sm.o[d][q][1] * inv), pack_h2(sm.o[d][q][2] * inv, sm.o[d][q][3] * inv)};
+        if (a.lse && g == 0) a.lse[rows.lse(a, r)] = none ? -INFINITY : (sm.m[q] + log2f(l)) * kLn2;
+    }
+}
+template <int DH, int QB>
+__global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void prefix_tiles(PrefixArgs a, TileWork w, float* ws) {
+    __shared__ __attribute__((aligned(1024))) f16 smem[4 * BK * Geo<DH>::W];
+    // an XCD takes items that follow each other, which share rows of K and V
+    tile_rows<DH, QB>(a, w, xcd_tile(blockIdx.x, gridDim.x), ws, smem);
+}
+
+// 16 rows of one sequence, the waves' steps over its own rows and, where nobody
+// else sees to it, the prefix before them.
+struct StepWork {
+    int tiles;
+    int prefix;               // rows of the prefix in the list: P or 0
+    int splits, slots, slot;  // parts of the list; states of a row (0: none) and this list's first
+};
+template <int DH, int NW>
+DEV void step_rows(const PrefixArgs& a, const StepWork& w, int item, float* ws, char* smem, float (*sm_m)[16], float (*sm_l)[16]) {
+    using G = Geo<DH>;
+    constexpr int KS = G::KS;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const int split = item % w.splits, tile = item / w.splits % w.tiles, bc = item / w.splits / w.tiles, c = bc % a.KV, b = bc / a.KV;
+    const Rows rows(a, c);
+    const int per = a.N * rows.group, R0 = b * per + tile * 16, end = (b + 1) * per, pre = w.prefix;
+    const int least = __builtin_amdgcn_readfirstlane(rows.own(a, R0)), most = __builtin_amdgcn_readfirstlane(rows.own(a, min(R0 + 16, end) - 1));
+    const int n = pre + most, steps = (n + 31) / 32;
+    const int c0 = (int)((int64_t)steps * split / w.splits), c1 = (int)((int64_t)steps * (split + 1) / w.splits), first = c0 + wave;
+    const int64_t ld = (int64_t)a.KV * a.dh, own0 = (int64_t)b * a.R * ld + (int64_t)c * a.dh;
+    const auto k_row = [&](int e) {
+        e = min(e, n - 1);
+        return e < pre ? a.pk + (int64_t)c * a.dh + e * ld : a.k + own0 + (e - pre) * ld;
+    };
+    const auto v_row = [&](int e) {
+        e = min(e, n - 1);
+        return e < pre ? a.pv + (int64_t)c * a.dh + e * ld : a.v + own0 + (e - pre) * ld;
+    };
+    Steps<DH, NW> walk(reinterpret_cast<f16*>(smem) + wave * 32 * G::W, lane);
+    if (first < c1) walk.load(first, k_row, v_row, a.dh);
+    const int r = min(R0 + l16, end - 1), last = pre + rows.own(a, r);
+    half8 qf[1][KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        qf[0][ks] = half8{};
+        if (32 * ks + 8 * g < a.dh) qf[0][ks] = *reinterpret_cast<const half8*>(a.q + rows.row(a, r) * a.dh + 32 * ks + 8 * g);
+    }
+    const float c2 = a.scale * kLog2e;
+    Softmax<DH, 1> sm;
+    const auto plain = [&](int step) { return 32 * step + 32 <= pre + least; };
+    const auto seen = [&] { return [last](int e) { return e < last; }; };
+    const uint64_t wild = walk.run(sm, qf, c2, first, c1, k_row, v_row, a.dh, plain, seen);
+    if (wild)
+        each_wild(plain, [&](int e) { return e < n ? v_row(e) : nullptr; }, a.dh, 32, first, c1, NW, lane, [&](int e) {
+            const bool sees[1] = {e < last};
+            sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g);
+        });
+    merge_waves<DH, NW>(sm, smem, sm_m, sm_l, lane, wave, [&](int q, int d, float m, float l, const floatx4& o) {
+        const int row = R0 + q;
+        if (row >= end) return;
+        if (w.slots) {
+            float* dst = state_at<DH>(ws, rows.row(a, row), w.slots, w.slot + split);
+            *reinterpret_cast<floatx4*>(dst + 4 + d) = o;
+            if (d == 0) dst[0] = m, dst[1] = l;
+            return;
+        }
+        const bool none = pre + rows.own(a, row) == 0;
+        const float inv = none ? 0.0f : 1.0f / l;
+        if (d < a.dh)
+            *reinterpret_cast<uint2*>(a.out + rows.row(a, row) * a.dh + d) = uint2{pack_h2(o[0] * inv, o[1] * inv), pack_h2(o[2] * inv, o[3] * inv)};
+        if (a.lse && d == 0) a.lse[rows.lse(a, row)] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+    });
+}
+template <int DH>
+struct StepGeo {
+    static constexpr int NW = DH <= 128 ? 8 : 4;  // waves; 256 values take the registers of two
+};
+template <int DH>
+__global__ __launch_bounds__(64 * StepGeo<DH>::NW, StepGeo<DH>::NW / 4) void prefix_steps(PrefixArgs a, StepWork w, float* ws) {
+    constexpr int NW = StepGeo<DH>::NW;
+    __shared__ __attribute__((aligned(16))) char smem[steps_bytes<DH, NW>()];
+    __shared__ float sm_m[NW][16], sm_l[NW][16];
+    step_rows<DH, NW>(a, w, xcd_tile(blockIdx.x, gridDim.x), ws, smem, sm_m, sm_l);
+}
+
+// The states of a row, added in order by one wave.
+constexpr int JOIN_MOST = 64;  // a lane weighs one
+template <int DH>
+__global__ __launch_bounds__(256) void prefix_join(PrefixArgs a, int slots, int64_t rows, const float* ws) {
+    constexpr int PER = (DH + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const float* src = ws + row * slots * (DH + 4);
+    const bool is = lane < slots;
+    const float mine = is ? src[lane * (DH + 4)] : -INFINITY, m = wave_max(mine);
+    const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - m);
+    const float l = wave_sum(is ? f * src[lane * (DH + 4) + 1] : 0.0f);
+    float o[PER] = {};
+#pragma unroll 8
+    for (int s = 0; s < slots; ++s) {
+        const float fs = __shfl(f, s, 64);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (lane + 64 * i < DH) o[i] += fs * src[s * (DH + 4) + 4 + lane + 64 * i];
+    }
+    const int h = (int)(row % a.H), t = (int)(row / a.H % a.N), b = (int)(row / a.H / a.N);
+    const bool none = a.P + own_rows(a, b, t) == 0;
+    const float inv = none ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (lane + 64 * i < a.dh) a.out[row * a.dh + lane + 64 * i] = (f16)(o[i] * inv);
+    if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+bool mfma_ok(const PrefixArgs& a) {
+    for (const void* p : {(const void*)a.q, (const void*)a.pk, (const void*)a.pv, (const void*)a.k, (const void*)a.v, (const void*)a.out})
+        if (!aligned16(p)) return false;
+    // a tile's rows behind one descriptor
+    return a.dh % 8 == 0 && (int64_t)a.KV * a.dh * 2 * (BK + 1) < INT32_MAX;
+}
+
+int query_blocks(int64_t rows, int64_t heads, int dh) { return dh <= 128 && heads * ((rows + 127) / 128) > 256 ? 2 : 1; }
+
+// How a shape runs.
+struct Plan {
+    enum { TILES, STEPS, SHARED } kind;
+    int qb;          // TILES, SHARED
+    TileWork tiles;  // TILES: all; SHARED: the prefix
+    StepWork steps;  // STEPS: all; SHARED: the own rows
+    int slots;
+};
+Plan plan_for(int64_t B, int64_t N, int64_t P, int64_t R, int64_t H, int64_t KV, int dh) {
+    Plan p{};
+    const int64_t per = N * (H / KV), heads = B * KV, waves = dh <= 128 ? 8 : 4;
+    auto ceil = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    if (per >= 64) {
+        p.kind = Plan::TILES;
+        p.qb = query_blocks(per, heads, dh);
+        const int64_t tiles = ceil(per, 64 * p.qb), groups = heads * tiles;
+        int64_t splits = std::max<int64_t>(1, std::min({512 / groups, ceil(P + R, 4 * BK), (int64_t)JOIN_MOST}));
+        p.slots = splits > 1 ? (int)splits : 0;
+        p.tiles = {(int)per, (int)tiles, 1, (int)splits, p.slots};
+        return p;
+    }
+    const int64_t tiles = ceil(per, 16), groups = heads * tiles;
+    const bool share = B > 1 && P >= 512 && B * per > 16;
+    if (!share) {
+        p.kind = Plan::STEPS;
+        const int64_t steps = ceil(P + R, 32);
+        const int64_t splits = steps <= 4 * waves ? 1 : std::max<int64_t>(1, std::min({ceil(steps, waves), 256 / groups, (int64_t)JOIN_MOST}));
+        p.slots = splits > 1 ? (int)splits : 0;
+        p.steps = {(int)tiles, (int)P, (int)splits, p.slots, 0};
+        return p;
+    }
+    p.kind = Plan::SHARED;
+    const int64_t all = B * per;
+    p.qb = query_blocks(all, KV * 16, dh);
+    const int64_t wide = ceil(all, 64 * p.qb) * KV;
+    const int64_t s1 = std::max<int64_t>(1, std::min({512 / wide, ceil(P, 4 * BK), (int64_t)JOIN_MOST / 2}));
+    const int64_t steps = ceil(R, 32);
+    const int64_t s2 = steps <= 4 * waves ? 1 : std::max<int64_t>(1, std::min({ceil(steps, waves), 256 / groups, (int64_t)JOIN_MOST / 2}));
+    p.slots = (int)(s1 + s2);
+    p.tiles = {(int)all, (int)ceil(all, 64 * p.qb), 0, (int)s1, p.slots};
+    p.steps = {(int)tiles, 0, (int)s2, p.slots, (int)s1};
+    return p;
+}
+
 }  // namespace
 
 uint64_t prefix_workspace(int B, int N, int P, int R, int H, int KV, int dh) {
-    (void)B, (void)N, (void)P, (void)R, (void)H, (void)KV, (void)dh;
-    return 0;
+    if (dh % 8) return 0;
+    return (uint64_t)plan_for(B, N, P, R, H, KV, dh).slots * B * N * H * (head_width(dh, 32) + 4) * sizeof(float);
 }
 
 int prefix_forward(const PrefixArgs& a, void* ws, hipStream_t st) {
-    (void)ws;
+    const char* op = "prefix_attention";
     const int64_t rows = (int64_t)a.B * a.N * a.H;
-    const int rc = check_grid("prefix_attention", rows, 64);
+    hipError_t e;
+    if (!mfma_ok(a)) {
+        const int rc = check_grid(op, rows, 64);
+        if (rc != EVKHIP_OK) return rc;
+        hipLaunchKernelGGL(prefix_rows, dim3((unsigned)rows), dim3(64), 0, st, a);
+        e = hipGetLastError();
+        return e == hipSuccess ? EVKHIP_OK : check_hip(e, "prefix_attention launch");
+    }
+    const Plan p = plan_for(a.B, a.N, a.P, a.R, a.H, a.KV, a.dh);
+    const int64_t seqs = p.kind == Plan::SHARED ? 1 : a.B;
+    const int64_t wide = p.kind == Plan::STEPS ? 0 : seqs * a.KV * p.tiles.tiles * p.tiles.splits;
+    const int64_t few = p.kind == Plan::TILES ? 0 : (int64_t)a.B * a.KV * p.steps.tiles * p.steps.splits;
+    int rc = check_grid(op, wide, 256);
+    if (rc == EVKHIP_OK) rc = check_grid(op, few, 512);
+    if (rc == EVKHIP_OK && p.slots) rc = check_grid(op, (rows + 3) / 4, 256);
     if (rc != EVKHIP_OK) return rc;
-    hipLaunchKernelGGL(prefix_rows, dim3((unsigned)rows), dim3(64), 0, st, a);
-    const hipError_t e = hipGetLastError();
+    e = by_head(a.dh, [&](auto dhc) {
+        constexpr int DH = decltype(dhc)::value;
+        float* const part = (float*)ws;
+        if (wide) {
+            auto go = [&](auto qb) {
+                hipLaunchKernelGGL((prefix_tiles<DH, decltype(qb)::value>), dim3((unsigned)wide), dim3(256), 0, st, a, p.tiles, part);
+            };
+            if constexpr (DH <= 128) {
+                if (p.qb == 2) go(std::integral_constant<int, 2>{});
+                else go(std::integral_constant<int, 1>{});
+            } else {
+                go(std::integral_constant<int, 1>{});
+            }
+        }
+        if (few) hipLaunchKernelGGL(prefix_steps<DH>, dim3((unsigned)few), dim3(64 * StepGeo<DH>::NW), 0, st, a, p.steps, part);
+        if (p.slots) hipLaunchKernelGGL(prefix_join<DH>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p.slots, rows, (const float*)part);
+    });
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "prefix_attention launch");
 }
 

@@ -14,18 +14,13 @@
 //
 // Rows that a query does not see are never read for it, so that whatever they
 // hold (stale cache rows, infinities, NaN) stays out of its sums.
-#include "kernels.h"
+#include "attention_tiles.h"
 
 #include <algorithm>
-
-#include <math.h>
 
 namespace evkhip {
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // The rows that a query at position p sees.
 struct Span {
@@ -70,12 +65,6 @@ struct RowLds {
     float x[SMAX], y[SMAX], p[64], q[64];
     int64_t j[64];
 };
-DEV void wave_sync() {  // the wave's LDS accesses before this are done
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // O and LSE of query row `row` = ((b N) + t) H + h
 DEV void fwd_row(const WindowArgs& a, int64_t row, RowLds& s, int lane) {
     const int dh = a.dh, h = (int)(row % a.H), t = (int)(row / a.H % a.N), b = (int)(row / a.H / a.N);
@@ -231,77 +220,7 @@ __global__ __launch_bounds__(64) void window_dkdv_rows(WindowArgs a) {
 // of the list is a tile of K and of V, so that a few sinks cost a few rows, no
 // tile of their own.  Only the tiles at the list's start and end hold rows that
 // some query does not see; the others run without a compare per score.
-//
-// v_mfma_f32_16x16x32_f16 throughout: S^T = K Q^T gives a lane one query
-// (column l16 = lane % 16) and rows 4 g + j (g = lane / 16) of each 16-row
-// block, which is the B operand of O^T += V^T P^T as it stands (slot s: row
-// 4 g + s of the first, 4 g + s - 4 of the second block); V^T comes from the
-// row-major tile by ds_read_b64_tr_b16.
 // ---------------------------------------------------------------------------
-constexpr int BK = 64;               // list entries per tile
-constexpr float RESCALE_LOG2 = 8.0f;  // O and l are rescaled when a score passes the reference by 2^8
-
-template <int DH>
-struct Geo {
-    static constexpr int KS = DH / 32, DT = DH / 16;
-    static constexpr int W = DH <= 32 ? 32 : DH <= 64 ? 64 : DH <= 128 ? 128 : 256;  // halves of an LDS row
-    static constexpr int CPR = W / 8;                                               // 16-byte chunks of it
-};
-// Chunk c of row r lies at slot c ^ swz(r).  LDS serves a transposed read in
-// halves of the wave (rows 0 .. 7, 8 .. 15 at one pair of chunks) and a 16-byte
-// read in four sets of lanes, each with all 16 rows, rows 4 .. 11 at the chunk
-// of the neighbouring g: both meet every bank once (measured: no conflicts).
-template <int W>
-DEV int swz(int r) {
-    return 2 * (W >= 128 ? r & 7 : W == 64 ? (r >> 1) & 3 : (r >> 2) & 1);
-}
-// A lane's places in a tile: offsets are sums of a row's and exclusive ors of
-// a chunk's part.
-template <int DH>
-struct Frag {
-    static constexpr int W = Geo<DH>::W;
-    int row_at, col_at;
-    DEV explicit Frag(int lane) {
-        const int l16 = lane & 15, g = lane >> 4, r = 4 * g + (l16 >> 2), c = l16 & 3;
-        row_at = l16 * W + ((g ^ swz<W>(l16)) << 3);
-        col_at = r * W + (((c >> 1) ^ swz<W>(r)) << 3) + (c & 1) * 4;
-    }
-    // row r0 + l16 (r0 a multiple of 16), chunk 4 ks + g
-    DEV half8 row(const f16* t, int r0, int ks) const {
-        return *reinterpret_cast<const half8*>(t + r0 * W + (row_at ^ (ks << 5)));
-    }
-    // column 16 d + l16 of rows r0 + 4 g .. + 3 and 16 further (r0 a multiple of 32): two transposed reads
-    DEV half8 col(const f16* t, int r0, int d) const {
-        const f16* p = t + r0 * W + (col_at ^ (d << 4));
-        return cat4(lds_read_tr(p), lds_read_tr(p + 16 * W));
-    }
-};
-
-// buf_rsrc of values that are the same in the whole wave, wherever they were computed
-DEV __amdgpu_buffer_rsrc_t wave_rsrc(const void* base, uint32_t bytes) {
-    const uint64_t p = (uint64_t)base;
-    const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)p), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32));
-    return buf_rsrc((const void*)(hi << 32 | lo), (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
-}
-
-// ROWS rows of 16-byte chunks into LDS by NWV waves: the lane's share of one
-// tile is chunk `chunk(i)` of row `row(i)`, i < PER, each 16 bytes to
-// lds + 1 KB (wave PER + i) + 16 lane.
-template <int DH, int ROWS, int NWV>
-struct TileDma {
-    using G = Geo<DH>;
-    static constexpr int RPI = 64 / G::CPR, PER = ROWS / RPI / NWV;
-    static_assert(PER >= 1 && ROWS % (RPI * NWV) == 0, "tile shape");
-    int wave, lane;
-    DEV int row(int i) const { return (wave * PER + i) * RPI + lane / G::CPR; }
-    DEV int chunk(int i) const { return (lane % G::CPR) ^ swz<G::W>(row(i)); }
-    DEV void go(__amdgpu_buffer_rsrc_t res, const uint32_t (&off)[PER], f16* lds) const {
-        const uint32_t at = lds_addr(lds) + wave * PER * 1024;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) dma16(res, off[i], at + i * 1024);
-    }
-};
-
 // The list of the rows that the queries t0 .. t1 of sequence b see.
 struct List {
     int pmin, pmax;  // positions of the first and last query (-1: sees nothing)
@@ -319,6 +238,7 @@ struct List {
         n = sl + hi - lo;
         first = lo ? s : a.sinks;
     }
+    DEV bool has(int i) const { return (i < n) & ((i < s) | (i >= sl)); }
     DEV int row(int i) const { return i < sl ? i : lo + (i - sl); }
     // every query of the tile sees the entries [i0, i0 + len)
     DEV bool plain(const WindowArgs& a, int i0, int len) const {
@@ -378,269 +298,12 @@ struct KvTiles {
     }
 };
 
-// This wave's loads have arrived, and no access moves ahead of that.  The builtin
-// tells the compiler as much, which otherwise waits in the loop for registers
-// that were loaded before it, and so for the loads into LDS.
-DEV void wait_loads() {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    asm volatile("" ::: "memory");
-}
-
-// N steps, each of M MFMAs on fragments that R LDS reads brought: the reads of
-// step i + AHEAD go out before the MFMAs of step i (read(i, slot) into slot
-// i % (AHEAD + 1) of a ring, use(i, slot)).  start() requests the first ones,
-// ahead of work that hides them; `pin` holds the scheduler to this order.
-template <int N, int AHEAD>
-struct Ring {
-    static constexpr int SLOTS = AHEAD + 1;
-    template <int R, class F>
-    static DEV void start(F&& read) {
-        static_for<AHEAD>([&](auto i) { read(i, i); });
-        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * R, 0);
-    }
-    template <int M, int R, class F, class U>
-    static DEV void run(F&& read, U&& use) {
-        static_for<N>([&](auto ic) {
-            constexpr int i = decltype(ic)::value;
-            if constexpr (i + AHEAD < N) {
-                read(std::integral_constant<int, i + AHEAD>{}, std::integral_constant<int, (i + AHEAD) % SLOTS>{});
-                __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
-            }
-            use(ic, std::integral_constant<int, i % SLOTS>{});
-            __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
-        });
-    }
-};
-
-DEV float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
-// over the four lanes of a query (16 and 32 apart)
-DEV float query_max(float m) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    m = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
-DEV float query_sum(float m) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    m = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
-}
-
 // n / d for 0 <= n < d + 2^16, d < 2^21: the quotient of n + 1/2 is at least
 // 1 / (2 d) from a whole number, its error at most 2^-22.
 struct SmallDiv {
     float inv;
     DEV explicit SmallDiv(int d) : inv(1.0f / (float)d) {}
     DEV int operator()(int n) const { return (int)(((float)n + 0.5f) * inv); }
-};
-
-// Hidden rows.  The MFMA's product of a weight of 0 and a NaN or an infinity is
-// NaN, and the rows of a tile that some of its columns (queries; keys in the
-// kernel of dK and dV) do not see may hold either: stale cache rows, padding, a
-// gradient that overflowed.  In tiles that are not seen whole, the wave that
-// loads a row looks at it and leaves zeros in LDS where it finds such a value;
-// the columns that do see the row add it at the end, from memory and in 32 bits,
-// unless their sums are NaN by then.  So it reaches those alone, and what it
-// costs goes by the rows at the ends of a list, not by pairs: 4096 queries of 8
-// heads over 2 of 128 values, window 512, both directions 111 us, with one
-// infinite row of dO 129, an infinity in every hundredth value of dO 497, a third
-// of all rows NaN 382.
-
-// NaN or infinity among the values: a product with 0 is 0 for every other one
-DEV half2_t wild2(const half8& x, half2_t w) {
-    const half2_t z = {(f16)0.0f, (f16)0.0f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w = __builtin_elementwise_fma(half2_t{x[2 * i], x[2 * i + 1]}, z, w);
-    return w;
-}
-
-DEV bool is_wild(half2_t w) { return !((float)w[0] == 0.0f && (float)w[1] == 0.0f); }
-DEV bool wild_row(const f16* p, int n) {  // n a multiple of 8
-    half2_t w = {(f16)0.0f, (f16)0.0f};
-    for (int i = 0; i < n; i += 8) w = wild2(*reinterpret_cast<const half8*>(p + i), w);
-    return is_wild(w);
-}
-// This wave's part of a tile in LDS, with zeros for the rows that hold a NaN or
-// an infinity; their bits, the part's first row lowest.
-template <class Dma>
-DEV uint32_t clean_rows(const Dma& dma, f16* tile) {
-    constexpr int CPR = Dma::G::CPR, RPI = Dma::RPI;
-    int lane = dma.lane;
-    asm volatile("" : "+v"(lane));  // addresses formed here, not kept through the kernel
-    uint32_t rows = 0;
-#pragma unroll
-    for (int i = 0; i < Dma::PER; ++i) {
-        u32x4* const p = reinterpret_cast<u32x4*>(tile + ((dma.wave * Dma::PER + i) * 64 + lane) * 8);
-        const uint64_t hit = __ballot(is_wild(wild2(as_half8(*p), half2_t{(f16)0.0f, (f16)0.0f})));
-        if (!hit) continue;
-        constexpr uint64_t ROW = (1ull << CPR) - 1;
-        if (hit >> (lane / CPR * CPR) & ROW) *p = u32x4{0u, 0u, 0u, 0u};
-        for (int k = 0; k < RPI; ++k) rows |= (hit >> (k * CPR) & ROW ? 1u : 0u) << (i * RPI + k);
-    }
-    return rows;
-}
-// What follows runs for such rows only, a few loads at a time and from places
-// formed on the spot: kept from the kernel's start, they would cost every call
-// the registers.
-//
-// products of the columns' operands (values 32 ks + 8 g and on) and a row, in each column's four lanes
-template <int KS, int QB>
-DEV void row_dot(float (&v)[QB], const half8 (&x)[QB][KS], const f16* row, int dh, int g) {
-    asm volatile("" : "+v"(g));
-#pragma unroll
-    for (int q = 0; q < QB; ++q) v[q] = 0.0f;
-#pragma unroll
-    for (int k0 = 0; k0 < KS; k0 += 4) {
-        u32x4 y[4];
-#pragma unroll
-        for (int k = 0; k < 4 && k0 + k < KS; ++k) y[k] = *reinterpret_cast<const u32x4*>(row + min(32 * (k0 + k) + 8 * g, dh - 8));
-#pragma unroll
-        for (int k = 0; k < 4 && k0 + k < KS; ++k) {
-            const half8 r = as_half8(32 * (k0 + k) + 8 * g < dh ? y[k] : u32x4{0u, 0u, 0u, 0u});
-#pragma unroll
-            for (int q = 0; q < QB; ++q) {
-                u32x4 u = as_u32x4(x[q][k0 + k]);
-                asm volatile("" : "+v"(u));  // else converted once, for the lengths at the start, and kept
-                const half8 c = as_half8(u);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[q] = __builtin_fmaf((float)c[i], (float)r[i], v[q]);
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int q = 0; q < QB; ++q) v[q] = query_sum(v[q]);
-}
-// acc[d][q] += w[q] row, for the columns that see it (and what nobody stores: values past dh)
-template <int DT, int QB>
-DEV void add_row(floatx4 (&acc)[DT][QB], const float (&w)[QB], const bool (&sees)[QB], const f16* row, int dh, int g) {
-    asm volatile("" : "+v"(g));
-#pragma unroll
-    for (int d0 = 0; d0 < DT; d0 += 8) {
-        half4 v[8];
-#pragma unroll
-        for (int d = 0; d < 8 && d0 + d < DT; ++d) v[d] = *reinterpret_cast<const half4*>(row + min(16 * (d0 + d) + 4 * g, dh - 4));
-#pragma unroll
-        for (int d = 0; d < 8 && d0 + d < DT; ++d)
-#pragma unroll
-            for (int q = 0; q < QB; ++q)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float o = acc[d0 + d][q][j];
-                    acc[d0 + d][q][j] = sees[q] ? __builtin_fmaf(w[q], (float)v[d][j], o) : o;
-                }
-        __builtin_amdgcn_sched_barrier(0);
-    }
-}
-// Columns whose sums in this lane are all NaN, which nothing that is added changes
-template <int DT, int QB>
-DEV void spoilt(bool (&nan)[QB], const floatx4 (&acc)[DT][QB]) {
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-        nan[q] = true;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) nan[q] &= acc[d][q][j] != acc[d][q][j];
-    }
-}
-template <int QB>
-DEV bool any_open(const bool (&sees)[QB], const bool (&nan)[QB]) {
-    bool open = false;
-#pragma unroll
-    for (int q = 0; q < QB; ++q) open |= sees[q] & !nan[q];
-    return __any(open);
-}
-// f(entry, row) for the entries of the list's tiles of `len`, from tile t0 in
-// steps of dt, that are not seen whole and whose rows of x (a row every ld
-// values) hold a NaN or an infinity
-template <class F>
-DEV void each_wild(const WindowArgs& a, const List& list, const f16* x, int64_t ld, int len, int t0, int t1, int dt, int lane, F&& f) {
-#pragma unroll 1
-    for (int t = t0; t < t1; t += dt) {
-        if (list.plain(a, t * len, len)) continue;
-        const int i = t * len + lane;
-        const bool is_row = (lane < len) & (i < list.n) & ((i < list.s) | (i >= list.sl));
-        uint64_t m = __ballot(is_row && wild_row(x + (int64_t)list.row(is_row ? i : 0) * ld, a.dh));
-#pragma unroll 1
-        for (; m; m &= m - 1) {
-            const int e = t * len + __builtin_ctzll(m);
-            f(e, (int64_t)list.row(e));
-        }
-    }
-}
-
-// The running softmax state of QB blocks of 16 queries (a lane: query l16 of
-// each) and the products of a tile of 16 KB rows into it.
-template <int DH, int QB>
-struct Softmax {
-    static constexpr int DT = Geo<DH>::DT, W = Geo<DH>::W;
-    floatx4 o[DT][QB];  // O^T: dh 16 d + 4 g + j, query l16
-    float m[QB], l[QB];  // reference of the exponents (base 2; -inf: none yet), this lane's part of the sum
-    DEV Softmax() {
-#pragma unroll
-        for (int q = 0; q < QB; ++q) {
-            m[q] = -INFINITY;
-            l[q] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[d][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-    }
-    // Scores s (raw) of KB blocks of rows to probabilities, as B operands: P is
-    // rounded to fp16 for the product (V is fp16 as well), the sum l is not.
-    template <int KB>
-    DEV void probs(floatx4 (&s)[KB][QB], float c2, half8 (&p)[KB / 2][QB]) {
-        float mx[QB];
-        bool grow = false;
-#pragma unroll
-        for (int q = 0; q < QB; ++q) {
-            mx[q] = fmaxf(max3(s[0][q][0], s[0][q][1], s[0][q][2]), s[0][q][3]);
-#pragma unroll
-            for (int kb = 1; kb < KB; ++kb)
-                mx[q] = max3(max3(s[kb][q][0], s[kb][q][1], mx[q]), s[kb][q][2], s[kb][q][3]);
-            mx[q] *= c2;
-            grow |= mx[q] > m[q] + RESCALE_LOG2;
-        }
-        if (__any(grow)) {
-#pragma unroll
-            for (int q = 0; q < QB; ++q) {
-                const float mn = fmaxf(m[q], query_max(mx[q]));
-                const float keep = m[q] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[q] - mn);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d][q] *= keep;
-                l[q] *= keep;
-                m[q] = mn;
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < QB; ++q) {
-            const float base = m[q] == -INFINITY ? 0.0f : -m[q];
-#pragma unroll
-            for (int k2 = 0; k2 < KB / 2; ++k2) {
-                float e[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * k2 + i / 4][q][i % 4], c2, base));
-                l[q] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-                p[k2][q] = as_half8(u32x4{pack_h2(e[0], e[1]), pack_h2(e[2], e[3]), pack_h2(e[4], e[5]), pack_h2(e[6], e[7])});
-            }
-        }
-    }
-    // V's row of entry e, whose probability the sums l already hold
-    DEV void add_row(const WindowArgs& a, const List& list, int e, const f16* k, const f16* v, const half8 (&qf)[QB][Geo<DH>::KS], const int (&qp)[QB],
-                     float c2, int g) {
-        float w[QB];
-        bool sees[QB], nan[QB];
-#pragma unroll
-        for (int q = 0; q < QB; ++q) sees[q] = Seen(a, list, qp[q])(e);
-        spoilt(nan, o);
-        if (!any_open(sees, nan)) return;
-        row_dot(w, qf, k, a.dh, g);
-#pragma unroll
-        for (int q = 0; q < QB; ++q) w[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[q], c2, m[q] == -INFINITY ? 0.0f : -m[q]));
-        ::evkhip::add_row(o, w, sees, v, a.dh, g);
-    }
 };
 
 // Forward.  Workgroup: 4 waves of 16 QB rows of one key head; K and V tiles in
@@ -655,11 +318,10 @@ struct Softmax {
 template <int DH, int QB>
 __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a, int tiles) {
     using G = Geo<DH>;
-    constexpr int KS = G::KS, DT = G::DT, W = G::W, TILE = BK * W, ROWS = 64 * QB;
+    constexpr int KS = G::KS, DT = G::DT, TILE = BK * G::W, ROWS = 64 * QB;
     __shared__ __attribute__((aligned(1024))) f16 smem[4 * TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const Frag<DH> fr(lane);
     // an XCD takes tiles that follow each other, which share most of their rows
     const int at = xcd_tile(blockIdx.x, gridDim.x);
     const int tile = tiles - 1 - at % tiles, bc = at / tiles, c = bc % a.KV, b = bc / a.KV;
@@ -686,52 +348,17 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
     }
     const float c2 = a.scale * kLog2e;
     Softmax<DH, QB> sm;
-    uint32_t wild = 0;
-    for (int t = 0; t < nt; ++t) {
-        f16* const sk = smem + (t & 1) * 2 * TILE;
-        f16* const sv = sk + TILE;
-        const bool plain = list.plain(a, t * BK, BK);  // workgroup-uniform
-        wait_loads();  // this wave's part of tile t is in LDS
-        if (!plain) wild |= clean_rows(kv.dma, sv);
-        __syncthreads();  // everyone's; the other stage is free
-        if (t + 1 < nt) {
-            f16* const nx = smem + ((t + 1) & 1) * 2 * TILE;
-            kv.load(list, (t + 1) * BK, nx, nx + TILE);
-        }
-        using Rows = Ring<4 * KS, 3>;
-        using Cols = Ring<2 * DT, 2>;
-        floatx4 s[4][QB];
-        half8 kf[Rows::SLOTS], vf[Cols::SLOTS];
-        auto row = [&](auto i, auto slot) { kf[slot] = fr.row(sk, 16 * (i / KS), i % KS); };
-        auto col = [&](auto i, auto slot) { vf[slot] = fr.col(sv, 32 * (i / DT), i % DT); };
-        Rows::template start<1>(row);
-        Rows::template run<QB, 1>(row, [&](auto i, auto slot) {
-#pragma unroll
-            for (int q = 0; q < QB; ++q)
-                s[i / KS][q] = mfma16(kf[slot], qf[q][i % KS], i % KS ? s[i / KS][q] : floatx4{0.0f, 0.0f, 0.0f, 0.0f});
-        });
-        if (!plain) {
-#pragma unroll
-            for (int q = 0; q < QB; ++q) {
-                const Seen see(a, list, qp[q]);
-#pragma unroll
-                for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        s[kb][q][j] = see(t * BK + 16 * kb + 4 * g + j) ? s[kb][q][j] : -INFINITY;
-            }
-        }
-        half8 p[2][QB];
-        sm.template probs<4>(s, c2, p);
-        Cols::template start<2>(col);
-        Cols::template run<QB, 2>(col, [&](auto i, auto slot) {
-#pragma unroll
-            for (int q = 0; q < QB; ++q) sm.o[i % DT][q] = mfma16(vf[slot], p[i / DT][q], sm.o[i % DT][q]);
-        });
-    }
+    const auto plain = [&](int t) { return list.plain(a, t * BK, BK); };
+    const uint32_t wild = attend_tiles<DH, QB>(sm, qf, c2, smem, kv.dma, 0, nt, [&](int t, f16* sk, f16* sv) { kv.load(list, t * BK, sk, sv); }, plain,
+                                               [&](int q) { return Seen(a, list, qp[q]); });
     if (__syncthreads_or(wild)) {
         const int64_t ld = (int64_t)a.KV * a.dh;
-        each_wild(a, list, kv.v, ld, BK, 0, nt, 1, lane, [&](int e, int64_t row) { sm.add_row(a, list, e, kv.k + row * ld, kv.v + row * ld, qf, qp, c2, g); });
+        each_wild(plain, [&](int e) { return list.has(e) ? kv.v + list.row(e) * ld : nullptr; }, a.dh, BK, 0, nt, 1, lane, [&](int e) {
+            bool sees[QB];
+#pragma unroll
+            for (int q = 0; q < QB; ++q) sees[q] = Seen(a, list, qp[q])(e);
+            sm.add_row(sees, kv.k + list.row(e) * ld, kv.v + list.row(e) * ld, qf, a.dh, c2, g);
+        });
     }
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
@@ -769,14 +396,11 @@ struct SplitGeo {
 template <int DH>
 __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void window_split(WindowArgs a, int tiles, int splits, float* ws) {
     using G = Geo<DH>;
-    constexpr int KS = G::KS, DT = G::DT, W = G::W, NW = SplitGeo<DH>::NW, VPER = 32 * G::CPR / 64, OW = DH + 4;
-    constexpr int SLOT = 32 * W * 2, STATE = 16 * OW * 4;  // bytes of a wave's V, then of its state
-    constexpr int BYTES = NW * (SLOT > STATE ? SLOT : STATE);
-    __shared__ __attribute__((aligned(16))) char smem[BYTES];
+    constexpr int KS = G::KS, NW = SplitGeo<DH>::NW;
+    __shared__ __attribute__((aligned(16))) char smem[steps_bytes<DH, NW>()];
     __shared__ float sm_m[NW][16], sm_l[NW][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const Frag<DH> fr(lane);
     const int at = xcd_tile(blockIdx.x, gridDim.x);
     const int split = at % splits, tile = at / splits % tiles, bc = at / splits / tiles, c = bc % a.KV, b = bc / a.KV;
     const int group = a.H / a.KV, NR = a.N * group, R0 = tile * 16;
@@ -784,34 +408,12 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
     const int steps = (list.n + 31) / 32;
     const int c0 = (int)((int64_t)steps * split / splits), c1 = (int)((int64_t)steps * (split + 1) / splits);
     const int64_t ld = (int64_t)a.KV * a.dh, kv0 = (int64_t)b * a.R * ld + (int64_t)c * a.dh;
-    f16* const slot = reinterpret_cast<f16*>(smem + wave * SLOT);
-
-    u32x4 kr[2][KS], vr[VPER];
-    auto load_k = [&](int step) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const f16* src = a.k + kv0 + list.row(min(32 * step + 16 * kb + l16, list.n - 1)) * ld;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                kr[kb][ks] = u32x4{0u, 0u, 0u, 0u};
-                if (32 * ks + 8 * g < a.dh) kr[kb][ks] = *reinterpret_cast<const u32x4*>(src + 32 * ks + 8 * g);
-            }
-        }
-    };
-    auto load_v = [&](int step) {
-#pragma unroll
-        for (int i = 0; i < VPER; ++i) {
-            const int row = (lane + 64 * i) / G::CPR, chunk = (lane + 64 * i) % G::CPR ^ swz<W>(row);
-            vr[i] = u32x4{0u, 0u, 0u, 0u};
-            if (chunk * 8 < a.dh)
-                vr[i] = *reinterpret_cast<const u32x4*>(a.v + kv0 + list.row(min(32 * step + row, list.n - 1)) * ld + chunk * 8);
-        }
-    };
-    int step = c0 + wave;
-    if (step < c1) {
-        load_k(step);
-        load_v(step);
-    }
+    const auto at_entry = [&](int e) { return kv0 + list.row(min(e, list.n - 1)) * ld; };
+    Steps<DH, NW> walk(reinterpret_cast<f16*>(smem) + wave * 32 * G::W, lane);
+    const auto k_row = [&](int e) { return a.k + at_entry(e); };
+    const auto v_row = [&](int e) { return a.v + at_entry(e); };
+    const int first = c0 + wave;
+    if (first < c1) walk.load(first, k_row, v_row, a.dh);
     const int r = min(R0 + l16, NR - 1), qp[1] = {position_of(a, b, r / group)};
     const int64_t q_at = ((int64_t)b * a.N + r / group) * a.H + c * group + r % group;  // row of q
     half8 qf[1][KS];
@@ -822,75 +424,21 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
     }
     const float c2 = a.scale * kLog2e;
     Softmax<DH, 1> sm;
-    uint64_t wild = 0;
-    for (; step < c1; step += NW) {
-        const bool plain = list.plain(a, 32 * step, 32);
-        if (!plain) {
-#pragma unroll
-            for (int i = 0; i < VPER; ++i) {
-                const uint64_t hit = __ballot(is_wild(wild2(as_half8(vr[i]), half2_t{(f16)0.0f, (f16)0.0f})));
-                if (hit >> (lane / G::CPR * G::CPR) & ((1ull << G::CPR) - 1)) vr[i] = u32x4{0u, 0u, 0u, 0u};
-                wild |= hit;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < VPER; ++i) *reinterpret_cast<u32x4*>(slot + (lane + 64 * i) * 8) = vr[i];
-        if (step + NW < c1) load_v(step + NW);
-        half8 vf[DT];
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vf[d] = fr.col(slot, 0, d);
-        floatx4 s[2][1];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            s[kb][0] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[kb][0] = mfma16(as_half8(kr[kb][ks]), qf[0][ks], s[kb][0]);
-        }
-        if (step + NW < c1) load_k(step + NW);
-        if (!plain) {
-            const Seen see(a, list, qp[0]);
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[kb][0][j] = see(32 * step + 16 * kb + 4 * g + j) ? s[kb][0][j] : -INFINITY;
-        }
-        half8 p[1][1];
-        sm.template probs<2>(s, c2, p);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) sm.o[d][0] = mfma16(vf[d], p[0][0], sm.o[d][0]);
-    }
+    const auto plain = [&](int step) { return list.plain(a, 32 * step, 32); };
+    const uint64_t wild = walk.run(sm, qf, c2, first, c1, k_row, v_row, a.dh, plain, [&] { return Seen(a, list, qp[0]); });
     if (wild)
-        each_wild(a, list, a.v + kv0, ld, 32, c0 + wave, c1, NW, lane,
-                  [&](int e, int64_t row) { sm.add_row(a, list, e, a.k + kv0 + row * ld, a.v + kv0 + row * ld, qf, qp, c2, g); });
-    // the states, one row of OW floats a query, once the slots have been read
-    __syncthreads();
-    float* const st = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<floatx4*>(st + (wave * 16 + l16) * OW + 16 * d + 4 * g) = sm.o[d][0];
-    const float l = query_sum(sm.l[0]);
-    if (g == 0) {
-        sm_m[wave][l16] = sm.m[0];
-        sm_l[wave][l16] = l;
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < 16 * (DH / 4); e += 64 * NW) {
-        const int q = e / (DH / 4), d = e % (DH / 4) * 4, row = R0 + q;
-        if (row >= NR) continue;
-        float m = -INFINITY, ls = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) m = fmaxf(m, sm_m[w][q]);
-        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float f = sm_m[w][q] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm_m[w][q] - m);
-            ls += f * sm_l[w][q];
-            o += f * *reinterpret_cast<const floatx4*>(st + (w * 16 + q) * OW + d);
-        }
+        each_wild(plain, [&](int e) { return list.has(e) ? v_row(e) : nullptr; }, a.dh, 32, first, c1, NW, lane, [&](int e) {
+            const bool sees[1] = {Seen(a, list, qp[0])(e)};
+            sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g);
+        });
+    merge_waves<DH, NW>(sm, smem, sm_m, sm_l, lane, wave, [&](int q, int d, float m, float ls, const floatx4& o) {
+        const int row = R0 + q;
+        if (row >= NR) return;
         if (splits > 1) {
             float* dst = ws + (((int64_t)bc * NR + row) * splits + split) * (DH + 4);
             *reinterpret_cast<floatx4*>(dst + 4 + d) = o;
             if (d == 0) dst[0] = m, dst[1] = ls;
-            continue;
+            return;
         }
         const int64_t at_row = ((int64_t)b * a.N + row / group) * a.H + c * group + row % group;
         const bool none = span_of(position_of(a, b, row / group), a).count() == 0;
@@ -899,7 +447,7 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
             *reinterpret_cast<uint2*>(a.out + at_row * a.dh + d) = uint2{pack_h2(o[0] * inv, o[1] * inv), pack_h2(o[2] * inv, o[3] * inv)};
         if (a.lse && d == 0)
             a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = none ? -INFINITY : (m + log2f(ls)) * kLn2;
-    }
+    });
 }
 
 // The states of one query row's splits (at most JOIN_MOST): each thread weighs
@@ -1152,7 +700,8 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_dq(WindowArgs a,
         kv.load(list, 0, smem, smem + TILE);
     }
     const int64_t ld = (int64_t)a.KV * a.dh;
-    each_wild(a, list, kv.k, ld, BK, 0, nt, 1, lane, [&](int i, int64_t row) {
+    each_wild([&](int t) { return list.plain(a, t * BK, BK); }, [&](int e) { return list.has(e) ? kv.k + list.row(e) * ld : nullptr; }, a.dh, BK, 0, nt, 1, lane, [&](int i) {
+        const int64_t row = list.row(i);
         float ds[QB], dp[QB];
         bool sees[QB], nan[QB];
 #pragma unroll
@@ -1528,27 +1077,6 @@ bool mfma_ok(const WindowArgs& a) {
     // a tile's rows behind one descriptor
     return (int64_t)a.KV * a.dh * 2 * (BK + 1) < INT32_MAX && (int64_t)a.H * a.dh * 2 * 260 < INT32_MAX;
 }
-// The DH that serves a head size, from `least` on
-uint64_t head_width(int dh, int least) {
-    return dh <= 32 && least <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : dh <= 128 ? 128 : 256;
-}
-template <class F>
-hipError_t by_head64(int dh, F&& f) {
-    switch (head_width(dh, 64)) {
-        case 64: f(std::integral_constant<int, 64>{}); break;
-        case 96: f(std::integral_constant<int, 96>{}); break;
-        case 128: f(std::integral_constant<int, 128>{}); break;
-        default: f(std::integral_constant<int, 256>{}); break;
-    }
-    return hipGetLastError();
-}
-template <class F>
-hipError_t by_head(int dh, F&& f) {
-    if (head_width(dh, 32) > 32) return by_head64(dh, f);
-    f(std::integral_constant<int, 32>{});
-    return hipGetLastError();
-}
-
 }  // namespace
 
 namespace {

@@ -130,6 +130,7 @@ def test_prefix_attention(L):
     assert prefix(L, m, k=(1, 9, 128)) == SHAPE
     assert prefix(L, m, v=(2, 9, 64)) == SHAPE
     assert prefix(L, m, pk=(1 << 30, 128)) == UNSUPPORTED
+    assert prefix(L, m, q=(1, 1, 64), pk=(1 << 29, 64), k=(1, (1 << 29) + 1, 64)) == UNSUPPORTED
     assert prefix(L, m, q=(1 << 29, 1, 256), k=(1 << 29, 1, 128)) == UNSUPPORTED
     for alias in (("o", "q"), ("o", "pk"), ("o", "pv"), ("o", "k"), ("o", "v")):
         assert prefix(L, m, alias=alias) == INVALID, alias
