@@ -225,6 +225,37 @@ DEV float lanes_sum(float v) {
     return v;
 }
 
+// over the whole wave, without LDS
+DEV float wave_add(float v) {
+    v = lanes_sum<16>(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
+DEV float wave_top(float v) {
+#define EVK_TOP(CTRL) v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false)))
+    EVK_TOP(0xB1);
+    EVK_TOP(0x4E);
+    EVK_TOP(0x141);
+    EVK_TOP(0x140);
+#undef EVK_TOP
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+// Values read or written once: past the caches
+DEV half8 ld_once(const f16* p) {
+    typedef half8 __attribute__((aligned(2))) half8_u;
+    return __builtin_nontemporal_load(reinterpret_cast<const half8_u*>(p));
+}
+DEV void st_once(f16* p, const half8& v) {
+    typedef half8 __attribute__((aligned(2))) half8_u;
+    __builtin_nontemporal_store(v, reinterpret_cast<half8_u*>(p));
+}
+
 // tanh GELU of gelu.comp (evk_ai.cpp:679-699)
 DEV float gelu_f(float x) {
     const float ka = 0.7978845608028654f, kb = 0.044715f;

@@ -112,6 +112,10 @@ struct TileWork {
     int own;           // their own rows are part of the list
     int splits, slots; // parts of the list; states of a row (0: none, the output is written)
 };
+struct Sees {  // the entries [0, P) and [sl, last), without && (as branches they cost more)
+    int P, sl, last;
+    DEV bool operator()(int e) const { return (e < P) | ((e >= sl) & (e < last)); }
+};
 template <int DH, int QB>
 DEV void tile_rows(const PrefixArgs& a, const TileWork& w, int item, float* ws, f16* smem) {
     using G = Geo<DH>;
@@ -162,13 +166,13 @@ DEV void tile_rows(const PrefixArgs& a, const TileWork& w, int item, float* ws, 
         const int i1 = (t + 1) * BK;
         return (i1 <= a.P) | ((i1 > sl) & (i1 <= sl + least));
     };
-    const auto seen = [&](int q) { return [P = a.P, sl, last = sl + own[q]](int e) { return (e < P) | ((e >= sl) & (e < last)); }; };
+    const auto seen = [&](int q) { return Sees{a.P, sl, sl + own[q]}; };
     const uint32_t wild = attend_tiles<DH, QB>(sm, qf, c2, smem, dma, t0, t1, load, plain, seen);
     if (__syncthreads_or(wild))
         each_wild(plain, [&](int e) { return ((e < a.P) | (e >= sl)) & (e < n) ? v_row(e) : nullptr; }, a.dh, BK, t0, t1, 1, lane, [&](int e) {
             bool sees[QB];
 #pragma unroll
-            for (int q = 0; q < QB; ++q) sees[q] = seen(q)(e);
+            for (int q = 0; q < QB; ++q) sees[q] = Sees{a.P, sl, sl + own[q]}(e);
             sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g);
         });
 #pragma unroll

@@ -177,7 +177,7 @@ def test_token_logprobs(L):
     assert scores(L, m, logits=(0, 100), tokens=(0,), lp=None, ent=None, ids=None, alt=None, stats=None) == OK
     past = (1 << 31, 1 << 31, 1 << 31, 64)
     assert scores(L, m, logits=past) == UNSUPPORTED
-    many = 1 << 23  # workgroups of 1024 threads
+    many = 1 << 24  # workgroups of 256 threads
     assert scores(L, m, logits=(many, 32000), tokens=(many,), lp=1 << 50, ent=1 << 51, ids=None, alt=None, stats=1 << 52) == UNSUPPORTED
 
 
