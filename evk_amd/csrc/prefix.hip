@@ -245,7 +245,7 @@ DEV void step_rows(const PrefixArgs& a, const StepWork& w, int item, float* ws, 
     const float c2 = a.scale * kLog2e;
     Softmax<DH, 1> sm;
     const auto plain = [&](int step) { return 32 * step + 32 <= pre + least; };
-    const auto seen = [&] { return [last](int e) { return e < last; }; };
+    const auto seen = [&](int) { return Sees{last, 0, 0}; };
     const uint64_t wild = walk.run(sm, qf, c2, first, c1, k_row, v_row, a.dh, plain, seen);
     if (wild)
         each_wild(plain, [&](int e) { return e < n ? v_row(e) : nullptr; }, a.dh, 32, first, c1, NW, lane, [&](int e) {
@@ -280,33 +280,62 @@ __global__ __launch_bounds__(64 * StepGeo<DH>::NW, StepGeo<DH>::NW / 4) void pre
     step_rows<DH, NW>(a, w, xcd_tile(blockIdx.x, gridDim.x), ws, smem, sm_m, sm_l);
 }
 
-// The states of a row, added in order by one wave.
+// The prefix by tiles and the own rows by steps in one launch: the former wait for
+// their products, the latter for memory.  Each XCD starts its part of the tiles
+// first, which take the same time all, and fills up with own rows, which end when
+// they end.
+template <int DH, int QB>
+__global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void prefix_mixed(PrefixArgs a, TileWork tw, int wide, StepWork sw, float* ws) {
+    constexpr int TILES = 4 * BK * Geo<DH>::W * 2, STEPS = steps_bytes<DH, 4>();
+    __shared__ __attribute__((aligned(1024))) char smem[TILES > STEPS ? TILES : STEPS];
+    __shared__ float sm_m[4][16], sm_l[4][16];
+    const int total = gridDim.x, x = blockIdx.x % 8, j = blockIdx.x / 8;
+    const int w0 = x * (wide / 8) + min(x, wide % 8), wn = wide / 8 + (x < wide % 8);  // this XCD's tiles
+    const int at = x * (total / 8) + min(x, total % 8) - w0 + j - wn;                   // own rows before this workgroup's
+    if (j < wn) tile_rows<DH, QB>(a, tw, w0 + j, ws, reinterpret_cast<f16*>(smem));
+    else step_rows<DH, 4>(a, sw, at, ws, smem, sm_m, sm_l);
+}
+
+// The states of a row, added in order by one wave: groups of DH / 4 lanes take
+// every HPW-th of them, 16 bytes a lane, all requested before the weights are
+// known.
 constexpr int JOIN_MOST = 64;  // a lane weighs one
 template <int DH>
 __global__ __launch_bounds__(256) void prefix_join(PrefixArgs a, int slots, int64_t rows, const float* ws) {
-    constexpr int PER = (DH + 63) / 64;
-    const int lane = threadIdx.x & 63;
+    constexpr int LPS = DH <= 32 ? 8 : DH <= 64 ? 16 : DH <= 128 ? 32 : 64, HPW = 64 / LPS, AHEAD = 8;
+    const int lane = threadIdx.x & 63, d = lane % LPS * 4, part = lane / LPS;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
     const float* src = ws + row * slots * (DH + 4);
     const bool is = lane < slots;
-    const float mine = is ? src[lane * (DH + 4)] : -INFINITY, m = wave_max(mine);
-    const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - m);
-    const float l = wave_sum(is ? f * src[lane * (DH + 4) + 1] : 0.0f);
-    float o[PER] = {};
-#pragma unroll 8
-    for (int s = 0; s < slots; ++s) {
-        const float fs = __shfl(f, s, 64);
+    const float mine = is ? src[lane * (DH + 4)] : -INFINITY, mine_l = is ? src[lane * (DH + 4) + 1] : 0.0f;
+    auto load = [&](int s) {
+        return *reinterpret_cast<const floatx4*>(src + min(s, slots - 1) * (DH + 4) + 4 + min(d, DH - 4));
+    };
+    floatx4 ahead[AHEAD];
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (lane + 64 * i < DH) o[i] += fs * src[s * (DH + 4) + 4 + lane + 64 * i];
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = load(part + HPW * i);
+    const float m = wave_top(mine), f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - m);
+    const float l = wave_add(is ? f * mine_l : 0.0f);
+    floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < slots; s0 += HPW * AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int s = s0 + part + HPW * i;
+            const float fs = __shfl(f, min(s, 63), 64);
+            if (s < slots) o += fs * ahead[i];
+            ahead[i] = load(s + HPW * AHEAD);
+        }
     }
+#pragma unroll
+    for (int k = LPS; k < 64; k *= 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], k, 64);
     const int h = (int)(row % a.H), t = (int)(row / a.H % a.N), b = (int)(row / a.H / a.N);
     const bool none = a.P + own_rows(a, b, t) == 0;
     const float inv = none ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (lane + 64 * i < a.dh) a.out[row * a.dh + lane + 64 * i] = (f16)(o[i] * inv);
+    if (part == 0 && d < a.dh)
+        *reinterpret_cast<uint2*>(a.out + row * a.dh + d) = uint2{pack_h2(o[0] * inv, o[1] * inv), pack_h2(o[2] * inv, o[3] * inv)};
     if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = none ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -322,43 +351,48 @@ int query_blocks(int64_t rows, int64_t heads, int dh) { return dh <= 128 && head
 // How a shape runs.
 struct Plan {
     enum { TILES, STEPS, SHARED } kind;
-    int qb;          // TILES, SHARED
+    int qb;          // query blocks of a wave in tiles
     TileWork tiles;  // TILES: all; SHARED: the prefix
     StepWork steps;  // STEPS: all; SHARED: the own rows
     int slots;
+    int64_t wide, few;  // workgroups of tiles and of steps
 };
 Plan plan_for(int64_t B, int64_t N, int64_t P, int64_t R, int64_t H, int64_t KV, int dh) {
     Plan p{};
-    const int64_t per = N * (H / KV), heads = B * KV, waves = dh <= 128 ? 8 : 4;
+    const int64_t per = N * (H / KV), heads = B * KV;
     auto ceil = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    auto some = [](int64_t most, int64_t a, int64_t b) { return std::max<int64_t>(1, std::min({most, a, b})); };
     if (per >= 64) {
         p.kind = Plan::TILES;
         p.qb = query_blocks(per, heads, dh);
         const int64_t tiles = ceil(per, 64 * p.qb), groups = heads * tiles;
-        int64_t splits = std::max<int64_t>(1, std::min({512 / groups, ceil(P + R, 4 * BK), (int64_t)JOIN_MOST}));
+        const int64_t splits = some(JOIN_MOST, 512 / groups, ceil(P + R, 4 * BK));
         p.slots = splits > 1 ? (int)splits : 0;
         p.tiles = {(int)per, (int)tiles, 1, (int)splits, p.slots};
+        p.wide = groups * splits;
         return p;
     }
-    const int64_t tiles = ceil(per, 16), groups = heads * tiles;
-    const bool share = B > 1 && P >= 512 && B * per > 16;
-    if (!share) {
+    const int64_t tiles = ceil(per, 16), groups = heads * tiles, all = B * per;
+    // steps of one workgroup, while its waves take no more than four each; else parts, and a second launch to join them
+    const int64_t steps = ceil(P + R, 32), waves = dh <= 128 ? 8 : 4;
+    const bool alone = steps <= 4 * waves;
+    if (B == 1 || (B - 1) * P * KV * dh * 4 < (alone ? 64 << 20 : 4 << 20)) {
         p.kind = Plan::STEPS;
-        const int64_t steps = ceil(P + R, 32);
-        const int64_t splits = steps <= 4 * waves ? 1 : std::max<int64_t>(1, std::min({ceil(steps, waves), 256 / groups, (int64_t)JOIN_MOST}));
+        const int64_t splits = alone ? 1 : some(JOIN_MOST, 256 / groups, ceil(steps, waves));
         p.slots = splits > 1 ? (int)splits : 0;
         p.steps = {(int)tiles, (int)P, (int)splits, p.slots, 0};
+        p.few = groups * splits;
         return p;
     }
     p.kind = Plan::SHARED;
-    const int64_t all = B * per;
-    p.qb = query_blocks(all, KV * 16, dh);
-    const int64_t wide = ceil(all, 64 * p.qb) * KV;
-    const int64_t s1 = std::max<int64_t>(1, std::min({512 / wide, ceil(P, 4 * BK), (int64_t)JOIN_MOST / 2}));
-    const int64_t steps = ceil(R, 32);
-    const int64_t s2 = steps <= 4 * waves ? 1 : std::max<int64_t>(1, std::min({ceil(steps, waves), 256 / groups, (int64_t)JOIN_MOST / 2}));
+    p.qb = dh <= 128 && KV * ceil(all, 128) * ceil(P, 512) >= 256 ? 2 : 1;
+    const int64_t wide = KV * ceil(all, 64 * p.qb);
+    const int64_t s1 = some(JOIN_MOST / 2, (p.qb == 2 ? 192 : 512) / wide, ceil(P, 4 * BK));
+    const int64_t s2 = some(JOIN_MOST / 2, JOIN_MOST / 2, ceil(R, dh <= 128 ? 512 : 256));
     p.slots = (int)(s1 + s2);
-    p.tiles = {(int)all, (int)ceil(all, 64 * p.qb), 0, (int)s1, p.slots};
+    p.wide = wide * s1;
+    p.few = groups * s2;
+    p.tiles = {(int)all, (int)(wide / KV), 0, (int)s1, p.slots};
     p.steps = {(int)tiles, 0, (int)s2, p.slots, (int)s1};
     return p;
 }
@@ -382,28 +416,28 @@ int prefix_forward(const PrefixArgs& a, void* ws, hipStream_t st) {
         return e == hipSuccess ? EVKHIP_OK : check_hip(e, "prefix_attention launch");
     }
     const Plan p = plan_for(a.B, a.N, a.P, a.R, a.H, a.KV, a.dh);
-    const int64_t seqs = p.kind == Plan::SHARED ? 1 : a.B;
-    const int64_t wide = p.kind == Plan::STEPS ? 0 : seqs * a.KV * p.tiles.tiles * p.tiles.splits;
-    const int64_t few = p.kind == Plan::TILES ? 0 : (int64_t)a.B * a.KV * p.steps.tiles * p.steps.splits;
-    int rc = check_grid(op, wide, 256);
-    if (rc == EVKHIP_OK) rc = check_grid(op, few, 512);
+    const dim3 grid((unsigned)(p.wide + p.few));
+    int rc = check_grid(op, p.wide + p.few, p.kind == Plan::STEPS ? 512 : 256);
     if (rc == EVKHIP_OK && p.slots) rc = check_grid(op, (rows + 3) / 4, 256);
     if (rc != EVKHIP_OK) return rc;
+    float* const part = (float*)ws;
     e = by_head(a.dh, [&](auto dhc) {
         constexpr int DH = decltype(dhc)::value;
-        float* const part = (float*)ws;
-        if (wide) {
-            auto go = [&](auto qb) {
-                hipLaunchKernelGGL((prefix_tiles<DH, decltype(qb)::value>), dim3((unsigned)wide), dim3(256), 0, st, a, p.tiles, part);
-            };
-            if constexpr (DH <= 128) {
-                if (p.qb == 2) go(std::integral_constant<int, 2>{});
-                else go(std::integral_constant<int, 1>{});
-            } else {
-                go(std::integral_constant<int, 1>{});
-            }
+        auto with = [&](auto qb) {
+            constexpr int QB = decltype(qb)::value;
+            if (p.kind == Plan::SHARED)
+                hipLaunchKernelGGL((prefix_mixed<DH, QB>), grid, dim3(256), 0, st, a, p.tiles, (int)p.wide, p.steps, part);
+            else
+                hipLaunchKernelGGL((prefix_tiles<DH, QB>), grid, dim3(256), 0, st, a, p.tiles, part);
+        };
+        if (p.kind == Plan::STEPS) {
+            hipLaunchKernelGGL(prefix_steps<DH>, grid, dim3(64 * StepGeo<DH>::NW), 0, st, a, p.steps, part);
+        } else if constexpr (DH > 128) {
+            with(std::integral_constant<int, 1>{});
+        } else {
+            if (p.qb == 2) with(std::integral_constant<int, 2>{});
+            else with(std::integral_constant<int, 1>{});
         }
-        if (few) hipLaunchKernelGGL(prefix_steps<DH>, dim3((unsigned)few), dim3(64 * StepGeo<DH>::NW), 0, st, a, p.steps, part);
         if (p.slots) hipLaunchKernelGGL(prefix_join<DH>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, p.slots, rows, (const float*)part);
     });
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "prefix_attention launch");

@@ -13,8 +13,8 @@
 // Memory-bound: every logit read once, a row in the registers of one workgroup
 // (ids have 16 bits, so a row is at most 65536 logits).  2560 rows of 32000: 31 us =
 // 5.3 TB/s (a copy of 1 GiB runs at 5.1), with 5 alternatives 37: a reading back of
-// the few logits that may be among them, two barriers more.  The gradient 66 us =
-// 5.0 TB/s.
+// the few logits that may be among them, two barriers more.  The gradient 64 us =
+// 5.1 TB/s.
 #include "kernels.h"
 
 #include <math.h>
@@ -267,7 +267,8 @@ __global__ __launch_bounds__(NT, NV == 16 ? 4 : 1) void token_logprobs_k(TokenLo
     }
 }
 
-template <int NT>
+// The gradient of NV vectors of each thread, all requested before the first is used.
+template <int NT, int NV>
 __global__ __launch_bounds__(NT) void token_logprobs_bwd_k(TokenLogprobsArgs a, int segments) {
     const int64_t row = blockIdx.x / segments;
     const int seg = blockIdx.x % segments, V = a.V, token = a.tokens[row];
@@ -275,32 +276,36 @@ __global__ __launch_bounds__(NT) void token_logprobs_bwd_k(TokenLogprobsArgs a, 
     const float m = a.stats[2 * row], L = a.stats[2 * row + 1], H = a.dentropy ? a.entropy[row] : 0.0f, c2 = a.scale * kLog2e;
     const f16* const l = a.logits + row * V;
     f16* const d = a.dlogits + row * V;
-    const int at = 8 * (threadIdx.x + NT * seg), n = V - at;
-    if (n <= 0) return;
-    half8 x = {};
+    auto at = [&](int v) { return 8 * (int)threadIdx.x + 8 * NT * (NV * seg + v); };
+    half8 x[NV];
     const bool idle = w == 0.0f && h == 0.0f;  // nothing asked of this row: zeros, whatever it holds
     if (!idle) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            if (at(v) + 8 <= V) x[v] = ld_once(l + at(v));
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int n = V - at(v);
+        if (n <= 0) break;
+        if (n < 8 && !idle) {
+#pragma unroll
+            for (int e = 0; e < 7; ++e) x[v][e] = e < n ? l[at(v) + e] : (f16)0.0f;
+        }
+        half8 g;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float t = ((float)x[v][e] - m) * c2 - L, p = __builtin_amdgcn_exp2f(t);
+            const float y = (at(v) + e == token ? w : 0.0f) - p * (w + h * (kLn2 * fmaxf(t, -1000.0f) + H));
+            g[e] = (f16)(idle ? 0.0f : a.scale * y);
+        }
         if (n >= 8) {
-            x = ld_h8(l + at);
+            st_once(d + at(v), g);
         } else {
 #pragma unroll
             for (int e = 0; e < 7; ++e)
-                if (e < n) x[e] = l[at + e];
+                if (e < n) d[at(v) + e] = g[e];
         }
-    }
-    half8 g;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float t = ((float)x[e] - m) * c2 - L, p = __builtin_amdgcn_exp2f(t);
-        const float v = (at + e == token ? w : 0.0f) - p * (w + h * (kLn2 * fmaxf(t, -1000.0f) + H));
-        g[e] = (f16)(idle ? 0.0f : a.scale * v);
-    }
-    if (n >= 8) {
-        st_once(d + at, g);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-            if (e < n) d[at + e] = g[e];
     }
 }
 
@@ -336,11 +341,11 @@ int token_logprobs_forward(const TokenLogprobsArgs& a, hipStream_t st) {
 }
 
 int token_logprobs_backward(const TokenLogprobsArgs& a, hipStream_t st) {
-    constexpr int NT = 256;
-    const int segments = (a.V + 8 * NT - 1) / (8 * NT);
+    constexpr int NT = 256, NV = 2;  // 2560 rows of 32000, us: one vector 80, two 64, four 66, eight 67
+    const int segments = (a.V + 8 * NT * NV - 1) / (8 * NT * NV);
     const int rc = check_grid("token_logprobs_backward", a.rows * segments, NT);
     if (rc != EVKHIP_OK) return rc;
-    hipLaunchKernelGGL(token_logprobs_bwd_k<NT>, dim3((unsigned)(a.rows * segments)), dim3(NT), 0, st, a, segments);
+    hipLaunchKernelGGL((token_logprobs_bwd_k<NT, NV>), dim3((unsigned)(a.rows * segments)), dim3(NT), 0, st, a, segments);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "token_logprobs_backward launch");
 }

@@ -425,7 +425,7 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
     const float c2 = a.scale * kLog2e;
     Softmax<DH, 1> sm;
     const auto plain = [&](int step) { return list.plain(a, 32 * step, 32); };
-    const uint64_t wild = walk.run(sm, qf, c2, first, c1, k_row, v_row, a.dh, plain, [&] { return Seen(a, list, qp[0]); });
+    const uint64_t wild = walk.run(sm, qf, c2, first, c1, k_row, v_row, a.dh, plain, [&](int q) { return Seen(a, list, qp[q]); });
     if (wild)
         each_wild(plain, [&](int e) { return list.has(e) ? v_row(e) : nullptr; }, a.dh, 32, first, c1, NW, lane, [&](int e) {
             const bool sees[1] = {Seen(a, list, qp[0])(e)};
