@@ -300,6 +300,18 @@ DEV half8 ld_h8(const f16* p) {
 }
 DEV void st_h8(f16* p, const half8& v) { __builtin_memcpy(p, &v, 16); }
 
+// What the compiler needs of these values it forms anew from here on, instead of
+// keeping it (each one's 32-bit form, say) from before.
+template <int N>
+DEV void forget(half8 (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        u32x4 u = as_u32x4(x[i]);
+        asm volatile("" : "+v"(u));
+        x[i] = as_half8(u);
+    }
+}
+
 // greedy_sample.comp's winner is the maximum under the total order
 // (value desc, bitrev8(j mod 256) asc, j asc); rank encodes the last two.
 DEV uint32_t greedy_rank(uint32_t j) {

@@ -66,7 +66,7 @@ struct RowSum {
     template <int M>
     DEV void operator()(float (&v)[M], float (*lds)[2][NW]) {
 #pragma unroll
-        for (int i = 0; i < M; ++i) v[i] = wave_sum(v[i]);
+        for (int i = 0; i < M; ++i) v[i] = wave_add(v[i]);
         if constexpr (NW > 1) {
             const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
             if (lane == 0)
@@ -175,17 +175,25 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
         wo[v] = a.wo ? ld_part(a.wo + at[v], n[v]) : ones();
         g[v] = a.gate ? ld_part(a.gate + (a.gate_rows ? gate * D : 0) + at[v], n[v]) : ones();
     }
-    for (int64_t row = first + threadIdx.x / TPR; row < end; row += RPW) {
+    half8 nx[NV], ny[NV], nds[NV] = {}, ndh[NV];
+    auto load = [&](int64_t row) {
+        const int64_t base = row * D;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            nx[v] = ld_part(a.x + base + at[v], n[v]);
+            if (Y) ny[v] = ld_part(a.y + base + at[v], n[v]);
+            ndh[v] = ld_part(a.dh + base + at[v], n[v]);
+            if (a.ds) nds[v] = ld_part(a.ds + base + at[v], n[v]);
+        }
+    };
+    const int64_t row0 = first + threadIdx.x / TPR;
+    if (row0 < end) load(row0);
+    for (int64_t row = row0; row < end; row += RPW) {
         const int64_t base = row * D;
         half8 x[NV], y[NV], ds[NV], dh[NV];
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            x[v] = ld_part(a.x + base + at[v], n[v]);
-            if (Y) y[v] = ld_part(a.y + base + at[v], n[v]);
-            dh[v] = ld_part(a.dh + base + at[v], n[v]);
-            ds[v] = half8{};
-            if (a.ds) ds[v] = ld_part(a.ds + base + at[v], n[v]);
-        }
+        for (int v = 0; v < NV; ++v) x[v] = nx[v], y[v] = ny[v], ds[v] = nds[v], dh[v] = ndh[v];
+        if (row + RPW < end) load(row + RPW);  // on their way during this row's sums
         float q = 1.0f;
         if (Y && a.post) {
             float yy[1] = {0.0f};
@@ -268,30 +276,69 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
     }
 }
 
-// Sums over the runs: block (job, 16 columns), job 0 dwi, 1 dwo, 2 + b the
-// gradient of gate b.  64 threads a column take every 64th run, in order, and
-// their sums are added in order.
-__global__ __launch_bounds__(1024) void residual_norm_sums_k(ResidualNormArgs a, const float* part, int parts, int gates, int blocks) {
-    __shared__ float red[64][17];
-    const int x = threadIdx.x % 16, u = threadIdx.x / 16, job = blockIdx.x / blocks, c = blockIdx.x % blocks * 16 + x, D = a.D;
-    f16* const out = job == 0 ? a.dwi : job == 1 ? a.dwo : a.dgate ? a.dgate + (int64_t)(job - 2) * D : nullptr;
-    if (!out) return;
-    const int64_t r0 = job < 2 ? 0 : (int64_t)(job - 2) * parts, r1 = job < 2 ? (int64_t)gates * parts : r0 + parts;
-    const float* const src = part + (job ? D : 0) + c;
-    float v = 0.0f;
-    if (c < D)
-#pragma unroll 4
-        for (int64_t r = r0 + u; r < r1; r += 64) {
-            const float f = job == 1 && a.gate ? (float)a.gate[(a.gate_rows ? r / parts * D : 0) + c] : 1.0f;
-            v += f * src[r * 2 * D];
+// Sums over the runs: block (job, 64 columns), job 0 dwi, 1 dwo (and the gradient
+// of the one gate that there is), from 2 on the gradients of 64 / lanes gates.  64
+// groups of 16 threads, four columns a thread: `lanes` of them (a power of two, no
+// more than the runs of a gate need) take a gate's runs in turn, all 64 those of
+// dwi and dwo, and their sums are added in order.
+constexpr int SUM_COLS = 64;
+__global__ __launch_bounds__(1024) void residual_norm_sums_k(ResidualNormArgs a, const float* part, int parts, int gates, int blocks, int gate_lanes) {
+    __shared__ float red[64][SUM_COLS + 4];
+    const int x = threadIdx.x % 16 * 4, u = threadIdx.x / 16, job = blockIdx.x / blocks, c0 = blockIdx.x % blocks * SUM_COLS, D = a.D;
+    const int lanes = job < 2 ? 64 : gate_lanes, gate0 = job < 2 ? 0 : (job - 2) * (64 / lanes), gate = gate0 + u / lanes;
+    const int64_t r0 = (int64_t)gate * parts + u % lanes, r1 = job < 2 ? (int64_t)gates * parts : gate < gates ? (int64_t)(gate + 1) * parts : 0;
+    const float* const src = part + (job ? D : 0) + c0 + x;
+    const bool weigh = job == 1 && a.gate_rows;
+    float v[4] = {};
+    if (c0 + x + 3 < D) {
+#pragma unroll 8
+        for (int64_t r = r0; r < r1; r += lanes) {
+            float p[4];
+            __builtin_memcpy(p, src + r * 2 * D, 16);
+            if (weigh) {
+                half4 g;
+                __builtin_memcpy(&g, a.gate + r / parts * D + c0 + x, 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] *= (float)g[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += p[i];
         }
-    red[u][x] = v;
+    } else {
+        for (int64_t r = r0; r < r1; r += lanes)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c0 + x + i < D) v[i] += src[r * 2 * D + i] * (weigh ? (float)a.gate[r / parts * D + c0 + x + i] : 1.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[u][x + i] = v[i];
     __syncthreads();
-    if (u || c >= D) return;
-    v = 0.0f;
-    for (int r = 0; r < 64; ++r) v += red[r][x];
-    if (job >= 2 && a.wo) v *= (float)a.wo[c];
-    out[c] = (f16)(a.accumulate ? v + (float)out[c] : v);
+    const int col = threadIdx.x % SUM_COLS, group = threadIdx.x / SUM_COLS, c = c0 + col;
+    auto put = [&](f16* out, float sum) {
+        if (out) out[c] = (f16)(a.accumulate ? sum + (float)out[c] : sum);
+    };
+    const float wo = a.wo && c < D ? (float)a.wo[c] : 1.0f;
+    if (lanes == 64) {  // four groups each, then the sixteen
+        float sum = ((red[4 * group][col] + red[4 * group + 1][col]) + red[4 * group + 2][col]) + red[4 * group + 3][col];
+        __syncthreads();
+        red[group][col] = sum;
+        __syncthreads();
+        if (group || c >= D) return;
+        sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += red[r][col];
+        if (job == 0) return put(a.dwi, sum);
+        if (job > 1) return put(a.dgate + (int64_t)gate0 * D, sum * wo);
+        put(a.dwo, a.gate && !a.gate_rows ? sum * (float)a.gate[c] : sum);
+        if (!a.gate_rows) put(a.dgate, sum * wo);
+        return;
+    }
+    if (c >= D) return;
+    for (int g = group; g < 64 / lanes && gate0 + g < gates; g += 16) {
+        float sum = 0.0f;
+        for (int r = 0; r < lanes; ++r) sum += red[g * lanes + r][col];
+        put(a.dgate + (int64_t)(gate0 + g) * D, sum * wo);
+    }
 }
 
 template <class F>
@@ -305,10 +352,13 @@ void by_width(int D, F&& f) {
 }
 static_assert(RESIDUAL_NORM_MOST == 1024 * 2 * 8, "the widest row");
 
-// Runs of rows of one gate
+// Runs of rows of one gate: long ones, whose sums cost less to write and add, as
+// far as every CU keeps rows in flight (us of the gradient with 256, 512 and 1024
+// runs: 7996 rows of 768 30, 27, 34; 4096 rows of 4096 54, 57, 66; 3000 of 8192
+// 81, 92, 101)
 int64_t runs(int64_t rows, int64_t gates, int D) {
-    const int64_t rows_gate = rows / gates;
-    return std::max<int64_t>(1, std::min((rows_gate + 3) / 4, (1024 + gates - 1) / gates));
+    const int64_t rows_gate = rows / gates, all = D <= 1024 ? 512 : 256;
+    return std::max<int64_t>(1, std::min((rows_gate + 3) / 4, (all + gates - 1) / gates));
 }
 
 }  // namespace
@@ -330,8 +380,10 @@ int residual_norm_forward(const ResidualNormArgs& a, hipStream_t st) {
 
 int residual_norm_backward(const ResidualNormArgs& a, float* part, hipStream_t st) {
     const int64_t gates = a.gate_rows ? a.rows / a.gate_rows : 1, parts = runs(a.rows, gates, a.D);
-    const int blocks = (a.D + 15) / 16;
-    const int64_t jobs = 2 + (a.dgate ? gates : 0);
+    const int blocks = (a.D + SUM_COLS - 1) / SUM_COLS;
+    int lanes = 1;
+    while (lanes < 64 && lanes < parts) lanes *= 2;
+    const int64_t jobs = 2 + (a.dgate && a.gate_rows ? (gates + 64 / lanes - 1) / (64 / lanes) : 0);
     int rc = EVKHIP_OK;
     by_width(a.D, [&](auto tpr, auto) { rc = check_grid("residual_norm_backward", gates * parts, threads_of(decltype(tpr)::value)); });
     if (rc == EVKHIP_OK && part) rc = check_grid("residual_norm_backward", jobs * blocks, 1024);
@@ -344,7 +396,7 @@ int residual_norm_backward(const ResidualNormArgs& a, float* part, hipStream_t s
     });
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && part) {
-        hipLaunchKernelGGL(residual_norm_sums_k, dim3((unsigned)(jobs * blocks)), dim3(1024), 0, st, a, part, (int)parts, (int)gates, blocks);
+        hipLaunchKernelGGL(residual_norm_sums_k, dim3((unsigned)(jobs * blocks)), dim3(1024), 0, st, a, part, (int)parts, (int)gates, blocks, lanes);
         e = hipGetLastError();
     }
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "residual_norm_backward launch");

@@ -70,19 +70,6 @@ DEV half8 row_part(const f16* l, int i, int V) {
     return h;
 }
 
-// The compiler forms what it needs of these values anew from here on: it would
-// keep each one's 32-bit form or exponential from pass to pass, in as many
-// registers as make the row's reads wait for each other.
-template <int NV>
-DEV void forget(half8 (&x)[NV]) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        u32x4 u = as_u32x4(x[v]);
-        asm volatile("" : "+v"(u));
-        x[v] = as_half8(u);
-    }
-}
-
 // The larger of two pairs of halves, as the instruction has it: the compiler's
 // own puts one before it for each side, for NaN that signal.  (One NaN is passed
 // over, in a row with NaN the sum is NaN.)
@@ -153,7 +140,7 @@ __global__ __launch_bounds__(NT, NV == 16 ? 4 : 1) void token_logprobs_k(TokenLo
     }
     const float c2 = a.scale * kLog2e;
     float sum = 0.0f, dot = 0.0f;
-    forget(x);
+    forget(x);  // else each value is kept as the maximum's pass had it, in as many registers as the reads then wait for
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
