@@ -24,7 +24,7 @@ ARCH = os.environ.get("EVK_OFFLOAD_ARCH", "gfx950")
 KERNEL_SOURCES = ["capi.hip", "gemm.hip", "flash.hip", "flash_wide.hip", "decode_ops.hip", "model.hip", "decode_persist.hip",
                   "kv_step.hip", "train_ops.hip", "capi_block.hip", "qkv_rope.hip", "window.hip",
                   "capi_group.hip", "residual_norm.hip", "token_logprobs.hip", "prefix.hip"]
-API_SOURCES = ["evk_runtime.cpp", "evk_ai.cpp", "evk_block.cpp"]
+API_SOURCES = ["evk_runtime.cpp", "evk_ai.cpp", "evk_block.cpp", "evk_group.cpp"]
 
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
@@ -85,7 +85,7 @@ def build(verbose: bool = False) -> None:
             os.replace(exe + ".tmp", exe)
 
         with cf.ThreadPoolExecutor(max_workers=3) as ex:
-            list(ex.map(program, ["api_tests", "kv_decoder_tool", "block_tests"]))
+            list(ex.map(program, ["api_tests", "kv_decoder_tool", "block_tests", "group_tests"]))
     if verbose:
         print("built", kern)
 

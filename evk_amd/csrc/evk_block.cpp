@@ -1,71 +1,17 @@
 // evk::ai's operators of a grouped-query block (no reference counterparts)
-// over the C ABI.  Workspaces are buffers of the runtime, released once the
-// stream has passed the call.
-#include <evk_ai.h>
-#include <evkhip.h>
+// over the C ABI.
+#include "evk_calls.h"
 
 namespace evk::ai {
-namespace {
-
-evkhip_tensor desc(Tensor& t) {
-    evkhip_tensor d{};
-    d.data = t.device_ptr();
-    d.rank = t.shape.rank();
-    for (uint32_t i = 0; i < d.rank; ++i) d.dims[i] = t.shape.values[i];
-    return d;
-}
-struct Opt {  // descriptor of a tensor that may be left out
-    evkhip_tensor d{};
-    const evkhip_tensor* p = nullptr;
-    explicit Opt(Tensor* t) {
-        if (t) {
-            d = desc(*t);
-            p = &d;
-        }
-    }
-};
-
-void check(int status, const char* op) {
-    if (status != EVKHIP_OK) {
-        std::fprintf(stderr, "evk::ai::%s failed (status %d): %s\n", op, status, evkhip_last_error());
-        std::abort();
-    }
-}
-void* stream() {
-    return GetCmd().stream();
-}
-
-// Address of `count` 32-bit values in the storage of an fp16 tensor.
-void* words(Tensor* t, uint64_t count, const char* op, const char* name) {
-    if (!t) return nullptr;
-    if (uint64_t(t->shape.count()) != 2 * count) {
-        std::fprintf(stderr, "evk::ai::%s: %s holds %u fp16 slots, needs %llu (%llu 32-bit values)\n", op, name, t->shape.count(),
-                     (unsigned long long)(2 * count), (unsigned long long)count);
-        std::abort();
-    }
-    return t->device_ptr();
-}
-uint64_t rows_of(Tensor& q, uint32_t head_dim) {
-    return head_dim ? uint64_t(q.shape.count()) / head_dim : 0;
-}
-
-struct Workspace {
-    evk::Buffer buffer;
-    uint64_t bytes;
-    explicit Workspace(uint64_t n) : bytes(n) {
-        if (n) buffer = evk::CreateBuffer({.size = n, .usage = evk::BufferUsage::Storage});
-    }
-    void* ptr() { return bytes ? reinterpret_cast<void*>(buffer.GetReference()) : nullptr; }
-};
-
-}  // namespace
+using namespace calls;
 
 void qkv_norm_rope(Tensor& qkv, Tensor& q, Tensor& k, Tensor& v, uint32_t head_dim, Tensor* q_weight, Tensor* k_weight,
-                   float eps, float rotary_base, uint32_t position_offset, Tensor* offsets) {
+                   float eps, float rotary_base, uint32_t position_offset, Tensor* offsets, uint32_t first_position) {
     evkhip_tensor X = desc(qkv), Q = desc(q), K = desc(k), V = desc(v);
     Opt wq(q_weight), wk(k_weight);
     const int32_t* off = static_cast<const int32_t*>(words(offsets, qkv.shape[0], "qkv_norm_rope", "offsets"));
-    check(evkhip_qkv_norm_rope(&X, wq.p, wk.p, &Q, &K, &V, head_dim, eps, rotary_base, position_offset, off, stream()),
+    check(evkhip_qkv_norm_rope_behind(&X, wq.p, wk.p, &Q, &K, &V, head_dim, eps, rotary_base, first_position, position_offset, off,
+                                      stream()),
           "qkv_norm_rope");
 }
 

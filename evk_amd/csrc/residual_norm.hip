@@ -297,7 +297,7 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_k(ResidualNormArgs a,
             __builtin_memcpy(p, src + r * 2 * D, 16);
             if (weigh) {
                 half4 g;
-                __builtin_memcpy(&g, a.gate + r / parts * D + c0 + x, 8);
+                __builtin_memcpy(&g, a.gate + (int64_t)((int)r / parts) * D + c0 + x, 8);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p[i] *= (float)g[i];
             }
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_k(ResidualNormArgs a,
         for (int64_t r = r0; r < r1; r += lanes)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (c0 + x + i < D) v[i] += src[r * 2 * D + i] * (weigh ? (float)a.gate[r / parts * D + c0 + x + i] : 1.0f);
+                if (c0 + x + i < D) v[i] += src[r * 2 * D + i] * (weigh ? (float)a.gate[(int64_t)((int)r / parts) * D + c0 + x + i] : 1.0f);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) red[u][x + i] = v[i];

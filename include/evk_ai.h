@@ -401,11 +401,12 @@ void zero(Tensor& tensor);
 
 // Norm and rotation of each query and key head of qkv (B, N, (H + 2 KV) *
 // head_dim): q (B, N, H * head_dim); k, v (B, rows, KV * head_dim), whose rows
-// position_offset + t (or offsets[b] + t, B int32 values) take token t.
+// position_offset + t (or offsets[b] + t, B int32 values) take token t.  Row 0
+// stands at position first_position: the length of a prefix that lies elsewhere.
 // Weights: head_dim values, nullptr for ones.
 void qkv_norm_rope(Tensor& qkv, Tensor& q, Tensor& k, Tensor& v, uint32_t head_dim, Tensor* q_weight = nullptr,
                    Tensor* k_weight = nullptr, float eps = 1e-4f, float rotary_base = 10000.0f, uint32_t position_offset = 0,
-                   Tensor* offsets = nullptr);
+                   Tensor* offsets = nullptr, uint32_t first_position = 0);
 // dqkv is written; the weights' gradients (nullptr: not wanted) are written or,
 // with accumulate, added to.
 void qkv_norm_rope_backward(Tensor& qkv, Tensor& dq, Tensor& dk, Tensor& dv, Tensor& dqkv, uint32_t head_dim,
@@ -429,6 +430,39 @@ void gated_linear(Tensor& x, Tensor& w, Tensor& h, Tensor* gate_up = nullptr, Ac
 // dx is written, dw written or, with accumulate, added to; nullptr: not wanted.
 void gated_linear_backward(Tensor& x, Tensor& w, Tensor& gate_up, Tensor& dh, Tensor* dx, Tensor* dw,
                            Activation activation = Activation::Silu, bool accumulate = false);
+
+// ---- operators of a group of continuations of one prompt (no reference
+// counterparts); 32-bit values lie in fp16 storage of twice as many elements ----
+
+// s = residual_scale x + gate * norm(y) * post_weight (gate * y without
+// post_norm), h = norm(s) * pre_weight; x, y, s, h (..., D), weights (D), gate (D)
+// or (B, D) with one for each of x's sequences; nullptr for ones.  y and s
+// nullptr: h = norm(x) * pre_weight, the norm before the first block.
+void residual_norm(Tensor& x, Tensor* y, Tensor* s, Tensor& h, Tensor* post_weight = nullptr, Tensor* gate = nullptr,
+                   Tensor* pre_weight = nullptr, float residual_scale = 1.0f, bool post_norm = true, float eps = 1e-4f);
+// From ds (nullptr: zeros) and dh: dx and dy are written; the gradients of weights
+// and gate (nullptr: not wanted) are written or, with accumulate, added to.
+void residual_norm_backward(Tensor& x, Tensor* y, Tensor* ds, Tensor& dh, Tensor& dx, Tensor* dy, Tensor* post_weight = nullptr,
+                            Tensor* gate = nullptr, Tensor* pre_weight = nullptr, Tensor* dpost_weight = nullptr, Tensor* dgate = nullptr,
+                            Tensor* dpre_weight = nullptr, float residual_scale = 1.0f, bool post_norm = true, float eps = 1e-4f,
+                            bool accumulate = false);
+
+// Attention of q (B, N, H * head_dim) over the prefix (P, KV * head_dim) that all
+// sequences share and each one's own rows of k, v (B, rows, KV * head_dim) up to
+// the query's, position_offset + t (or offsets[b] + t, B int32 values).  lse: B * H
+// * N fp32 values.
+void prefix_attention(Tensor& q, Tensor& prefix_k, Tensor& prefix_v, Tensor& k, Tensor& v, Tensor& o, uint32_t head_dim,
+                      uint32_t position_offset = 0, Tensor* offsets = nullptr, Tensor* lse = nullptr);
+
+// log p of `tokens` (one a row of logits (..., V); 0 for ids of V and above), p =
+// softmax(input_scale * logits), fp32; where given, the rows' entropies, the K most
+// likely ids (..., K) with their log p, and stats (2 a row) for the gradient.
+void token_logprobs(Tensor& logits, Tensor& tokens, Tensor& logprobs, Tensor* entropy = nullptr, Tensor* top_ids = nullptr,
+                    Tensor* top_logprobs = nullptr, Tensor* stats = nullptr, float input_scale = 1.0f);
+// dlogits is written from fp32 dlogprobs and, with the forward's entropy, dentropy
+// (one of the two may be nullptr).
+void token_logprobs_backward(Tensor& logits, Tensor& tokens, Tensor& stats, Tensor* dlogprobs, Tensor& dlogits, Tensor* entropy = nullptr,
+                             Tensor* dentropy = nullptr, float input_scale = 1.0f);
 
 // ---- training ops (evk_ai.h:476-614).  *_backward ops accumulate into
 // their grad_in, as the reference's shaders do. ----
@@ -789,6 +823,69 @@ struct Graph {
             evk::ai::add(x.grad(), dx, x.grad());
         };
         return out;
+    }
+
+    // x (.., D) joined with the block's output y as evk::ai::residual_norm joins
+    // them: the stream s behind the block and h, what the next one reads.
+    struct Joined {
+        Tensor &s, &h;
+    };
+    Joined residual_norm(Tensor& x, Tensor& y, Tensor* post_weight = nullptr, Tensor* gate = nullptr, Tensor* pre_weight = nullptr,
+                         float residual_scale = 1.0f, bool post_norm = true, float eps = 1e-4f) {
+        assert(x.shape.rank() == y.shape.rank() && x.shape.count() == y.shape.count() && "residual_norm: x and y (.., D)");
+        Tensor& dx = node(x.shape);
+        Tensor& dy = node(x.shape);
+        Tensor& s = node(x.shape);
+        Tensor& h = node(x.shape);
+        s.forward_fn = [&x, &y, &s, &h, post_weight, gate, pre_weight, residual_scale, post_norm, eps]() {
+            evk::ai::residual_norm(x, &y, &s, h, post_weight, gate, pre_weight, residual_scale, post_norm, eps);
+        };
+        // runs after the backward functions of every node that reads s or h
+        s.backward_fn = [&x, &y, &s, &h, &dx, &dy, post_weight, gate, pre_weight, residual_scale, post_norm, eps]() {
+            evk::ai::residual_norm_backward(x, &y, &s.grad(), h.grad(), dx, &dy, post_weight, gate, pre_weight,
+                                            post_weight ? &post_weight->grad() : nullptr, gate ? &gate->grad() : nullptr,
+                                            pre_weight ? &pre_weight->grad() : nullptr, residual_scale, post_norm, eps, true);
+            evk::ai::add(x.grad(), dx, x.grad());
+            evk::ai::add(y.grad(), dy, y.grad());
+        };
+        return {s, h};
+    }
+
+    // norm(x) * weight, the norm before the first block.
+    Tensor& weighted_norm(Tensor& x, Tensor& weight, float eps = 1e-4f) {
+        Tensor& dx = node(x.shape);
+        Tensor& h = node(x.shape);
+        h.forward_fn = [&x, &h, &weight, eps]() { evk::ai::residual_norm(x, nullptr, nullptr, h, nullptr, nullptr, &weight, 1.0f, true, eps); };
+        h.backward_fn = [&x, &h, &dx, &weight, eps]() {
+            evk::ai::residual_norm_backward(x, nullptr, nullptr, h.grad(), dx, nullptr, nullptr, nullptr, &weight, nullptr, nullptr,
+                                            &weight.grad(), 1.0f, true, eps, true);
+            evk::ai::add(x.grad(), dx, x.grad());
+        };
+        return h;
+    }
+
+    // Log-probabilities of tokens (B, N) under logits (B, N, V), and entropies; the
+    // backward pass starts from their gradients, fp32 values that the caller has
+    // written (advantages with their sign, say): dlogprobs and dentropy, two fp16
+    // slots for each of the B * N rows, dentropy nullptr for none.
+    struct Scores {
+        Tensor &logprobs, &entropy;  // (B, N, 2), fp32 values
+    };
+    Scores token_logprobs(Tensor& logits, Tensor& tokens, Tensor& dlogprobs, Tensor* dentropy = nullptr, float input_scale = 1.0f) {
+        assert(logits.shape.rank() == 3 && tokens.shape.rank() == 2 && "token_logprobs: logits (B, N, V), tokens (B, N)");
+        const uint32_t B = logits.shape[0], N = logits.shape[1];
+        Tensor& stats = node(Shape({B, N, 4}));
+        Tensor& dlogits = node(logits.shape);
+        Tensor& entropy = node(Shape({B, N, 2}));
+        Tensor& logprobs = node(Shape({B, N, 2}));
+        logprobs.forward_fn = [&logits, &tokens, &logprobs, &entropy, &stats, input_scale]() {
+            evk::ai::token_logprobs(logits, tokens, logprobs, &entropy, nullptr, nullptr, &stats, input_scale);
+        };
+        logprobs.backward_fn = [&logits, &tokens, &dlogprobs, dentropy, &entropy, &stats, &dlogits, input_scale]() {
+            evk::ai::token_logprobs_backward(logits, tokens, stats, &dlogprobs, dlogits, dentropy ? &entropy : nullptr, dentropy, input_scale);
+            evk::ai::add(logits.grad(), dlogits, logits.grad());
+        };
+        return {logprobs, entropy};
     }
 
     // The reference's composition: scores = q k^T, mask, softmax(scale), @ v.
