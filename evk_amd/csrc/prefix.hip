@@ -346,9 +346,7 @@ bool mfma_ok(const PrefixArgs& a) {
     return a.dh % 8 == 0 && (int64_t)a.KV * a.dh * 2 * (BK + 1) < INT32_MAX;
 }
 
-int query_blocks(int64_t rows, int64_t heads, int dh) { return dh <= 128 && heads * ((rows + 127) / 128) > 256 ? 2 : 1; }
-
-// How a shape runs.
+// How a shape runs.  us in the comments: one side of a rule and the other.
 struct Plan {
     enum { TILES, STEPS, SHARED } kind;
     int qb;          // query blocks of a wave in tiles
@@ -359,24 +357,34 @@ struct Plan {
 };
 Plan plan_for(int64_t B, int64_t N, int64_t P, int64_t R, int64_t H, int64_t KV, int dh) {
     Plan p{};
-    const int64_t per = N * (H / KV), heads = B * KV;
+    const int64_t per = N * (H / KV), heads = B * KV, all = B * per;
     auto ceil = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     auto some = [](int64_t most, int64_t a, int64_t b) { return std::max<int64_t>(1, std::min({most, a, b})); };
-    if (per >= 64) {
+    // Prompts: tiles of one sequence's rows over the prefix and its own.  From 256 rows of a key head on (8 sequences of 120
+    // tokens, 16 heads over 4 of 128, behind 4096 rows: 62, the other way 89), from 128 on where that gives every CU a
+    // tile (32 of 50 tokens behind 1000 rows 32 and 58; 8 of 40, 8 over 2 of 64, behind 200 rows, 48 tiles: 11.2 and 6.0;
+    // 64 rows each, 64 sequences behind 8192 rows: 269 and 184).
+    if (per >= 256 || (per >= 128 && heads * ceil(per, 64) >= 256)) {
         p.kind = Plan::TILES;
-        p.qb = query_blocks(per, heads, dh);
+        p.qb = dh <= 128 && heads * ceil(per, 128) > 256 ? 2 : 1;  // as in window_attention
         const int64_t tiles = ceil(per, 64 * p.qb), groups = heads * tiles;
-        const int64_t splits = some(JOIN_MOST, 512 / groups, ceil(P + R, 4 * BK));
+        // parts of the list where CUs are idle: of 4 tiles and more, of 16 where a quarter is busy (10 tiles over 4200 rows:
+        // 15.7, with 16 tiles a part 21; 104 over 600 rows, parts of 8 15.1, none 10.3; 256 over 300: 21.6 and 8.5)
+        const int64_t splits = groups >= 256 ? 1 : some(JOIN_MOST, 512 / groups, ceil(P + R, (groups >= 64 ? 16 : 4) * BK));
         p.slots = splits > 1 ? (int)splits : 0;
         p.tiles = {(int)per, (int)tiles, 1, (int)splits, p.slots};
         p.wide = groups * splits;
         return p;
     }
-    const int64_t tiles = ceil(per, 16), groups = heads * tiles, all = B * per;
-    // steps of one workgroup, while its waves take no more than four each; else parts, and a second launch to join them
+    const int64_t tiles = ceil(per, 16), groups = heads * tiles;
+    // A few rows: each sequence's steps over both, in one workgroup while its waves take no more than four each, else in
+    // parts with a second launch to join them; while reading the prefix again for each costs less than sharing it: 64 MB
+    // against a second launch (64 sequences, 12 heads over 4 of 64, 300 rows, 19 MB: 7.4 and 10.4; 32 over 8 of 128, 500 rows,
+    // 129 MB: 28.8 and 23.4), 4 MB where there is one anyway (16 sequences of 8 over 1 of 64, 4096 rows, 16 MB: 9.6 and 9.3;
+    // 4 of 32 over 8 of 128, 16000 rows, 197 MB: 45 and 22).
     const int64_t steps = ceil(P + R, 32), waves = dh <= 128 ? 8 : 4;
     const bool alone = steps <= 4 * waves;
-    if (B == 1 || (B - 1) * P * KV * dh * 4 < (alone ? 64 << 20 : 4 << 20)) {
+    if (B == 1 || (double)(B - 1) * P * KV * dh * 4 < (alone ? 64 << 20 : 4 << 20)) {
         p.kind = Plan::STEPS;
         const int64_t splits = alone ? 1 : some(JOIN_MOST, 256 / groups, ceil(steps, waves));
         p.slots = splits > 1 ? (int)splits : 0;
@@ -384,6 +392,9 @@ Plan plan_for(int64_t B, int64_t N, int64_t P, int64_t R, int64_t H, int64_t KV,
         p.few = groups * splits;
         return p;
     }
+    // The prefix for all sequences at once, by tiles of 64 rows, of 128 where those are enough to keep the products busy
+    // (256 rows of 8 heads over 8192 rows 52 and 60; 64 rows over 2048 13.4 and 11.6); the own rows in parts of up to 16
+    // steps of 128 values, which end at about the same time (one part 55, two 50; 256 values, 500 rows: 22 and 16).
     p.kind = Plan::SHARED;
     p.qb = dh <= 128 && KV * ceil(all, 128) * ceil(P, 512) >= 256 ? 2 : 1;
     const int64_t wide = KV * ceil(all, 64 * p.qb);
