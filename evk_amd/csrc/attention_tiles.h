@@ -396,10 +396,10 @@ DEV uint32_t attend_tiles(Softmax<DH, QB>& sm, const half8 (&qf)[QB][Geo<DH>::KS
     return wild;
 }
 
-// Every NW-th step of 32 entries into the states of 16 QB queries, by one wave: K
+// Every NW-th step of 32 entries into the states of 16 queries, by one wave: K
 // goes from memory straight into A operands, V through the wave's own LDS slot
 // (32 rows), no barrier; the next step's loads are in flight meanwhile.
-template <int DH, int NW, int QB = 1>
+template <int DH, int NW>
 struct Steps {
     using G = Geo<DH>;
     static constexpr int KS = G::KS, DT = G::DT, W = G::W, VPER = 32 * G::CPR / 64;
@@ -437,7 +437,7 @@ struct Steps {
     }
     // from `step`, which is loaded, on; k_row, v_row: an entry's row, past the list's end any row that is there
     template <class KRow, class VRow, class Plain, class Seen>
-    DEV uint64_t run(Softmax<DH, QB>& sm, const half8 (&qf)[QB][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
+    DEV uint64_t run(Softmax<DH, 1>& sm, const half8 (&qf)[1][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
                      Seen&& seen) {
         const int g = lane >> 4;
         uint64_t wild = 0;
@@ -457,33 +457,25 @@ struct Steps {
             half8 vf[DT];
 #pragma unroll
             for (int d = 0; d < DT; ++d) vf[d] = fr.col(slot, 0, d);
-            floatx4 s[2][QB];
+            floatx4 s[2][1];
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
+                s[kb][0] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int q = 0; q < QB; ++q) s[kb][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int q = 0; q < QB; ++q) s[kb][q] = mfma16(as_half8(kr[kb][ks]), qf[q][ks], s[kb][q]);
+                for (int ks = 0; ks < KS; ++ks) s[kb][0] = mfma16(as_half8(kr[kb][ks]), qf[0][ks], s[kb][0]);
             }
             if (step + NW < end) load_k(step + NW, k_row, dh);
             if (!whole) {
+                const auto see = seen(0);
 #pragma unroll
-                for (int q = 0; q < QB; ++q) {
-                    const auto see = seen(q);
+                for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) s[kb][q][j] = see(32 * step + 16 * kb + 4 * g + j) ? s[kb][q][j] : -INFINITY;
-                }
+                    for (int j = 0; j < 4; ++j) s[kb][0][j] = see(32 * step + 16 * kb + 4 * g + j) ? s[kb][0][j] : -INFINITY;
             }
-            half8 p[1][QB];
+            half8 p[1][1];
             sm.template probs<2>(s, c2, p);
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int q = 0; q < QB; ++q) sm.o[d][q] = mfma16(vf[d], p[0][q], sm.o[d][q]);
+            for (int d = 0; d < DT; ++d) sm.o[d][0] = mfma16(vf[d], p[0][0], sm.o[d][0]);
         }
         return wild;
     }
@@ -495,19 +487,19 @@ constexpr int steps_bytes() {
     constexpr int SLOT = 32 * Geo<DH>::W * 2, STATE = 16 * (DH + 4) * 4;  // of a wave's V, then of its state
     return NW * (SLOT > STATE ? SLOT : STATE);
 }
-// The waves' states of 16 queries (block QI) as one: store(query, value, m, l, four
-// values of O^T) for all of them
-template <int DH, int NW, int QI = 0, int QB, class Store>
-DEV void merge_waves(const Softmax<DH, QB>& sm, char* smem, float (*sm_m)[16], float (*sm_l)[16], int lane, int wave, Store&& store) {
+// The waves' states of 16 queries as one: store(query, value, m, l, four values of
+// O^T) for all of them
+template <int DH, int NW, class Store>
+DEV void merge_waves(const Softmax<DH, 1>& sm, char* smem, float (*sm_m)[16], float (*sm_l)[16], int lane, int wave, Store&& store) {
     constexpr int DT = Geo<DH>::DT, OW = DH + 4;
     const int l16 = lane & 15, g = lane >> 4;
     __syncthreads();  // the slots have been read
     float* const st = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<floatx4*>(st + (wave * 16 + l16) * OW + 16 * d + 4 * g) = sm.o[d][QI];
-    const float l = query_sum(sm.l[QI]);
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<floatx4*>(st + (wave * 16 + l16) * OW + 16 * d + 4 * g) = sm.o[d][0];
+    const float l = query_sum(sm.l[0]);
     if (g == 0) {
-        sm_m[wave][l16] = sm.m[QI];
+        sm_m[wave][l16] = sm.m[0];
         sm_l[wave][l16] = l;
     }
     __syncthreads();
