@@ -23,7 +23,10 @@ DEV int own_rows(const PrefixArgs& a, int b, int t) {
 }
 
 // ---------------------------------------------------------------------------
-// One wave per query row, any head size and alignment.
+// One wave per query row, any head size and alignment: 64 rows of K at a time, a
+// lane each, then V's columns over the lanes.  For what the MFMA kernels do not
+// take; bounded by the latency of its scalar loads (16 sequences, 8 heads over 2 of
+// 100 values, 1000 rows and up to 300: 218 us).
 // ---------------------------------------------------------------------------
 constexpr int SMAX = 256;  // largest head size
 
@@ -106,7 +109,12 @@ DEV float* state_at(float* ws, int64_t row, int slots, int slot) {
 }
 
 // Tiles of 64 QB rows over the prefix and, where they are one sequence's, its own
-// rows behind it.  The prefix is padded to whole tiles of the list.
+// rows behind it.  The prefix is padded to whole tiles of the list, so that a tile
+// lies behind one descriptor.
+//
+// Bounded by the softmax's instructions beside the MFMA: 8 x 500 tokens, 16 heads
+// over 4 of 128, behind 4096 rows, 142 GFLOP in 150 us = 950 TFLOP/s (a product of
+// the library at 8192^3 runs at 1156).
 struct TileWork {
     int per, tiles;    // rows of one sequence (B N G: all of them together, over the prefix alone), tiles of them
     int own;           // their own rows are part of the list
@@ -206,7 +214,10 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void prefix_tiles(PrefixArgs
 }
 
 // 16 rows of one sequence, the waves' steps over its own rows and, where nobody
-// else sees to it, the prefix before them.
+// else sees to it, the prefix before them: a few queries use few of a product's
+// columns, and nothing waits but for memory.  One token, 32 heads over 8 of 128
+// behind 16000 rows: 17.9 us with the join = 3.7 TB/s; 64 sequences of 12 over 4 of
+// 64, 300 rows and up to 300: 8.0.
 struct StepWork {
     int tiles;
     int prefix;               // rows of the prefix in the list: P or 0
@@ -283,7 +294,10 @@ __global__ __launch_bounds__(64 * StepGeo<DH>::NW, StepGeo<DH>::NW / 4) void pre
 // The prefix by tiles and the own rows by steps in one launch: the former wait for
 // their products, the latter for memory.  Each XCD starts its part of the tiles
 // first, which take the same time all, and fills up with own rows, which end when
-// they end.
+// they end.  64 tokens, 32 heads over 8 of 128 behind 8192 rows, up to 1024 of their
+// own: 44 us for 34 MB of prefix, whose products are 8.6 GFLOP, and 134 MB of own
+// rows, which alone take 31-38.  4 tokens each behind 4096 rows, with the join: 42, in
+// launches of their own 52.
 template <int DH, int QB>
 __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void prefix_mixed(PrefixArgs a, TileWork tw, int wide, StepWork sw, float* ws) {
     constexpr int TILES = 4 * BK * Geo<DH>::W * 2, STEPS = steps_bytes<DH, 4>();
@@ -298,7 +312,7 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void prefix_mixed(PrefixArgs
 
 // The states of a row, added in order by one wave: groups of DH / 4 lanes take
 // every HPW-th of them, 16 bytes a lane, all requested before the weights are
-// known.
+// known.  2048 rows of 14 states: 5.0 us, a launch and two latencies.
 constexpr int JOIN_MOST = 64;  // a lane weighs one
 template <int DH>
 __global__ __launch_bounds__(256) void prefix_join(PrefixArgs a, int slots, int64_t rows, const float* ws) {

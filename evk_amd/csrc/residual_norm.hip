@@ -15,7 +15,8 @@
 // threads' registers, NV vectors of eight values each, at any alignment (the
 // last vector takes what is left); weights and gates stay in registers from row
 // to row.  The sums of a row are in 32 bits, as is everything between the loads
-// and the stores.
+// and the stores.  8192 rows of 4096: 50 us = 5.3 TB/s (a copy of 1 GiB runs at
+// 5.1); 7996 of 768, where the launch counts, 13.8 = 3.6; 16 rows 3.9.
 #include "kernels.h"
 
 #include <algorithm>
@@ -154,7 +155,8 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_k(ResidualNormA
 // The gradient.  A workgroup takes a run of rows of one gate (`parts` runs a
 // gate), keeps the columns' sums dh u and S n in registers and leaves them in the
 // workspace, one row of 2 D sums, which residual_norm_sums_k adds in a fixed
-// order.
+// order.  A row's sums wait for each other three times; the next row is on its way
+// meanwhile.  4096 rows of 4096: 44 us = 4.6 TB/s; 7996 of 768: 20 = 3.7.
 template <int TPR, int NV, bool Y>
 __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualNormArgs a, int64_t rows_gate, int parts, float* part) {
     constexpr int RPW = threads_of(TPR) / TPR;
@@ -280,7 +282,8 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
 // of the one gate that there is), from 2 on the gradients of 64 / lanes gates.  64
 // groups of 16 threads, four columns a thread: `lanes` of them (a power of two, no
 // more than the runs of a gate need) take a gate's runs in turn, all 64 those of
-// dwi and dwo, and their sums are added in order.
+// dwi and dwo, and their sums are added in order.  512 runs of 768, 4 gates: 6.8 us,
+// 256 of 4096: 5.3, the latency of eight rows a thread and the launch.
 constexpr int SUM_COLS = 64;
 __global__ __launch_bounds__(1024) void residual_norm_sums_k(ResidualNormArgs a, const float* part, int parts, int gates, int blocks, int gate_lanes) {
     __shared__ float red[64][SUM_COLS + 4];
