@@ -54,10 +54,10 @@ inline int check_workspace(const char* op, const void* p, uint64_t have, uint64_
     return EVKHIP_OK;
 }
 
-inline int check_weight(const char* op, const char* name, const evkhip_tensor* w, uint32_t head_dim) {
+inline int check_weight(const char* op, const char* name, const evkhip_tensor* w, uint32_t values) {
     if (!w) return EVKHIP_OK;
     CHECK(check_tensor(w, name, 1, 1));
-    EVK_RETURN_IF(w->dims[0] != head_dim, EVKHIP_ERR_SHAPE, "%s: %s must hold head_dim = %u values", op, name, head_dim);
+    EVK_RETURN_IF(w->dims[0] != values, EVKHIP_ERR_SHAPE, "%s: %s must hold %u values", op, name, values);
     return EVKHIP_OK;
 }
 
@@ -66,7 +66,7 @@ struct Heads {
 };
 // q (B,N,H dh); k, v (B,R,KV dh)
 inline int head_shapes(const char* op, const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v, uint32_t dh,
-                Heads* s) {
+                       Heads* s) {
     CHECK(check_tensor(q, op, 3, 3));
     CHECK(check_tensor(k, op, 3, 3));
     CHECK(check_tensor(v, op, 3, 3));

@@ -236,6 +236,7 @@ int evkhip_token_logprobs(const evkhip_tensor* logits, const evkhip_tensor* toke
     uint64_t rows, top = 0;
     CHECK(logits_shapes(op, logits, tokens, input_scale, &rows));
     EVK_RETURN_IF(rows && !logprobs, EVKHIP_ERR_INVALID_ARG, "%s: null logprobs", op);
+    if (top_ids) CHECK(check_tensor(top_ids, op, 1, EVKHIP_MAX_DIMS));
     EVK_RETURN_IF(!top_ids != !top_logprobs && !(top_ids && numel(top_ids) == 0), EVKHIP_ERR_INVALID_ARG,
                   "%s: top_ids and top_logprobs come together", op);
     CHECK(check_floats(op, "logprobs", logprobs));
@@ -244,7 +245,6 @@ int evkhip_token_logprobs(const evkhip_tensor* logits, const evkhip_tensor* toke
     CHECK(check_floats(op, "stats", stats));
     if (top_ids) {
         uint64_t n;
-        CHECK(check_tensor(top_ids, op, 1, EVKHIP_MAX_DIMS));
         CHECK(rows_of(op, top_ids, &n));
         top = dim_at(top_ids, -1);
         EVK_RETURN_IF(top && n != rows, EVKHIP_ERR_SHAPE, "%s: alternatives of %llu rows, %llu are there", op, (unsigned long long)n,

@@ -209,3 +209,15 @@ def test_python_checks():
                  lambda: evk.residual_norm_backward(h, h, h, h, h, h), lambda: evk.token_logprobs_backward(h, x, x, x, h)):
         with pytest.raises((ValueError, RuntimeError)):
             call()
+
+
+@pytest.mark.parametrize("rank", [0, 9, 1 << 31])
+def test_alternatives_of_a_rank_that_is_none(L, rank):
+    """The descriptor's sizes are not read before its rank has been checked, with or without a place for their log p."""
+    m = Mem()
+    for alt in (None, 1 << 16):
+        ids = m(6, 5)
+        ids.rank = rank
+        logits, tokens = m(6, 100), m(6)
+        assert L.evkhip_token_logprobs(b(logits), b(tokens), 4096, None, b(ids), alt, None, 1.0, None) == SHAPE
+        assert b"rank" in L.evkhip_last_error()
