@@ -177,7 +177,7 @@ DEV void tile_rows(const PrefixArgs& a, const TileWork& w, int item, float* ws, 
     const auto seen = [&](int q) { return Sees{a.P, sl, sl + own[q]}; };
     const uint32_t wild = attend_tiles<DH, QB>(sm, qf, c2, smem, dma, t0, t1, load, plain, seen);
     if (__syncthreads_or(wild))
-        each_wild(plain, [&](int e) { return ((e < a.P) | (e >= sl)) & (e < n) ? v_row(e) : nullptr; }, a.dh, BK, t0, t1, 1, lane, [&](int e) {
+        each_wild(plain, [&](int e) { return (((e < a.P) | (e >= sl)) & (e < n)) ? v_row(e) : nullptr; }, a.dh, BK, t0, t1, 1, lane, [&](int e) {
             bool sees[QB];
 #pragma unroll
             for (int q = 0; q < QB; ++q) sees[q] = Sees{a.P, sl, sl + own[q]}(e);
@@ -222,6 +222,7 @@ struct StepWork {
     int tiles;
     int prefix;               // rows of the prefix in the list: P or 0
     int splits, slots, slot;  // parts of the list; states of a row (0: none) and this list's first
+    int groups;               // parts of all lists
 };
 template <int DH, int NW>
 DEV void step_rows(const PrefixArgs& a, const StepWork& w, int item, float* ws, char* smem, float (*sm_m)[16], float (*sm_l)[16]) {
@@ -229,7 +230,11 @@ DEV void step_rows(const PrefixArgs& a, const StepWork& w, int item, float* ws, 
     constexpr int KS = G::KS;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const int split = item % w.splits, tile = item / w.splits % w.tiles, bc = item / w.splits / w.tiles, c = bc % a.KV, b = bc / a.KV;
+    // Parts go round the XCDs, so that each gets as many long ones, a part's tiles on one of them (sequences in turn on an XCD:
+    // 64 tokens, 32 heads over 8 of 128 behind 4096 rows, up to 1024 of their own, longest first: 52, now 43).
+    const int part = item / 8 / w.tiles * 8 + item % 8, tile = item / 8 % w.tiles;
+    const int split = part % w.splits, bc = part / w.splits, c = bc % a.KV, b = bc / a.KV;
+    if (part >= w.groups) return;
     const Rows rows(a, c);
     const int per = a.N * rows.group, R0 = b * per + tile * 16, end = (b + 1) * per, pre = w.prefix;
     const int least = __builtin_amdgcn_readfirstlane(rows.own(a, R0)), most = __builtin_amdgcn_readfirstlane(rows.own(a, min(R0 + 16, end) - 1));
@@ -288,7 +293,7 @@ __global__ __launch_bounds__(64 * StepGeo<DH>::NW, StepGeo<DH>::NW / 4) void pre
     constexpr int NW = StepGeo<DH>::NW;
     __shared__ __attribute__((aligned(16))) char smem[steps_bytes<DH, NW>()];
     __shared__ float sm_m[NW][16], sm_l[NW][16];
-    step_rows<DH, NW>(a, w, xcd_tile(blockIdx.x, gridDim.x), ws, smem, sm_m, sm_l);
+    step_rows<DH, NW>(a, w, blockIdx.x, ws, smem, sm_m, sm_l);
 }
 
 // The prefix by tiles and the own rows by steps in one launch: the former wait for
@@ -303,11 +308,9 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void prefix_mixed(PrefixArgs
     constexpr int TILES = 4 * BK * Geo<DH>::W * 2, STEPS = steps_bytes<DH, 4>();
     __shared__ __attribute__((aligned(1024))) char smem[TILES > STEPS ? TILES : STEPS];
     __shared__ float sm_m[4][16], sm_l[4][16];
-    const int total = gridDim.x, x = blockIdx.x % 8, j = blockIdx.x / 8;
-    const int w0 = x * (wide / 8) + min(x, wide % 8), wn = wide / 8 + (x < wide % 8);  // this XCD's tiles
-    const int at = x * (total / 8) + min(x, total % 8) - w0 + j - wn;                   // own rows before this workgroup's
-    if (j < wn) tile_rows<DH, QB>(a, tw, w0 + j, ws, reinterpret_cast<f16*>(smem));
-    else step_rows<DH, 4>(a, sw, at, ws, smem, sm_m, sm_l);
+    const int tiles = (wide + 7) / 8 * 8, tile = xcd_tile(blockIdx.x, tiles);
+    if ((int)blockIdx.x >= tiles) step_rows<DH, 4>(a, sw, blockIdx.x - tiles, ws, smem, sm_m, sm_l);
+    else if (tile < wide) tile_rows<DH, QB>(a, tw, tile, ws, reinterpret_cast<f16*>(smem));
 }
 
 // The states of a row, added in order by one wave: groups of DH / 4 lanes take
@@ -402,8 +405,8 @@ Plan plan_for(int64_t B, int64_t N, int64_t P, int64_t R, int64_t H, int64_t KV,
         p.kind = Plan::STEPS;
         const int64_t splits = alone ? 1 : some(JOIN_MOST, 256 / groups, ceil(steps, waves));
         p.slots = splits > 1 ? (int)splits : 0;
-        p.steps = {(int)tiles, (int)P, (int)splits, p.slots, 0};
-        p.few = groups * splits;
+        p.steps = {(int)tiles, (int)P, (int)splits, p.slots, 0, (int)(heads * splits)};
+        p.few = ceil(heads * splits, 8) * 8 * tiles;
         return p;
     }
     // The prefix for all sequences at once, by tiles of 64 rows, of 128 where those are enough to keep the products busy
@@ -416,9 +419,9 @@ Plan plan_for(int64_t B, int64_t N, int64_t P, int64_t R, int64_t H, int64_t KV,
     const int64_t s2 = some(JOIN_MOST / 2, JOIN_MOST / 2, ceil(R, dh <= 128 ? 512 : 256));
     p.slots = (int)(s1 + s2);
     p.wide = wide * s1;
-    p.few = groups * s2;
+    p.few = ceil(heads * s2, 8) * 8 * tiles;
     p.tiles = {(int)all, (int)(wide / KV), 0, (int)s1, p.slots};
-    p.steps = {(int)tiles, 0, (int)s2, p.slots, (int)s1};
+    p.steps = {(int)tiles, 0, (int)s2, p.slots, (int)s1, (int)(heads * s2)};
     return p;
 }
 
@@ -441,8 +444,9 @@ int prefix_forward(const PrefixArgs& a, void* ws, hipStream_t st) {
         return e == hipSuccess ? EVKHIP_OK : check_hip(e, "prefix_attention launch");
     }
     const Plan p = plan_for(a.B, a.N, a.P, a.R, a.H, a.KV, a.dh);
-    const dim3 grid((unsigned)(p.wide + p.few));
-    int rc = check_grid(op, p.wide + p.few, p.kind == Plan::STEPS ? 512 : 256);
+    const int64_t groups = p.kind == Plan::SHARED ? (p.wide + 7) / 8 * 8 + p.few : p.wide + p.few;
+    const dim3 grid((unsigned)groups);
+    int rc = check_grid(op, groups, p.kind == Plan::STEPS ? 512 : 256);
     if (rc == EVKHIP_OK && p.slots) rc = check_grid(op, (rows + 3) / 4, 256);
     if (rc != EVKHIP_OK) return rc;
     float* const part = (float*)ws;
