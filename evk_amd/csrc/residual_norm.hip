@@ -13,7 +13,8 @@
 //
 // Memory-bound: every value read once and written once.  A row lies in TPR
 // threads' registers, NV vectors of eight values each, at any alignment (the
-// last vector takes what is left); weights and gates stay in registers from row
+// last vector takes what is left; narrow rows share a wave: 40000 rows of 256 14 us
+// and 30 with gradient, a wave each 21 and 50); weights and gates stay in registers from row
 // to row.  The sums of a row are in 32 bits, as is everything between the loads
 // and the stores.  8192 rows of 4096: 50 us = 5.3 TB/s (a copy of 1 GiB runs at
 // 5.1); 7996 of 768, where the launch counts, 13.8 = 3.6; 16 rows 3.9.
@@ -56,18 +57,19 @@ DEV half8 ones() {
 }
 
 constexpr int threads_of(int tpr) { return tpr < 256 ? 256 : tpr; }
+constexpr int waves_of(int tpr) { return tpr < 64 ? 1 : tpr / 64; }  // of a row
 
 // Sums over the TPR threads of a row.  Wider rows than a wave meet in LDS, in two
 // places in turn: who writes one again has passed the barrier of the other,
 // which everyone reaches after reading the first.
 template <int TPR>
 struct RowSum {
-    static constexpr int NW = TPR / 64;
+    static constexpr int NW = waves_of(TPR);
     int turn = 0;
     template <int M>
     DEV void operator()(float (&v)[M], float (*lds)[2][NW]) {
 #pragma unroll
-        for (int i = 0; i < M; ++i) v[i] = wave_add(v[i]);
+        for (int i = 0; i < M; ++i) v[i] = TPR < 64 ? lanes_sum<TPR < 64 ? TPR : 1>(v[i]) : wave_add(v[i]);
         if constexpr (NW > 1) {
             const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
             if (lane == 0)
@@ -99,7 +101,7 @@ DEV void stream(const ResidualNormArgs& a, const half8 (&x)[NV], const half8 (&y
 template <int TPR, int NV, bool Y>
 __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_k(ResidualNormArgs a) {
     constexpr int RPW = threads_of(TPR) / TPR;
-    __shared__ float red[2][2][TPR / 64];
+    __shared__ float red[2][2][waves_of(TPR)];
     const int t = threadIdx.x % TPR, D = a.D;
     RowSum<TPR> sum;
     int at[NV], n[NV];
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_k(ResidualNormA
 template <int TPR, int NV, bool Y>
 __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualNormArgs a, int64_t rows_gate, int parts, float* part) {
     constexpr int RPW = threads_of(TPR) / TPR;
-    __shared__ float red[2][2][TPR / 64];
+    __shared__ float red[2][2][waves_of(TPR)];
     __shared__ float cols[RPW > 1 ? RPW : 1][RPW > 1 ? 2 * TPR * NV * 8 : 1];
     const int t = threadIdx.x % TPR, D = a.D;
     const int64_t gate = blockIdx.x / parts, r0 = blockIdx.x % parts;
@@ -346,6 +348,9 @@ __global__ __launch_bounds__(1024) void residual_norm_sums_k(ResidualNormArgs a,
 
 template <class F>
 void by_width(int D, F&& f) {
+    if (D <= 64) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+    if (D <= 128) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+    if (D <= 256) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
     if (D <= 512) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
     if (D <= 1024) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
     if (D <= 2048) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
@@ -358,10 +363,13 @@ static_assert(RESIDUAL_NORM_MOST == 1024 * 2 * 8, "the widest row");
 // Runs of rows of one gate: long ones, whose sums cost less to write and add, as
 // far as every CU keeps rows in flight (us of the gradient with 256, 512 and 1024
 // runs: 7996 rows of 768 30, 27, 34; 4096 rows of 4096 54, 57, 66; 3000 of 8192
-// 81, 92, 101)
+// 81, 92, 101), each with a row for all of a workgroup's threads and two at least
+// (1, 2 and 4: 64 rows of 4096 12.7, 13.4, 16.8; 256 rows 19.4, 17.0, 19.2)
 int64_t runs(int64_t rows, int64_t gates, int D) {
     const int64_t rows_gate = rows / gates, all = D <= 1024 ? 512 : 256;
-    return std::max<int64_t>(1, std::min((rows_gate + 3) / 4, (all + gates - 1) / gates));
+    int64_t least = 0;
+    by_width(D, [&](auto tpr, auto) { least = std::max(2, threads_of(decltype(tpr)::value) / decltype(tpr)::value); });
+    return std::max<int64_t>(1, std::min((rows_gate + least - 1) / least, (all + gates - 1) / gates));
 }
 
 }  // namespace

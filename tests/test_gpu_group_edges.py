@@ -8,7 +8,7 @@ import torch
 
 import evk_amd as evk
 from test_gpu_block import E, F16, F64, H, T, Rng, close, empty
-from test_gpu_group import ids16, prefix_check, prefix_want, scores_check, some_tokens
+from test_gpu_group import Norms, ids16, prefix_check, prefix_want, scores_check, some_tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +148,30 @@ def test_candidates_past_their_list(dev):
         x[3] = 0.0
         x[4, ::3] = 1.0
         scores_check(dev, x, some_tokens(6, v, dev, 4, pad=False), 1.0, 32)
+
+
+@pytest.mark.parametrize("d", [8, 63, 64, 65, 127, 128, 129, 200, 255, 256, 257])
+@pytest.mark.parametrize("b,n,gate", [(1, 1, "channel"), (5, 37, "sequence"), (1, 3001, None), (33, 1, "sequence")])
+def test_residual_norm_narrow_rows(dev, d, b, n, gate):
+    """Rows that share a wave, as many as fill it and not, of one gate and several."""
+    c = Norms(dev, 700 + d + n, b, n, d, True, gate, scale=0.5, odd=d % 2 == 1)
+    s, h = c.forward()
+    want, size = c.want()
+    c.check(dict(s=s, h=h), want, size)
+    c.check(c.backward(), want, size)
+
+
+@pytest.mark.parametrize("d", [24, 100, 250])
+def test_residual_norm_narrow_rows_apart(dev, d):
+    """A row that holds NaN or infinities leaves its neighbours in the wave alone."""
+    c = Norms(dev, 720 + d, 1, 70, d, True, "channel")
+    s0, h0 = c.forward()
+    g0 = c.backward()
+    c.x[0, 9], c.y[0, 34, d - 1], c.x[0, 69, 0] = math.nan, math.inf, -math.inf
+    s, h = c.forward()
+    g = c.backward()
+    same = torch.ones(70, dtype=torch.bool, device=dev)
+    same[[9, 34, 69]] = False
+    for got, was in ((s, s0), (h, h0), (g["dx"], g0["dx"]), (g["dy"], g0["dy"])):
+        assert torch.equal(got[0, same], was[0, same])
+        assert not torch.isfinite(got[0, ~same]).all()
