@@ -258,16 +258,18 @@ __global__ __launch_bounds__(NT, NV == 16 ? 4 : 1) void token_logprobs_k(TokenLo
     }
 }
 
-// The gradient of NV vectors of each thread, all requested before the first is used.
-template <int NT, int NV>
+// The gradient of NV vectors of each thread, all requested before the first is
+// used: TPR threads on a segment of a row, short rows several a workgroup.
+template <int NT, int TPR, int NV>
 __global__ __launch_bounds__(NT) void token_logprobs_bwd_k(TokenLogprobsArgs a, int segments) {
-    const int64_t row = blockIdx.x / segments;
-    const int seg = blockIdx.x % segments, V = a.V, token = a.tokens[row];
+    const int64_t row = TPR < NT ? (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR : blockIdx.x / segments;
+    if (TPR < NT && row >= a.rows) return;
+    const int seg = TPR < NT ? 0 : blockIdx.x % segments, V = a.V, token = a.tokens[row];
     const float w = a.dlogprobs && token < V ? a.dlogprobs[row] : 0.0f, h = a.dentropy ? a.dentropy[row] : 0.0f;
     const float m = a.stats[2 * row], L = a.stats[2 * row + 1], H = a.dentropy ? a.entropy[row] : 0.0f, c2 = a.scale * kLog2e;
     const f16* const l = a.logits + row * V;
     f16* const d = a.dlogits + row * V;
-    auto at = [&](int v) { return 8 * (int)threadIdx.x + 8 * NT * (NV * seg + v); };
+    auto at = [&](int v) { return 8 * (int)(threadIdx.x % TPR) + 8 * TPR * (NV * seg + v); };
     half8 x[NV];
     const bool idle = w == 0.0f && h == 0.0f;  // nothing asked of this row: zeros, whatever it holds
     if (!idle) {
@@ -333,10 +335,22 @@ int token_logprobs_forward(const TokenLogprobsArgs& a, hipStream_t st) {
 
 int token_logprobs_backward(const TokenLogprobsArgs& a, hipStream_t st) {
     constexpr int NT = 256, NV = 2;  // 2560 rows of 32000, us: one vector 80, two 64, four 66, eight 67
-    const int segments = (a.V + 8 * NT * NV - 1) / (8 * NT * NV);
-    const int rc = check_grid("token_logprobs_backward", a.rows * segments, NT);
+    int rc = EVKHIP_OK;
+    auto launch = [&](auto tprc) {
+        constexpr int TPR = decltype(tprc)::value;
+        const int segments = TPR < NT ? 1 : (a.V + 8 * NT * NV - 1) / (8 * NT * NV);
+        const int64_t groups = TPR < NT ? (a.rows + NT / TPR - 1) / (NT / TPR) : a.rows * segments;
+        rc = check_grid("token_logprobs_backward", groups, NT);
+        if (rc == EVKHIP_OK) hipLaunchKernelGGL((token_logprobs_bwd_k<NT, TPR, NV>), dim3((unsigned)groups), dim3(NT), 0, st, a, segments);
+    };
+    // As few threads as a row fills (us, and with a workgroup a row: 2560 rows of 144 3.3 and 3.9, 65536 12.6 and 47.5, 30000 of
+    // 500 15.8 and 29.8, 20000 of 1001 18.5 and 27.4).
+    if (a.V <= 256) launch(std::integral_constant<int, 16>{});
+    else if (a.V <= 512) launch(std::integral_constant<int, 32>{});
+    else if (a.V <= 1024) launch(std::integral_constant<int, 64>{});
+    else if (a.V <= 2048) launch(std::integral_constant<int, 128>{});
+    else launch(std::integral_constant<int, NT>{});
     if (rc != EVKHIP_OK) return rc;
-    hipLaunchKernelGGL((token_logprobs_bwd_k<NT, NV>), dim3((unsigned)(a.rows * segments)), dim3(NT), 0, st, a, segments);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? EVKHIP_OK : check_hip(e, "token_logprobs_backward launch");
 }

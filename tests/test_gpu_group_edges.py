@@ -8,7 +8,7 @@ import torch
 
 import evk_amd as evk
 from test_gpu_block import E, F16, F64, H, T, Rng, close, empty
-from test_gpu_group import Norms, ids16, prefix_check, prefix_want, scores_check, some_tokens
+from test_gpu_group import Norms, grad_check, ids16, prefix_check, prefix_want, scores_check, some_tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -175,3 +175,18 @@ def test_residual_norm_narrow_rows_apart(dev, d):
     for got, was in ((s, s0), (h, h0), (g["dx"], g0["dx"]), (g["dy"], g0["dy"])):
         assert torch.equal(got[0, same], was[0, same])
         assert not torch.isfinite(got[0, ~same]).all()
+
+
+@pytest.mark.parametrize("v", [8, 120, 144, 256, 257, 512, 513, 1001, 1024, 1025, 2048, 2049])
+@pytest.mark.parametrize("rows", [1, 15, 17, 2000])
+def test_token_logprobs_backward_short_rows(dev, v, rows):
+    """Rows that share a workgroup, as many as fill it and not; behind the last one nothing is written."""
+    r = Rng(dev, 740 + v + rows)
+    logits, tokens = r(rows, v, std=3.0, odd=v % 2 == 1), some_tokens(rows, v, dev, v)
+    dlp, dent = r(rows, std=20.0).float(), r(rows, std=5.0).float()
+    d, _ = grad_check(dev, logits, tokens, 0.7, dlp, dent, odd=v % 2 == 0)
+    lp, ent, stats = torch.empty(rows, device=dev), torch.empty(rows, device=dev), torch.empty(rows, 2, device=dev)
+    evk.token_logprobs(logits, tokens, lp, ent, stats=stats, input_scale=0.7)
+    longer = torch.full((rows + 40, v), 9.0, dtype=F16, device=dev)
+    evk.token_logprobs_backward(logits, tokens, stats, dlp, longer[:rows], ent, dent, input_scale=0.7)
+    assert torch.equal(longer[:rows], d) and (longer[rows:] == 9.0).all()
