@@ -158,7 +158,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_k(ResidualNormA
 // gate), keeps the columns' sums dh u and S n in registers and leaves them in the
 // workspace, one row of 2 D sums, which residual_norm_sums_k adds in a fixed
 // order.  A row's sums wait for each other three times; the next row is on its way
-// meanwhile.  4096 rows of 4096: 44 us = 4.6 TB/s; 7996 of 768: 20 = 3.7.
+// meanwhile.  4096 rows of 4096: 41 us = 4.9 TB/s; 7996 of 768: 20 = 3.7.
 template <int TPR, int NV, bool Y>
 __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualNormArgs a, int64_t rows_gate, int parts, float* part) {
     constexpr int RPW = threads_of(TPR) / TPR;
@@ -254,12 +254,17 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
     if constexpr (RPW == 1) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
+            if (n[v] >= 8) {
+                __builtin_memcpy(dst + at[v], dwi[v], 32);
+                if (Y) __builtin_memcpy(dst + D + at[v], dsn[v], 32);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < n[v]) {
-                    dst[at[v] + e] = dwi[v][e];
-                    if (Y) dst[D + at[v] + e] = dsn[v][e];
-                }
+                for (int e = 0; e < 7; ++e)
+                    if (e < n[v]) {
+                        dst[at[v] + e] = dwi[v][e];
+                        if (Y) dst[D + at[v] + e] = dsn[v][e];
+                    }
+            }
     } else {
         constexpr int W = TPR * NV * 8;
 #pragma unroll
@@ -284,39 +289,44 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
 // of the one gate that there is), from 2 on the gradients of 64 / lanes gates.  64
 // groups of 16 threads, four columns a thread: `lanes` of them (a power of two, no
 // more than the runs of a gate need) take a gate's runs in turn, all 64 those of
-// dwi and dwo, and their sums are added in order.  512 runs of 768, 4 gates: 6.8 us,
-// 256 of 4096: 5.3, the latency of eight rows a thread and the launch.
+// dwi and dwo, eight at once, and their sums are added in order.  512 runs of 768, 4
+// gates: 5.6 us, 256 of 4096: 5.5, a launch and the latency of what other XCDs wrote.
 constexpr int SUM_COLS = 64;
 __global__ __launch_bounds__(1024) void residual_norm_sums_k(ResidualNormArgs a, const float* part, int parts, int gates, int blocks, int gate_lanes) {
     __shared__ float red[64][SUM_COLS + 4];
     const int x = threadIdx.x % 16 * 4, u = threadIdx.x / 16, job = blockIdx.x / blocks, c0 = blockIdx.x % blocks * SUM_COLS, D = a.D;
     const int lanes = job < 2 ? 64 : gate_lanes, gate0 = job < 2 ? 0 : (job - 2) * (64 / lanes), gate = gate0 + u / lanes;
     const int64_t r0 = (int64_t)gate * parts + u % lanes, r1 = job < 2 ? (int64_t)gates * parts : gate < gates ? (int64_t)(gate + 1) * parts : 0;
-    const float* const src = part + (job ? D : 0) + c0 + x;
+    const int cx = min(c0 + x, max(D - 4, 0));  // the row's last columns are read with those before them
+    const float* const src = part + (job ? D : 0) + cx;
     const bool weigh = job == 1 && a.gate_rows;
     float v[4] = {};
-    if (c0 + x + 3 < D) {
-#pragma unroll 8
-        for (int64_t r = r0; r < r1; r += lanes) {
-            float p[4];
-            __builtin_memcpy(p, src + r * 2 * D, 16);
-            if (weigh) {
-                half4 g;
-                __builtin_memcpy(&g, a.gate + (int64_t)((int)r / parts) * D + c0 + x, 8);
+    if (D >= 4) {
+        constexpr int AHEAD = 8;
+        for (int64_t r = r0; r < r1; r += AHEAD * lanes) {
+            float p[AHEAD][4];
+            half4 g[AHEAD];
+            auto at = [&](int k) { return min(r + k * lanes, r1 - 1); };
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] *= (float)g[i];
-            }
+            for (int k = 0; k < AHEAD; ++k) __builtin_memcpy(p[k], src + at(k) * 2 * D, 16);
+            if (weigh)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += p[i];
+                for (int k = 0; k < AHEAD; ++k) __builtin_memcpy(&g[k], a.gate + (int64_t)((int)at(k) / parts) * D + cx, 8);
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (r + k * lanes < r1) v[i] += weigh ? p[k][i] * (float)g[k][i] : p[k][i];
         }
     } else {
         for (int64_t r = r0; r < r1; r += lanes)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (c0 + x + i < D) v[i] += src[r * 2 * D + i] * (weigh ? (float)a.gate[(int64_t)((int)r / parts) * D + c0 + x + i] : 1.0f);
+                if (cx + i < D) v[i] += src[r * 2 * D + i] * (weigh ? (float)a.gate[(int64_t)((int)r / parts) * D + cx + i] : 1.0f);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[u][x + i] = v[i];
+    for (int i = 0; i < 4; ++i)
+        if (cx + i >= c0) red[u][cx + i - c0] = v[i];
     __syncthreads();
     const int col = threadIdx.x % SUM_COLS, group = threadIdx.x / SUM_COLS, c = c0 + col;
     auto put = [&](f16* out, float sum) {
