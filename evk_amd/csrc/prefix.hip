@@ -410,14 +410,18 @@ Plan plan_for(int64_t B, int64_t N, int64_t P, int64_t R, int64_t H, int64_t KV,
         return p;
     }
     // The prefix for all sequences at once, by tiles of 64 rows, of 128 where those are enough to keep the products busy
-    // (256 rows of 8 heads over 8192 rows 52 and 60; 64 rows over 2048 13.4 and 11.6); the own rows in parts of up to 16
-    // steps of 128 values, which end at about the same time (one part 55, two 50; 256 values, 500 rows: 22 and 16).  Few rows
-    // leave the join's other states to the prefix (5 tokens, 2 heads over one of 256 behind 16000 rows: 32 parts 21.1, 61 18.9).
+    // (256 rows of 8 heads over 8192 rows 52 and 60; 64 rows over 2048 13.4 and 11.6); of the latter 192 workgroups beside the
+    // own rows, up to two a CU where each would have more than 18 tiles of the prefix (64 x 8
+    // tokens, 32 heads over 8 of 128, 8192 rows: 167 and 129; 16 x 40, 16 over 4, 4096 rows: 53 and 44; 18 or 10 tiles at 64
+    // tokens, 32 over 8, 16000 rows: 58 and 65).  The own rows in parts of up to 16 steps of 128 values, which end at about the
+    // same time (one part 55, two 50; 256 values, 500 rows: 22 and 16).  Few rows leave the join's other states to the prefix
+    // (5 tokens, 2 heads over one of 256 behind 16000 rows: 32 parts 21.1, 61 18.9).
     p.kind = Plan::SHARED;
     p.qb = dh <= 128 && KV * ceil(all, 128) * ceil(P, 512) >= 256 ? 2 : 1;
     const int64_t wide = KV * ceil(all, 64 * p.qb);
     const int64_t s2 = some(JOIN_MOST / 2, JOIN_MOST / 2, ceil(R, dh <= 128 ? 512 : 256));
-    const int64_t s1 = some(JOIN_MOST - s2, (p.qb == 2 ? 192 : 512) / wide, ceil(P, 4 * BK));
+    const int64_t fill = p.qb == 2 ? std::max<int64_t>(192, std::min<int64_t>(512, wide * ceil(P, BK) / 18)) : 512;
+    const int64_t s1 = some(JOIN_MOST - s2, fill / wide, ceil(P, 4 * BK));
     p.slots = (int)(s1 + s2);
     p.wide = wide * s1;
     p.few = ceil(heads * s2, 8) * 8 * tiles;
