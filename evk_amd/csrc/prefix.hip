@@ -25,8 +25,8 @@ DEV int own_rows(const PrefixArgs& a, int b, int t) {
 // ---------------------------------------------------------------------------
 // One wave per query row, any head size and alignment: 64 rows of K at a time, a
 // lane each, then V's columns over the lanes.  For what the MFMA kernels do not
-// take; bounded by the latency of its scalar loads (16 sequences, 8 heads over 2 of
-// 100 values, 1000 rows and up to 300: 218 us).
+// take; bounded by the latency of its loads (16 sequences, 8 heads over 2 of 100
+// values, 1000 rows and up to 300: 120 us).
 // ---------------------------------------------------------------------------
 constexpr int SMAX = 256;  // largest head size
 
@@ -54,7 +54,13 @@ __global__ __launch_bounds__(64) void prefix_rows(PrefixArgs a) {
         if (lane < n) {
             const f16* const k = at(a.pk, a.k, j);
             sc = 0.0f;
-            for (int d = 0; d < dh; ++d) sc += (float)k[d] * s.x[d];
+            int d = 0;
+            for (; d + 8 <= dh; d += 8) {
+                const half8 x = ld_h8(k + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sc += (float)x[e] * s.x[d + e];
+            }
+            for (; d < dh; ++d) sc += (float)k[d] * s.x[d];
             sc *= a.scale * kLog2e;
         }
         const float m_new = fmaxf(m, wave_max(sc));
@@ -70,6 +76,7 @@ __global__ __launch_bounds__(64) void prefix_rows(PrefixArgs a) {
             const int d = lane + 64 * u;
             if (d >= dh) break;
             float v = o[u] * keep;
+#pragma unroll 16
             for (int i = 0; i < n; ++i) v += s.p[i] * (float)s.v[i][d];
             o[u] = v;
         }
