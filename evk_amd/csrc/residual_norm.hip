@@ -162,6 +162,11 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_k(ResidualNormA
 template <int TPR, int NV, bool Y>
 __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualNormArgs a, int64_t rows_gate, int parts, float* part) {
     constexpr int RPW = threads_of(TPR) / TPR;
+    // Room for the weights, the next row and the sums beside a row in the registers of its threads: else the former are read
+    // when they are needed and the sums lie in LDS (1000 rows of 16384, both directions: 108 us; all in registers, which then
+    // do not suffice, 230).
+    constexpr bool ROOM = TPR < 1024;
+    __shared__ floatx4 kept[ROOM ? 1 : 4 * NV][ROOM ? 1 : TPR];  // dwi and dsn of a thread's vectors, in halves
     __shared__ float red[2][2][waves_of(TPR)];
     __shared__ float cols[RPW > 1 ? RPW : 1][RPW > 1 ? 2 * TPR * NV * 8 : 1];
     const int t = threadIdx.x % TPR, D = a.D;
@@ -175,10 +180,21 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
     for (int v = 0; v < NV; ++v) {
         at[v] = 8 * (t + TPR * v);
         n[v] = D - at[v];
-        wi[v] = a.wi ? ld_part(a.wi + at[v], n[v]) : ones();
-        wo[v] = a.wo ? ld_part(a.wo + at[v], n[v]) : ones();
-        g[v] = a.gate ? ld_part(a.gate + (a.gate_rows ? gate * D : 0) + at[v], n[v]) : ones();
     }
+    auto weights = [&] {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            wi[v] = a.wi ? ld_part(a.wi + at[v], n[v]) : ones();
+            wo[v] = a.wo ? ld_part(a.wo + at[v], n[v]) : ones();
+            g[v] = a.gate ? ld_part(a.gate + (a.gate_rows ? gate * D : 0) + at[v], n[v]) : ones();
+        }
+    };
+    if (!ROOM)
+#pragma unroll
+        for (int k = 0; k < 4 * NV; ++k) kept[k][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto anew = [](auto&... values) {  // formed anew behind a barrier, not kept as 32 bits across it
+        if (!ROOM) (forget(values), ...);
+    };
     half8 nx[NV], ny[NV], nds[NV] = {}, ndh[NV];
     auto load = [&](int64_t row) {
         const int64_t base = row * D;
@@ -191,13 +207,20 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
         }
     };
     const int64_t row0 = first + threadIdx.x / TPR;
-    if (row0 < end) load(row0);
+    if (ROOM) {
+        if (row0 < end) load(row0);
+        weights();
+    }
     for (int64_t row = row0; row < end; row += RPW) {
         const int64_t base = row * D;
         half8 x[NV], y[NV], ds[NV], dh[NV];
+        if (!ROOM) {
+            weights();
+            load(row);
+        }
 #pragma unroll
         for (int v = 0; v < NV; ++v) x[v] = nx[v], y[v] = ny[v], ds[v] = nds[v], dh[v] = ndh[v];
-        if (row + RPW < end) load(row + RPW);  // on their way during this row's sums
+        if (ROOM && row + RPW < end) load(row + RPW);  // on their way during this row's sums
         float q = 1.0f;
         if (Y && a.post) {
             float yy[1] = {0.0f};
@@ -208,6 +231,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
             sum(yy, red);
             q = rsqrtf(yy[0] / (float)D + a.eps);
         }
+        anew(x, y, g, wo);
         float s[NV][8], sc[2] = {0.0f, 0.0f};
         stream<Y>(a, x, y, g, wo, q, s);
 #pragma unroll
@@ -218,6 +242,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
                 sc[1] += s[v][e] * ((float)dh[v][e] * (float)wi[v][e]);
             }
         sum(sc, red);
+        anew(y, ds, dh, wi, g, wo);
         const float r = rsqrtf(sc[0] / (float)D + a.eps), back = sc[1] * r / (float)D;  // mean(c u)
         float en[1] = {0.0f};
 #pragma unroll
@@ -226,20 +251,31 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float u = s[v][e] * r, d = (float)dh[v][e];
-                dwi[v][e] += d * u;
+                if (ROOM) dwi[v][e] += d * u;
+                else dwi[v][e] = d * u;
                 const float S = (float)ds[v][e] + r * (d * (float)wi[v][e] - u * back);
                 s[v][e] = S;
                 dx[e] = (Y ? a.scale : 1.0f) * S;
                 if (Y) {
                     const float m = (float)y[v][e] * q;
-                    dsn[v][e] += S * m;
+                    if (ROOM) dsn[v][e] += S * m;
+                    else dsn[v][e] = S * m;
                     en[0] += S * (float)g[v][e] * (float)wo[v][e] * m;
                 }
             }
             st_part(a.dx + base + at[v], n[v], dx);
+            if (!ROOM)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        kept[4 * v + k][t][e] += dwi[v][4 * k + e];
+                        if (Y) kept[4 * v + 2 + k][t][e] += dsn[v][4 * k + e];
+                    }
         }
         if (!Y) continue;
         if (a.post) sum(en, red);
+        anew(y, g, wo);
         const float mean = a.post ? en[0] / (float)D : 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -249,6 +285,14 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
             st_part(a.dy + base + at[v], n[v], dy);
         }
     }
+    if (!ROOM)
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                dwi[v][e] = kept[4 * v + e / 4][t][e % 4];
+                dsn[v][e] = kept[4 * v + 2 + e / 4][t][e % 4];
+            }
     if (!part) return;  // launch-uniform: neither weights nor gates have gradients
     float* const dst = part + (int64_t)blockIdx.x * 2 * D;
     if constexpr (RPW == 1) {

@@ -190,3 +190,19 @@ def test_token_logprobs_backward_short_rows(dev, v, rows):
     longer = torch.full((rows + 40, v), 9.0, dtype=F16, device=dev)
     evk.token_logprobs_backward(logits, tokens, stats, dlp, longer[:rows], ent, dent, input_scale=0.7)
     assert torch.equal(longer[:rows], d) and (longer[rows:] == 9.0).all()
+
+
+@pytest.mark.parametrize("b,n,d,gate", [(1, 1, 8193, None), (2, 5, 9000, "sequence"), (1, 700, 12001, "channel"), (3, 130, 16384, "sequence")])
+def test_residual_norm_widest_rows(dev, b, n, d, gate):
+    """Rows whose sums over a run lie in LDS, runs of one row and of several."""
+    c = Norms(dev, 760 + d, b, n, d, True, gate, scale=1.5, odd=d % 2 == 1)
+    s, h = c.forward()
+    want, size = c.want()
+    c.check(dict(s=s, h=h), want, size)
+    got = c.backward()
+    c.check(got, want, size)
+    again = c.backward()
+    assert all(v is None or torch.equal(v, again[k]) for k, v in got.items())
+    c = Norms(dev, 761 + d, b, n, d, y=False)  # and the norm alone
+    want, size = c.want()
+    c.check(c.backward(), want, size)
