@@ -256,8 +256,10 @@ DEV bool any_open(const bool (&sees)[QB], const bool (&nan)[QB]) {
 }
 
 // The running softmax state of QB blocks of 16 queries (a lane: query l16 of
-// each) and the products of a tile of 16 KB rows into it.
-template <int DH, int QB>
+// each) and the products of a tile of 16 KB rows into it.  P, l and O carry 2^LIFT,
+// up to 7: P then is 2^15 at most, and 2^-14 and below, where fp16 holds fewer bits,
+// LIFT further from the reference.
+template <int DH, int QB, int LIFT = 0>
 struct Softmax {
     static constexpr int DT = Geo<DH>::DT, W = Geo<DH>::W;
     floatx4 o[DT][QB];  // O^T: dh 16 d + 4 g + j, query l16
@@ -299,7 +301,7 @@ struct Softmax {
         }
 #pragma unroll
         for (int q = 0; q < QB; ++q) {
-            const float base = m[q] == -INFINITY ? 0.0f : -m[q];
+            const float base = m[q] == -INFINITY ? 0.0f : LIFT - m[q];
 #pragma unroll
             for (int k2 = 0; k2 < KB / 2; ++k2) {
                 float e[8];
@@ -319,7 +321,7 @@ struct Softmax {
         if (!any_open(sees, nan)) return;
         row_dot(w, qf, k, dh, g);
 #pragma unroll
-        for (int q = 0; q < QB; ++q) w[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[q], c2, m[q] == -INFINITY ? 0.0f : -m[q]));
+        for (int q = 0; q < QB; ++q) w[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[q], c2, m[q] == -INFINITY ? 0.0f : LIFT - m[q]));
         ::evkhip::add_row(o, w, sees, v, dh, g);
     }
 };
@@ -344,8 +346,8 @@ DEV void each_wild(Plain&& plain, Row&& row, int dh, int len, int t0, int t1, in
 // tile before is used; one barrier a tile.  plain(t): every query of the
 // workgroup sees the whole tile; seen(q)(entry): whether the lane's query of block
 // q does.  Non-zero: rows were left out (clean_rows).
-template <int DH, int QB, class Dma, class Load, class Plain, class Seen>
-DEV uint32_t attend_tiles(Softmax<DH, QB>& sm, const half8 (&qf)[QB][Geo<DH>::KS], float c2, f16* smem, const Dma& dma, int t0, int t1, Load&& load,
+template <int DH, int QB, int LIFT, class Dma, class Load, class Plain, class Seen>
+DEV uint32_t attend_tiles(Softmax<DH, QB, LIFT>& sm, const half8 (&qf)[QB][Geo<DH>::KS], float c2, f16* smem, const Dma& dma, int t0, int t1, Load&& load,
                           Plain&& plain, Seen&& seen) {
     constexpr int KS = Geo<DH>::KS, DT = Geo<DH>::DT, TILE = BK * Geo<DH>::W;
     const int g = dma.lane >> 4;
@@ -436,8 +438,8 @@ struct Steps {
         load_v(step, v_row, dh);
     }
     // from `step`, which is loaded, on; k_row, v_row: an entry's row, past the list's end any row that is there
-    template <class KRow, class VRow, class Plain, class Seen>
-    DEV uint64_t run(Softmax<DH, 1>& sm, const half8 (&qf)[1][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
+    template <int LIFT, class KRow, class VRow, class Plain, class Seen>
+    DEV uint64_t run(Softmax<DH, 1, LIFT>& sm, const half8 (&qf)[1][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
                      Seen&& seen) {
         const int g = lane >> 4;
         uint64_t wild = 0;
@@ -489,8 +491,8 @@ constexpr int steps_bytes() {
 }
 // The waves' states of 16 queries as one: store(query, value, m, l, four values of
 // O^T) for all of them
-template <int DH, int NW, class Store>
-DEV void merge_waves(const Softmax<DH, 1>& sm, char* smem, float (*sm_m)[16], float (*sm_l)[16], int lane, int wave, Store&& store) {
+template <int DH, int NW, int LIFT, class Store>
+DEV void merge_waves(const Softmax<DH, 1, LIFT>& sm, char* smem, float (*sm_m)[16], float (*sm_l)[16], int lane, int wave, Store&& store) {
     constexpr int DT = Geo<DH>::DT, OW = DH + 4;
     const int l16 = lane & 15, g = lane >> 4;
     __syncthreads();  // the slots have been read

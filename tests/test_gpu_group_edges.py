@@ -206,3 +206,25 @@ def test_residual_norm_widest_rows(dev, b, n, d, gate):
     c = Norms(dev, 761 + d, b, n, d, y=False)  # and the norm alone
     want, size = c.want()
     c.check(c.backward(), want, size)
+
+
+@pytest.mark.parametrize("b,n,h,kv,dh,p", [(1, 1, 8, 2, 64, 9000), (8, 3, 8, 2, 128, 9000), (16, 40, 4, 4, 64, 9000), (2, 300, 4, 2, 96, 9000), (3, 1, 2, 1, 256, 300)])
+def test_prefix_a_row_that_draws_most(dev, b, n, h, kv, dh, p):
+    """The first row's score is 2^18 above the others' and its values are zeros, so that the output is a sum of small
+    weights.  A weight of 2^-18 of the largest, with 2^7 in front 2^-11, is off by half a step of its 11 bits, as is the
+    result: 2^-12 each in quadrature of the uniform error, below 2^-11 of the norm together."""
+    r = Rng(dev, 780 + dh)
+    q, pk, pv = torch.zeros(b, n, h * dh, dtype=F16, device=dev), torch.zeros(p, kv * dh, dtype=F16, device=dev), r(p, kv * dh)
+    rows = n + 9
+    k, v = torch.zeros(b, rows, kv * dh, dtype=F16, device=dev), r(b, rows, kv * dh)
+    q.view(b, n, h, dh)[..., 0] = 4.0
+    q.view(b, n, h, dh)[..., 1:] = r(b, n, h, dh - 1, std=0.1)
+    pk.view(p, kv, dh)[..., 1:] = r(p, kv, dh - 1)
+    pk.view(p, kv, dh)[0] = 0.0
+    pk.view(p, kv, dh)[0, :, 0] = 18.0 * math.log(2.0) * dh ** 0.5 / 4.0
+    pv[0] = 0.0
+    o, lse = empty(dev, b, n, h * dh), torch.empty(b, h, n, device=dev)
+    evk.prefix_attention(q, pk, pv, k, v, o, dh, lse=lse)
+    w = prefix_want(q, pk, pv, k, v, h, kv, dh, [0] * b)
+    assert float((o.to(F64) - w["o"]).norm() / w["o"].norm()) <= 2.0 ** -11
+    assert ((lse.to(F64) - w["lse"]).abs() <= w["lse_t"]).all()
