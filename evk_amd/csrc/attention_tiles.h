@@ -214,6 +214,30 @@ DEV void row_dot(float (&v)[QB], const half8 (&x)[QB][KS], const f16* row, int d
 #pragma unroll
     for (int q = 0; q < QB; ++q) v[q] = query_sum(v[q]);
 }
+// The same of the queries of an MFMA's columns and a row of K, as the MFMA had it: with any other order of the sum,
+// exponents of large scores would differ from those that the sums l hold.
+template <int KS, int QB>
+DEV void row_scores(float (&v)[QB], const half8 (&x)[QB][KS], const f16* row, int dh, int g) {
+    asm volatile("" : "+v"(g));
+    floatx4 s[QB];
+#pragma unroll
+    for (int q = 0; q < QB; ++q) s[q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k0 = 0; k0 < KS; k0 += 4) {
+        u32x4 y[4];
+#pragma unroll
+        for (int k = 0; k < 4 && k0 + k < KS; ++k) y[k] = *reinterpret_cast<const u32x4*>(row + min(32 * (k0 + k) + 8 * g, dh - 8));
+#pragma unroll
+        for (int k = 0; k < 4 && k0 + k < KS; ++k) {
+            const half8 r = as_half8(32 * (k0 + k) + 8 * g < dh ? y[k] : u32x4{0u, 0u, 0u, 0u});  // each of 16 rows
+#pragma unroll
+            for (int q = 0; q < QB; ++q) s[q] = mfma16(r, x[q][k0 + k], s[q]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int q = 0; q < QB; ++q) v[q] = s[q][0];
+}
 // acc[d][q] += w[q] row, for the columns that see it (and what nobody stores: values past dh)
 template <int DT, int QB>
 DEV void add_row(floatx4 (&acc)[DT][QB], const float (&w)[QB], const bool (&sees)[QB], const f16* row, int dh, int g) {
@@ -255,6 +279,15 @@ DEV bool any_open(const bool (&sees)[QB], const bool (&nan)[QB]) {
     return __any(open);
 }
 
+// Exponents, in powers of two: (s - m) c2 + LIFT with m a score (raw, as s is), in one product and sum from the rounded
+// LIFT - m c2.  While |m| c2 stays below 2^12, that rounding moves a weight by 2^-13 at most.  From there on (FAR) the
+// difference is formed first, which 32 bits hold: a rounding of m c2 would shift all weights of a row, by powers of two
+// from 2^24 on (at 2^29 past fp16's largest value), and those of every part of its list by another one.  Such rows are
+// done again from the list's start (8 x 500 tokens, 16 heads over 4 of 128, behind 4096 rows: 156 us, with scores of tens
+// of thousands 302): both ways in one loop, by a branch, cost every prompt 3 to 5% (the products no longer run under the
+// exponentials) or a third more registers.
+constexpr float FAR_LOG2 = 4096.0f;
+
 // The running softmax state of QB blocks of 16 queries (a lane: query l16 of
 // each) and the products of a tile of 16 KB rows into it.  P, l and O carry 2^LIFT,
 // up to 7: P then is 2^15 at most, and 2^-14 and below, where fp16 holds fewer bits,
@@ -263,8 +296,11 @@ template <int DH, int QB, int LIFT = 0>
 struct Softmax {
     static constexpr int DT = Geo<DH>::DT, W = Geo<DH>::W;
     floatx4 o[DT][QB];  // O^T: dh 16 d + 4 g + j, query l16
-    float m[QB], l[QB];  // reference of the exponents (base 2; -inf: none yet), this lane's part of the sum
-    DEV Softmax() {
+    float m[QB], l[QB];  // the score that exponents refer to (-inf: none yet), this lane's part of the sum
+    bool far;            // |m| c2 has passed FAR_LOG2 for some query of the wave
+    DEV Softmax() { reset(); }
+    DEV void reset() {
+        far = false;
 #pragma unroll
         for (int q = 0; q < QB; ++q) {
             m[q] = -INFINITY;
@@ -273,10 +309,17 @@ struct Softmax {
             for (int d = 0; d < DT; ++d) o[d][q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
+    // What a score's difference to m starts from, and what is taken off first
+    template <bool FAR>
+    DEV void refer(int q, float c2, float& base, float& off) const {
+        const bool none = m[q] == -INFINITY;
+        base = FAR ? (float)LIFT : none ? 0.0f : __builtin_fmaf(-m[q], c2, (float)LIFT);
+        off = FAR && !none ? m[q] : 0.0f;
+    }
     // Scores s (raw) of KB blocks of rows to probabilities, as B operands: P is
     // rounded to fp16 for the product (V is fp16 as well), the sum l is not.
-    template <int KB>
-    DEV void probs(floatx4 (&s)[KB][QB], float c2, half8 (&p)[KB / 2][QB]) {
+    template <bool FAR, int KB>
+    DEV void probs(const floatx4 (&s)[KB][QB], float c2, half8 (&p)[KB / 2][QB]) {
         float mx[QB];
         bool grow = false;
 #pragma unroll
@@ -285,46 +328,58 @@ struct Softmax {
 #pragma unroll
             for (int kb = 1; kb < KB; ++kb)
                 mx[q] = max3(max3(s[kb][q][0], s[kb][q][1], mx[q]), s[kb][q][2], s[kb][q][3]);
-            mx[q] *= c2;
-            grow |= mx[q] > m[q] + RESCALE_LOG2;
+            grow |= (mx[q] - m[q]) * c2 > RESCALE_LOG2;
         }
         if (__any(grow)) {
 #pragma unroll
             for (int q = 0; q < QB; ++q) {
                 const float mn = fmaxf(m[q], query_max(mx[q]));
-                const float keep = m[q] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[q] - mn);
+                const float keep = m[q] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[q] - mn) * c2);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[d][q] *= keep;
                 l[q] *= keep;
                 m[q] = mn;
+                if (!FAR) far |= __any((fabsf(mn) * c2 >= FAR_LOG2) & (fabsf(mn) < INFINITY));
             }
         }
 #pragma unroll
         for (int q = 0; q < QB; ++q) {
-            const float base = m[q] == -INFINITY ? 0.0f : LIFT - m[q];
+            float base, off;
+            refer<FAR>(q, c2, base, off);
 #pragma unroll
             for (int k2 = 0; k2 < KB / 2; ++k2) {
                 float e[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * k2 + i / 4][q][i % 4], c2, base));
+                for (int i = 0; i < 8; ++i) {
+                    const float x = s[2 * k2 + i / 4][q][i % 4];
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(FAR ? x - off : x, c2, base));
+                }
                 l[q] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
                 p[k2][q] = as_half8(u32x4{pack_h2(e[0], e[1]), pack_h2(e[2], e[3]), pack_h2(e[4], e[5]), pack_h2(e[6], e[7])});
             }
         }
     }
-    // V's row of an entry that the queries of `sees` see, whose probability the sums l already hold
-    DEV void add_row(const bool (&sees)[QB], const f16* k, const f16* v, const half8 (&qf)[QB][Geo<DH>::KS], int dh, float c2, int g) {
+    // V's row of an entry that the queries of `sees` see, whose probability the sums l already hold (`again`: by FAR's way)
+    DEV void add_row(const bool (&sees)[QB], const f16* k, const f16* v, const half8 (&qf)[QB][Geo<DH>::KS], int dh, float c2, int g, bool again) {
         float w[QB];
         bool nan[QB];
         spoilt(nan, o);
         if (!any_open(sees, nan)) return;
-        row_dot(w, qf, k, dh, g);
+        row_scores(w, qf, k, dh, g);
 #pragma unroll
-        for (int q = 0; q < QB; ++q) w[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[q], c2, m[q] == -INFINITY ? 0.0f : LIFT - m[q]));
+        for (int q = 0; q < QB; ++q) {
+            float base, off, far_base, far_off;
+            refer<false>(q, c2, base, off);
+            refer<true>(q, c2, far_base, far_off);
+            w[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[q] - (again ? far_off : off), c2, again ? far_base : base));
+        }
         ::evkhip::add_row(o, w, sees, v, dh, g);
     }
+    // log-sum-exp, l the whole sum
+    static DEV float lse(float m, float l, float scale) { return __builtin_fmaf(m, scale, (log2f(l) - (float)LIFT) * kLn2); }
 };
+// The factor of a state whose exponents refer to m in one that refer to `most`
+DEV float state_weight(float m, float most, float c2) { return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - most) * c2); }
 
 // f(entry) for the entries of the tiles of `len`, from tile t0 in steps of dt, that
 // are not seen whole (plain) and whose rows (null: none) hold a NaN or an infinity
@@ -346,8 +401,8 @@ DEV void each_wild(Plain&& plain, Row&& row, int dh, int len, int t0, int t1, in
 // tile before is used; one barrier a tile.  plain(t): every query of the
 // workgroup sees the whole tile; seen(q)(entry): whether the lane's query of block
 // q does.  Non-zero: rows were left out (clean_rows).
-template <int DH, int QB, int LIFT, class Dma, class Load, class Plain, class Seen>
-DEV uint32_t attend_tiles(Softmax<DH, QB, LIFT>& sm, const half8 (&qf)[QB][Geo<DH>::KS], float c2, f16* smem, const Dma& dma, int t0, int t1, Load&& load,
+template <bool FAR, int DH, int QB, int LIFT, class Dma, class Load, class Plain, class Seen>
+DEV uint32_t walk_tiles(Softmax<DH, QB, LIFT>& sm, const half8 (&qf)[QB][Geo<DH>::KS], float c2, f16* smem, const Dma& dma, int t0, int t1, Load&& load,
                           Plain&& plain, Seen&& seen) {
     constexpr int KS = Geo<DH>::KS, DT = Geo<DH>::DT, TILE = BK * Geo<DH>::W;
     const int g = dma.lane >> 4;
@@ -388,7 +443,7 @@ DEV uint32_t attend_tiles(Softmax<DH, QB, LIFT>& sm, const half8 (&qf)[QB][Geo<D
             }
         }
         half8 p[2][QB];
-        sm.template probs<4>(s, c2, p);
+        sm.template probs<FAR, 4>(s, c2, p);
         Cols::template start<2>(col);
         Cols::template run<QB, 2>(col, [&](auto i, auto slot) {
 #pragma unroll
@@ -396,6 +451,21 @@ DEV uint32_t attend_tiles(Softmax<DH, QB, LIFT>& sm, const half8 (&qf)[QB][Geo<D
         });
     }
     return wild;
+}
+// The same, and again where scores are FAR: then sm.far is true for the whole
+// workgroup.  f(): rows that were left out, to be added.
+template <int DH, int QB, int LIFT, class Dma, class Load, class Plain, class Seen, class F>
+DEV void attend_tiles(Softmax<DH, QB, LIFT>& sm, const half8 (&qf)[QB][Geo<DH>::KS], float c2, f16* smem, const Dma& dma, int t0, int t1, Load&& load,
+                      Plain&& plain, Seen&& seen, F&& f) {
+    const uint32_t wild = walk_tiles<false>(sm, qf, c2, smem, dma, t0, t1, load, plain, seen);
+    if (!__syncthreads_or(wild | (sm.far ? 1u : 0u))) return;
+    if (__syncthreads_or(sm.far)) {
+        sm.reset();
+        load(t0, smem, smem + BK * Geo<DH>::W);
+        walk_tiles<true>(sm, qf, c2, smem, dma, t0, t1, load, plain, seen);
+        sm.far = true;
+    }
+    if (__syncthreads_or(wild)) f();
 }
 
 // Every NW-th step of 32 entries into the states of 16 queries, by one wave: K
@@ -437,10 +507,23 @@ struct Steps {
         load_k(step, k_row, dh);
         load_v(step, v_row, dh);
     }
-    // from `step`, which is loaded, on; k_row, v_row: an entry's row, past the list's end any row that is there
+    // from `step`, which is loaded, on; k_row, v_row: an entry's row, past the list's end any row that is there.  Again
+    // where scores are FAR.
     template <int LIFT, class KRow, class VRow, class Plain, class Seen>
     DEV uint64_t run(Softmax<DH, 1, LIFT>& sm, const half8 (&qf)[1][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
                      Seen&& seen) {
+        const uint64_t wild = walk<false>(sm, qf, c2, step, end, k_row, v_row, dh, plain, seen);
+        if (__builtin_expect(sm.far, 0)) {  // code behind the kernel's (between the loop and what follows: 16 tokens of a head of 256 10.8 us, 11.2)
+            sm.reset();
+            load(step, k_row, v_row, dh);
+            walk<true>(sm, qf, c2, step, end, k_row, v_row, dh, plain, seen);
+            sm.far = true;
+        }
+        return wild;
+    }
+    template <bool FAR, int LIFT, class KRow, class VRow, class Plain, class Seen>
+    DEV uint64_t walk(Softmax<DH, 1, LIFT>& sm, const half8 (&qf)[1][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
+                      Seen&& seen) {
         const int g = lane >> 4;
         uint64_t wild = 0;
         for (; step < end; step += NW) {
@@ -475,7 +558,7 @@ struct Steps {
                     for (int j = 0; j < 4; ++j) s[kb][0][j] = see(32 * step + 16 * kb + 4 * g + j) ? s[kb][0][j] : -INFINITY;
             }
             half8 p[1][1];
-            sm.template probs<2>(s, c2, p);
+            sm.template probs<FAR, 2>(s, c2, p);
 #pragma unroll
             for (int d = 0; d < DT; ++d) sm.o[d][0] = mfma16(vf[d], p[0][0], sm.o[d][0]);
         }
@@ -492,7 +575,7 @@ constexpr int steps_bytes() {
 // The waves' states of 16 queries as one: store(query, value, m, l, four values of
 // O^T) for all of them
 template <int DH, int NW, int LIFT, class Store>
-DEV void merge_waves(const Softmax<DH, 1, LIFT>& sm, char* smem, float (*sm_m)[16], float (*sm_l)[16], int lane, int wave, Store&& store) {
+DEV void merge_waves(const Softmax<DH, 1, LIFT>& sm, float c2, char* smem, float (*sm_m)[16], float (*sm_l)[16], int lane, int wave, Store&& store) {
     constexpr int DT = Geo<DH>::DT, OW = DH + 4;
     const int l16 = lane & 15, g = lane >> 4;
     __syncthreads();  // the slots have been read
@@ -513,7 +596,7 @@ DEV void merge_waves(const Softmax<DH, 1, LIFT>& sm, char* smem, float (*sm_m)[1
         floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const float f = sm_m[w][q] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm_m[w][q] - m);
+            const float f = state_weight(sm_m[w][q], m, c2);
             ls += f * sm_l[w][q];
             o += f * *reinterpret_cast<const floatx4*>(st + (w * 16 + q) * OW + d);
         }

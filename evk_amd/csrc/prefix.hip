@@ -46,7 +46,8 @@ __global__ __launch_bounds__(64) void prefix_rows(PrefixArgs a) {
     };
     for (int d = lane; d < dh; d += 64) s.x[d] = (float)a.q[row * dh + d];
     wave_sync();
-    float m = -INFINITY, l = 0.0f, o[SMAX / 64] = {};
+    const float c2 = a.scale * kLog2e;
+    float m = -INFINITY, l = 0.0f, o[SMAX / 64] = {};  // m a score, not scaled
     for (int64_t i0 = 0; i0 < total; i0 += 64) {
         const int n = (int)min((int64_t)64, total - i0);
         const int64_t j = min(i0 + lane, total - 1);
@@ -61,11 +62,10 @@ __global__ __launch_bounds__(64) void prefix_rows(PrefixArgs a) {
                 for (int e = 0; e < 8; ++e) sc += (float)x[e] * s.x[d + e];
             }
             for (; d < dh; ++d) sc += (float)k[d] * s.x[d];
-            sc *= a.scale * kLog2e;
         }
         const float m_new = fmaxf(m, wave_max(sc));
-        const float keep = m == -INFINITY ? 0.0f : exp2f(m - m_new);
-        const float e = lane < n ? exp2f(sc - (m_new == -INFINITY ? 0.0f : m_new)) : 0.0f;
+        const float keep = m == -INFINITY ? 0.0f : exp2f((m - m_new) * c2);
+        const float e = lane < n ? exp2f((sc - (m_new == -INFINITY ? 0.0f : m_new)) * c2) : 0.0f;
         l = l * keep + wave_sum(e);
         m = m_new;
         s.p[lane] = e;
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(64) void prefix_rows(PrefixArgs a) {
 #pragma unroll
     for (int u = 0; u < SMAX / 64; ++u)
         if (lane + 64 * u < dh) a.out[row * dh + lane + 64 * u] = (f16)(total ? o[u] / l : 0.0f);
-    if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = total ? (m + log2f(l)) * kLn2 : -INFINITY;
+    if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = total ? __builtin_fmaf(m, a.scale, log2f(l) * kLn2) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -187,14 +187,14 @@ DEV void tile_rows(const PrefixArgs& a, const TileWork& w, int item, float* ws, 
         return (i1 <= a.P) | ((i1 > sl) & (i1 <= sl + least));
     };
     const auto seen = [&](int q) { return Sees{a.P, sl, sl + own[q]}; };
-    const uint32_t wild = attend_tiles(sm, qf, c2, smem, dma, t0, t1, load, plain, seen);
-    if (__syncthreads_or(wild))
+    attend_tiles(sm, qf, c2, smem, dma, t0, t1, load, plain, seen, [&] {
         each_wild(plain, [&](int e) { return (((e < a.P) | (e >= sl)) & (e < n)) ? v_row(e) : nullptr; }, a.dh, BK, t0, t1, 1, lane, [&](int e) {
             bool sees[QB];
 #pragma unroll
             for (int q = 0; q < QB; ++q) sees[q] = Sees{a.P, sl, sl + own[q]}(e);
-            sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g);
+            sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g, sm.far);
         });
+    });
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int r = wr0 + 16 * q + l16;
@@ -215,7 +215,7 @@ DEV void tile_rows(const PrefixArgs& a, const TileWork& w, int item, float* ws, 
             if (16 * d + 4 * g < a.dh)
                 *reinterpret_cast<uint2*>(dst + 16 * d + 4 * g) =
                     uint2{pack_h2(sm.o[d][q][0] * inv, sm.o[d][q][1] * inv), pack_h2(sm.o[d][q][2] * inv, sm.o[d][q][3] * inv)};
-        if (a.lse && g == 0) a.lse[rows.lse(a, r)] = none ? -INFINITY : (sm.m[q] - LIFT + log2f(l)) * kLn2;
+        if (a.lse && g == 0) a.lse[rows.lse(a, r)] = none ? -INFINITY : sm.lse(sm.m[q], l, a.scale);
     }
 }
 template <int DH, int QB>
@@ -278,9 +278,9 @@ DEV void step_rows(const PrefixArgs& a, const StepWork& w, int item, float* ws, 
     if (wild)
         each_wild(plain, [&](int e) { return e < n ? v_row(e) : nullptr; }, a.dh, 32, first, c1, NW, lane, [&](int e) {
             const bool sees[1] = {e < last};
-            sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g);
+            sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g, sm.far);
         });
-    merge_waves<DH, NW>(sm, smem, sm_m, sm_l, lane, wave, [&](int q, int d, float m, float l, const floatx4& o) {
+    merge_waves<DH, NW>(sm, c2, smem, sm_m, sm_l, lane, wave, [&](int q, int d, float m, float l, const floatx4& o) {
         const int row = R0 + q;
         if (row >= end) return;
         if (w.slots) {
@@ -293,7 +293,7 @@ DEV void step_rows(const PrefixArgs& a, const StepWork& w, int item, float* ws, 
         const float inv = none ? 0.0f : 1.0f / l;
         if (d < a.dh)
             *reinterpret_cast<uint2*>(a.out + rows.row(a, row) * a.dh + d) = uint2{pack_h2(o[0] * inv, o[1] * inv), pack_h2(o[2] * inv, o[3] * inv)};
-        if (a.lse && d == 0) a.lse[rows.lse(a, row)] = none ? -INFINITY : (m - LIFT + log2f(l)) * kLn2;
+        if (a.lse && d == 0) a.lse[rows.lse(a, row)] = none ? -INFINITY : sm.lse(m, l, a.scale);
     });
 }
 template <int DH>
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256) void prefix_join(PrefixArgs a, int slots, int6
     floatx4 ahead[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) ahead[i] = load(part + HPW * i);
-    const float m = wave_top(mine), f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - m);
+    const float m = wave_top(mine), f = state_weight(mine, m, a.scale * kLog2e);
     const float l = wave_add(is ? f * mine_l : 0.0f);
     floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < slots; s0 += HPW * AHEAD) {
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(256) void prefix_join(PrefixArgs a, int slots, int6
     const float inv = none ? 0.0f : 1.0f / l;
     if (part == 0 && d < a.dh)
         *reinterpret_cast<uint2*>(a.out + row * a.dh + d) = uint2{pack_h2(o[0] * inv, o[1] * inv), pack_h2(o[2] * inv, o[3] * inv)};
-    if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = none ? -INFINITY : (m - LIFT + log2f(l)) * kLn2;
+    if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = none ? -INFINITY : Softmax<DH, 1, LIFT>::lse(m, l, a.scale);
 }
 
 bool mfma_ok(const PrefixArgs& a) {

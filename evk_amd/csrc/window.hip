@@ -74,14 +74,15 @@ DEV void fwd_row(const WindowArgs& a, int64_t row, RowLds& s, int lane) {
     wave_sync();
     for (int d = lane; d < dh; d += 64) s.x[d] = (float)a.q[row * dh + d];
     wave_sync();
-    float m = -INFINITY, l = 0.0f, o[SMAX / 64] = {};
+    const float c2 = a.scale * kLog2e;
+    float m = -INFINITY, l = 0.0f, o[SMAX / 64] = {};  // m a score, not scaled
     for (int i0 = 0; i0 < sp.count(); i0 += 64) {
         const int n = min(64, sp.count() - i0);
         const int64_t j = sp.row(min(i0 + lane, sp.count() - 1)) * kv_ld;
-        const float sc = lane < n ? dot_row(a.k + kv0 + j, s.x, dh) * a.scale * kLog2e : -INFINITY;
+        const float sc = lane < n ? dot_row(a.k + kv0 + j, s.x, dh) : -INFINITY;
         const float m_new = fmaxf(m, wave_max(sc));
-        const float keep = m == -INFINITY ? 0.0f : exp2f(m - m_new);
-        const float e = lane < n ? exp2f(sc - (m_new == -INFINITY ? 0.0f : m_new)) : 0.0f;
+        const float keep = m == -INFINITY ? 0.0f : exp2f((m - m_new) * c2);
+        const float e = lane < n ? exp2f((sc - (m_new == -INFINITY ? 0.0f : m_new)) * c2) : 0.0f;
         l = l * keep + wave_sum(e);
         m = m_new;
         s.p[lane] = e;
@@ -100,7 +101,7 @@ DEV void fwd_row(const WindowArgs& a, int64_t row, RowLds& s, int lane) {
 #pragma unroll
     for (int u = 0; u < SMAX / 64; ++u)
         if (lane + 64 * u < dh) a.out[row * dh + lane + 64 * u] = (f16)(sp.count() ? o[u] / l : 0.0f);
-    if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = sp.count() ? (m + log2f(l)) * kLn2 : -INFINITY;
+    if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = sp.count() ? __builtin_fmaf(m, a.scale, log2f(l) * kLn2) : -INFINITY;
 }
 
 // dQ of one query row
@@ -349,17 +350,16 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
     const float c2 = a.scale * kLog2e;
     Softmax<DH, QB> sm;
     const auto plain = [&](int t) { return list.plain(a, t * BK, BK); };
-    const uint32_t wild = attend_tiles<DH, QB>(sm, qf, c2, smem, kv.dma, 0, nt, [&](int t, f16* sk, f16* sv) { kv.load(list, t * BK, sk, sv); }, plain,
-                                               [&](int q) { return Seen(a, list, qp[q]); });
-    if (__syncthreads_or(wild)) {
+    attend_tiles(sm, qf, c2, smem, kv.dma, 0, nt, [&](int t, f16* sk, f16* sv) { kv.load(list, t * BK, sk, sv); }, plain,
+                 [&](int q) { return Seen(a, list, qp[q]); }, [&] {
         const int64_t ld = (int64_t)a.KV * a.dh;
         each_wild(plain, [&](int e) { return list.has(e) ? kv.v + list.row(e) * ld : nullptr; }, a.dh, BK, 0, nt, 1, lane, [&](int e) {
             bool sees[QB];
 #pragma unroll
             for (int q = 0; q < QB; ++q) sees[q] = Seen(a, list, qp[q])(e);
-            sm.add_row(sees, kv.k + list.row(e) * ld, kv.v + list.row(e) * ld, qf, a.dh, c2, g);
+            sm.add_row(sees, kv.k + list.row(e) * ld, kv.v + list.row(e) * ld, qf, a.dh, c2, g, sm.far);
         });
-    }
+    });
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
         const int r = wr0 + 16 * q + l16;
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(256, DH > 128 ? 1 : 2) void window_fwd(WindowArgs a
                 *reinterpret_cast<uint2*>(dst + 16 * d + 4 * g) =
                     uint2{pack_h2(sm.o[d][q][0] * inv, sm.o[d][q][1] * inv), pack_h2(sm.o[d][q][2] * inv, sm.o[d][q][3] * inv)};
         if (a.lse && g == 0)
-            a.lse[((int64_t)b * a.H + c * group + r % group) * a.N + r / group] = none ? -INFINITY : (sm.m[q] + log2f(l)) * kLn2;
+            a.lse[((int64_t)b * a.H + c * group + r % group) * a.N + r / group] = none ? -INFINITY : sm.lse(sm.m[q], l, a.scale);
     }
 }
 
@@ -429,9 +429,9 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
     if (wild)
         each_wild(plain, [&](int e) { return list.has(e) ? v_row(e) : nullptr; }, a.dh, 32, first, c1, NW, lane, [&](int e) {
             const bool sees[1] = {Seen(a, list, qp[0])(e)};
-            sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g);
+            sm.add_row(sees, k_row(e), v_row(e), qf, a.dh, c2, g, sm.far);
         });
-    merge_waves<DH, NW>(sm, smem, sm_m, sm_l, lane, wave, [&](int q, int d, float m, float ls, const floatx4& o) {
+    merge_waves<DH, NW>(sm, c2, smem, sm_m, sm_l, lane, wave, [&](int q, int d, float m, float ls, const floatx4& o) {
         const int row = R0 + q;
         if (row >= NR) return;
         if (splits > 1) {
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(64 * SplitGeo<DH>::NW, SplitGeo<DH>::NW / 4) void w
         if (d < a.dh)
             *reinterpret_cast<uint2*>(a.out + at_row * a.dh + d) = uint2{pack_h2(o[0] * inv, o[1] * inv), pack_h2(o[2] * inv, o[3] * inv)};
         if (a.lse && d == 0)
-            a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = none ? -INFINITY : (m + log2f(ls)) * kLn2;
+            a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = none ? -INFINITY : sm.lse(m, ls, a.scale);
     });
 }
 
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int split
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NW; ++w) m = fmaxf(m, red[0][w]);
-    const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - m);
+    const float f = state_weight(mine, m, a.scale * kLog2e);
     weight[tid] = f;
     l = wave_sum(f * l);
     if (lane == 0) red[1][wave] = l;
@@ -488,7 +488,7 @@ __global__ __launch_bounds__(JOIN_MOST) void window_join(WindowArgs a, int split
     for (int d = tid; d < a.dh; d += 256)
         a.out[at * a.dh + d] = (f16)(((part[0][d] + part[1][d]) + (part[2][d] + part[3][d])) * inv);
     if (a.lse && tid == 0)
-        a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+        a.lse[((int64_t)b * a.H + c * group + row % group) * a.N + row / group] = none ? -INFINITY : Softmax<DH, 1>::lse(m, l, a.scale);
 }
 
 // P and dS are rounded to fp16 for their products, which has 30 powers of two

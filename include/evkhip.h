@@ -356,7 +356,9 @@ int evkhip_qkv_norm_rope_backward(const evkhip_tensor* qkv, const evkhip_tensor*
  * do not reach its output, whatever they hold.  A query that sees no row (an
  * offset below 0) has output 0 and log-sum-exp -inf; one whose scores are all
  * -inf has output NaN (it has no softmax) and log-sum-exp -inf.  lse: NULL or
- * fp32 (B,H,N).  N == 1 is a decode step.  head_dim up to 256. */
+ * fp32 (B,H,N).  N == 1 is a decode step.  head_dim up to 256.  Scores may have
+ * any size: weights come from their differences to the row's largest, as 32 bits
+ * hold them (a row's time about doubles past 2800). */
 uint64_t evkhip_window_attention_workspace(uint32_t batch, uint32_t n, uint32_t rows, uint32_t heads,
                                            uint32_t kv_heads, uint32_t head_dim, uint32_t window, uint32_t sinks);
 int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,
@@ -366,7 +368,9 @@ int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, cons
 
 /* Its gradient over a whole sequence (rows == N, positions from 0) from the
  * forward's o and lse: dQ (as q), dK and dV (as k) are written, dK and dV
- * summed over the heads that share them, in a fixed order. */
+ * summed over the heads that share them, in a fixed order.  Weights come from
+ * scores and lse in 32 bits: they are off by up to |lse| 2^-22 of themselves, so
+ * that there is no gradient of scores past some millions. */
 uint64_t evkhip_window_attention_bwd_workspace(uint32_t batch, uint32_t n, uint32_t heads, uint32_t kv_heads,
                                                uint32_t head_dim, uint32_t window, uint32_t sinks);
 int evkhip_window_attention_bwd(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,
@@ -438,7 +442,7 @@ int evkhip_residual_norm_backward(const evkhip_tensor* x, const evkhip_tensor* y
  * whatever they hold.  A query that sees no row (P 0 and p below 0) has output 0
  * and log-sum-exp -inf; one whose scores are all -inf has output NaN and
  * log-sum-exp -inf.  lse: NULL or fp32 (B,H,N).  N == 1 is a decode step.
- * head_dim up to 256. */
+ * head_dim up to 256.  Scores of any size, as evkhip_window_attention. */
 uint64_t evkhip_prefix_attention_workspace(uint32_t batch, uint32_t n, uint32_t prefix, uint32_t rows, uint32_t heads, uint32_t kv_heads,
                                            uint32_t head_dim);
 int evkhip_prefix_attention(const evkhip_tensor* q, const evkhip_tensor* prefix_k, const evkhip_tensor* prefix_v, const evkhip_tensor* k,
