@@ -288,11 +288,14 @@ DEV bool any_open(const bool (&sees)[QB], const bool (&nan)[QB]) {
 // exponentials) or a third more registers.
 constexpr float FAR_LOG2 = 4096.0f;
 
+// P, l and O carry 2^LIFT: P then is 2^15 at most, and fp16 holds all its bits down to 2^-21 of the reference (2^-14
+// without).  A first row that draws most of the weight and holds little of the values, as models have it (what sinks are
+// kept for), leaves the output to many small weights.
+constexpr int LIFT = 7;
+
 // The running softmax state of QB blocks of 16 queries (a lane: query l16 of
-// each) and the products of a tile of 16 KB rows into it.  P, l and O carry 2^LIFT,
-// up to 7: P then is 2^15 at most, and 2^-14 and below, where fp16 holds fewer bits,
-// LIFT further from the reference.
-template <int DH, int QB, int LIFT = 0>
+// each) and the products of a tile of 16 KB rows into it.
+template <int DH, int QB>
 struct Softmax {
     static constexpr int DT = Geo<DH>::DT, W = Geo<DH>::W;
     floatx4 o[DT][QB];  // O^T: dh 16 d + 4 g + j, query l16
@@ -401,8 +404,8 @@ DEV void each_wild(Plain&& plain, Row&& row, int dh, int len, int t0, int t1, in
 // tile before is used; one barrier a tile.  plain(t): every query of the
 // workgroup sees the whole tile; seen(q)(entry): whether the lane's query of block
 // q does.  Non-zero: rows were left out (clean_rows).
-template <bool FAR, int DH, int QB, int LIFT, class Dma, class Load, class Plain, class Seen>
-DEV uint32_t walk_tiles(Softmax<DH, QB, LIFT>& sm, const half8 (&qf)[QB][Geo<DH>::KS], float c2, f16* smem, const Dma& dma, int t0, int t1, Load&& load,
+template <bool FAR, int DH, int QB, class Dma, class Load, class Plain, class Seen>
+DEV uint32_t walk_tiles(Softmax<DH, QB>& sm, const half8 (&qf)[QB][Geo<DH>::KS], float c2, f16* smem, const Dma& dma, int t0, int t1, Load&& load,
                           Plain&& plain, Seen&& seen) {
     constexpr int KS = Geo<DH>::KS, DT = Geo<DH>::DT, TILE = BK * Geo<DH>::W;
     const int g = dma.lane >> 4;
@@ -454,8 +457,8 @@ DEV uint32_t walk_tiles(Softmax<DH, QB, LIFT>& sm, const half8 (&qf)[QB][Geo<DH>
 }
 // The same, and again where scores are FAR: then sm.far is true for the whole
 // workgroup.  f(): rows that were left out, to be added.
-template <int DH, int QB, int LIFT, class Dma, class Load, class Plain, class Seen, class F>
-DEV void attend_tiles(Softmax<DH, QB, LIFT>& sm, const half8 (&qf)[QB][Geo<DH>::KS], float c2, f16* smem, const Dma& dma, int t0, int t1, Load&& load,
+template <int DH, int QB, class Dma, class Load, class Plain, class Seen, class F>
+DEV void attend_tiles(Softmax<DH, QB>& sm, const half8 (&qf)[QB][Geo<DH>::KS], float c2, f16* smem, const Dma& dma, int t0, int t1, Load&& load,
                       Plain&& plain, Seen&& seen, F&& f) {
     const uint32_t wild = walk_tiles<false>(sm, qf, c2, smem, dma, t0, t1, load, plain, seen);
     if (!__syncthreads_or(wild | (sm.far ? 1u : 0u))) return;
@@ -509,8 +512,8 @@ struct Steps {
     }
     // from `step`, which is loaded, on; k_row, v_row: an entry's row, past the list's end any row that is there.  Again
     // where scores are FAR.
-    template <int LIFT, class KRow, class VRow, class Plain, class Seen>
-    DEV uint64_t run(Softmax<DH, 1, LIFT>& sm, const half8 (&qf)[1][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
+    template <class KRow, class VRow, class Plain, class Seen>
+    DEV uint64_t run(Softmax<DH, 1>& sm, const half8 (&qf)[1][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
                      Seen&& seen) {
         const uint64_t wild = walk<false>(sm, qf, c2, step, end, k_row, v_row, dh, plain, seen);
         if (__builtin_expect(sm.far, 0)) {  // code behind the kernel's (between the loop and what follows: 16 tokens of a head of 256 10.8 us, 11.2)
@@ -521,8 +524,8 @@ struct Steps {
         }
         return wild;
     }
-    template <bool FAR, int LIFT, class KRow, class VRow, class Plain, class Seen>
-    DEV uint64_t walk(Softmax<DH, 1, LIFT>& sm, const half8 (&qf)[1][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
+    template <bool FAR, class KRow, class VRow, class Plain, class Seen>
+    DEV uint64_t walk(Softmax<DH, 1>& sm, const half8 (&qf)[1][KS], float c2, int step, int end, KRow&& k_row, VRow&& v_row, int dh, Plain&& plain,
                       Seen&& seen) {
         const int g = lane >> 4;
         uint64_t wild = 0;
@@ -574,8 +577,8 @@ constexpr int steps_bytes() {
 }
 // The waves' states of 16 queries as one: store(query, value, m, l, four values of
 // O^T) for all of them
-template <int DH, int NW, int LIFT, class Store>
-DEV void merge_waves(const Softmax<DH, 1, LIFT>& sm, float c2, char* smem, float (*sm_m)[16], float (*sm_l)[16], int lane, int wave, Store&& store) {
+template <int DH, int NW, class Store>
+DEV void merge_waves(const Softmax<DH, 1>& sm, float c2, char* smem, float (*sm_m)[16], float (*sm_l)[16], int lane, int wave, Store&& store) {
     constexpr int DT = Geo<DH>::DT, OW = DH + 4;
     const int l16 = lane & 15, g = lane >> 4;
     __syncthreads();  // the slots have been read

@@ -97,11 +97,6 @@ __global__ __launch_bounds__(64) void prefix_rows(PrefixArgs a) {
 // sequences see the same prefix, so that a tile of them reads it once.
 // ---------------------------------------------------------------------------
 
-// A first row that draws most of the weight and holds little of the values, as
-// models have it, leaves the output to many small weights: with 2^7 they keep fp16's
-// bits down to 2^-21 of the largest.
-constexpr int LIFT = 7;
-
 // Where a row of the matrix lies, and what it sees
 struct Rows {
     int group;
@@ -181,7 +176,7 @@ DEV void tile_rows(const PrefixArgs& a, const TileWork& w, int item, float* ws, 
         }
     }
     const float c2 = a.scale * kLog2e;
-    Softmax<DH, QB, LIFT> sm;
+    Softmax<DH, QB> sm;
     const auto plain = [&](int t) {
         const int i1 = (t + 1) * BK;
         return (i1 <= a.P) | ((i1 > sl) & (i1 <= sl + least));
@@ -271,7 +266,7 @@ DEV void step_rows(const PrefixArgs& a, const StepWork& w, int item, float* ws, 
         if (32 * ks + 8 * g < a.dh) qf[0][ks] = *reinterpret_cast<const half8*>(a.q + rows.row(a, r) * a.dh + 32 * ks + 8 * g);
     }
     const float c2 = a.scale * kLog2e;
-    Softmax<DH, 1, LIFT> sm;
+    Softmax<DH, 1> sm;
     const auto plain = [&](int step) { return 32 * step + 32 <= pre + least; };
     const auto seen = [&](int) { return Sees{last, 0, 0}; };
     const uint64_t wild = walk.run(sm, qf, c2, first, c1, k_row, v_row, a.dh, plain, seen);
@@ -365,7 +360,7 @@ __global__ __launch_bounds__(256) void prefix_join(PrefixArgs a, int slots, int6
     const float inv = none ? 0.0f : 1.0f / l;
     if (part == 0 && d < a.dh)
         *reinterpret_cast<uint2*>(a.out + row * a.dh + d) = uint2{pack_h2(o[0] * inv, o[1] * inv), pack_h2(o[2] * inv, o[3] * inv)};
-    if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = none ? -INFINITY : Softmax<DH, 1, LIFT>::lse(m, l, a.scale);
+    if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + t] = none ? -INFINITY : Softmax<DH, 1>::lse(m, l, a.scale);
 }
 
 bool mfma_ok(const PrefixArgs& a) {
