@@ -456,7 +456,9 @@ def greedy_sample(logits, out_tokens, position, token_base, token_count, stream=
 # device (offsets int32, lse fp32).  `workspace` is a uint8 tensor of at least
 # the bytes that the library names for the shapes; without one the call takes it
 # from torch's allocator, in the order of the current stream, and so needs
-# `stream` to be that stream.
+# `stream` to be that stream.  A call on another stream runs in that one's order
+# alone: who allocates, fills or frees its tensors on the current stream has one
+# wait for the other (torch.cuda.Stream.wait_stream), before the call and after.
 
 _F16 = None
 _U32 = (1 << 32) - 1
