@@ -120,7 +120,7 @@ DEV float* state_at(float* ws, int64_t row, int slots, int slot) {
 // lies behind one descriptor.
 //
 // Bounded by the softmax's instructions beside the MFMA: 8 x 500 tokens, 16 heads
-// over 4 of 128, behind 4096 rows, 142 GFLOP in 150 us = 950 TFLOP/s (a product of
+// over 4 of 128, behind 4096 rows, 142 GFLOP in 150-159 us = 890-950 TFLOP/s (a product of
 // the library at 8192^3 runs at 1156).
 struct TileWork {
     int per, tiles;    // rows of one sequence (B N G: all of them together, over the prefix alone), tiles of them
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * StepGeo<DH>::NW, StepGeo<DH>::NW / 4) void pre
 // their products, the latter for memory.  Each XCD starts its part of the tiles
 // first, which take the same time all, and fills up with own rows, which end when
 // they end.  64 tokens, 32 heads over 8 of 128 behind 8192 rows, up to 1024 of their
-// own: 44 us for 34 MB of prefix, whose products are 8.6 GFLOP, and 134 MB of own
+// own: 45-48 us for 34 MB of prefix, whose products are 8.6 GFLOP, and 134 MB of own
 // rows, which alone take 31-38.  4 tokens each behind 4096 rows, with the join: 42, in
 // launches of their own 52.
 template <int DH, int QB>

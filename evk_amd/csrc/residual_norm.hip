@@ -17,7 +17,9 @@
 // and 30 with gradient, a wave each 21 and 50); weights and gates stay in registers from row
 // to row.  The sums of a row are in 32 bits, as is everything between the loads
 // and the stores.  8192 rows of 4096: 50 us = 5.3 TB/s (a copy of 1 GiB runs at
-// 5.1); 7996 of 768, where the launch counts, 13.8 = 3.6; 16 rows 3.9.
+// 5.1), the norm alone (no y) 26 = 5.2; 7996 of 768, where the launch counts, 13.8 =
+// 3.6; 16 rows 3.8.  Rows that are no multiple of 8, whose last values come one by
+// one: 8000 of 1001 15.0 = 4.3 TB/s, of 5001 114 = 2.8 (of 5000 77 = 4.2).
 #include "kernels.h"
 
 #include <algorithm>
@@ -158,7 +160,8 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_k(ResidualNormA
 // gate), keeps the columns' sums dh u and S n in registers and leaves them in the
 // workspace, one row of 2 D sums, which residual_norm_sums_k adds in a fixed
 // order.  A row's sums wait for each other three times; the next row is on its way
-// meanwhile.  4096 rows of 4096: 41 us = 4.9 TB/s; 7996 of 768: 20 = 3.7.
+// meanwhile.  4096 rows of 4096: 41 us = 4.9 TB/s; 7996 of 768: 20 = 3.8; 8000
+// of 5001, with the sums, 205 = 2.3 (of 5000 114 = 4.2).
 template <int TPR, int NV, bool Y>
 __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualNormArgs a, int64_t rows_gate, int parts, float* part) {
     constexpr int RPW = threads_of(TPR) / TPR;
@@ -334,7 +337,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void residual_norm_bwd_k(ResidualN
 // groups of 16 threads, four columns a thread: `lanes` of them (a power of two, no
 // more than the runs of a gate need) take a gate's runs in turn, all 64 those of
 // dwi and dwo, eight at once, and their sums are added in order.  512 runs of 768, 4
-// gates: 5.6 us, 256 of 4096: 5.5, a launch and the latency of what other XCDs wrote.
+// gates: 5.0 us, 256 of 4096: 5.0, a launch and the latency of what other XCDs wrote.
 constexpr int SUM_COLS = 64;
 __global__ __launch_bounds__(1024) void residual_norm_sums_k(ResidualNormArgs a, const float* part, int parts, int gates, int blocks, int gate_lanes) {
     __shared__ float red[64][SUM_COLS + 4];

@@ -305,7 +305,10 @@ __global__ __launch_bounds__(NT) void token_logprobs_bwd_k(TokenLogprobsArgs a, 
 // Threads and vectors of a row: as few waves as its registers fit.  Their barriers
 // cost less than more loads at once save, for few rows too (with 5 alternatives,
 // us of 256 threads and of 1024: 64 rows of 32000 8.1 and 9.0, 1024 rows 19.5 and
-// 25.1; of 512 threads 4001 rows 64.3, of 256 61.3).
+// 25.1; of 512 threads 4001 rows 64.3, of 256 61.3).  A row pays for all vectors of
+// its shape: TB/s of thousands of rows at a shape's end and past it, 4.2 (4000) and
+// 2.7 (4200), 4.9 (8000) and 3.1 (9000), 5.0 (16000) and 3.0 (17000), 4.9 (32000) and
+// 2.9 (33000); 4.4 at 24000, 3.9 at 50257.
 template <class F>
 void by_vocab(int V, F&& f) {
 #define EVK_SHAPE(NT, NV) f(std::integral_constant<int, NT>{}, std::integral_constant<int, NV>{})
