@@ -369,8 +369,8 @@ int evkhip_window_attention(const evkhip_tensor* q, const evkhip_tensor* k, cons
 /* Its gradient over a whole sequence (rows == N, positions from 0) from the
  * forward's o and lse: dQ (as q), dK and dV (as k) are written, dK and dV
  * summed over the heads that share them, in a fixed order.  Weights come from
- * scores and lse in 32 bits: they are off by up to |lse| 2^-22 of themselves, so
- * that there is no gradient of scores past some millions. */
+ * scores and lse in 32 bits: they are off by up to |lse| 2^-20 of themselves, so
+ * that scores past some hundred thousands have no gradient. */
 uint64_t evkhip_window_attention_bwd_workspace(uint32_t batch, uint32_t n, uint32_t heads, uint32_t kv_heads,
                                                uint32_t head_dim, uint32_t window, uint32_t sinks);
 int evkhip_window_attention_bwd(const evkhip_tensor* q, const evkhip_tensor* k, const evkhip_tensor* v,
